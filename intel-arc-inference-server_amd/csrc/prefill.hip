@@ -95,12 +95,6 @@ __device__ __forceinline__ u4_t dequant_scaled(uint32_t w, h2_t s2, const DqCons
   return u4_t{h2_bits(p0 * s2), h2_bits(p1 * s2), h2_bits(p2 * s2), h2_bits(p3 * s2)};
 }
 
-// outputs are stored in pieces of several elements at the elements' own alignment
-typedef f4_t f4_any __attribute__((aligned(4)));
-typedef uint32_t h2_any __attribute__((aligned(2)));
-typedef u2_t h4_any __attribute__((aligned(2)));
-typedef u4_t h8_any __attribute__((aligned(2)));
-
 // A wave's 64 columns: lane (fr, fq) = (l % 16, l / 16) reads word row fq of a half group's four at
 // columns 4 fr .. 4 fr + 3 (one 16-byte load), and column 4 fr + j is column fr of the wave's matrix
 // tile j: the B operand is the lane's own word, and the lane ends with four adjacent columns.
@@ -734,19 +728,6 @@ __device__ __forceinline__ u4_t widen_i8x8(uint32_t x0, uint32_t x1) {
               h2_bits(as_h2(__builtin_amdgcn_perm(hi, x0, 0x04030402u)) - bias),
               h2_bits(as_h2(__builtin_amdgcn_perm(hi, x1, 0x04010400u)) - bias),
               h2_bits(as_h2(__builtin_amdgcn_perm(hi, x1, 0x04030402u)) - bias)};
-}
-
-// (v_maximum3_f32: fmaxf would quieten each operand first, an instruction per operand)
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x, y), z);
-}
-// the max over the four lanes l % 16 + 16 k that hold one column's scores
-__device__ __forceinline__ float col_max(float x) {
-  float a0 = x, a1 = x;
-  lane_swap16(a0, a1);
-  float b0 = __builtin_elementwise_maximum(a0, a1), b1 = b0;
-  lane_swap32(b0, b1);
-  return __builtin_elementwise_maximum(b0, b1);
 }
 
 // 8 consecutive elements of a cache row as loaded, and as f16
