@@ -36,6 +36,8 @@ extern "C" {
  * activation left the fp16 range): the argmax kernels set it when the word was 0, and the
  * step's token is not to be used. */
 #define MI_STATUS_NONFINITE 0xDEAD0004u
+/* mi_attn_masked's flag word after a page table entry outside the cache. */
+#define MI_STATUS_BAD_PAGE 0xDEAD0005u
 
 enum {
   MI_OK = 0,
@@ -496,6 +498,78 @@ int mi_moe_prefill(const uint32_t* route, const uint16_t* x, const uint32_t* gu_
                    const uint32_t* dn_blocks, uint16_t* resid, uint32_t T, uint32_t experts,
                    uint32_t top_k, uint32_t hidden, uint32_t inter, uint32_t* list, uint32_t* tiles,
                    uint32_t* tiles_n, uint16_t* h, uint16_t* d, void* stream);
+
+/* ---- scoring many positions of a text: the linear in 8-bit integers, log probabilities, attention
+ * with masks. No counterpart in the reference, which scores nothing; the conventions are those of the
+ * entries above. Each may be captured into a hipGraph: sizes and pointers are the launch's, what the
+ * device arrays hold (tokens, spans, positions, pages, activations) is read at every replay. Calls that
+ * overlap need workspaces of their own. ---- */
+enum { MI_OUT_F32 = 0, MI_OUT_F16 = 1 };
+/* Rows of activations to 8 bits: s[m] = max_k |x[m][k]| / 127 (fp32), q = rne(x / s), as
+ * mi_lm_head_int8_quantise does to a head's rows; a zero row s = 0, q = 0; a row with a value that is not
+ * finite s = NaN, q = 0 (its outputs are then NaN, the other rows' untouched). x f16 [M][K], rows x_stride
+ * apart (a multiple of 8, x 16-byte aligned); q_tiled in mi_i8w_index(K, k, m)'s layout, M rounded up to 16
+ * times K bytes (the rows behind M are set to zero). K a multiple of 64 up to 131072, M up to 2^20. */
+int mi_quant_rows_i8(const uint16_t* x, size_t x_stride, uint32_t M, uint32_t K, int8_t* q_tiled,
+                     float* row_scales, void* stream);
+/* out [M][N] = ((float)(sum_k q[m][k] w[n][k]) * row_scales[m]) * w_scales[n]: the sum exact in int32, one
+ * rounding to fp32 and two products, for MI_OUT_F16 one more to f16. w_tiled and w_scales as
+ * mi_lm_head_int8_quantise gives them, for any linear with N a multiple of 16; rows of out out_stride
+ * elements apart. An output's bits depend on its row and its column alone. */
+int mi_gemm_w8a8(const int8_t* q_tiled, const float* row_scales, const int8_t* w_tiled,
+                 const float* w_scales, void* out, uint32_t out_kind, size_t out_stride, uint32_t M,
+                 uint32_t K, uint32_t N, void* stream);
+/* mi_quant_rows_i8 and mi_gemm_w8a8 in one call, bit for bit; ws: mi_linear_w8a8_ws(M, K) bytes of device
+ * scratch, 16-byte aligned. */
+size_t mi_linear_w8a8_ws(uint32_t M, uint32_t K);
+int mi_linear_w8a8(const uint16_t* x, size_t x_stride, const int8_t* w_tiled, const float* w_scales,
+                   void* ws, size_t ws_bytes, void* out, uint32_t out_kind, size_t out_stride, uint32_t M,
+                   uint32_t K, uint32_t N, void* stream);
+/* Log probabilities over logits fp32 [M][vocab_used], rows row_stride apart: of tokens[m] the log
+ * probability and the rank (how many tokens come before it: a larger logit, or an equal one and a lower
+ * id), the entropy of the row's distribution (nats), and its `top` most likely tokens with their log
+ * probabilities, [M][top], best first. Any of logprob, rank, entropy may be NULL; tokens too, without the
+ * first two; top 0..64, 0 with NULL arrays. A token id >= vocab_used: logprob NaN, rank 0xFFFFFFFF. A logit
+ * of -inf has probability 0 (and counts nothing in the entropy). A NaN, a +inf or nothing but -inf in a row makes its
+ * probabilities and entropy NaN, as the formulas say; a NaN is behind every token, and has the rank
+ * 0xFFFFFFFF. Places past vocab_used hold the id 0xFFFFFFFF and -inf. ws: mi_logprobs_ws bytes of device
+ * scratch, 16-byte aligned (NULL where that is 0). M up to 65535, vocab_used up to 2^23. */
+size_t mi_logprobs_ws(uint32_t M, uint32_t vocab_used, uint32_t top);
+int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, uint32_t M,
+                uint32_t vocab_used, uint32_t top, float* logprob, uint32_t* rank, float* entropy,
+                uint32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes, void* stream);
+/* What the rows of mi_attn_masked see, device arrays of T (slopes: q_heads). Row t stands at cache position
+ * pos[t] (NULL: pos0 + t) and sees the keys j < hi[t] (NULL: pos + 1, causal) that are at or behind lo[t]
+ * (NULL: 0) or before `prefix`:
+ *   a sliding window   lo = pos + 1 - window
+ *   packed documents   lo = the document's first position (with prefix: a prompt that all of them share)
+ *   a prompt that sees itself whole   hi = max(pos + 1, the prompt's end)
+ *   padding            hi = 0
+ * cap > 0: scores become cap * tanh(score / cap). slopes: slopes[h] * |pos - j| is taken off a score of
+ * head h (after the cap). */
+typedef struct mi_attn_mask {
+  const uint32_t* lo;
+  const uint32_t* hi;
+  const uint32_t* pos;
+  uint32_t pos0;
+  uint32_t prefix;
+  float cap;
+  const float* slopes;
+} mi_attn_mask;
+/* Attention of T rows, one or many (q fp32 [T][q_heads][head_dim] as mi_attn_prep and mi_attn_prep_rows
+ * write it, magnitudes below 65504), over the f16 cache: row layout as mi_attn_prefill, keys at or behind
+ * kv_len are never read. attn_out [T][q_heads * head_dim] f16 (shape->act as mi_attn_reduce); a row that sees
+ * no key gives zeros. What a row does not see has no part in it, infinities and NaN included. pages: cache row
+ * of key j = pages[j / page] * page + j % page, n_pages the pages that the cache holds; an entry that is not
+ * below n_pages sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL), the call's outputs are then not to be
+ * used, and nothing outside the cache is read. head_dim 128 or 256, up to 64 q heads per kv head, not gated;
+ * T up to 65535. ws: mi_attn_masked_ws(T, kv_len, shape) bytes of device scratch, 16-byte aligned (NULL
+ * where that is 0). */
+size_t mi_attn_masked_ws(uint32_t T, uint32_t kv_len, const mi_attn_shape* shape);
+int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v, size_t row_stride,
+                   size_t head_stride, const uint32_t* pages, uint32_t page, uint32_t n_pages,
+                   uint32_t kv_len, uint32_t T, const mi_attn_shape* shape, const mi_attn_mask* mask,
+                   void* ws, size_t ws_bytes, uint16_t* attn_out, uint32_t* flag, void* stream);
 
 /* ---- the decode loop (src/runtime/engine.h:52-331, capture.cc, control.h) ----
  * Model shape as data (model::ModelDesc, src/model/model_desc.h:67-229), restricted to the

@@ -109,6 +109,14 @@ SIGNATURES = {
     "mi_moe_gate_up_routed": (i32, [vp, u32, vp, vp, vp, vp, u32, u32, u32, u32, u32, vp]),
     "mi_moe_down_norm": (i32, [vp, vp, vp, vp, u32, u32, u32, u32, u32, vp, vp, vp, f32, vp, vp, u32, u32, vp]),
     "mi_moe_down": (i32, [vp, vp, vp, vp, u32, u32, u32, u32, u32, vp]),
+    "mi_quant_rows_i8": (i32, [vp, sz, u32, u32, vp, vp, vp]),
+    "mi_gemm_w8a8": (i32, [vp, vp, vp, vp, vp, u32, sz, u32, u32, u32, vp]),
+    "mi_linear_w8a8_ws": (sz, [u32, u32]),
+    "mi_linear_w8a8": (i32, [vp, sz, vp, vp, vp, sz, vp, u32, sz, u32, u32, u32, vp]),
+    "mi_logprobs_ws": (sz, [u32, u32, u32]),
+    "mi_logprobs": (i32, [vp, sz, vp, u32, u32, u32, vp, vp, vp, vp, vp, vp, sz, vp]),
+    "mi_attn_masked_ws": (sz, [u32, u32, vp]),
+    "mi_attn_masked": (i32, [vp, vp, vp, sz, sz, vp, u32, u32, u32, u32, vp, vp, vp, sz, vp, vp, vp]),
 }
 
 
@@ -128,6 +136,8 @@ class GemvEpilogue(C.Structure):
 
 
 STATUS_HANDOFF_TIMEOUT = 0xDEAD0003
+STATUS_BAD_PAGE = 0xDEAD0005
+OUT_F32, OUT_F16 = 0, 1  # mi_gemm_w8a8's and mi_linear_w8a8's out_kind
 
 
 class MiError(RuntimeError):
@@ -181,6 +191,11 @@ class AttnShape(C.Structure):
     _fields_ = [("q_heads", u32), ("kv_heads", u32), ("head_dim", u32), ("rot_dim", u32),
                 ("gated", u32), ("qkv_n", u32), ("k_off", u32), ("v_off", u32), ("scale", f32),
                 ("eps", f32), ("act", u32)]
+
+
+class AttnMask(C.Structure):
+    """mi_attn_mask: the rows' spans of keys, the cap of the scores and the bias by distance."""
+    _fields_ = [("lo", vp), ("hi", vp), ("pos", vp), ("pos0", u32), ("prefix", u32), ("cap", f32), ("slopes", vp)]
 
 
 def lib_shape(sh, act=0):

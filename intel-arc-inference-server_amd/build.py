@@ -27,6 +27,7 @@ HIP_ONLY = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-
 # fp32 accumulators by the vector ALUs at once, so it too is kept out of AGPRs (no copies out of
 # them: 27B step 4.23 -> 4.13 ms, verify steps at 2..8 rows 0.5-2 % faster).
 PER_FILE = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+            "attn_masked.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],  # as attn.hip
             "gemv_w4a16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
             # the prefill GEMM and attention: 27B prefill 20.4 -> 21.1 k tokens/s, MoE 69.7 -> 72.0 k
             "prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
