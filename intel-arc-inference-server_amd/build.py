@@ -28,6 +28,9 @@ HIP_ONLY = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-
 # them: 27B step 4.23 -> 4.13 ms, verify steps at 2..8 rows 0.5-2 % faster).
 PER_FILE = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
             "attn_masked.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],  # as attn.hip
+            # as attn.hip (one work-group per CU leaves 512 registers, and the accumulators then go to AGPRs and
+            # back: 128 x 5120 x 34816 in 128 x 128 tiles 72.5 us against 64.2)
+            "gemm_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
             "gemv_w4a16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
             # the prefill GEMM and attention: 27B prefill 20.4 -> 21.1 k tokens/s, MoE 69.7 -> 72.0 k
             "prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],

@@ -32,47 +32,98 @@ __device__ __forceinline__ uint32_t max_abs8(uint32_t m, u4_t v) {
   const uint32_t a = max_u16x2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), b = max_u16x2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu);
   return max_u16x2(m, max_u16x2(a, b));
 }
-// rne(x / s) as the low byte: |x / s| < 2^22, and 1.5 * 2^23 + r rounds r to an integer in the sum's low bits
-__device__ __forceinline__ uint32_t quant_word(uint32_t p0, uint32_t p1, float s) {
+// rne(x / s) as the low byte, |x / s| <= 127: 1.5 * 2^23 + r rounds r to an integer in the sum's low bits. The
+// quotient is the fp32 one of the definition wherever that matters: x times the rounded 1 / s is within 2^-15 of it,
+// so only a product nearer than 2^-13 to a border between integers (one in 4096) is divided.
+__device__ __forceinline__ uint32_t quant_word(uint32_t p0, uint32_t p1, float s, float inv) {
+  constexpr float kMagic = 12582912.0f;
   uint32_t b[4];
+  bool near = false;
+  float v[4];
 #pragma unroll
   for (uint32_t i = 0; i < 4; ++i) {
-    const float v = h2f((uint16_t)((i < 2 ? p0 : p1) >> (16u * (i & 1u))));
-    b[i] = __builtin_bit_cast(uint32_t, v / s + 12582912.0f);
+    v[i] = h2f((uint16_t)((i < 2 ? p0 : p1) >> (16u * (i & 1u))));
+    const float r = v[i] * inv, m = r + kMagic;
+    near |= fabsf(r - (m - kMagic)) > 0.5f - 0x1p-13f;
+    b[i] = __builtin_bit_cast(uint32_t, m);
+  }
+  if (near) {
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) b[i] = __builtin_bit_cast(uint32_t, v[i] / s + kMagic);
   }
   const uint32_t lo = __builtin_amdgcn_perm(b[1], b[0], 0x0C0C0400u), hi = __builtin_amdgcn_perm(b[3], b[2], 0x0C0C0400u);
   return lo | (hi << 16);
 }
+// A unit is 16 of a row's values, the 16 bytes of one lane of a fragment: unit u = 4 c + q holds
+// k = 64 c + 8 q .. + 7 (a) and 64 c + 32 + 8 q .. + 7 (b).
+struct Unit {
+  u4_t a, b;
+};
+__device__ __forceinline__ Unit load_unit(const uint16_t* row, uint32_t u) {
+  const u4_t* p = reinterpret_cast<const u4_t*>(row + 64u * (u >> 2) + 8u * (u & 3u));
+  return {p[0], p[4]};
+}
+// the row's scale from its largest magnitude's bits (f16 magnitudes are ordered as their bits; an infinity or a NaN is at
+// or above 0x7C00)
+struct Scale {
+  float s, inv;
+  bool zero;  // the row's integers are zeros: a zero row, or one that is not finite
+};
+__device__ __forceinline__ Scale row_scale(uint32_t bits) {
+  const bool finite = bits < 0x7C00u;
+  const float s = finite ? h2f((uint16_t)bits) / 127.0f : __builtin_bit_cast(float, kNanBits);
+  return {s, 1.0f / s, !finite || bits == 0u};
+}
+__device__ __forceinline__ u4_t quant_unit(const Unit& v, const Scale& s) {
+  const u4_t w = {quant_word(v.a.x, v.a.y, s.s, s.inv), quant_word(v.a.z, v.a.w, s.s, s.inv), quant_word(v.b.x, v.b.y, s.s, s.inv),
+                  quant_word(v.b.z, v.b.w, s.s, s.inv)};
+  return s.zero ? u4_t{0u, 0u, 0u, 0u} : w;
+}
+__device__ __forceinline__ uint32_t max_bits(uint32_t m) { return (uint32_t)wave_max((float)max(m & 0xFFFFu, m >> 16)); }
 
-// One wave per row, four rows per work-group; a unit is 16 of the row's values, the 16 bytes of one lane of a
-// fragment: k = 64 c + 8 q .. + 7 and 64 c + 32 + 8 q .. + 7.
-__global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restrict__ x, size_t x_stride, uint32_t M,
-                                                         uint32_t K, int8_t* __restrict__ q_tiled,
-                                                         float* __restrict__ scales) {
-  const uint32_t lane = threadIdx.x & 63u, m = blockIdx.x * 4u + (threadIdx.x >> 6), units = K / 16u;
+// W waves per row, up to U units per lane held in registers between the maximum and the quotients; 4 rows per work-group of
+// single waves (their units are 64 adjacent bytes).
+template <uint32_t W, uint32_t U>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void quant_rows_kernel(const uint16_t* __restrict__ x, size_t x_stride,
+                                                                           uint32_t M, uint32_t K, int8_t* __restrict__ q_tiled,
+                                                                           float* __restrict__ scales) {
+  const uint32_t wave = threadIdx.x >> 6, t = W == 1 ? threadIdx.x & 63u : threadIdx.x;
+  const uint32_t m = W == 1 ? blockIdx.x * 4u + wave : blockIdx.x, units = K / 16u;
   u4_t* to = reinterpret_cast<u4_t*>(q_tiled + (size_t)(m / 16u) * 16u * K) + m % 16u;
   if (m >= M) {  // the last fragment's rows behind the matrix
-    for (uint32_t u = lane; u < units; u += 64u) to[16u * u] = u4_t{0u, 0u, 0u, 0u};
+    for (uint32_t u = t; u < units; u += 64u * W) to[16u * u] = u4_t{0u, 0u, 0u, 0u};
     return;
   }
   const uint16_t* row = x + (size_t)m * x_stride;
-  auto piece = [&](uint32_t u, uint32_t half) {
-    return *reinterpret_cast<const u4_t*>(row + 64u * (u >> 2) + 32u * half + 8u * (u & 3u));
-  };
+  Unit v[U];
   uint32_t mx = 0;
-  for (uint32_t u = lane; u < units; u += 64u) mx = max_abs8(max_abs8(mx, piece(u, 0)), piece(u, 1));
-  // (f16 magnitudes are ordered as their bits; an infinity or a NaN is at or above 0x7C00)
-  const uint32_t bits = (uint32_t)wave_max((float)max(mx & 0xFFFFu, mx >> 16));
-  const bool finite = bits < 0x7C00u;
-  const float s = finite ? h2f((uint16_t)bits) / 127.0f : __builtin_bit_cast(float, kNanBits);
-  if (lane == 0) scales[m] = s;
-  const bool zero = !finite || bits == 0;
-  for (uint32_t u = lane; u < units; u += 64u) {
-    const u4_t a = piece(u, 0), b = piece(u, 1);
-    u4_t w = {quant_word(a.x, a.y, s), quant_word(a.z, a.w, s), quant_word(b.x, b.y, s), quant_word(b.z, b.w, s)};
-    if (zero) w = u4_t{0u, 0u, 0u, 0u};
-    to[16u * u] = w;
+#pragma unroll
+  for (uint32_t i = 0; i < U; ++i)
+    if (t + 64u * W * i < units) v[i] = load_unit(row, t + 64u * W * i);
+#pragma unroll
+  for (uint32_t i = 0; i < U; ++i)
+    if (t + 64u * W * i < units) mx = max_abs8(max_abs8(mx, v[i].a), v[i].b);
+  uint32_t bits = max_bits(mx);
+  if constexpr (W > 1) {
+    __shared__ uint32_t part[W];
+    if ((threadIdx.x & 63u) == 0) part[wave] = bits;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < W; ++i) bits = max(bits, part[i]);
   }
+  const Scale s = row_scale(bits);
+  if (t == 0) scales[m] = s.s;
+#pragma unroll
+  for (uint32_t i = 0; i < U; ++i)
+    if (t + 64u * W * i < units) to[16u * (t + 64u * W * i)] = quant_unit(v[i], s);
+}
+// One wave per row where the rows alone fill the chip, else four, or as many as its units take.
+void launch_quant(const uint16_t* x, size_t x_stride, uint32_t M, uint32_t K, int8_t* q, float* s, hipStream_t st) {
+  const uint32_t rows = (M + 15u) / 16u * 16u;
+  if (K <= 8192 && M >= 1024) quant_rows_kernel<1, 8><<<rows / 4u, 256, 0, st>>>(x, x_stride, M, K, q, s);
+  else if (K <= 8192) quant_rows_kernel<4, 2><<<rows, 256, 0, st>>>(x, x_stride, M, K, q, s);
+  else if (K <= 32768) quant_rows_kernel<8, 4><<<rows, 512, 0, st>>>(x, x_stride, M, K, q, s);
+  else quant_rows_kernel<16, 8><<<rows, 1024, 0, st>>>(x, x_stride, M, K, q, s);
 }
 
 struct GemmArgs {
@@ -102,50 +153,269 @@ __device__ __forceinline__ void store4(const GemmArgs& a, uint32_t m, uint32_t n
   }
 }
 
-// 2 x 2 waves of 64 x 64 outputs each, operands straight from memory. A is the weights, so a lane ends with four
-// adjacent columns of one row.
-template <bool F32>
-__global__ __launch_bounds__(256) void gemm_w8a8_kernel(GemmArgs a) {
+// Few rows: MT x 16 rows and NT x 16 columns per work-group, whose W waves deal the chunks of k out among them, U at a
+// time each. Both operands come straight from memory (a lane without a row loads none); A is the weights, so a lane
+// ends with four adjacent columns of one row. The waves' sums join through LDS.
+template <bool F32, uint32_t MT, uint32_t NT, uint32_t W, uint32_t U>
+__global__ __launch_bounds__(64 * W) void gemm_w8a8_few_kernel(GemmArgs a) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const uint32_t nc = a.K / 64u, nt = a.N / 16u, mt = (a.M + 15u) / 16u;
-  const uint32_t n0 = (blockIdx.x * 2u + (wave & 1u)) * 4u, m0 = (blockIdx.y * 2u + (wave >> 1)) * 4u;
-  const u4_t *wp[4], *qp[4];
+  const uint32_t nc = a.K / 64u, nt = a.N / 16u;
+  const uint32_t n0 = blockIdx.x * NT, m0 = blockIdx.y * MT;
+  const u4_t* wp[NT];
+  const u4_t* qp[MT];
+  bool have[MT];
 #pragma unroll
-  for (uint32_t i = 0; i < 4; ++i) {  // (a tile behind the matrix reads its last one and stores nothing)
-    wp[i] = a.w + (size_t)min(n0 + i, nt - 1u) * nc * 64u + lane;
-    qp[i] = a.q + (size_t)min(m0 + i, mt - 1u) * nc * 64u + lane;
+  for (uint32_t i = 0; i < NT; ++i) wp[i] = a.w + (size_t)min(n0 + i, nt - 1u) * nc * 64u + lane;
+#pragma unroll
+  for (uint32_t j = 0; j < MT; ++j) {
+    have[j] = (m0 + j) * 16u + (lane & 15u) < a.M;
+    qp[j] = a.q + (size_t)(have[j] ? m0 + j : 0u) * nc * 64u + lane;
   }
-  i4_t acc[4][4];
+  i4_t acc[MT][NT];
 #pragma unroll
-  for (uint32_t i = 0; i < 4; ++i)
+  for (uint32_t j = 0; j < MT; ++j)
 #pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) acc[i][j] = i4_t{0, 0, 0, 0};
-  for (uint32_t c = 0; c < nc; ++c) {
-    i4_t wv[4], qv[4];
+    for (uint32_t i = 0; i < NT; ++i) acc[j][i] = i4_t{0, 0, 0, 0};
+  for (uint32_t c0 = wave * U; c0 < nc; c0 += W * U) {
+    u4_t wv[U][NT], qv[U][MT];
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      wv[i] = __builtin_bit_cast(i4_t, wp[i][(size_t)c * 64u]);
-      qv[i] = __builtin_bit_cast(i4_t, qp[i][(size_t)c * 64u]);
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t c = min(c0 + u, nc - 1u);
+#pragma unroll
+      for (uint32_t i = 0; i < NT; ++i) wv[u][i] = load_stream16(reinterpret_cast<const uint32_t*>(wp[i] + (size_t)c * 64u));
+#pragma unroll
+      for (uint32_t j = 0; j < MT; ++j) {
+        qv[u][j] = u4_t{0u, 0u, 0u, 0u};
+        if (have[j] && c0 + u < nc) qv[u][j] = *as_global(qp[j] + (size_t)c * 64u);
+      }
     }
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
+    for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
-      for (uint32_t j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[i], qv[j], acc[i][j], 0, 0, 0);
+      for (uint32_t j = 0; j < MT; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < NT; ++i)
+          acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4_t, wv[u][i]), __builtin_bit_cast(i4_t, qv[u][j]),
+                                                            acc[j][i], 0, 0, 0);
   }
+  __shared__ __align__(16) i4_t part[W][MT * NT][64];
 #pragma unroll
-  for (uint32_t j = 0; j < 4; ++j) {
-    const uint32_t m = (m0 + j) * 16u + (lane & 15u);
-    if (m >= a.M) continue;
+  for (uint32_t j = 0; j < MT; ++j)
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-      if (n0 + i < nt) store4<F32>(a, m, (n0 + i) * 16u + 4u * (lane >> 4), acc[i][j]);
+    for (uint32_t i = 0; i < NT; ++i) part[wave][j * NT + i][lane] = acc[j][i];
+  __syncthreads();
+  for (uint32_t t = wave; t < MT * NT; t += W) {
+    const uint32_t m = (m0 + t / NT) * 16u + (lane & 15u), tile = n0 + t % NT;
+    if (m >= a.M || tile >= nt) continue;
+    i4_t sum = part[0][t][lane];
+#pragma unroll
+    for (uint32_t p = 1; p < W; ++p) sum += part[p][t][lane];
+    store4<F32>(a, m, tile * 16u + 4u * (lane >> 4), sum);
   }
 }
 
+// One fragment (1 KiB, 16 bytes per lane) from memory straight into LDS. The compiler does not see what this writes, nor
+// count the load: a kernel that uses it leaves no load of its own in flight and waits by vmcnt itself.
+__device__ __forceinline__ void load_fragment(uint32_t lds, const u4_t* from, uint32_t lane16) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(lane16), "s"(from) : "memory");
+}
+
+// Many rows: WM x WN waves of 16 RM rows x 16 CN columns, KS times over the parts of k. Both operands go into LDS in
+// fragment order, by direct loads into a ring of NS chunks, and from there into registers a chunk ahead of the products.
+// A is the weights: a lane ends with four adjacent columns of a row.
+template <bool F32, uint32_t RM, uint32_t CN, uint32_t WM, uint32_t WN, uint32_t KS, uint32_t NS>
+__global__ __launch_bounds__(64 * WM * WN * KS, 2) void gemm_w8a8_kernel(GemmArgs a, uint32_t m_tiles) {
+  constexpr uint32_t TM = RM * WM, TN = CN * WN, TT = TM + TN;  // 16-row and 16-column tiles of the work-group
+  constexpr uint32_t PW = WM * WN;                              // waves of a part
+  constexpr uint32_t L = (TT + PW - 1) / PW;                    // fragments a wave loads per chunk
+  constexpr uint32_t kSums = KS > 1 ? (KS - 1) * RM * CN * PW * 64 : 1;  // 16-byte pieces of the other parts' sums
+  __shared__ __align__(16) union {
+    u4_t stage[KS][NS][TT][64];
+    i4_t sums[kSums];
+  } sm;
+  // An XCD takes a run of column tiles with all their row tiles (the rows fastest): what it holds in its L2 at a time is
+  // shared by the work-groups it runs at a time.
+  const uint32_t per = gridDim.x / 8u, id = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+  const uint32_t nt = a.N / 16u, mt = (a.M + 15u) / 16u, nc = a.K / 64u;
+  const uint32_t m0 = id % m_tiles * TM, n0 = id / m_tiles * TN;
+  if (n0 >= nt) return;
+  const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const uint32_t ks = wave / PW, pw = wave % PW, wm = pw / WN, wn = pw % WN;
+  // this wave's fragments of a chunk: tile ft of the rows, then the columns (a tile behind the matrix is its last one, and
+  // a wave without a fragment loads the last once more)
+  const u4_t* from[L];
+  uint32_t at[L];
+#pragma unroll
+  for (uint32_t i = 0; i < L; ++i) {
+    const uint32_t ft = min(pw + PW * i, TT - 1u);
+    from[i] = ft < TM ? a.q + (size_t)min(m0 + ft, mt - 1u) * nc * 64u : a.w + (size_t)min(n0 + ft - TM, nt - 1u) * nc * 64u;
+    at[i] = (uint32_t)(uintptr_t)&sm.stage[ks][0][ft][0];
+  }
+  // this part's i-th chunk is KS i + ks (one behind the last is that one again, times zeros)
+  const uint32_t steps = (nc + KS - 1u) / KS;
+  auto load = [&](uint32_t k, uint32_t i, uint32_t slot) {
+    load_fragment(at[k] + slot * (TT * 1024u), from[k] + (size_t)min(KS * i + ks, nc - 1u) * 64u, 16u * lane);
+  };
+  struct Operands {
+    i4_t w[CN], x[RM];
+  } f0, f1;
+  auto read = [&](uint32_t k, Operands& f, uint32_t slot) {
+    const u4_t(*st)[64] = sm.stage[ks][slot];
+    if (k < CN) f.w[k] = __builtin_bit_cast(i4_t, st[TM + wn * CN + k][lane]);
+    else f.x[k - CN] = __builtin_bit_cast(i4_t, st[wm * RM + k - CN][lane]);
+  };
+  i4_t acc[RM][CN];
+#pragma unroll
+  for (uint32_t j = 0; j < RM; ++j)
+#pragma unroll
+    for (uint32_t i = 0; i < CN; ++i) acc[j][i] = i4_t{0, 0, 0, 0};
+#pragma unroll
+  for (uint32_t i = 0; i < NS; ++i)
+#pragma unroll
+    for (uint32_t k = 0; k < L; ++k) load(k, i, i);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1u) * L) : "memory");
+#pragma unroll
+  for (uint32_t k = 0; k < RM + CN; ++k) read(k, f0, 0);
+  uint32_t slot = 0;
+  auto step = [&](uint32_t i, Operands& now, Operands& next) {
+    // the next chunk is in LDS once every wave's fragments are, and this one's slot is free once every wave has read it
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2u) * L) : "memory");
+    const uint32_t freed = slot;
+    slot = slot + 1u == NS ? 0u : slot + 1u;
+    // The reads of the next chunk's operands and the loads of a later chunk's fragments, dealt out between the products:
+    // one behind the other they would leave the matrix core idle for as long as they take to issue.
+    constexpr uint32_t OPS = RM + CN + L, PER = RM * CN >= OPS ? RM * CN / OPS : 1, MORE = (OPS + RM * CN / PER - 1) / (RM * CN / PER);
+    if (KS > 1 && KS * i + ks >= nc) {
+#pragma unroll
+      for (uint32_t k = 0; k < CN; ++k) now.w[k] = i4_t{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (uint32_t p = 0; p < RM * CN; ++p) {
+      if (p % PER == 0) {
+#pragma unroll
+        for (uint32_t o = p / PER * MORE; o < (p / PER + 1u) * MORE; ++o) {
+          if (o < RM + CN) read(o, next, slot);
+          else if (o < OPS) load(o - RM - CN, i + NS, freed);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      acc[p / CN][p % CN] = __builtin_amdgcn_mfma_i32_16x16x64_i8(now.w[p % CN], now.x[p / CN], acc[p / CN][p % CN], 0, 0, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  uint32_t i = 0;
+  for (; i + 2u <= steps; i += 2u) {
+    step(i, f0, f1);
+    step(i + 1u, f1, f0);
+  }
+  if (i < steps) step(i, f0, f1);
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  if constexpr (KS > 1) {
+    // the other parts hand their sums to the first
+    i4_t* sums = sm.sums + pw * RM * CN * 64u + lane;
+    constexpr uint32_t kPart = PW * RM * CN * 64;
+    if (ks)
+#pragma unroll
+      for (uint32_t j = 0; j < RM; ++j)
+#pragma unroll
+        for (uint32_t k = 0; k < CN; ++k) sums[(ks - 1u) * kPart + (j * CN + k) * 64u] = acc[j][k];
+    __syncthreads();
+    if (ks) return;
+#pragma unroll
+    for (uint32_t p = 0; p + 1u < KS; ++p)
+#pragma unroll
+      for (uint32_t j = 0; j < RM; ++j)
+#pragma unroll
+        for (uint32_t k = 0; k < CN; ++k) acc[j][k] += sums[p * kPart + (j * CN + k) * 64u];
+  }
+#pragma unroll
+  for (uint32_t j = 0; j < RM; ++j) {
+    const uint32_t m = (m0 + wm * RM + j) * 16u + (lane & 15u);
+    if (m >= a.M) continue;
+#pragma unroll
+    for (uint32_t k = 0; k < CN; ++k) {
+      const uint32_t tile = n0 + wn * CN + k;
+      if (tile < nt) store4<F32>(a, m, tile * 16u + 4u * (lane >> 4), acc[j][k]);
+    }
+  }
+}
+
+template <bool F32, uint32_t RM, uint32_t CN, uint32_t WM, uint32_t WN, uint32_t KS, uint32_t NS>
+void launch_tiles(const GemmArgs& a, hipStream_t st) {
+  const uint32_t m_tiles = (a.M + 16u * RM * WM - 1u) / (16u * RM * WM), n_tiles = (a.N + 16u * CN * WN - 1u) / (16u * CN * WN);
+  gemm_w8a8_kernel<F32, RM, CN, WM, WN, KS, NS><<<(m_tiles * n_tiles + 7u) / 8u * 8u, 64 * WM * WN * KS, 0, st>>>(a, m_tiles);
+}
+template <bool F32, uint32_t MT, uint32_t NT, uint32_t W, uint32_t U>
+void launch_few(const GemmArgs& a, hipStream_t st) {
+  gemm_w8a8_few_kernel<F32, MT, NT, W, U><<<dim3((a.N + 16u * NT - 1u) / (16u * NT), (a.M + 16u * MT - 1u) / (16u * MT)), 64 * W, 0, st>>>(a);
+}
+
+// The work-group's shape by the least modelled time in ns,
+//   launch + turn r + step s c + work w s / 256 + weights K N / 10^6 + out M N / 10^6
+// with w work-groups, s = K / (64 parts) steps of each, c = ceil(w / 256) work-groups a CU runs and r of them one after
+// another (`occ` fit a CU at once). The constants were fitted to every shape's times at 790 random sizes (1..2048 rows,
+// K 256..17408, N 256..151936; a fifth of them this library's layers): the choice is 2.8 % off the best shape on average.
+// Measured (us; the chosen shape, then others) at K -> N:
+//   5120 -> 7168:   1 row 7.4 (16 x 16, 16 parts), 16 x 32 8.3, 64 x 64 10.3; 128 rows 12.3 (64 x 64, 4 parts), 64 x 32 18.8, 128 x 128 21.6;
+//                   1000 rows 38.8 (128 x 256), 128 x 128 41.0, 256 x 256 55.6
+//   5120 -> 34816:  13 rows 30.4 (16 x 32), 16 x 16 32.7; 128 rows 54.3 (128 x 256), 64 x 128 69.5; 2048 rows 329 (256 x 256), 128 x 256 385
+//   17408 -> 5120:  333 rows 53.8 (64 x 128), 64 x 64 67.0, 128 x 256 107; 1000 rows 106 (192 x 256), 128 x 256 111
+//   5120 -> 151936: 500 rows 374 (256 x 256), 128 x 256 453
+enum Shape { kFew16x16, kFew16x16w, kFew16x32, kFew32x32, kFew64x16, kTile64p4, kTile64, kTile64x128, kTile128, kTile128x256, kTile192x256, kTile256 };
+Shape pick(uint32_t M, uint32_t K, uint32_t N) {
+  static constexpr struct {
+    Shape shape;
+    uint32_t rows, cols, parts, occ, most;  // most: rows it is meant for
+    double launch, turn, step, work, weights, out;
+  } kShapes[] = {{kFew16x16, 16, 16, 4, 8, 64u, 3757, 0, 89, 54, 0, 429},
+                  {kFew16x16w, 16, 16, 16, 2, 64u, 3837, 0, 251, 294, 0, 2498},
+                  {kFew16x32, 16, 32, 4, 8, 64u, 3475, 209, 187, 72, 1, 0},
+                  {kFew32x32, 32, 32, 4, 6, 128u, 3634, 0, 221, 67, 0, 641},
+                  {kFew64x16, 64, 16, 8, 4, 256u, 3666, 0, 263, 65, 0, 2705},
+                  {kTile64p4, 64, 64, 4, 1, ~0u, 1859, 2180, 291, 140, 45, 1213},
+                  {kTile64, 64, 64, 2, 2, ~0u, 2417, 1485, 162, 32, 54, 833},
+                  {kTile64x128, 64, 128, 2, 1, ~0u, 1702, 2425, 195, 113, 80, 615},
+                  {kTile128, 128, 128, 1, 2, ~0u, 3826, 118, 167, 51, 55, 871},
+                  {kTile128x256, 128, 256, 1, 1, ~0u, 2392, 1775, 291, 97, 61, 797},
+                  {kTile192x256, 192, 256, 1, 1, ~0u, 1798, 2791, 401, 125, 41, 830},
+                  {kTile256, 256, 256, 1, 1, ~0u, 1714, 2879, 491, 146, 35, 871}};
+  Shape best = kTile128;
+  double least = 1e300;
+  for (const auto& s : kShapes) {
+    if (M > s.most) continue;
+    const uint64_t w = (uint64_t)((M + s.rows - 1u) / s.rows) * ((N + s.cols - 1u) / s.cols);
+    const double steps = (K / 64u + s.parts - 1u) / s.parts;
+    const double t = s.launch + s.turn * (double)((w + 256u * s.occ - 1u) / (256u * s.occ)) + s.step * steps * (double)((w + 255u) / 256u) +
+                     s.work * steps * (double)w / 256.0 + s.weights * 1e-6 * K * N + s.out * 1e-6 * M * N;
+    if (t < least) {
+      least = t;
+      best = s.shape;
+    }
+  }
+  return best;
+}
+
+template <bool F32>
+void launch_shape(Shape p, const GemmArgs& a, hipStream_t st) {
+  switch (p) {
+    case kFew16x16: return launch_few<F32, 1, 1, 4, 8>(a, st);
+    case kFew16x16w: return launch_few<F32, 1, 1, 16, 4>(a, st);
+    case kFew16x32: return launch_few<F32, 1, 2, 4, 4>(a, st);
+    case kFew32x32: return launch_few<F32, 2, 2, 4, 4>(a, st);
+    case kFew64x16: return launch_few<F32, 4, 1, 8, 2>(a, st);
+    case kTile64p4: return launch_tiles<F32, 4, 2, 1, 2, 4, 4>(a, st);
+    case kTile64: return launch_tiles<F32, 4, 2, 1, 2, 2, 5>(a, st);
+    case kTile64x128: return launch_tiles<F32, 2, 4, 2, 2, 2, 6>(a, st);
+    case kTile128: return launch_tiles<F32, 4, 4, 2, 2, 1, 5>(a, st);
+    case kTile128x256: return launch_tiles<F32, 4, 4, 2, 4, 1, 6>(a, st);
+    case kTile192x256: return launch_tiles<F32, 6, 4, 2, 4, 1, 5>(a, st);
+    case kTile256: return launch_tiles<F32, 8, 4, 2, 4, 1, 4>(a, st);
+  }
+}
 int launch_gemm(const GemmArgs& a, uint32_t out_kind, hipStream_t st) {
-  const dim3 grid((a.N + 127u) / 128u, (a.M + 127u) / 128u);
-  if (out_kind == MI_OUT_F32) gemm_w8a8_kernel<true><<<grid, 256, 0, st>>>(a);
-  else gemm_w8a8_kernel<false><<<grid, 256, 0, st>>>(a);
+  const Shape p = pick(a.M, a.K, a.N);
+  if (out_kind == MI_OUT_F32) launch_shape<true>(p, a, st);
+  else launch_shape<false>(p, a, st);
   return mi_hip((int)hipGetLastError(), "gemm_w8a8");
 }
 
@@ -196,7 +466,7 @@ int mi_quant_rows_i8(const uint16_t* x, size_t x_stride, uint32_t M, uint32_t K,
   if (int e = check_rows("quant_rows_i8", x, x_stride, M, K)) return e;
   if (!q_tiled || !row_scales || misaligned(q_tiled, 16) || misaligned(row_scales, 4))
     return mi_fail(MI_ERR_ARG, "quant_rows_i8: null or misaligned output (the rows 16 bytes, the scales 4)");
-  quant_rows_kernel<<<(M + 15u) / 16u * 4u, 256, 0, (hipStream_t)stream>>>(x, x_stride, M, K, q_tiled, row_scales);
+  launch_quant(x, x_stride, M, K, q_tiled, row_scales, (hipStream_t)stream);
   return mi_hip((int)hipGetLastError(), "quant_rows_i8");
 }
 
