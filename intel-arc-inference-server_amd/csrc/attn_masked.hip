@@ -52,24 +52,36 @@ struct Tiles {
   uint32_t n_a, b0, n;
   __device__ __forceinline__ uint32_t key(uint32_t i) const { return kTile * (i < n_a ? i : b0 + (i - n_a)); }
 };
-__device__ __forceinline__ uint32_t row_pos(const MaskedArgs& a, uint32_t t) { return a.pos ? a.pos[t] : a.pos0 + t; }
 
+// a row's span as loaded: thread t's row t0 + t
+struct RowSpan {
+  uint32_t lo = 0, hi = 0, pos = 0;
+};
+__device__ __forceinline__ RowSpan load_span(const MaskedArgs& a, uint32_t t0, uint32_t rows_here) {
+  RowSpan s;
+  if (threadIdx.x < rows_here) {
+    const uint32_t t = t0 + threadIdx.x;
+    s.pos = a.pos ? a.pos[t] : a.pos0 + t;
+    s.lo = a.lo ? a.lo[t] : 0u;
+    s.hi = a.hi ? a.hi[t] : s.pos + 1u;
+  }
+  return s;
+}
 // every thread of the work-group; rows_here <= its threads
-__device__ __forceinline__ Tiles block_begin(const MaskedArgs& a, Block& b, uint32_t t0, uint32_t rows_here) {
+__device__ __forceinline__ Tiles block_begin(const MaskedArgs& a, Block& b, const RowSpan& s, uint32_t rows_here) {
   const uint32_t t = threadIdx.x;
   if (t == 0) {
     b.min_lo = b.min_hi = 0xFFFFFFFFu;
     b.max_lo = b.max_hi = 0u;
     b.again = 0;
   }
-  __syncthreads();
+  lds_barrier();
   if (t < rows_here) {
-    const uint32_t p = row_pos(a, t0 + t);
-    uint32_t hi = min(a.hi ? a.hi[t0 + t] : p + 1u, a.kv_len), lo = min(a.lo ? a.lo[t0 + t] : 0u, hi);
+    uint32_t hi = min(s.hi, a.kv_len), lo = min(s.lo, hi);
     if (lo == hi && min(a.prefix, hi) == 0u) lo = hi = 0u;  // nothing
     b.lo[t] = lo;
     b.hi[t] = hi;
-    b.pos[t] = p;
+    b.pos[t] = s.pos;
     if (hi) {
       atomicMin(&b.min_lo, lo);
       atomicMax(&b.max_lo, lo);
@@ -77,12 +89,14 @@ __device__ __forceinline__ Tiles block_begin(const MaskedArgs& a, Block& b, uint
       atomicMax(&b.max_hi, hi);
     }
   }
-  __syncthreads();
+  lds_barrier();
   Tiles w{0u, 0u, 0u};
-  if (b.max_hi) {
-    w.n_a = (min(a.prefix, b.max_hi) + kTile - 1u) / kTile;
-    w.b0 = max(b.min_lo / kTile, w.n_a);
-    const uint32_t end = (b.max_hi + kTile - 1u) / kTile;
+  auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+  const uint32_t min_lo = uniform(b.min_lo), max_hi = uniform(b.max_hi);
+  if (max_hi) {
+    w.n_a = (min(a.prefix, max_hi) + kTile - 1u) / kTile;
+    w.b0 = max(min_lo / kTile, w.n_a);
+    const uint32_t end = (max_hi + kTile - 1u) / kTile;
     w.n = w.n_a + (end > w.b0 ? end - w.b0 : 0u);
   }
   return w;
@@ -99,6 +113,9 @@ __device__ __forceinline__ uint32_t cache_row(const MaskedArgs& a, uint32_t key)
   }
   return pg * a.page + (key - at * a.page);
 }
+
+// The cache's order: contiguous, pages that hold whole tiles (one table entry for a tile's 32 keys), any pages.
+enum Order { kContiguous, kWholeTiles, kAnyPages };
 
 // A column of a wave's 16 x CT: its span and what its scores take.
 struct Column {
@@ -120,16 +137,15 @@ __device__ __forceinline__ Column column(const MaskedArgs& a, const Block& b, ui
 __device__ __forceinline__ bool sees(const MaskedArgs& a, const Column& c, uint32_t key) {
   return key < c.hi && (key >= c.lo || key < a.prefix);
 }
-// The scores of keys key0 + 16 (e / 4) + e % 4 (e < 8) in base 2, -inf for a key that the column does not see.
-__device__ __forceinline__ void scores(const MaskedArgs& a, const Column& c, uint32_t key0, bool masked, float (&w)[8]) {
-  if (a.cap != 0.f) {
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e)
-      w[e] = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(w[e] * a.c2) + 1.f), a.cap);
-  } else {
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) w[e] *= a.c;
-  }
+// A score in base 2, the cap applied.
+template <bool CAP>
+__device__ __forceinline__ float score(const MaskedArgs& a, float s) {
+  if constexpr (CAP) return __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.c2) + 1.f), a.cap);
+  return s * a.c;
+}
+// The rest for the scores of keys key0 + 16 (e / 4) + e % 4 (e < 8): the bias, and -inf for a key that the column does not
+// see.
+__device__ __forceinline__ void bias_and_mask(const MaskedArgs& a, const Column& c, uint32_t key0, bool masked, float (&w)[8]) {
   if (a.slopes) {
     const float d = (float)(int)(c.pos - key0);
 #pragma unroll
@@ -139,6 +155,16 @@ __device__ __forceinline__ void scores(const MaskedArgs& a, const Column& c, uin
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) w[e] = sees(a, c, key0 + 16u * (e / 4) + e % 4) ? w[e] : -INFINITY;
   }
+}
+__device__ __forceinline__ void scores(const MaskedArgs& a, const Column& c, uint32_t key0, bool masked, float (&w)[8]) {
+  if (a.cap != 0.f) {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) w[e] = score<true>(a, w[e]);
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) w[e] = score<false>(a, w[e]);
+  }
+  bias_and_mask(a, c, key0, masked, w);
 }
 // whether some column of the block does not see some key of the tile (uniform)
 __device__ __forceinline__ bool tile_masked(const MaskedArgs& a, const Block& b, uint32_t key) {
@@ -209,13 +235,13 @@ __device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, 
   }
 }
 
-// q of a column as the B operand, f16 high and low parts: k = 32 kk + 8 qq + e
-template <int HD>
-__device__ __forceinline__ void load_q(const float* qp, h8_t (&qh)[HD / 32], h8_t (&ql)[HD / 32]) {
+// KK x 32 dims of a column's q as the B operand, f16 high and low parts: k = 32 kk + 8 qq + e
+template <uint32_t KK>
+__device__ __forceinline__ void load_q(const float* qp, h8_t (&qh)[KK], h8_t (&ql)[KK]) {
   float neg1 = -1.f;
   asm("" : "+s"(neg1));
 #pragma unroll
-  for (uint32_t kk = 0; kk < HD / 32; ++kk) {
+  for (uint32_t kk = 0; kk < KK; ++kk) {
     const f4_t q0 = *reinterpret_cast<const f4_any*>(qp + 32u * kk), q1 = *reinterpret_cast<const f4_any*>(qp + 32u * kk + 4);
     u4_t h, l;
     uint32_t hh, ll;
@@ -228,27 +254,47 @@ __device__ __forceinline__ void load_q(const float* qp, h8_t (&qh)[HD / 32], h8_
   }
 }
 
-// One step of a column's softmax: the scores w become weights (in place and as the B operand of P V).
-template <uint32_t NT>
-__device__ __forceinline__ h8_t weigh(float (&w)[8], uint32_t qi, float& r, float& l, f4_t (&acc)[NT]) {
-  const float mx = max3(max3(w[0], w[1], w[2]), max3(w[3], w[4], w[5]), max3(w[6], w[7], w[7]));
-  if (const uint64_t over = __ballot(mx > r + kRaise)) {
-    // (each column by its own four lanes, whatever its neighbours need)
-    const uint32_t o = (uint32_t)over | (uint32_t)(over >> 32);
-    const float cm = col_max(mx), to = ((o | o >> 16) >> qi) & 1u ? fmaxf(r, cm - kBelow) : r;
-    const float alpha = __builtin_amdgcn_exp2f(r - to);
-    r = to;
-    l *= alpha;
+// One step of the softmax of a wave's CT column tiles. The references first: raised, with what was formed by them, where a
+// score passes one (each column by its own four lanes, whatever its neighbours need).
+template <uint32_t CT, uint32_t NT>
+__device__ __forceinline__ void raise(const float (&w)[CT][8], uint32_t qi, float (&r)[CT], float (&l)[CT], f4_t (&acc)[CT][NT]) {
+  float mx[CT];
+  bool over = false;
 #pragma unroll
-    for (uint32_t tt = 0; tt < NT; ++tt) acc[tt] *= alpha;
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    mx[ct] = max3(max3(w[ct][0], w[ct][1], w[ct][2]), max3(w[ct][3], w[ct][4], w[ct][5]), max3(w[ct][6], w[ct][7], w[ct][7]));
+    over |= mx[ct] > r[ct] + kRaise;
   }
+  if (!__ballot(over)) return;
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    const uint64_t lanes = __ballot(mx[ct] > r[ct] + kRaise);
+    const uint32_t o = (uint32_t)lanes | (uint32_t)(lanes >> 32);
+    const float cm = col_max(mx[ct]), to = ((o | o >> 16) >> qi) & 1u ? fmaxf(r[ct], cm - kBelow) : r[ct];
+    const float alpha = __builtin_amdgcn_exp2f(r[ct] - to);
+    r[ct] = to;
+    l[ct] *= alpha;
+#pragma unroll
+    for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] *= alpha;
+  }
+}
+// Then the weights, as the B operands of P V in f16 high and low parts; their sum goes to l.
+__device__ __forceinline__ void weights(float (&w)[8], float r, float& l, h8_t& hi, h8_t& lo) {
 #pragma unroll
   for (uint32_t e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(w[e] - r);
   l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-  u4_t b;
+  float neg1 = -1.f;
+  asm("" : "+s"(neg1));
+  u4_t h, m;
 #pragma unroll
-  for (uint32_t e = 0; e < 4; ++e) b[e] = h2_bits(__builtin_convertvector((f2_t{w[2 * e], w[2 * e + 1]}), h2_t));
-  return __builtin_bit_cast(h8_t, b);
+  for (uint32_t e = 0; e < 4; ++e) {
+    uint32_t hh, mm;
+    f16_parts(w[2 * e], w[2 * e + 1], neg1, hh, mm);
+    h[e] = hh;
+    m[e] = mm;
+  }
+  hi = __builtin_bit_cast(h8_t, h);
+  lo = __builtin_bit_cast(h8_t, m);
 }
 typedef short v4s_t __attribute__((ext_vector_type(4)));
 typedef v4s_t __attribute__((address_space(3)))* v4s_lds;
@@ -300,16 +346,16 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
   const uint32_t j = blockIdx.x, t0 = blockIdx.y * a.rows, split = blockIdx.z;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, qi = lane & 15u, qq = lane >> 4;
   const uint32_t rows_here = min(a.rows, a.T - t0);
-  const Tiles tiles = block_begin(a, b, t0, rows_here);
+  const Tiles tiles = block_begin(a, b, load_span(a, t0, rows_here), rows_here);
   const uint32_t from = (uint32_t)((uint64_t)tiles.n * split / a.splits), to = (uint32_t)((uint64_t)tiles.n * (split + 1u) / a.splits);
   const uint32_t row = qi / a.gqa, g = qi % a.gqa;
   const Column col = column(a, b, j, row, g, rows_here);
   h8_t qh[KK], ql[KK];
-  load_q<HD>(a.q + ((size_t)(t0 + (row < rows_here ? row : 0u)) * a.q_heads + j * a.gqa + g) * HD + 8u * qq, qh, ql);
-  float r = kNoKey, l = 0.f;
-  f4_t acc[NT];
+  load_q<KK>(a.q + ((size_t)(t0 + (row < rows_here ? row : 0u)) * a.q_heads + j * a.gqa + g) * HD + 8u * qq, qh, ql);
+  float r[1] = {kNoKey}, l[1] = {0.f};
+  f4_t acc[1][NT];
 #pragma unroll
-  for (uint32_t tt = 0; tt < NT; ++tt) acc[tt] = f4_t{0.f, 0.f, 0.f, 0.f};
+  for (uint32_t tt = 0; tt < NT; ++tt) acc[0][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
 
   const size_t hoff = (size_t)j * a.head_stride;
   const uint32_t last = b.max_hi - 1u;
@@ -354,27 +400,33 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
       load(crow);
       if (i + 8u < to) crow = rows_of(i + 8u);
     }
-    float w[8];
+    float w[1][8];
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) w[e] = d[e / 4][e % 4];
-    scores(a, col, key + 4u * qq, tile_masked(a, b, key), w);
-    const h8_t p = weigh<NT>(w, qi, r, l, acc);
+    for (uint32_t e = 0; e < 8; ++e) w[0][e] = d[e / 4][e % 4];
+    scores(a, col, key + 4u * qq, tile_masked(a, b, key), w[0]);
+    raise<1, NT>(w, qi, r, l, acc);
+    h8_t ph, pl;
+    weights(w[0], r[0], l[0], ph, pl);
 #pragma unroll
-    for (uint32_t tt = 0; tt < NT; ++tt) acc[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v_operand<VROW>(vb, tt), p, acc[tt], 0, 0, 0);
+    for (uint32_t tt = 0; tt < NT; ++tt) {
+      const h8_t av = v_operand<VROW>(vb, tt);
+      acc[0][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ph, acc[0][tt], 0, 0, 0);
+      acc[0][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pl, acc[0][tt], 0, 0, 0);
+    }
   }
-  l = col_sum(l);
+  l[0] = col_sum(l[0]);
   float bad = 0.f;
 #pragma unroll
-  for (uint32_t tt = 0; tt < NT; ++tt) bad += not_finite(acc[tt]);
-  if (col.live && (bad != 0.f || l - l != 0.f)) b.again = 1;
+  for (uint32_t tt = 0; tt < NT; ++tt) bad += not_finite(acc[0][tt]);
+  if (col.live && (bad != 0.f || l[0] - l[0] != 0.f)) b.again = 1;
   wave_lds_sync();
   auto& mine = slab[wave].part;
 #pragma unroll
   for (uint32_t tt = 0; tt < NT; ++tt)
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) mine.acc[4u * tt + e][lane] = acc[tt][e];
-  mine.r[lane] = r;
-  mine.l[lane] = l;
+    for (uint32_t e = 0; e < 4; ++e) mine.acc[4u * tt + e][lane] = acc[0][tt][e];
+  mine.r[lane] = r[0];
+  mine.l[lane] = l[0];
   __syncthreads();
   if (b.again) {
     slow_block<HD>(a, b, tiles, j, t0, rows_here, from, to, split);
@@ -409,122 +461,220 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
   }
 }
 
-// A chunk: grid (kv_heads, row blocks, splits); 4 waves side by side of CT column tiles each walk the same 32-key tiles,
-// staged in LDS for all of them, the next tile's rows in registers meanwhile.
-template <int HD, int CT>
-__global__ __launch_bounds__(256, 2) void attn_masked_kernel(MaskedArgs a) {
-  constexpr uint32_t KK = HD / 32, NT = HD / 16, KROW = HD + 8, VROW = HD + 16;
-  constexpr uint32_t PPR = HD / 8, RPP = 256 / PPR, CH = kTile / RPP;  // 16-byte pieces per row, rows per pass, passes
-  struct Stage {
-    uint16_t k[kTile * KROW], v[kTile * VROW];
-  };
+// A chunk: grid (kv_heads, row blocks, splits). Four waves side by side take CT column tiles each and 128 of the dims; at
+// rows of 256 four more take the other half (a wave's registers hold 32 columns of 128 dims with two waves per SIMD, and
+// every LDS read then serves 32 columns). All walk the same 32-key tiles, K and V staged in LDS for all of them, the rows
+// after them in registers meanwhile. A step i has two halves with a barrier between them:
+//   the products of tile i + 1's scores, dealt out among the exponentials that make tile i's weights;
+//   P V of tile i, dealt out among the scaling (and the tanh) of tile i + 1's scores, whose maxima follow.
+// So the matrix core has products while the vector ALUs work in the same wave. The halves of the dims exchange their parts
+// of the scores through LDS across the barrier.
+template <int HD, int CT, bool CAP, Order ORDER>
+__global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
+  constexpr uint32_t DS = HD / 128, KK = 4, NT = 8, KROW = HD + 8, VROW = HD + 16, THREADS = 2 * HD;
+  constexpr uint32_t PPR = HD / 8, RPP = THREADS / PPR, CH = kTile / RPP;  // 16-byte pieces per row, rows per pass, passes
   __shared__ Block b;
-  __shared__ __align__(16) Stage st[2];
+  __shared__ __align__(16) struct {
+    uint16_t k[2][kTile * KROW], v[2][kTile * VROW];
+    f4_t s[DS > 1 ? 2 : 1][DS > 1 ? 4 * DS : 1][2 * CT][DS > 1 ? 64 : 1];
+  } st;
   // the last row blocks of a causal chunk see the most keys: they are dispatched first
   const uint32_t j = blockIdx.x, t0 = (gridDim.y - 1u - blockIdx.y) * a.rows, split = blockIdx.z;
-  const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6, qi = lane & 15u, qq = lane >> 4;
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 6)), qi = lane & 15u, qq = lane >> 4;
+  const uint32_t cw = wave % 4u, ds = wave / 4u;
   const uint32_t rows_here = min(a.rows, a.T - t0);
-  const Tiles tiles = block_begin(a, b, t0, rows_here);
-  const uint32_t from = (uint32_t)((uint64_t)tiles.n * split / a.splits), to = (uint32_t)((uint64_t)tiles.n * (split + 1u) / a.splits);
-  const size_t hoff = (size_t)j * a.head_stride;
-  const uint32_t last = b.max_hi - 1u, srow = t / PPR, sp = 8u * (t % PPR);
-  u4_t kr[CH], vr[CH];
-  uint32_t crow[CH];
-  auto rows_of = [&](uint32_t i) {
-#pragma unroll
-    for (uint32_t n = 0; n < CH; ++n) crow[n] = cache_row(a, min(tiles.key(i) + RPP * n + srow, last));
-  };
-  auto load = [&]() {
-#pragma unroll
-    for (uint32_t n = 0; n < CH; ++n) {
-      const size_t at = (size_t)crow[n] * a.row_stride + hoff + sp;
-      kr[n] = *reinterpret_cast<const u4_t*>(a.k + at);
-      vr[n] = *reinterpret_cast<const u4_t*>(a.v + at);
-    }
-  };
-  auto store = [&](Stage& s) {
-#pragma unroll
-    for (uint32_t n = 0; n < CH; ++n) {
-      *reinterpret_cast<u4_t*>(s.k + (RPP * n + srow) * KROW + sp) = kr[n];
-      *reinterpret_cast<u4_t*>(s.v + (RPP * n + srow) * VROW + sp) = vr[n];
-    }
-  };
-  if (from < to) {
-    rows_of(from);
-    load();
-    if (from + 1u < to) rows_of(from + 1u);
-  }
-  const bool computes = 16u * CT * wave < rows_here * a.gqa;  // a wave without a live column only stages
+  const RowSpan span = load_span(a, t0, rows_here);
   uint32_t row[CT], g[CT];
-  Column col[CT];
-  h8_t qh[CT][KK], ql[CT][KK];
-  float r[CT], l[CT];
-  f4_t acc[CT][NT];
+  const float* qp[CT];
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
-    const uint32_t p = 16u * (CT * wave + ct) + qi;
+    const uint32_t p = 16u * (CT * cw + ct) + qi;
     row[ct] = p / a.gqa;
     g[ct] = p % a.gqa;
+    qp[ct] = a.q + ((size_t)(t0 + (row[ct] < rows_here ? row[ct] : 0u)) * a.q_heads + j * a.gqa + g[ct]) * HD + 128u * ds + 8u * qq;
+  }
+  const Tiles tiles = block_begin(a, b, span, rows_here);
+  const uint32_t from = (uint32_t)((uint64_t)tiles.n * split / a.splits), n = (uint32_t)((uint64_t)tiles.n * (split + 1u) / a.splits) - from;
+  auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+  const uint32_t min_hi = uniform(b.min_hi), max_lo = uniform(b.max_lo), last = uniform(b.max_hi) - 1u;
+  const size_t hoff = (size_t)j * a.head_stride;
+  const uint32_t srow = t / PPR, sp = 8u * (t % PPR);
+  u4_t kr[CH], vr[CH];
+  // the cache rows of tile i: its first (r[0]) where they follow one another, else those that the thread loads
+  struct Rows {
+    uint32_t r[CH];
+  };
+  auto rows_of = [&](uint32_t i) {
+    Rows w;
+    const uint32_t key0 = tiles.key(from + min(i, n - 1u));
+    if constexpr (ORDER == kContiguous) {
+      w.r[0] = key0;
+    } else if constexpr (ORDER == kWholeTiles) {
+      w.r[0] = cache_row(a, key0);
+    } else {
+#pragma unroll
+      for (uint32_t c = 0; c < CH; ++c) w.r[c] = cache_row(a, min(key0 + RPP * c + srow, last));
+    }
+    return w;
+  };
+  // (a tile behind the last is that one again, and its loads are not used)
+  auto load = [&](const uint16_t* cache, uint32_t i, const Rows& w, u4_t (&to)[CH]) {
+    const uint32_t left = last - tiles.key(from + min(i, n - 1u));
+#pragma unroll
+    for (uint32_t c = 0; c < CH; ++c) {
+      const uint32_t r = ORDER == kAnyPages ? w.r[c] : uniform(w.r[0]) + min(RPP * c + srow, left);
+      to[c] = *as_global(reinterpret_cast<const u4_t*>(cache + (size_t)r * a.row_stride + hoff + sp));
+    }
+  };
+  auto store = [&](uint16_t* to, uint32_t pitch, const u4_t (&v)[CH]) {
+#pragma unroll
+    for (uint32_t c = 0; c < CH; ++c) *reinterpret_cast<u4_t*>(to + (RPP * c + srow) * pitch + sp) = v[c];
+  };
+  // the rows of the tiles i + 1 .. i + 3 of a step i: V of the first and K of the last are loaded in it (a page's entry is
+  // fetched a step before the loads that need it)
+  Rows r1, r2, r3;
+  u4_t k1[CH];
+  if (n) {
+    const Rows r0 = rows_of(0);
+    r1 = rows_of(1);
+    r2 = rows_of(2);
+    r3 = rows_of(3);
+    load(a.k, 0, r0, kr);
+    load(a.v, 0, r0, vr);
+    load(a.k, 1, r1, k1);
+  }
+  Column col[CT];
+  float r[CT], l[CT];
+  f4_t acc[CT][NT], d[CT][2];
+  h8_t qh[CT][KK], ql[CT][KK];
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    load_q<KK>(qp[ct], qh[ct], ql[ct]);
     col[ct] = column(a, b, j, row[ct], g[ct], rows_here);
-    load_q<HD>(a.q + ((size_t)(t0 + (row[ct] < rows_here ? row[ct] : 0u)) * a.q_heads + j * a.gqa + g[ct]) * HD + 8u * qq, qh[ct],
-               ql[ct]);
     r[ct] = kNoKey;
     l[ct] = 0.f;
 #pragma unroll
     for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
   }
-  if (from < to) {
-    store(st[0]);
-    if (from + 1u < to) {
-      load();
-      if (from + 2u < to) rows_of(from + 2u);
+  // One K operand (16 keys x 32 dims, number s = 2 kk + gg) and its products: this wave's part of the scores
+  // S^T[key 16 gg + 4 qq + e][column qi].
+  auto k_operand = [&](uint32_t buf, uint32_t s) {
+    return *reinterpret_cast<const h8_t*>(st.k[buf] + (16u * (s % 2u) + qi) * KROW + 128u * ds + 8u * qq + 32u * (s / 2u));
+  };
+  auto product = [&](h8_t kh, uint32_t s, uint32_t part) {  // part < 2 CT: the columns' high parts, then the low ones
+    const uint32_t ct = part % CT;
+    d[ct][s % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, part < CT ? qh[ct][s / 2] : ql[ct][s / 2], d[ct][s % 2], 0, 0, 0);
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (uint32_t ct = 0; ct < CT; ++ct) d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+  };
+  auto hand_over = [&](uint32_t buf) {
+    if constexpr (DS > 1) {
+#pragma unroll
+      for (uint32_t ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (uint32_t gg = 0; gg < 2; ++gg) st.s[buf][wave][2 * ct + gg][lane] = d[ct][gg];
     }
+  };
+  auto take_over = [&](uint32_t buf) {
+    if constexpr (DS > 1) {
+#pragma unroll
+      for (uint32_t ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (uint32_t gg = 0; gg < 2; ++gg) d[ct][gg] += st.s[buf][wave ^ 4u][2 * ct + gg][lane];
+    }
+  };
+  float w[CT][8];
+  // the scores w of tile i: bias, mask, and the columns' references
+  auto settle = [&](uint32_t i) {
+    const uint32_t key = tiles.key(from + i);
+    const bool masked = key + kTile > min_hi || (key < max_lo && key + kTile > a.prefix);  // uniform
+#pragma unroll
+    for (uint32_t ct = 0; ct < CT; ++ct) bias_and_mask(a, col[ct], key + 4u * qq, masked, w[ct]);
+    raise<CT, NT>(w, qi, r, l, acc);
+  };
+  if (n) {
+    store(st.k[0], KROW, kr);
+    store(st.k[1], KROW, k1);
+    load(a.k, 2, r2, kr);
+    lds_barrier();
+    clear();
+#pragma unroll
+    for (uint32_t s = 0; s < 2 * KK; ++s) {
+      const h8_t kh = k_operand(0, s);
+#pragma unroll
+      for (uint32_t part = 0; part < 2 * CT; ++part) product(kh, s, part);
+    }
+    hand_over(0);
+    lds_barrier();
+    take_over(0);
+#pragma unroll
+    for (uint32_t ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) w[ct][e] = score<CAP>(a, d[ct][e / 4][e % 4]);
+    settle(0);
   }
-  lds_barrier();
-  for (uint32_t i = from; i < to; ++i) {
-    const Stage& s = st[(i - from) & 1u];
-    if (computes) {
-      const uint32_t key = tiles.key(i);
-      f4_t d[CT][2];
+  for (uint32_t i = 0; i < n; ++i) {
+    const uint32_t cur = i & 1u, nxt = cur ^ 1u;
+    // V of tile i and K of tile i + 2 into the buffers that were last read before the barrier behind us; then the loads of
+    // the next step's
+    store(st.v[cur], VROW, vr);
+    store(st.k[cur], KROW, kr);
+    const Rows r4 = rows_of(i + 4u);
+    load(a.v, i + 1u, r1, vr);
+    load(a.k, i + 3u, r3, kr);
+    r1 = r2;
+    r2 = r3;
+    r3 = r4;
+    h8_t p[CT];
+    {  // (behind the last tile the products are of a tile that is not used)
+      constexpr uint32_t S = 2 * KK, AHEAD = 3;
+      h8_t kh[S];
+      clear();
 #pragma unroll
-      for (uint32_t ct = 0; ct < CT; ++ct) d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+      for (uint32_t s = 0; s < AHEAD; ++s) kh[s] = k_operand(nxt, s);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (uint32_t kk = 0; kk < KK; ++kk)
+      for (uint32_t s = 0; s < S; ++s) {
+        if (s + AHEAD < S) kh[s + AHEAD] = k_operand(nxt, s + AHEAD);
 #pragma unroll
-        for (uint32_t gg = 0; gg < 2; ++gg) {
-          const h8_t kh = *reinterpret_cast<const h8_t*>(s.k + (16u * gg + qi) * KROW + 32u * kk + 8u * qq);
-#pragma unroll
-          for (uint32_t ct = 0; ct < CT; ++ct) d[ct][gg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[ct][kk], d[ct][gg], 0, 0, 0);
-#pragma unroll
-          for (uint32_t ct = 0; ct < CT; ++ct) d[ct][gg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[ct][kk], d[ct][gg], 0, 0, 0);
+        for (uint32_t h = 0; h < CT; ++h) {  // two products, one weight
+          product(kh[s], s, 2 * h);
+          product(kh[s], s, 2 * h + 1);
+          const uint32_t x = s * CT + h, ct = x / 8, e = x % 8;
+          w[ct][e] = __builtin_amdgcn_exp2f(w[ct][e] - r[ct]);
+          l[ct] += w[ct][e];
+          if (e % 2) {
+            u4_t pk = __builtin_bit_cast(u4_t, p[ct]);
+            pk[e / 2] = h2_bits(__builtin_convertvector((f2_t{w[ct][e - 1], w[ct][e]}), h2_t));
+            p[ct] = __builtin_bit_cast(h8_t, pk);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
-      const bool masked = tile_masked(a, b, key);
-      h8_t p[CT];
-#pragma unroll
-      for (uint32_t ct = 0; ct < CT; ++ct) {
-        float w[8];
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) w[e] = d[ct][e / 4][e % 4];
-        scores(a, col[ct], key + 4u * qq, masked, w);
-        p[ct] = weigh<NT>(w, qi, r[ct], l[ct], acc[ct]);
       }
-      const uint16_t* vb = s.v + (4u * qq + (qi >> 2)) * VROW + 4u * (qi & 3u);
-#pragma unroll
-      for (uint32_t tt = 0; tt < NT; ++tt) {
-        const h8_t av = v_operand<VROW>(vb, tt);
-#pragma unroll
-        for (uint32_t ct = 0; ct < CT; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, p[ct], acc[ct][tt], 0, 0, 0);
-      }
-    }
-    // (the other buffer was last read before the previous barrier)
-    if (i + 1u < to) {
-      store(st[(i + 1u - from) & 1u]);
-      if (i + 2u < to) {
-        load();
-        if (i + 3u < to) rows_of(i + 3u);
-      }
+      hand_over(nxt);
     }
     lds_barrier();
+    {
+      const uint16_t* vb = st.v[cur] + (4u * qq + (qi >> 2)) * VROW + 128u * ds + 4u * (qi & 3u);
+      constexpr uint32_t AHEAD = 3;
+      h8_t av[NT];
+#pragma unroll
+      for (uint32_t tt = 0; tt < AHEAD; ++tt) av[tt] = v_operand<VROW>(vb, tt);
+      take_over(nxt);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (uint32_t tt = 0; tt < NT; ++tt) {
+        if (tt + AHEAD < NT) av[tt + AHEAD] = v_operand<VROW>(vb, tt + AHEAD);
+#pragma unroll
+        for (uint32_t ct = 0; ct < CT; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[tt], p[ct], acc[ct][tt], 0, 0, 0);
+#pragma unroll
+        for (uint32_t ct = 0; ct < CT; ++ct) w[ct][tt] = score<CAP>(a, d[ct][tt / 4][tt % 4]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (i + 1u < n) settle(i + 1u);
+    }
   }
   float sum[CT];
 #pragma unroll
@@ -537,7 +687,7 @@ __global__ __launch_bounds__(256, 2) void attn_masked_kernel(MaskedArgs a) {
   }
   __syncthreads();
   if (b.again) {
-    slow_block<HD>(a, b, tiles, j, t0, rows_here, from, to, split);
+    slow_block<HD>(a, b, tiles, j, t0, rows_here, from, from + n, split);
     return;
   }
 #pragma unroll
@@ -545,8 +695,8 @@ __global__ __launch_bounds__(256, 2) void attn_masked_kernel(MaskedArgs a) {
     if (row[ct] >= rows_here) continue;
     if (a.splits > 1) {
 #pragma unroll
-      for (uint32_t tt = 0; tt < NT; ++tt) store_part<HD>(a, j, t0 + row[ct], g[ct], split, qq, tt, acc[ct][tt]);
-      if (qq == 0) {
+      for (uint32_t tt = 0; tt < NT; ++tt) store_part<HD>(a, j, t0 + row[ct], g[ct], split, qq, 8u * ds + tt, acc[ct][tt]);
+      if (qq == 0 && ds == 0) {
         float* o = part_at<HD>(a, j, t0 + row[ct], g[ct], split);
         o[HD] = r[ct];
         o[HD + 1] = col[ct].live ? sum[ct] : 0.f;
@@ -554,44 +704,146 @@ __global__ __launch_bounds__(256, 2) void attn_masked_kernel(MaskedArgs a) {
     } else {
       const float inv = col[ct].live && sum[ct] != 0.f ? 1.0f / sum[ct] : 0.f;
 #pragma unroll
-      for (uint32_t tt = 0; tt < NT; ++tt) store_out<HD>(a, j, t0 + row[ct], g[ct], qq, tt, inv == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : acc[ct][tt] * inv);
+      for (uint32_t tt = 0; tt < NT; ++tt)
+        store_out<HD>(a, j, t0 + row[ct], g[ct], qq, 8u * ds + tt, inv == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : acc[ct][tt] * inv);
     }
   }
 }
-
-// grid (q_heads, T): one column's splits, a thread per dim
-template <int HD>
-__global__ __launch_bounds__(HD) void attn_masked_join_kernel(MaskedArgs a) {
-  const uint32_t h = blockIdx.x, t = blockIdx.y, d = threadIdx.x;
-  const float* p = a.part + (size_t)(t * a.q_heads + h) * a.splits * (HD + 4);
-  float top = kNoKey, sum = 0.f, v = 0.f;
-  for (uint32_t s = 0; s < a.splits; ++s)
-    if (p[s * (HD + 4) + HD + 1] != 0.f) top = fmaxf(top, p[s * (HD + 4) + HD]);
-  for (uint32_t s = 0; s < a.splits; ++s) {
-    const float l = p[s * (HD + 4) + HD + 1];
-    if (l == 0.f) continue;  // (no key of the row in that part)
-    const float f = __builtin_amdgcn_exp2f(p[s * (HD + 4) + HD] - top);
-    sum = __builtin_fmaf(l, f, sum);
-    v = __builtin_fmaf(p[s * (HD + 4) + d], f, v);
-  }
-  a.out[((size_t)t * a.q_heads + h) * HD + d] = act_enc(sum == 0.f ? 0.f : v / sum, a.act);
+template <int HD, int CT, bool CAP>
+void launch_order(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
+  if (!a.pages) attn_masked_kernel<HD, CT, CAP, kContiguous><<<grid, 2 * HD, 0, st>>>(a);
+  else if (a.page % kTile == 0) attn_masked_kernel<HD, CT, CAP, kWholeTiles><<<grid, 2 * HD, 0, st>>>(a);
+  else attn_masked_kernel<HD, CT, CAP, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
+}
+template <int HD, int CT>
+void launch_chunk(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
+  if (a.cap != 0.f) launch_order<HD, CT, true>(a, grid, st);
+  else launch_order<HD, CT, false>(a, grid, st);
 }
 
-// The launch: few columns per block, or a chunk's, and the parts that the keys are split in.
+// grid (q_heads, T): one column's splits. Each split's factor first, a thread each; then HD / 4 threads side by side take
+// four dims each, of every G-th split.
+constexpr uint32_t kMaxSplits = 256;
+template <int HD>
+__global__ __launch_bounds__(256) void attn_masked_join_kernel(MaskedArgs a) {
+  constexpr uint32_t G = 256 / (HD / 4);
+  __shared__ float factor[kMaxSplits], most[4], total[4];
+  __shared__ __align__(16) f4_t sums[G][HD / 4];
+  const uint32_t h = blockIdx.x, t = blockIdx.y, i = threadIdx.x, lane = i & 63u, wave = i >> 6;
+  const float* p = a.part + (size_t)(t * a.q_heads + h) * a.splits * (HD + 4);
+  float r = kNoKey, l = 0.f;
+  if (i < a.splits) {
+    r = p[i * (HD + 4) + HD];
+    l = p[i * (HD + 4) + HD + 1];
+  }
+  if (l == 0.f) r = kNoKey;  // (no key of the row in that part)
+  const float m = wave_max(r);
+  if (lane == 0) most[wave] = m;
+  __syncthreads();
+  const float f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(r - fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
+  if (i < a.splits) factor[i] = f;
+  const float sum = wave_sum(l * f);
+  if (lane == 0) total[wave] = sum;
+  __syncthreads();
+  const uint32_t g = i / (HD / 4), d = i % (HD / 4);
+  f4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (uint32_t s = g; s < a.splits; s += G) {
+    const float w = factor[s];
+    const f4_t x = *reinterpret_cast<const f4_t*>(p + s * (HD + 4) + 4u * d);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) v[e] = __builtin_fmaf(x[e], w, v[e]);
+  }
+  sums[g][d] = v;
+  __syncthreads();
+  if (i >= HD / 4) return;
+#pragma unroll
+  for (uint32_t k = 1; k < G; ++k) v += sums[k][d];
+  const float all = (total[0] + total[1]) + (total[2] + total[3]), inv = all == 0.f ? 0.f : 1.0f / all;
+  const u2_t o = {(uint32_t)act_enc(v[0] * inv, a.act) | ((uint32_t)act_enc(v[1] * inv, a.act) << 16),
+                  (uint32_t)act_enc(v[2] * inv, a.act) | ((uint32_t)act_enc(v[3] * inv, a.act) << 16)};
+  *reinterpret_cast<h4_any*>(a.out + ((size_t)t * a.q_heads + h) * HD + 4u * d) = o;
+}
+
+// The same for few splits: HD / 4 threads take a column, each four dims of all its splits; several columns per work-group.
+constexpr uint32_t kFewSplits = 8;
+template <int HD>
+__global__ __launch_bounds__(256) void attn_masked_join_few_kernel(MaskedArgs a, uint32_t columns) {
+  constexpr uint32_t C = 256 / (HD / 4);
+  const uint32_t c = blockIdx.x * C + threadIdx.x / (HD / 4), d = threadIdx.x % (HD / 4);
+  if (c >= columns) return;
+  const float* p = a.part + (size_t)c * a.splits * (HD + 4);
+  f4_t v[kFewSplits];
+  float r[kFewSplits], l[kFewSplits], top = kNoKey;
+#pragma unroll
+  for (uint32_t s = 0; s < kFewSplits; ++s) {
+    const float* q = p + (s < a.splits ? s : 0u) * (HD + 4);
+    v[s] = *reinterpret_cast<const f4_t*>(q + 4u * d);
+    r[s] = q[HD];
+    l[s] = s < a.splits ? q[HD + 1] : 0.f;
+  }
+#pragma unroll
+  for (uint32_t s = 0; s < kFewSplits; ++s) top = l[s] == 0.f ? top : fmaxf(top, r[s]);
+  f4_t o = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+#pragma unroll
+  for (uint32_t s = 0; s < kFewSplits; ++s) {
+    const float f = l[s] == 0.f ? 0.f : __builtin_amdgcn_exp2f(r[s] - top);  // (no key of the row in that part)
+    sum = __builtin_fmaf(l[s], f, sum);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[s][e], f, o[e]);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const u2_t h = {(uint32_t)act_enc(o[0] * inv, a.act) | ((uint32_t)act_enc(o[1] * inv, a.act) << 16),
+                  (uint32_t)act_enc(o[2] * inv, a.act) | ((uint32_t)act_enc(o[3] * inv, a.act) << 16)};
+  *reinterpret_cast<h4_any*>(a.out + (size_t)c * HD + 4u * d) = h;
+}
+
+// The launch: the few-rows kernel up to 16 columns, else the chunk's with CT column tiles, and the parts that the keys are
+// split in.
+//   few: as many parts as fill the CUs (two work-groups each at rows of 128, one at 256), of 128 keys at least. Measured
+//   (us): one row, 40 / 8 heads of 128, 4099 keys 17.6 / 12.9 / 11.3 / 10.0 / 11.2 in 4 / 8 / 16 / 32 / 64 parts; 131072 keys
+//   105 / 100 / 103 / 110 in 32 / 64 / 128 / 256; 16 / 2 heads of 256, 65536 keys 37.6 / 31.3 / 38.3 in 64 / 128 / 256.
+//   chunk: the least modelled time over both CT and the parts s, in us:
+//     rounds (3 + tiles / s tau) + join,  join = 3 + T q_heads s (head_dim + 4) 8 bytes at 3.5 TB/s for s > 1
+//   with tiles of 32 keys (all that the cache may hold: what the rows see is the device's) and tau a tile's time with k
+//   work-groups on a CU. Measured (us; CT 1 then 2, in 1 / 2 / 3 / 4 parts): 500 rows over 4500 keys, 32 / 8 heads of 128:
+//   103 / 89 / 83 / 84, 148 / 90 / 86 / 75; 777 over 3778, 16 / 2 of 256: 148 / 152 / 153 / 158, 218 / 128 / 155 / 136; 333 over 333,
+//   40 / 8 of 128: 15 / 23 / 25 / 27, 23 / 26 / 28 / 29; 20 over 4020: 89 / 51 / 38 / 31 (16 parts 19), 131 / 73 / 53 / 44.
 struct Pick {
   bool few;
   uint32_t ct, rows, splits;
 };
 constexpr uint32_t kCus = 256;
 Pick pick(uint32_t T, uint32_t keys, uint32_t kv_heads, uint32_t gqa, uint32_t hd) {
-  Pick p;
-  p.few = gqa <= 16 && T * gqa <= 16;
-  p.ct = !p.few && hd == 128 && (uint64_t)kv_heads * ((T + 128 / gqa - 1) / (128 / gqa)) > kCus ? 2 : 1;
-  p.rows = (p.few ? 16u : 64u * p.ct) / gqa;
-  const uint64_t blocks = (uint64_t)kv_heads * ((T + p.rows - 1) / p.rows);
-  const uint64_t want = p.few ? (4 * kCus + blocks - 1) / blocks : (2 * kCus + blocks - 1) / blocks;
-  const uint64_t most = (keys + 255u) / 256u;  // (at least 256 keys each)
-  p.splits = blocks >= kCus ? 1u : (uint32_t)std::max<uint64_t>(1, std::min(want, most));
+  Pick p{gqa <= 16 && (uint64_t)T * gqa <= 16, 1, 0, 1};
+  if (p.few) {
+    p.rows = 16u / gqa;
+    const uint32_t slots = hd == 128 ? 2 * kCus : kCus;
+    p.splits = std::max(1u, std::min({slots / kv_heads, (keys + 127u) / 128u, kMaxSplits}));
+    return p;
+  }
+  static constexpr double kTau[2][2][3] = {{{0.73, 1.15, 1.53}, {1.05, 1.45, 1.45}}, {{1.2, 1.2, 1.2}, {1.85, 1.85, 1.85}}};
+  const double tiles = (keys + kTile - 1u) / kTile;
+  double least = 1e300;
+  for (uint32_t ct = 1; ct <= 2; ++ct) {
+    const uint32_t rows = 64u * ct / gqa, cap = hd == 128 ? 4u - ct : 1u;  // work-groups that a CU holds
+    const double* tau = kTau[hd == 256][ct - 1];
+    const uint64_t blocks = (uint64_t)kv_heads * ((T + rows - 1u) / rows);
+    for (uint32_t s = 1; s <= 64u && (s == 1 || s * 4u <= tiles); ++s) {
+      const uint64_t w = blocks * s, full = w / (kCus * cap), rest = w % (kCus * cap);
+      const double step = tiles / s;
+      double us = (double)full * (3.0 + step * tau[cap - 1]);
+      if (rest) us += 3.0 + step * tau[(rest + kCus - 1) / kCus - 1];
+      if (s > 1) us += 3.0 + (double)T * (kv_heads * gqa) * s * (hd + 4) * 8.0 / 3.5e6;
+      if (us < least) {
+        least = us;
+        p.ct = ct;
+        p.rows = rows;
+        p.splits = s;
+      }
+    }
+  }
   return p;
 }
 size_t part_bytes(const Pick& p, uint32_t T, uint32_t q_heads, uint32_t hd) {
@@ -674,14 +926,19 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
     if (narrow) attn_masked_few_kernel<128><<<grid, 256, 0, st>>>(a);
     else attn_masked_few_kernel<256><<<grid, 256, 0, st>>>(a);
   } else if (narrow) {
-    if (p.ct == 2) attn_masked_kernel<128, 2><<<grid, 256, 0, st>>>(a);
-    else attn_masked_kernel<128, 1><<<grid, 256, 0, st>>>(a);
+    if (p.ct == 2) launch_chunk<128, 2>(a, grid, st);
+    else launch_chunk<128, 1>(a, grid, st);
   } else {
-    attn_masked_kernel<256, 1><<<grid, 256, 0, st>>>(a);
+    if (p.ct == 2) launch_chunk<256, 2>(a, grid, st);
+    else launch_chunk<256, 1>(a, grid, st);
   }
-  if (p.splits > 1) {
-    if (narrow) attn_masked_join_kernel<128><<<dim3(shape->q_heads, T), 128, 0, st>>>(a);
+  const uint32_t columns = T * shape->q_heads;
+  if (p.splits > kFewSplits) {
+    if (narrow) attn_masked_join_kernel<128><<<dim3(shape->q_heads, T), 256, 0, st>>>(a);
     else attn_masked_join_kernel<256><<<dim3(shape->q_heads, T), 256, 0, st>>>(a);
+  } else if (p.splits > 1) {
+    if (narrow) attn_masked_join_few_kernel<128><<<(columns + 7u) / 8u, 256, 0, st>>>(a, columns);
+    else attn_masked_join_few_kernel<256><<<(columns + 3u) / 4u, 256, 0, st>>>(a, columns);
   }
   return mi_hip((int)hipGetLastError(), "attn_masked");
 }
