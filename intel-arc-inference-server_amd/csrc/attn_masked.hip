@@ -16,6 +16,7 @@
 // A key that a row does not see has weight 0, but 0 times an infinity or a NaN of its V row is a NaN. A block whose
 // result is not finite is therefore formed again, key by key, over the keys that each row sees.
 #include <algorithm>
+#include <type_traits>
 
 #include "mi_capi_internal.h"
 #include "mi_common.h"
@@ -26,7 +27,6 @@ namespace {
 constexpr float kNoKey = -1e30f, kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 15.f, kBelow = 7.f;
 constexpr uint32_t kTile = 32;      // keys per step of a wave
-constexpr uint32_t kMaxRows = 128;  // rows of a block at most
 
 struct MaskedArgs {
   const float* q;        // [T][q_heads][HD]
@@ -42,64 +42,63 @@ struct MaskedArgs {
   float c, c2, cap;      // y = c s, or cap - 2 cap / (2^(c2 s) + 1) (cap here in base 2)
 };
 
-// What a block's rows see, and the 32-key tiles that hold it: tiles [0, n_a) of the prefix, then from b0 on.
-struct Block {
-  uint32_t lo[kMaxRows], hi[kMaxRows], pos[kMaxRows];  // hi 0: the row sees nothing
-  uint32_t min_lo, max_lo, min_hi, max_hi;
-  int again;
+// A row's span: lo <= hi <= kv_len; hi 0: it sees nothing.
+struct Span {
+  uint32_t lo, hi, pos;
 };
-struct Tiles {
-  uint32_t n_a, b0, n;
-  __device__ __forceinline__ uint32_t key(uint32_t i) const { return kTile * (i < n_a ? i : b0 + (i - n_a)); }
-};
-
-// a row's span as loaded: thread t's row t0 + t
-struct RowSpan {
-  uint32_t lo = 0, hi = 0, pos = 0;
-};
-__device__ __forceinline__ RowSpan load_span(const MaskedArgs& a, uint32_t t0, uint32_t rows_here) {
-  RowSpan s;
-  if (threadIdx.x < rows_here) {
-    const uint32_t t = t0 + threadIdx.x;
-    s.pos = a.pos ? a.pos[t] : a.pos0 + t;
-    s.lo = a.lo ? a.lo[t] : 0u;
-    s.hi = a.hi ? a.hi[t] : s.pos + 1u;
-  }
+__device__ __forceinline__ Span row_span(const MaskedArgs& a, uint32_t t) {
+  Span s;
+  s.pos = a.pos ? a.pos[t] : a.pos0 + t;
+  s.hi = min(a.hi ? a.hi[t] : s.pos + 1u, a.kv_len);
+  s.lo = min(a.lo ? a.lo[t] : 0u, s.hi);
+  if (s.lo == s.hi && min(a.prefix, s.hi) == 0u) s.lo = s.hi = 0u;
   return s;
 }
-// every thread of the work-group; rows_here <= its threads
-__device__ __forceinline__ Tiles block_begin(const MaskedArgs& a, Block& b, const RowSpan& s, uint32_t rows_here) {
-  const uint32_t t = threadIdx.x;
-  if (t == 0) {
-    b.min_lo = b.min_hi = 0xFFFFFFFFu;
-    b.max_lo = b.max_hi = 0u;
-    b.again = 0;
+// What a block's rows see, and the 32-key tiles that hold it: tiles [0, n_a) of the prefix, then from b0 on. Every wave
+// forms it by itself from the rows' spans, a row (or two) per lane: no barrier stands before the first loads.
+struct Block {
+  uint32_t min_hi, max_lo, last;  // the last key that a row sees
+  uint32_t n_a, b0, n;
+  __device__ __forceinline__ uint32_t key(uint32_t i) const { return kTile * (i < n_a ? i : b0 + (i - n_a)); }
+  // whether some column of the block does not see some key of the tile (uniform)
+  __device__ __forceinline__ bool masked(const MaskedArgs& a, uint32_t key) const {
+    return key + kTile > min_hi || (key < max_lo && key + kTile > a.prefix);
   }
-  lds_barrier();
-  if (t < rows_here) {
-    uint32_t hi = min(s.hi, a.kv_len), lo = min(s.lo, hi);
-    if (lo == hi && min(a.prefix, hi) == 0u) lo = hi = 0u;  // nothing
-    b.lo[t] = lo;
-    b.hi[t] = hi;
-    b.pos[t] = s.pos;
-    if (hi) {
-      atomicMin(&b.min_lo, lo);
-      atomicMax(&b.max_lo, lo);
-      atomicMin(&b.min_hi, hi);
-      atomicMax(&b.max_hi, hi);
+};
+template <typename F>
+__device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
+  auto swap = [](uint32_t x, auto c) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(c)::value, 0xF, 0xF, false); };
+  v = f(v, swap(v, std::integral_constant<int, 0xB1>{}));
+  v = f(v, swap(v, std::integral_constant<int, 0x4E>{}));
+  v = f(v, swap(v, std::integral_constant<int, 0x141>{}));
+  v = f(v, swap(v, std::integral_constant<int, 0x140>{}));
+  auto at = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); };
+  return f(f(at(0), at(16)), f(at(32), at(48)));
+}
+__device__ __forceinline__ Block block_of(const MaskedArgs& a, uint32_t t0, uint32_t rows_here) {
+  const uint32_t lane = threadIdx.x & 63u;
+  uint32_t min_lo = 0xFFFFFFFFu, min_hi = 0xFFFFFFFFu, max_lo = 0u, max_hi = 0u;
+  for (uint32_t r = lane; r < rows_here; r += 64u) {
+    const Span s = row_span(a, t0 + r);
+    if (s.hi) {
+      min_lo = min(min_lo, s.lo);
+      max_lo = max(max_lo, s.lo);
+      min_hi = min(min_hi, s.hi);
+      max_hi = max(max_hi, s.hi);
     }
   }
-  lds_barrier();
-  Tiles w{0u, 0u, 0u};
-  auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
-  const uint32_t min_lo = uniform(b.min_lo), max_hi = uniform(b.max_hi);
+  auto lesser = [](uint32_t x, uint32_t y) { return min(x, y); };
+  auto greater = [](uint32_t x, uint32_t y) { return max(x, y); };
+  min_lo = wave_fold(min_lo, lesser);
+  max_hi = wave_fold(max_hi, greater);
+  Block b{wave_fold(min_hi, lesser), wave_fold(max_lo, greater), max_hi - 1u, 0u, 0u, 0u};
   if (max_hi) {
-    w.n_a = (min(a.prefix, max_hi) + kTile - 1u) / kTile;
-    w.b0 = max(min_lo / kTile, w.n_a);
+    b.n_a = (min(a.prefix, max_hi) + kTile - 1u) / kTile;
+    b.b0 = max(min_lo / kTile, b.n_a);
     const uint32_t end = (max_hi + kTile - 1u) / kTile;
-    w.n = w.n_a + (end > w.b0 ? end - w.b0 : 0u);
+    b.n = b.n_a + (end > b.b0 ? end - b.b0 : 0u);
   }
-  return w;
+  return b;
 }
 
 // the cache row of a key below kv_len
@@ -123,13 +122,12 @@ struct Column {
   float slope;
   bool live;  // a row and a head, and the row sees something
 };
-__device__ __forceinline__ Column column(const MaskedArgs& a, const Block& b, uint32_t j, uint32_t row, uint32_t g,
-                                         uint32_t rows_here) {
-  Column c{0u, 0xFFFFFFFFu, 0u, 0.f, row < rows_here && b.hi[min(row, kMaxRows - 1u)] != 0u};
-  if (row < rows_here) c.pos = b.pos[row];
-  if (c.live) {  // (any other column sees every key and is not written)
-    c.lo = b.lo[row];
-    c.hi = b.hi[row];
+__device__ __forceinline__ Column column(const MaskedArgs& a, uint32_t j, uint32_t t0, uint32_t row, uint32_t g, uint32_t rows_here) {
+  const Span s = row_span(a, t0 + min(row, rows_here - 1u));
+  Column c{s.lo, s.hi, s.pos, 0.f, row < rows_here && s.hi != 0u};
+  if (!c.live) {  // (it sees every key and is not written)
+    c.lo = 0u;
+    c.hi = 0xFFFFFFFFu;
   }
   if (a.slopes) c.slope = a.slopes[j * a.gqa + g] * kLog2e;
   return c;
@@ -166,11 +164,6 @@ __device__ __forceinline__ void scores(const MaskedArgs& a, const Column& c, uin
   }
   bias_and_mask(a, c, key0, masked, w);
 }
-// whether some column of the block does not see some key of the tile (uniform)
-__device__ __forceinline__ bool tile_masked(const MaskedArgs& a, const Block& b, uint32_t key) {
-  return key + kTile > b.min_hi || (key < b.max_lo && key + kTile > a.prefix);
-}
-
 // where a split leaves column `col` of its block: HD values (sums of weight times V), then r and the weights' sum
 template <int HD>
 __device__ __forceinline__ float* part_at(const MaskedArgs& a, uint32_t j, uint32_t t, uint32_t g, uint32_t split) {
@@ -179,7 +172,7 @@ __device__ __forceinline__ float* part_at(const MaskedArgs& a, uint32_t j, uint3
 
 // The columns of a block one by one, over the keys that they see only: a lane holds dims lane + 64 i.
 template <int HD>
-__device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, const Tiles& tiles, uint32_t j, uint32_t t0,
+__device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, uint32_t j, uint32_t t0,
                                            uint32_t rows_here, uint32_t from, uint32_t to, uint32_t split) {
   constexpr uint32_t D = HD / 64;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
@@ -187,7 +180,7 @@ __device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, 
 #pragma unroll 1
   for (uint32_t p = wave; p < rows_here * a.gqa; p += blockDim.x / 64u) {
     const uint32_t row = p / a.gqa, g = p % a.gqa;
-    const Column c = column(a, b, j, row, g, rows_here);
+    const Column c = column(a, j, t0, row, g, rows_here);
     const float* q = a.q + ((size_t)(t0 + row) * a.q_heads + j * a.gqa + g) * HD + lane;
     float r = kNoKey, l = 0.f, acc[D];
 #pragma unroll
@@ -195,7 +188,7 @@ __device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, 
     if (c.live) {
 #pragma unroll 1
       for (uint32_t i = from; i < to; ++i) {
-        const uint32_t k0 = tiles.key(i);
+        const uint32_t k0 = b.key(i);
 #pragma unroll 1
         for (uint32_t key = k0; key < k0 + kTile; ++key) {
           if (!sees(a, c, key)) continue;
@@ -237,21 +230,29 @@ __device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, 
 
 // KK x 32 dims of a column's q as the B operand, f16 high and low parts: k = 32 kk + 8 qq + e
 template <uint32_t KK>
-__device__ __forceinline__ void load_q(const float* qp, h8_t (&qh)[KK], h8_t (&ql)[KK]) {
+__device__ __forceinline__ void split_q(const f4_t (&q)[2 * KK], h8_t (&qh)[KK], h8_t (&ql)[KK]) {
   float neg1 = -1.f;
   asm("" : "+s"(neg1));
 #pragma unroll
   for (uint32_t kk = 0; kk < KK; ++kk) {
-    const f4_t q0 = *reinterpret_cast<const f4_any*>(qp + 32u * kk), q1 = *reinterpret_cast<const f4_any*>(qp + 32u * kk + 4);
     u4_t h, l;
-    uint32_t hh, ll;
-    f16_parts(q0.x, q0.y, neg1, hh, ll); h.x = hh; l.x = ll;
-    f16_parts(q0.z, q0.w, neg1, hh, ll); h.y = hh; l.y = ll;
-    f16_parts(q1.x, q1.y, neg1, hh, ll); h.z = hh; l.z = ll;
-    f16_parts(q1.z, q1.w, neg1, hh, ll); h.w = hh; l.w = ll;
+#pragma unroll
+    for (uint32_t x = 0; x < 4; ++x) {
+      uint32_t hh, ll;
+      f16_parts(q[2 * kk + x / 2][2 * (x % 2)], q[2 * kk + x / 2][2 * (x % 2) + 1], neg1, hh, ll);
+      h[x] = hh;
+      l[x] = ll;
+    }
     qh[kk] = __builtin_bit_cast(h8_t, h);
     ql[kk] = __builtin_bit_cast(h8_t, l);
   }
+}
+template <uint32_t KK>
+__device__ __forceinline__ void load_q(const float* qp, h8_t (&qh)[KK], h8_t (&ql)[KK]) {
+  f4_t q[2 * KK];
+#pragma unroll
+  for (uint32_t x = 0; x < 2 * KK; ++x) q[x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2)));
+  split_q<KK>(q, qh, ql);
 }
 
 // One step of the softmax of a wave's CT column tiles. The references first: raised, with what was formed by them, where a
@@ -325,8 +326,10 @@ __device__ __forceinline__ void store_out(const MaskedArgs& a, uint32_t j, uint3
                   (uint32_t)act_enc(v[2], a.act) | ((uint32_t)act_enc(v[3], a.act) << 16)};
   *reinterpret_cast<h4_any*>(a.out + ((size_t)t * a.q_heads + j * a.gqa + g) * HD + 16u * tt + 4u * qq) = h;
 }
-__device__ __forceinline__ float not_finite(f4_t v) {  // 0, or NaN
-  return ((v[0] - v[0]) + (v[1] - v[1])) + ((v[2] - v[2]) + (v[3] - v[3]));
+__device__ __forceinline__ float not_finite(float z, f4_t v) {  // 0 (a zero z), or NaN
+#pragma unroll
+  for (uint32_t e = 0; e < 4; ++e) z = __builtin_fmaf(v[e], 0.f, z);
+  return z;
 }
 
 // Few rows (16 columns per block): grid (kv_heads, row blocks, splits), 4 waves. A wave walks its own 32-key tiles,
@@ -336,7 +339,6 @@ template <int HD>
 __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel(MaskedArgs a) {
   constexpr uint32_t KK = HD / 32, NT = HD / 16, VROW = HD + 16;
   constexpr uint32_t PPR = HD / 8, RPP = 64 / PPR, NV = kTile / RPP;  // 16-byte pieces per V row, rows per load, loads per tile
-  __shared__ Block b;
   __shared__ __align__(16) union Slab {
     uint16_t v[kTile * VROW];
     struct {
@@ -346,22 +348,20 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
   const uint32_t j = blockIdx.x, t0 = blockIdx.y * a.rows, split = blockIdx.z;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, qi = lane & 15u, qq = lane >> 4;
   const uint32_t rows_here = min(a.rows, a.T - t0);
-  const Tiles tiles = block_begin(a, b, load_span(a, t0, rows_here), rows_here);
-  const uint32_t from = (uint32_t)((uint64_t)tiles.n * split / a.splits), to = (uint32_t)((uint64_t)tiles.n * (split + 1u) / a.splits);
   const uint32_t row = qi / a.gqa, g = qi % a.gqa;
-  const Column col = column(a, b, j, row, g, rows_here);
-  h8_t qh[KK], ql[KK];
-  load_q<KK>(a.q + ((size_t)(t0 + (row < rows_here ? row : 0u)) * a.q_heads + j * a.gqa + g) * HD + 8u * qq, qh, ql);
+  const Block b = block_of(a, t0, rows_here);
+  const Column col = column(a, j, t0, row, g, rows_here);
+  const uint32_t from = (uint32_t)((uint64_t)b.n * split / a.splits), to = (uint32_t)((uint64_t)b.n * (split + 1u) / a.splits);
+  const float* qp = a.q + ((size_t)(t0 + (row < rows_here ? row : 0u)) * a.q_heads + j * a.gqa + g) * HD + 8u * qq;
   float r[1] = {kNoKey}, l[1] = {0.f};
   f4_t acc[1][NT];
 #pragma unroll
   for (uint32_t tt = 0; tt < NT; ++tt) acc[0][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
 
   const size_t hoff = (size_t)j * a.head_stride;
-  const uint32_t last = b.max_hi - 1u;
   u4_t kr[2][KK], vr[NV];
   // a lane's cache row: of key 16 (lane / 16 % 2) + lane % 16 of the tile (keys behind the last one read it again)
-  auto rows_of = [&](uint32_t i) { return cache_row(a, min(tiles.key(i) + (lane & 31u), last)); };
+  auto rows_of = [&](uint32_t i) { return cache_row(a, min(b.key(i) + (lane & 31u), b.last)); };
   auto load = [&](uint32_t crow) {
 #pragma unroll
     for (uint32_t gg = 0; gg < 2; ++gg) {
@@ -380,10 +380,12 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
     load(rows_of(i));
     if (i + 4u < to) crow = rows_of(i + 4u);
   }
+  h8_t qh[KK], ql[KK];
+  load_q<KK>(qp, qh, ql);
   uint16_t* vs = slab[wave].v;
   const uint16_t* vb = vs + (4u * qq + (qi >> 2)) * VROW + 4u * (qi & 3u);
   for (; i < to; i += 4u) {
-    const uint32_t key = tiles.key(i);
+    const uint32_t key = b.key(i);
     f4_t d[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
     for (uint32_t kk = 0; kk < KK; ++kk)
@@ -403,7 +405,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
     float w[1][8];
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) w[0][e] = d[e / 4][e % 4];
-    scores(a, col, key + 4u * qq, tile_masked(a, b, key), w[0]);
+    scores(a, col, key + 4u * qq, b.masked(a, key), w[0]);
     raise<1, NT>(w, qi, r, l, acc);
     h8_t ph, pl;
     weights(w[0], r[0], l[0], ph, pl);
@@ -417,8 +419,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
   l[0] = col_sum(l[0]);
   float bad = 0.f;
 #pragma unroll
-  for (uint32_t tt = 0; tt < NT; ++tt) bad += not_finite(acc[0][tt]);
-  if (col.live && (bad != 0.f || l[0] - l[0] != 0.f)) b.again = 1;
+  for (uint32_t tt = 0; tt < NT; ++tt) bad = not_finite(bad, acc[0][tt]);
+  bad += l[0] - l[0];
   wave_lds_sync();
   auto& mine = slab[wave].part;
 #pragma unroll
@@ -427,9 +429,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
     for (uint32_t e = 0; e < 4; ++e) mine.acc[4u * tt + e][lane] = acc[0][tt][e];
   mine.r[lane] = r[0];
   mine.l[lane] = l[0];
-  __syncthreads();
-  if (b.again) {
-    slow_block<HD>(a, b, tiles, j, t0, rows_here, from, to, split);
+  if (__syncthreads_or(col.live && bad != 0.f)) {
+    slow_block<HD>(a, b, j, t0, rows_here, from, to, split);
     return;
   }
   // wave w joins the dims 16 tt + .. of its quarter of the tiles
@@ -473,7 +474,6 @@ template <int HD, int CT, bool CAP, Order ORDER>
 __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   constexpr uint32_t DS = HD / 128, KK = 4, NT = 8, KROW = HD + 8, VROW = HD + 16, THREADS = 2 * HD;
   constexpr uint32_t PPR = HD / 8, RPP = THREADS / PPR, CH = kTile / RPP;  // 16-byte pieces per row, rows per pass, passes
-  __shared__ Block b;
   __shared__ __align__(16) struct {
     uint16_t k[2][kTile * KROW], v[2][kTile * VROW];
     f4_t s[DS > 1 ? 2 : 1][DS > 1 ? 4 * DS : 1][2 * CT][DS > 1 ? 64 : 1];
@@ -483,20 +483,22 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   const uint32_t t = threadIdx.x, lane = t & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 6)), qi = lane & 15u, qq = lane >> 4;
   const uint32_t cw = wave % 4u, ds = wave / 4u;
   const uint32_t rows_here = min(a.rows, a.T - t0);
-  const RowSpan span = load_span(a, t0, rows_here);
+  const Block b = block_of(a, t0, rows_here);
   uint32_t row[CT], g[CT];
-  const float* qp[CT];
+  Column col[CT];
+  f4_t qraw[CT][2 * KK];  // (converted behind the first tiles' loads)
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
     const uint32_t p = 16u * (CT * cw + ct) + qi;
     row[ct] = p / a.gqa;
     g[ct] = p % a.gqa;
-    qp[ct] = a.q + ((size_t)(t0 + (row[ct] < rows_here ? row[ct] : 0u)) * a.q_heads + j * a.gqa + g[ct]) * HD + 128u * ds + 8u * qq;
+    col[ct] = column(a, j, t0, row[ct], g[ct], rows_here);
+    const float* qp = a.q + ((size_t)(t0 + (row[ct] < rows_here ? row[ct] : 0u)) * a.q_heads + j * a.gqa + g[ct]) * HD + 128u * ds + 8u * qq;
+#pragma unroll
+    for (uint32_t x = 0; x < 2 * KK; ++x) qraw[ct][x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2)));
   }
-  const Tiles tiles = block_begin(a, b, span, rows_here);
-  const uint32_t from = (uint32_t)((uint64_t)tiles.n * split / a.splits), n = (uint32_t)((uint64_t)tiles.n * (split + 1u) / a.splits) - from;
+  const uint32_t from = (uint32_t)((uint64_t)b.n * split / a.splits), n = (uint32_t)((uint64_t)b.n * (split + 1u) / a.splits) - from;
   auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
-  const uint32_t min_hi = uniform(b.min_hi), max_lo = uniform(b.max_lo), last = uniform(b.max_hi) - 1u;
   const size_t hoff = (size_t)j * a.head_stride;
   const uint32_t srow = t / PPR, sp = 8u * (t % PPR);
   u4_t kr[CH], vr[CH];
@@ -506,20 +508,20 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   };
   auto rows_of = [&](uint32_t i) {
     Rows w;
-    const uint32_t key0 = tiles.key(from + min(i, n - 1u));
+    const uint32_t key0 = b.key(from + min(i, n - 1u));
     if constexpr (ORDER == kContiguous) {
       w.r[0] = key0;
     } else if constexpr (ORDER == kWholeTiles) {
       w.r[0] = cache_row(a, key0);
     } else {
 #pragma unroll
-      for (uint32_t c = 0; c < CH; ++c) w.r[c] = cache_row(a, min(key0 + RPP * c + srow, last));
+      for (uint32_t c = 0; c < CH; ++c) w.r[c] = cache_row(a, min(key0 + RPP * c + srow, b.last));
     }
     return w;
   };
   // (a tile behind the last is that one again, and its loads are not used)
   auto load = [&](const uint16_t* cache, uint32_t i, const Rows& w, u4_t (&to)[CH]) {
-    const uint32_t left = last - tiles.key(from + min(i, n - 1u));
+    const uint32_t left = b.last - b.key(from + min(i, n - 1u));
 #pragma unroll
     for (uint32_t c = 0; c < CH; ++c) {
       const uint32_t r = ORDER == kAnyPages ? w.r[c] : uniform(w.r[0]) + min(RPP * c + srow, left);
@@ -543,14 +545,12 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
     load(a.v, 0, r0, vr);
     load(a.k, 1, r1, k1);
   }
-  Column col[CT];
   float r[CT], l[CT];
   f4_t acc[CT][NT], d[CT][2];
   h8_t qh[CT][KK], ql[CT][KK];
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
-    load_q<KK>(qp[ct], qh[ct], ql[ct]);
-    col[ct] = column(a, b, j, row[ct], g[ct], rows_here);
+    split_q<KK>(qraw[ct], qh[ct], ql[ct]);
     r[ct] = kNoKey;
     l[ct] = 0.f;
 #pragma unroll
@@ -588,8 +588,8 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   float w[CT][8];
   // the scores w of tile i: bias, mask, and the columns' references
   auto settle = [&](uint32_t i) {
-    const uint32_t key = tiles.key(from + i);
-    const bool masked = key + kTile > min_hi || (key < max_lo && key + kTile > a.prefix);  // uniform
+    const uint32_t key = b.key(from + i);
+    const bool masked = b.masked(a, key);
 #pragma unroll
     for (uint32_t ct = 0; ct < CT; ++ct) bias_and_mask(a, col[ct], key + 4u * qq, masked, w[ct]);
     raise<CT, NT>(w, qi, r, l, acc);
@@ -677,17 +677,17 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
     }
   }
   float sum[CT];
+  bool bad = false;
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
     sum[ct] = col_sum(l[ct]);
-    float bad = 0.f;
+    float z = sum[ct] - sum[ct];
 #pragma unroll
-    for (uint32_t tt = 0; tt < NT; ++tt) bad += not_finite(acc[ct][tt]);
-    if (col[ct].live && (bad != 0.f || sum[ct] - sum[ct] != 0.f)) b.again = 1;
+    for (uint32_t tt = 0; tt < NT; ++tt) z = not_finite(z, acc[ct][tt]);
+    bad |= col[ct].live && z != 0.f;
   }
-  __syncthreads();
-  if (b.again) {
-    slow_block<HD>(a, b, tiles, j, t0, rows_here, from, from + n, split);
+  if (__syncthreads_or(bad)) {
+    slow_block<HD>(a, b, j, t0, rows_here, from, from + n, split);
     return;
   }
 #pragma unroll
@@ -804,12 +804,15 @@ __global__ __launch_bounds__(256) void attn_masked_join_few_kernel(MaskedArgs a,
 //   few: as many parts as fill the CUs (two work-groups each at rows of 128, one at 256), of 128 keys at least. Measured
 //   (us): one row, 40 / 8 heads of 128, 4099 keys 17.6 / 12.9 / 11.3 / 10.0 / 11.2 in 4 / 8 / 16 / 32 / 64 parts; 131072 keys
 //   105 / 100 / 103 / 110 in 32 / 64 / 128 / 256; 16 / 2 heads of 256, 65536 keys 37.6 / 31.3 / 38.3 in 64 / 128 / 256.
-//   chunk: the least modelled time over both CT and the parts s, in us:
-//     rounds (3 + tiles / s tau) + join,  join = 3 + T q_heads s (head_dim + 4) 8 bytes at 3.5 TB/s for s > 1
-//   with tiles of 32 keys (all that the cache may hold: what the rows see is the device's) and tau a tile's time with k
-//   work-groups on a CU. Measured (us; CT 1 then 2, in 1 / 2 / 3 / 4 parts): 500 rows over 4500 keys, 32 / 8 heads of 128:
-//   103 / 89 / 83 / 84, 148 / 90 / 86 / 75; 777 over 3778, 16 / 2 of 256: 148 / 152 / 153 / 158, 218 / 128 / 155 / 136; 333 over 333,
-//   40 / 8 of 128: 15 / 23 / 25 / 27, 23 / 26 / 28 / 29; 20 over 4020: 89 / 51 / 38 / 31 (16 parts 19), 131 / 73 / 53 / 44.
+//   chunk: the least modelled time over both CT and the parts s, in us. What the rows see is the device's; the model takes
+//   them for the last T of the cache and causal, so that a work-group has between (keys - T) / 32 and keys / 32 tiles:
+//     the longest, 3 + most / s tau, or all of them over the CUs, rounds (3 + mean / s tau), and for s > 1
+//     join = 3 + T q_heads s (head_dim + 4) 8 bytes at 3.5 TB/s
+//   with cap the work-groups that a CU holds, tau a tile's time with that many on it, and rounds between w / (256 cap), where
+//   short work-groups fill up behind long ones, and the next whole number, where all are alike. Measured (us; CT 1 then 2, in
+//   1 / 2 / 3 / 4 parts): 500 rows over 4500 keys, 32 / 8 heads of 128: 108 / 88 / 79 / 82, 148 / 88 / 81 / 71; 777 over 3778,
+//   16 / 2 of 256: 147 / 151 / 152 / 157, 221 / 129 / 155 / 136 (122 in 5); 2048 over 2048, 40 / 8 of 128: 106 / 126, 86 / 112, 16 / 2 of 256:
+//   87 / 116, 110 / 97; 333 over 333, 40 / 8 of 128: 14 / 21 / 23, 20 / 24 / 26; 20 over 4020: 87 / 50 / 36 / 30 (16 parts 18), 129 / 71 / 51 / 42.
 struct Pick {
   bool few;
   uint32_t ct, rows, splits;
@@ -824,17 +827,18 @@ Pick pick(uint32_t T, uint32_t keys, uint32_t kv_heads, uint32_t gqa, uint32_t h
     return p;
   }
   static constexpr double kTau[2][2][3] = {{{0.73, 1.15, 1.53}, {1.05, 1.45, 1.45}}, {{1.2, 1.2, 1.2}, {1.85, 1.85, 1.85}}};
-  const double tiles = (keys + kTile - 1u) / kTile;
+  const double most = (keys + kTile - 1u) / kTile, mean = most - std::min(T, keys) / (2.0 * kTile);
+  const double alike = (double)(keys - std::min(T, keys)) / keys;
   double least = 1e300;
   for (uint32_t ct = 1; ct <= 2; ++ct) {
-    const uint32_t rows = 64u * ct / gqa, cap = hd == 128 ? 4u - ct : 1u;  // work-groups that a CU holds
+    const uint32_t rows = 64u * ct / gqa, cap = hd == 128 ? 4u - ct : 1u;
     const double* tau = kTau[hd == 256][ct - 1];
     const uint64_t blocks = (uint64_t)kv_heads * ((T + rows - 1u) / rows);
-    for (uint32_t s = 1; s <= 64u && (s == 1 || s * 4u <= tiles); ++s) {
-      const uint64_t w = blocks * s, full = w / (kCus * cap), rest = w % (kCus * cap);
-      const double step = tiles / s;
-      double us = (double)full * (3.0 + step * tau[cap - 1]);
-      if (rest) us += 3.0 + step * tau[(rest + kCus - 1) / kCus - 1];
+    for (uint32_t s = 1; s <= 64u && (s == 1 || s * 4u <= most); ++s) {
+      const uint64_t w = blocks * s;
+      const double at = tau[std::min<uint64_t>((w + kCus - 1u) / kCus, cap) - 1u];
+      const double turns = (double)w / (kCus * cap), whole = (double)((w + kCus * cap - 1u) / (kCus * cap));
+      double us = std::max(3.0 + most / s * at, (turns + (whole - turns) * alike) * (3.0 + mean / s * at));
       if (s > 1) us += 3.0 + (double)T * (kv_heads * gqa) * s * (hd + 4) * 8.0 / 3.5e6;
       if (us < least) {
         least = us;
