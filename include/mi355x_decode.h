@@ -520,7 +520,7 @@ int mi_gemm_w8a8(const int8_t* q_tiled, const float* row_scales, const int8_t* w
                  const float* w_scales, void* out, uint32_t out_kind, size_t out_stride, uint32_t M,
                  uint32_t K, uint32_t N, void* stream);
 /* mi_quant_rows_i8 and mi_gemm_w8a8 in one call, bit for bit; ws: mi_linear_w8a8_ws(M, K) bytes of device
- * scratch, 16-byte aligned. */
+ * scratch, 16-byte aligned; out overlaps neither x nor ws. */
 size_t mi_linear_w8a8_ws(uint32_t M, uint32_t K);
 int mi_linear_w8a8(const uint16_t* x, size_t x_stride, const int8_t* w_tiled, const float* w_scales,
                    void* ws, size_t ws_bytes, void* out, uint32_t out_kind, size_t out_stride, uint32_t M,

@@ -22,6 +22,7 @@ typedef int i4_t __attribute__((ext_vector_type(4)));
 typedef unsigned short us2_t __attribute__((ext_vector_type(2)));
 
 constexpr uint32_t kMaxK = 131072;  // the int32 sums stay below 2^31
+constexpr uint32_t kFusedK = 32768;  // the longest single row that a product quantises for itself, one byte of LDS for each k
 
 __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t,
@@ -138,8 +139,7 @@ struct GemmArgs {
 
 // the four outputs n .. n + 3 of row m
 template <bool F32>
-__device__ __forceinline__ void store4(const GemmArgs& a, uint32_t m, uint32_t n, i4_t acc) {
-  const float s = a.qs[m];
+__device__ __forceinline__ void store4(const GemmArgs& a, float s, uint32_t m, uint32_t n, i4_t acc) {
   const f4_t ws = *reinterpret_cast<const f4_any*>(a.ws + n);
   f4_t v;
 #pragma unroll
@@ -154,10 +154,16 @@ __device__ __forceinline__ void store4(const GemmArgs& a, uint32_t m, uint32_t n
 }
 
 // Few rows: MT x 16 rows and NT x 16 columns per work-group, whose W waves deal the chunks of k out among them, U at a
-// time each. Both operands come straight from memory (a lane without a row loads none); A is the weights, so a lane
-// ends with four adjacent columns of one row. The waves' sums join through LDS.
-template <bool F32, uint32_t MT, uint32_t NT, uint32_t W, uint32_t U>
-__global__ __launch_bounds__(64 * W) void gemm_w8a8_few_kernel(GemmArgs a) {
+// time each. Both operands come straight from memory (a lane without a row loads none); A is the weights, so a lane ends
+// with four adjacent columns of a row. The waves' sums join through LDS.
+// FUSED (MT 1, a single row): the row is the f16 one, which every work-group quantises for itself into LDS behind its
+// first weights' loads, in place of a launch whose 4 us the weights wait for. Against the two launches: 5120 -> 7168
+// 9.4 us (12.2), 17408 -> 5120 21.0 (23.6), 1024 -> 512 4.2 (7.5), 5120 -> 151936 113.0 (114.5), 32768 -> 4096 27.3
+// (27.6). More rows cost each work-group more of that work: two are 33.6 (30.3) at 5120 -> 34816, four 14.8 (12.4) at
+// 5120 -> 7168, so they take the two launches.
+template <bool F32, uint32_t MT, uint32_t NT, uint32_t W, uint32_t U, bool FUSED>
+__global__ __launch_bounds__(64 * W) void gemm_w8a8_few_kernel(GemmArgs a, const uint16_t* x) {
+  static_assert(!FUSED || MT == 1);
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const uint32_t nc = a.K / 64u, nt = a.N / 16u;
   const uint32_t n0 = blockIdx.x * NT, m0 = blockIdx.y * MT;
@@ -169,26 +175,55 @@ __global__ __launch_bounds__(64 * W) void gemm_w8a8_few_kernel(GemmArgs a) {
 #pragma unroll
   for (uint32_t j = 0; j < MT; ++j) {
     have[j] = (m0 + j) * 16u + (lane & 15u) < a.M;
-    qp[j] = a.q + (size_t)(have[j] ? m0 + j : 0u) * nc * 64u + lane;
+    qp[j] = FUSED ? nullptr : a.q + (size_t)(have[j] ? m0 + j : 0u) * nc * 64u + lane;
+  }
+  u4_t wv[U][NT];
+  auto load_w = [&](uint32_t c0) {
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+      for (uint32_t i = 0; i < NT; ++i)
+        wv[u][i] = load_stream16(reinterpret_cast<const uint32_t*>(wp[i] + (size_t)min(c0 + u, nc - 1u) * 64u));
+  };
+  uint32_t c0 = wave * U;
+  if constexpr (FUSED) load_w(c0);
+  extern __shared__ __align__(16) u4_t row_units[];  // FUSED: the row's K bytes, as [K / 64][4][16]
+  __shared__ uint32_t top[W];
+  Scale row{};
+  if constexpr (FUSED) {
+    const uint32_t units = a.K / 16u;
+    uint32_t mx = 0;
+    for (uint32_t u = threadIdx.x; u < units; u += 64u * W) {
+      const Unit v = load_unit(x, u);
+      mx = max_abs8(max_abs8(mx, v.a), v.b);
+    }
+    mx = max_bits(mx);
+    if (lane == 0) top[wave] = mx;
+    lds_barrier();
+    uint32_t bits = top[0];
+#pragma unroll
+    for (uint32_t i = 1; i < W; ++i) bits = max(bits, top[i]);
+    row = row_scale(bits);
+    for (uint32_t u = threadIdx.x; u < units; u += 64u * W) row_units[u] = quant_unit(load_unit(x, u), row);
+    lds_barrier();
   }
   i4_t acc[MT][NT];
 #pragma unroll
   for (uint32_t j = 0; j < MT; ++j)
 #pragma unroll
     for (uint32_t i = 0; i < NT; ++i) acc[j][i] = i4_t{0, 0, 0, 0};
-  for (uint32_t c0 = wave * U; c0 < nc; c0 += W * U) {
-    u4_t wv[U][NT], qv[U][MT];
+  auto multiply = [&](uint32_t at) {
+    u4_t qv[U][MT];
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-      const uint32_t c = min(c0 + u, nc - 1u);
-#pragma unroll
-      for (uint32_t i = 0; i < NT; ++i) wv[u][i] = load_stream16(reinterpret_cast<const uint32_t*>(wp[i] + (size_t)c * 64u));
+    for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
       for (uint32_t j = 0; j < MT; ++j) {
         qv[u][j] = u4_t{0u, 0u, 0u, 0u};
-        if (have[j] && c0 + u < nc) qv[u][j] = *as_global(qp[j] + (size_t)c * 64u);
+        if (have[j] && at + u < nc) {
+          if constexpr (FUSED) qv[u][j] = row_units[4u * (at + u) + (lane >> 4)];
+          else qv[u][j] = *as_global(qp[j] + (size_t)(at + u) * 64u);
+        }
       }
-    }
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
@@ -197,6 +232,15 @@ __global__ __launch_bounds__(64 * W) void gemm_w8a8_few_kernel(GemmArgs a) {
         for (uint32_t i = 0; i < NT; ++i)
           acc[j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4_t, wv[u][i]), __builtin_bit_cast(i4_t, qv[u][j]),
                                                             acc[j][i], 0, 0, 0);
+  };
+  if constexpr (FUSED) {
+    multiply(c0);
+    c0 += W * U;
+  }
+#pragma unroll 1
+  for (; c0 < nc; c0 += W * U) {
+    load_w(c0);
+    multiply(c0);
   }
   __shared__ __align__(16) i4_t part[W][MT * NT][64];
 #pragma unroll
@@ -210,7 +254,7 @@ __global__ __launch_bounds__(64 * W) void gemm_w8a8_few_kernel(GemmArgs a) {
     i4_t sum = part[0][t][lane];
 #pragma unroll
     for (uint32_t p = 1; p < W; ++p) sum += part[p][t][lane];
-    store4<F32>(a, m, tile * 16u + 4u * (lane >> 4), sum);
+    store4<F32>(a, FUSED ? row.s : a.qs[m], m, tile * 16u + 4u * (lane >> 4), sum);
   }
 }
 
@@ -332,10 +376,11 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void gemm_w8a8_kernel(GemmArg
   for (uint32_t j = 0; j < RM; ++j) {
     const uint32_t m = (m0 + wm * RM + j) * 16u + (lane & 15u);
     if (m >= a.M) continue;
+    const float s = a.qs[m];
 #pragma unroll
     for (uint32_t k = 0; k < CN; ++k) {
       const uint32_t tile = n0 + wn * CN + k;
-      if (tile < nt) store4<F32>(a, m, tile * 16u + 4u * (lane >> 4), acc[j][k]);
+      if (tile < nt) store4<F32>(a, s, m, tile * 16u + 4u * (lane >> 4), acc[j][k]);
     }
   }
 }
@@ -347,7 +392,14 @@ void launch_tiles(const GemmArgs& a, hipStream_t st) {
 }
 template <bool F32, uint32_t MT, uint32_t NT, uint32_t W, uint32_t U>
 void launch_few(const GemmArgs& a, hipStream_t st) {
-  gemm_w8a8_few_kernel<F32, MT, NT, W, U><<<dim3((a.N + 16u * NT - 1u) / (16u * NT), (a.M + 16u * MT - 1u) / (16u * MT)), 64 * W, 0, st>>>(a);
+  gemm_w8a8_few_kernel<F32, MT, NT, W, U, false>
+      <<<dim3((a.N + 16u * NT - 1u) / (16u * NT), (a.M + 16u * MT - 1u) / (16u * MT)), 64 * W, 0, st>>>(a, nullptr);
+}
+template <uint32_t NT, uint32_t U>
+void launch_fused(const GemmArgs& a, uint32_t out_kind, const uint16_t* x, hipStream_t st) {
+  const uint32_t wgs = (a.N + 16u * NT - 1u) / (16u * NT);
+  if (out_kind == MI_OUT_F32) gemm_w8a8_few_kernel<true, 1, NT, 4, U, true><<<wgs, 256, a.K, st>>>(a, x);
+  else gemm_w8a8_few_kernel<false, 1, NT, 4, U, true><<<wgs, 256, a.K, st>>>(a, x);
 }
 
 // The work-group's shape by the least modelled time in ns,
@@ -491,6 +543,12 @@ int mi_linear_w8a8(const uint16_t* x, size_t x_stride, const int8_t* w_tiled, co
     return mi_fail(MI_ERR_ARG, "linear_w8a8: the workspace is null, misaligned (16 bytes) or below mi_linear_w8a8_ws");
   int8_t* q = static_cast<int8_t*>(ws);
   float* qs = reinterpret_cast<float*>(q + tiled_bytes(M, K));
+  if (M == 1 && K <= kFusedK) {
+    const GemmArgs a{nullptr, nullptr, reinterpret_cast<const u4_t*>(w_tiled), w_scales, out, out_stride, M, K, N};
+    if (pick(M, K, N) == kFew16x32) launch_fused<2, 4>(a, out_kind, x, (hipStream_t)stream);
+    else launch_fused<1, 8>(a, out_kind, x, (hipStream_t)stream);
+    return mi_hip((int)hipGetLastError(), "linear_w8a8");
+  }
   if (int e = mi_quant_rows_i8(x, x_stride, M, K, q, qs, stream)) return e;
   const GemmArgs a{reinterpret_cast<const u4_t*>(q), qs, reinterpret_cast<const u4_t*>(w_tiled), w_scales, out,
                    out_stride, M, K, N};

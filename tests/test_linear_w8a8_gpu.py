@@ -192,3 +192,49 @@ def test_other_stream_and_replayed_graph():
             g.replay()
             sync()
             check(host(out, np.float32).reshape(M, N), x, w, ws, 0)
+
+
+# sizes that between them take every shape of the product's work-groups, each with rows, columns or chunks that end
+# inside one
+WIDE = [(9, 2112, 5136), (27, 1088, 6160), (33, 5184, 7184), (61, 1088, 10256), (515, 8256, 80), (250, 64, 4112), (131, 2112, 10256),
+        (333, 5184, 5136), (390, 576, 7184), (131, 64, 20496), (515, 1088, 7184), (1021, 64, 10256), (131, 2112, 34832),
+        (1500, 192, 10256), (2045, 448, 7184)]
+
+
+@pytest.mark.parametrize("M,K,N", WIDE)
+def test_wide_products_are_the_exact_sums(M, K, N):
+    """outputs compared bit for bit: the sums are integers below 2^53, so a product in fp64 is exact, and the two fp32
+    products that follow round alike"""
+    T = torch()
+    rng = np.random.default_rng(M + K + N)
+    q = rng.integers(-127, 128, (M, K)).astype(np.int8)
+    w = rng.integers(-127, 128, (N, K)).astype(np.int8)
+    qs, ws = dev(rng.uniform(0.01, 0.02, M).astype(np.float32)), dev(rng.uniform(0.01, 0.02, N).astype(np.float32))
+    dq, dw = dev(tile(q)), dev(tile(w))
+    stride = N + 5
+    out = T.full((M * stride + GUARD,), 5.0, dtype=T.float32, device="cuda")
+    print(f"gemm_w8a8 M={M} K={K} N={N}", flush=True)
+    mi.call("mi_gemm_w8a8", ptr(dq), ptr(qs), ptr(dw), ptr(ws), ptr(out), mi.OUT_F32, stride, M, K, N, stream())
+    sync()
+    sums = T.mm(T.from_numpy(q).cuda().double(), T.from_numpy(w).cuda().double().t().contiguous())
+    want = (sums.float() * qs[:, None]) * ws
+    body = out[:M * stride].view(M, stride)
+    assert T.equal(body[:, :N], want)
+    assert (body[:, N:] == 5).all() and (out[M * stride:] == 5).all()
+
+
+@pytest.mark.parametrize("kind", [0, 1])
+@pytest.mark.parametrize("K,N", [(64, 16), (320, 7184), (448, 4112), (5120, 7168), (17408, 80), (32768, 48), (32832, 48)])
+def test_a_single_row(K, N, kind):
+    rng = np.random.default_rng(K + N)
+    w, ws = weights(rng, N, K)
+    for special in (None, 0, np.inf, np.nan, 65504):
+        x = rows(rng, 1, K)
+        if special == 0:
+            x[:] = 0
+        elif special is not None:
+            x[0, K - 1] = special
+        got = call_linear(x, w, ws, kind, x_stride=K + 8)
+        if special in (0, None, 65504):
+            assert np.isfinite(got).all()
+        check(got, x, w, ws, kind)
