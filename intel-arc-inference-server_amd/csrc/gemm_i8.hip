@@ -158,7 +158,7 @@ __device__ __forceinline__ void store4(const GemmArgs& a, float s, uint32_t m, u
 // with four adjacent columns of a row. The waves' sums join through LDS.
 // FUSED (MT 1, a single row): the row is the f16 one, which every work-group quantises for itself into LDS behind its
 // first weights' loads, in place of a launch whose 4 us the weights wait for. Against the two launches: 5120 -> 7168
-// 9.4 us (12.2), 17408 -> 5120 21.0 (23.6), 1024 -> 512 4.2 (7.5), 5120 -> 151936 113.0 (114.5), 32768 -> 4096 27.3
+// 9.4 us (12.3), 17408 -> 5120 20.4 (23.7), 1024 -> 512 3.6 (6.6), 5120 -> 151936 111.8 (114.4), 32768 -> 4096 24.5
 // (27.6). More rows cost each work-group more of that work: two are 33.6 (30.3) at 5120 -> 34816, four 14.8 (12.4) at
 // 5120 -> 7168, so they take the two launches.
 template <bool F32, uint32_t MT, uint32_t NT, uint32_t W, uint32_t U, bool FUSED>
@@ -395,11 +395,11 @@ void launch_few(const GemmArgs& a, hipStream_t st) {
   gemm_w8a8_few_kernel<F32, MT, NT, W, U, false>
       <<<dim3((a.N + 16u * NT - 1u) / (16u * NT), (a.M + 16u * MT - 1u) / (16u * MT)), 64 * W, 0, st>>>(a, nullptr);
 }
-template <uint32_t NT, uint32_t U>
+template <uint32_t NT, uint32_t W, uint32_t U>
 void launch_fused(const GemmArgs& a, uint32_t out_kind, const uint16_t* x, hipStream_t st) {
   const uint32_t wgs = (a.N + 16u * NT - 1u) / (16u * NT);
-  if (out_kind == MI_OUT_F32) gemm_w8a8_few_kernel<true, 1, NT, 4, U, true><<<wgs, 256, a.K, st>>>(a, x);
-  else gemm_w8a8_few_kernel<false, 1, NT, 4, U, true><<<wgs, 256, a.K, st>>>(a, x);
+  if (out_kind == MI_OUT_F32) gemm_w8a8_few_kernel<true, 1, NT, W, U, true><<<wgs, 64 * W, a.K, st>>>(a, x);
+  else gemm_w8a8_few_kernel<false, 1, NT, W, U, true><<<wgs, 64 * W, a.K, st>>>(a, x);
 }
 
 // The work-group's shape by the least modelled time in ns,
@@ -545,8 +545,12 @@ int mi_linear_w8a8(const uint16_t* x, size_t x_stride, const int8_t* w_tiled, co
   float* qs = reinterpret_cast<float*>(q + tiled_bytes(M, K));
   if (M == 1 && K <= kFusedK) {
     const GemmArgs a{nullptr, nullptr, reinterpret_cast<const u4_t*>(w_tiled), w_scales, out, out_stride, M, K, N};
-    if (pick(M, K, N) == kFew16x32) launch_fused<2, 4>(a, out_kind, x, (hipStream_t)stream);
-    else launch_fused<1, 8>(a, out_kind, x, (hipStream_t)stream);
+    // 16 waves where all work-groups run at once, two to a CU: 24.5 us (4 waves 27.1) at 32768 -> 4096; where they take
+    // turns each turn waits for its row again: 30.7 (28.1) at 5120 -> 34816
+    const Shape p = pick(M, K, N);
+    if (p == kFew16x32) launch_fused<2, 4, 4>(a, out_kind, x, (hipStream_t)stream);
+    else if (p == kFew16x16w && N <= 8192u) launch_fused<1, 16, 4>(a, out_kind, x, (hipStream_t)stream);
+    else launch_fused<1, 4, 8>(a, out_kind, x, (hipStream_t)stream);
     return mi_hip((int)hipGetLastError(), "linear_w8a8");
   }
   if (int e = mi_quant_rows_i8(x, x_stride, M, K, q, qs, stream)) return e;
