@@ -4,17 +4,20 @@
 // With m = max_i x_i, d_i = x_i - m, Z = sum_i e^(d_i), T = sum_i e^(d_i) d_i over the vocabulary:
 //   log p_i = d_i - log Z,   entropy = log Z - T / Z,   rank(t) = #{i : x_i > x_t, or x_i = x_t and i < t}
 // One pass: a lane keeps its own running maximum with its Z and T in base 2 (a maximum that rises by -delta turns them into
-// Z 2^delta and (T + delta Z) 2^delta), a wave its 64 best tokens sorted over its lanes, best first. A token is better than
-// another when its logit is larger, or equal with the lower index. What beats the wave's k-th best and reaches the
-// work-group's bound is put in: few at once by a shift of the lanes behind its place, many at once as a sorted 64 merged
-// with the list. The bound: with W waves each publishes its ceil(k / W)-th best, and k logits reach the least of these,
-// which is close to the k-th best of all. In the first step a wave takes it from its lanes' maxima, so that of the first
-// 4096 tokens hardly more than k go into a list (each wave by its own k-th best alone put in four times as many).
+// Z 2^delta and (T + delta Z) 2^delta). A token is better than another when its logit is larger, or equal with the lower
+// index.
+// Many rows, one work-group each: a wave keeps its 64 best tokens sorted over its lanes, best first. What beats the wave's
+// k-th best and reaches the work-group's bound is put in: few at once by a shift of the lanes behind its place, many at once
+// as a sorted 64 merged with the list. The bound: with W waves each publishes its ceil(k / W)-th best, and k logits reach
+// the least of these, which is close to the k-th best of all. In the first step a wave takes it from its lanes' maxima, so
+// that of the first 4096 tokens hardly more than k go into a list (each wave by its own k-th best alone put in four times
+// as many). Few rows are cut into slices, which leave their statistics and the largest logit of each 256 tokens; a second
+// launch joins them and reads again the few runs that can hold one of the k best.
 // What bounds it: the memory's stream, with the vector ALUs close behind (about ten instructions per logit); few rows are
 // bound by their two launches' chains of loads. Each wave's next 4 KiB are loaded ahead of the work on the present ones.
-// Measured (MI355X, vocabulary 151936): 2048 rows with the 20 best 323 -> 271 us by the bound (-30) and the loads ahead (-22), 246
-// with the 5 best, 234 with none (5.3 TB/s; a plain read of those bytes 6.7); 333 rows with 5 66 -> 55; one row with 20
-// 33 -> 18.7 in 149 slices (the lanes' statistics by one wave maximum, eight waves in the join, its loads all at its start).
+// Measured (MI355X, vocabulary 151936): 2048 rows with the 20 best 323 -> 271 us by the bound (-30) and the loads ahead
+// (-22), 245 with the 5 best, 232 with none (5.4 TB/s; a plain read of those bytes 6.7); 333 rows with 5 66 -> 52.5; one
+// row with 20 33 -> 12.0 in 149 slices.
 #include <algorithm>
 #include <type_traits>
 
@@ -31,12 +34,12 @@ struct LogprobArgs {
   const float* logits;
   size_t row_stride;
   const uint32_t* tokens;
-  uint32_t vocab, top, slices, slice;  // `slice` tokens each, a multiple of 4
+  uint32_t vocab, top, slices, slice;  // `slice` tokens each; a multiple of 1024 where there are several
   float *logprob, *entropy, *top_logprobs;
   uint32_t *rank, *top_ids;
-  // per (row, slice): (m, Z, T, count) and `top` (value, id) pairs
+  // where a row has several slices: (m, Z, T, count) per (row, slice), the largest logit per (row, 256 tokens)
   f4_t* stats;
-  u2_t* lists;
+  float* peaks;
 };
 
 // ---- the statistics ----
@@ -184,8 +187,10 @@ __device__ __forceinline__ bool join_waves(Joint<W>& j, Stats& s, uint32_t& coun
       j.t[wave] = s.t;
       j.count[wave] = count;
     }
-    j.v[wave][lane] = list.v;
-    j.id[wave][lane] = list.id;
+    if (top) {
+      j.v[wave][lane] = list.v;
+      j.id[wave][lane] = list.id;
+    }
     __syncthreads();
     if (wave >= step) return false;
     Stats o;
@@ -203,22 +208,37 @@ __device__ __forceinline__ float token_logit(const LogprobArgs& a, uint32_t row,
   const uint32_t t = *token = a.tokens ? a.tokens[row] : kNone;
   return t < a.vocab ? a.logits[(size_t)row * a.row_stride + t] : __builtin_bit_cast(float, kNanBits);
 }
-// the row's answers, from its whole statistics and list and its token's logit (one wave)
-__device__ __forceinline__ void answer(const LogprobArgs& a, uint32_t row, const Stats& s, uint32_t count, Entry list, float xt,
+// the row's answers, from its whole statistics (log_z = logf(s.z)) and its token's logit
+__device__ __forceinline__ void answer(const LogprobArgs& a, uint32_t row, const Stats& s, uint32_t count, float log_z, float xt,
                                        uint32_t lane) {
-  const float log_z = logf(s.z);
-  if (lane == 0) {
-    if (a.entropy) a.entropy[row] = log_z - s.t / s.z * kLn2;
-    if (a.logprob) a.logprob[row] = (xt - s.m) - log_z;
-    if (a.rank) a.rank[row] = xt != xt ? kNone : count;
-  }
-  if (lane < a.top) {
-    a.top_ids[(size_t)row * a.top + lane] = list.id;
-    a.top_logprobs[(size_t)row * a.top + lane] = list.id == kNone ? -INFINITY : (list.v - s.m) - log_z;
-  }
+  if (lane != 0) return;
+  if (a.entropy) a.entropy[row] = log_z - s.t / s.z * kLn2;
+  if (a.logprob) a.logprob[row] = (xt - s.m) - log_z;
+  if (a.rank) a.rank[row] = xt != xt ? kNone : count;
+}
+__device__ __forceinline__ void answer_top(const LogprobArgs& a, uint32_t row, uint32_t place, Entry e, const Stats& s, float log_z) {
+  a.top_ids[(size_t)row * a.top + place] = e.id;
+  a.top_logprobs[(size_t)row * a.top + place] = e.id == kNone ? -INFINITY : (e.v - s.m) - log_z;
 }
 
-// grid (slices, rows): 4 waves walk a slice of the row's tokens, each 256 at a time
+// four values' maxima over the wave: lane 0 the first's, 32 the second's, 16 the third's, 48 the fourth's
+__device__ __forceinline__ float wave_max4(float a, float b, float c, float d) {
+  lane_swap32(a, b);
+  lane_swap32(c, d);
+  float m = fmaxf(a, b), n = fmaxf(c, d);
+  lane_swap16(m, n);
+  m = fmaxf(m, n);
+  auto with = [&](auto x) { m = fmaxf(m, __builtin_bit_cast(float, xor_lane<decltype(x)::value>(__builtin_bit_cast(uint32_t, m)))); };
+  with(std::integral_constant<uint32_t, 1>{});
+  with(std::integral_constant<uint32_t, 2>{});
+  with(std::integral_constant<uint32_t, 4>{});
+  with(std::integral_constant<uint32_t, 8>{});
+  return m;
+}
+
+// grid (slices, rows): 4 waves walk a slice of the row's tokens, each 256 at a time. LISTS: the slice is the whole row, and
+// the waves keep its best tokens; otherwise they leave the largest logit of each 256.
+template <bool LISTS>
 __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.y;
   const float* x = a.logits + (size_t)row * a.row_stride;
@@ -269,7 +289,7 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
         s.z += e;
         s.t = __builtin_fmaf(e, __builtin_elementwise_maximum(d, -1e30f), s.t);  // (-inf counts nothing)
       }
-    if (a.top) {
+    if (LISTS && a.top) {
       if (first) {
         bound.publish(wave, lane, kth_largest(all, share, lane));
         __syncthreads();
@@ -298,8 +318,13 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
         if (mine > -INFINITY) bound.publish(wave, lane, mine);
       }
     }
-    // the tokens before t count where they are equal too; t lies within one step of one wave
     const uint32_t w0 = i0 - 4u * lane;
+    if (!LISTS && a.top) {
+      const float peak = wave_max4(most[0], most[1], most[2], most[3]);
+      const uint32_t at = w0 + 1024u * ((lane >> 5) + ((lane >> 3) & 2u));
+      if ((lane & 15u) == 0 && at < end) a.peaks[(size_t)row * ((a.vocab + 255u) / 256u) + at / 256u] = peak;
+    }
+    // the tokens before t count where they are equal too; t lies within one step of one wave
     if (w0 + 1024u * (U - 1u) + 256u <= ahead) {
 #pragma unroll
       for (uint32_t u = 0; u < U; ++u)
@@ -319,80 +344,217 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
     }
   }
   __shared__ Joint<4> joint;
-  if (!join_waves<4>(joint, s, count, list, a.top, wave, lane)) return;
-  if (a.slices == 1) {
-    answer(a, row, s, count, list, xt, lane);
-    return;
-  }
-  const size_t at = (size_t)row * a.slices + blockIdx.x;
-  if (lane == 0) a.stats[at] = f4_t{s.m, s.z, s.t, (float)count};
-  if (lane < a.top) a.lists[at * a.top + lane] = u2_t{__builtin_bit_cast(uint32_t, list.v), list.id};
+  if (!join_waves<4>(joint, s, count, list, LISTS ? a.top : 0u, wave, lane)) return;
+  if constexpr (LISTS) {
+    const float log_z = logf(s.z);
+    answer(a, row, s, count, log_z, xt, lane);
+    if (lane < a.top) answer_top(a, row, lane, list, s, log_z);
+  } else if (lane == 0) a.stats[(size_t)row * a.slices + blockIdx.x] = f4_t{s.m, s.z, s.t, (float)count};
 }
 
-// one work-group of W waves per row: its slices' statistics, and their lists as one set of entries, 4 per lane at a time
-template <uint32_t W>
-__global__ __launch_bounds__(64 * W) void logprobs_join_kernel(LogprobArgs a) {
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x, n = a.slices * a.top;
+// A work-group per row of several slices: joins their statistics, and finds the best tokens among the runs of 256 whose
+// largest logit reaches a bound that k runs' reach, which it reads again: about 50 runs and 60 tokens at 151936 tokens and
+// k = 20. The bound: of runs by their largest logit, equal ones by their place, the worst of the waves' ceil(k / W)-th best
+// (k runs have a token at least as good as any token of a run behind it). A token's place among the best is the number of
+// those read that are better. Where more tokens reach the bound than fit (equal logits, or fewer finite ones than k), the
+// waves keep lists. One row of 151936 with the 20 best takes 12.0 us, 16 rows 15.7, 333 with the 5 best 52.5 (lists from
+// every slice, as a row in one has them: 18.6, 23 and 54.2); one row of equal logits 21.4 (20.9).
+__global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
+  constexpr uint32_t W = 8, U = 4, B = 8, kFit = 1024;  // waves; a lane's runs looked at together; runs read together; tokens
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x, runs = (a.vocab + 255u) / 256u;
+  const float* x = a.logits + (size_t)row * a.row_stride;
   const f4_t* stats = a.stats + (size_t)row * a.slices;
-  const u2_t* entries = a.lists + (size_t)row * n;
-  Stats s;
-  uint32_t count = 0, token;
-  Entry list, last;
-  constexpr uint32_t U = 4;
-  __shared__ Bound<W> bound;
-  __shared__ Joint<W> joint;
+  const float* peaks = a.peaks + (size_t)row * runs;
+  __shared__ union {
+    Joint<W> joint;
+    struct {
+      float v[kFit];
+      uint32_t id[kFit];
+    } fit;
+  } sm;
+  __shared__ float m[W], z[W], t[W];
+  __shared__ uint32_t counts[W], fits, place[W];
+  __shared__ float least[W];
   const uint32_t share = (a.top + W - 1u) / W;
-  float xt = 0.f;
-  for (uint32_t i0 = 0, first = 1; first || i0 < n; i0 += 64u * W * U, first = 0) {
-    u2_t p[U];
+  // (every load that the answers wait for goes out at once)
+  f4_t q = {-INFINITY, 0.f, 0.f, 0.f};
+  if (threadIdx.x < a.slices) q = stats[threadIdx.x];
+  float p[U];
+  auto load = [&](uint32_t r0) {  // run r is wave r % W's
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
-      const uint32_t i = i0 + 64u * W * u + threadIdx.x;
-      p[u] = i < n ? entries[i] : u2_t{0xFF800000u, kNone};
+      const uint32_t r = r0 + W * (64u * u + lane) + wave;
+      p[u] = r < runs ? peaks[r] : -INFINITY;
     }
-    if (first) {  // (every load that the answers wait for is out before the first entry is looked at)
-      f4_t q = {-INFINITY, 0.f, 0.f, 0.f};
-      if (threadIdx.x < a.slices) q = stats[threadIdx.x];
-      xt = token_logit(a, row, &token);
-      float all = -INFINITY;
+  };
+  if (a.top) load(0);
+  uint32_t token;
+  const float xt = token_logit(a, row, &token);
+  if (threadIdx.x == 0) fits = 0;
+  if (a.top) {  // this wave's share of the bound, each lane with the best of its runs
+    float v = p[0], low = -INFINITY;
+    uint32_t run = W * lane + wave, worst = 0;
 #pragma unroll
-      for (uint32_t u = 0; u < U; ++u) all = fmaxf(all, __builtin_bit_cast(float, p[u].x));
-      if (a.top) {
-        bound.publish(wave, lane, kth_largest(all, share, lane));
-        if constexpr (W > 1) __syncthreads();
+    for (uint32_t u = 1; u < U; ++u)
+      if (p[u] > v || v != v) {
+        v = p[u];
+        run = W * (64u * u + lane) + wave;
       }
-      s.m = q[0];
-      s.z = q[1];
-      s.t = q[2];
-      count = (uint32_t)q[3];  // (below 2^24: exact)
+    uint64_t left = __ballot(run < runs);
+#pragma unroll 1
+    for (uint32_t i = 0; i < share; ++i) {
+      const float most = wave_max(v);
+      const uint64_t who = __ballot(v == most) & left;
+      if (!who) {  // (fewer runs than the share: every token reaches the bound)
+        low = -INFINITY;
+        worst = kNone;
+        break;
+      }
+      const uint32_t l = (uint32_t)__builtin_ctzll(who), r = (uint32_t)__builtin_amdgcn_readlane((int)run, (int)l);
+      worst = i && most == low ? max(worst, r) : r;
+      low = most;
+      left &= ~(1ull << l);
+      if (lane == l) v = -INFINITY;
     }
-    if (a.top) {
-      const float cut = fmaxf(last.v, bound.get());
+    if (lane == 0) {
+      least[wave] = low;
+      place[wave] = worst;
+    }
+  }
+  __syncthreads();
+  float cut = INFINITY;
+  uint32_t last_run = 0;  // of runs whose largest logit is `cut`
+  if (a.top)
+#pragma unroll
+    for (uint32_t w = 0; w < W; ++w) {
+      last_run = least[w] < cut ? place[w] : least[w] == cut ? max(last_run, place[w]) : last_run;
+      cut = fminf(cut, least[w]);
+    }
+  // `take` gets this wave's runs that reach `cut`, each lane 4 tokens from `at` of every one
+  auto walk = [&](auto take) {
+    for (uint32_t r0 = 0;;) {
 #pragma unroll 1
       for (uint32_t u = 0; u < U; ++u) {
-        const u2_t q = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2] : p[3];
-        put(list, last, Entry{__builtin_bit_cast(float, q.x), q.y}, cut, a.top, lane);
+        const float peak = u == 0 ? p[0] : u == 1 ? p[1] : u == 2 ? p[2] : p[3];
+        const uint32_t run = r0 + W * (64u * u + lane) + wave;
+        for (uint64_t who = __ballot(run < runs && (peak > cut || (peak == cut && run <= last_run))); who;) {
+          f4_t v[B];
+          uint32_t at[B] = {}, n = 0;
+#pragma unroll
+          for (uint32_t b = 0; b < B; ++b) {
+            v[b] = f4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            if (!who) continue;
+            at[b] = 256u * (r0 + W * (64u * u + (uint32_t)__builtin_ctzll(who)) + wave) + 4u * lane;
+            who &= who - 1u;
+            n = b + 1u;
+            if (at[b] + 4u <= a.vocab) v[b] = *as_global(reinterpret_cast<const f4_any*>(x + at[b]));
+            else
+#pragma unroll
+              for (uint32_t i = 0; i < 4; ++i)
+                if (at[b] + i < a.vocab) v[b][i] = *as_global(x + at[b] + i);
+          }
+          take(v, at, n);
+        }
       }
+      r0 += 64u * W * U;
+      if (r0 >= runs) break;
+      load(r0);
     }
-  }
+  };
+  if (a.top)
+    walk([&](f4_t(&v)[B], uint32_t(&at)[B], uint32_t n) {
+#pragma unroll
+      for (uint32_t b = 0; b < B; ++b) {
+        if (b >= n) break;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+          if (v[b][i] >= cut && at[b] + i < a.vocab) {
+            const uint32_t to = atomicAdd(&fits, 1u);
+            if (to < kFit) {
+              sm.fit.v[to] = v[b][i];
+              sm.fit.id[to] = at[b] + i;
+            }
+          }
+      }
+    });
+  Stats s;
+  s.m = q[0];
+  s.z = q[1];
+  s.t = q[2];
+  uint32_t count = (uint32_t)q[3];  // (below 2^24: exact)
   for (uint32_t i = threadIdx.x + 64u * W; i < a.slices; i += 64u * W) {
-    const f4_t p = stats[i];
+    const f4_t r = stats[i];
     Stats o;
-    o.m = p[0];
-    o.z = p[1];
-    o.t = p[2];
+    o.m = r[0];
+    o.z = r[1];
+    o.t = r[2];
     s.merge(o);
-    count += (uint32_t)p[3];
+    count += (uint32_t)r[3];
   }
+  merge_lanes(s);
   count = (uint32_t)wave_sum((float)count);
-  if (join_waves<W>(joint, s, count, list, a.top, wave, lane)) answer(a, row, s, count, list, xt, lane);
+  if (lane == 0) {
+    m[wave] = s.m;
+    z[wave] = s.z;
+    t[wave] = s.t;
+    counts[wave] = count;
+  }
+  __syncthreads();
+  s = Stats{};
+  if (lane < W) {
+    s.m = m[lane];
+    s.z = z[lane];
+    s.t = t[lane];
+  }
+  merge_lanes(s);
+  count = (uint32_t)wave_sum(lane < W ? (float)counts[lane] : 0.f);
+  const float log_z = logf(s.z);
+  if (wave == 0) answer(a, row, s, count, log_z, xt, lane);
+  const uint32_t n = fits;
+  if (n <= kFit) {
+    for (uint32_t i0 = 0; i0 < n; i0 += 8u * W) {  // 8 lanes for each
+      const uint32_t i = i0 + threadIdx.x / 8u, at = min(i, n - 1u);
+      const Entry e = {sm.fit.v[at], sm.fit.id[at]};
+      uint32_t place = 0;
+#pragma unroll 4
+      for (uint32_t o = lane & 7u; o < n; o += 8u) place += better(Entry{sm.fit.v[o], sm.fit.id[o]}, e) ? 1u : 0u;
+      place += xor_lane<1>(place);
+      place += xor_lane<2>(place);
+      place += xor_lane<4>(place);
+      if (i < n && place < a.top && (lane & 7u) == 0) answer_top(a, row, place, e, s, log_z);
+    }
+    for (uint32_t i = n + threadIdx.x; i < a.top; i += 64u * W) answer_top(a, row, i, Entry{}, s, log_z);  // (no such token)
+    return;
+  }
+  Entry list, last;
+  load(0);
+  walk([&](f4_t(&v)[B], uint32_t(&at)[B], uint32_t n) {
+#pragma unroll 1
+    for (uint32_t b = 0; b < n; ++b) {  // (the first; the others move up)
+#pragma unroll 1
+      for (uint32_t i = 0; i < 4; ++i) {
+        const float e = i == 0 ? v[0][0] : i == 1 ? v[0][1] : i == 2 ? v[0][2] : v[0][3];
+        put(list, last, Entry{e, at[0] + i < a.vocab ? at[0] + i : kNone}, cut, a.top, lane);
+      }
+#pragma unroll
+      for (uint32_t c = 0; c + 1u < B; ++c) {
+        v[c] = v[c + 1u];
+        at[c] = at[c + 1u];
+      }
+      cut = fmaxf(cut, last.v);
+    }
+  });
+  __syncthreads();  // (the waves have read `fits`; what it counted is written over)
+  Stats none;
+  if (!join_waves<W>(sm.joint, none, count, list, a.top, wave, lane)) return;
+  if (lane < a.top) answer_top(a, row, lane, list, s, log_z);
 }
 
 // The slices of a row: one where the rows alone fill the chip.
 void pick_slices(uint32_t M, uint32_t vocab, uint32_t* slices, uint32_t* slice) {
   const uint32_t want = std::max(1u, 1024u / M), most = (vocab + 1023u) / 1024u;
   const uint32_t n = std::min(want, most);
-  *slice = ((vocab + n - 1u) / n + 3u) / 4u * 4u;
+  *slice = n == 1 ? vocab : ((vocab + n - 1u) / n + 1023u) / 1024u * 1024u;
   *slices = (vocab + *slice - 1u) / *slice;
 }
 
@@ -407,7 +569,7 @@ size_t mi_logprobs_ws(uint32_t M, uint32_t vocab_used, uint32_t top) {
   if (M == 0 || vocab_used == 0) return 0;
   uint32_t slices, slice;
   pick_slices(M, vocab_used, &slices, &slice);
-  return slices == 1 ? 0 : (size_t)M * slices * (16u + 8u * (size_t)top);
+  return slices == 1 ? 0 : (size_t)M * (16u * (size_t)slices + (top ? (vocab_used + 255u) / 256u * 4u : 0u));
 }
 
 int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, uint32_t M, uint32_t vocab_used,
@@ -430,12 +592,15 @@ int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, 
   pick_slices(M, vocab_used, &a.slices, &a.slice);
   if (need) {
     a.stats = static_cast<f4_t*>(ws);
-    a.lists = reinterpret_cast<u2_t*>(a.stats + (size_t)M * a.slices);
+    a.peaks = reinterpret_cast<float*>(a.stats + (size_t)M * a.slices);
   }
   hipStream_t st = (hipStream_t)stream;
-  logprobs_kernel<<<dim3(a.slices, M), 256, 0, st>>>(a);
-  if (a.slices > 8) logprobs_join_kernel<8><<<M, 512, 0, st>>>(a);
-  else if (a.slices > 1) logprobs_join_kernel<1><<<M, 64, 0, st>>>(a);
+  if (a.slices == 1) {
+    logprobs_kernel<true><<<dim3(1, M), 256, 0, st>>>(a);
+  } else {
+    logprobs_kernel<false><<<dim3(a.slices, M), 256, 0, st>>>(a);
+    logprobs_join_kernel<<<M, 512, 0, st>>>(a);
+  }
   return mi_hip((int)hipGetLastError(), "logprobs");
 }
 

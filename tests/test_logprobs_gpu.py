@@ -104,6 +104,38 @@ def test_against_the_definition(M, n, top, kind):
         check_row(x[r, :n], int(tokens[r]), top, got, r)
 
 
+@pytest.mark.parametrize("kind", ["normal", "ties", "flat", "falling", "rising", "few", "last", "nan"])
+@pytest.mark.parametrize("M,n,top", [(1, 700001, 20), (2, 530000, 64), (1, 151936, 33), (3, 2500, 64), (1, 1 << 23, 5)])
+def test_best_tokens_of_a_cut_row(M, n, top, kind):
+    """rows in slices: the best tokens come from few runs, from runs of equal logits, from all of them"""
+    rng = np.random.default_rng(n + top)
+    x = rng.normal(0, 2, (M, n)).astype(np.float32)
+    if kind == "ties":
+        x = np.round(x)
+    elif kind == "flat":
+        x[:] = -1.5
+    elif kind == "falling":
+        x = -np.sort(-x, 1)
+    elif kind == "rising":
+        x = np.sort(x, 1)
+    elif kind == "few":  # fewer finite than asked, at the end
+        x[:, :n - 3] = -np.inf
+    elif kind == "last":  # equal ones but for the last, and one large
+        x[:] = 0
+        x[:, n - 1] = 1
+    elif kind == "nan":  # a NaN is behind every token, the others keep their places
+        x[:, ::3] = np.nan
+        x[:, :1024] = np.nan
+    tokens = rng.integers(0, n, M)
+    got = call(x, tokens, n, top)
+    for r in range(M):
+        if kind != "nan":
+            check_row(x[r, :n], int(tokens[r]) if x[r, tokens[r]] > -np.inf else None, top, got, r)
+        else:
+            order = np.lexsort((np.arange(n), np.where(np.isnan(x[r]), np.inf, -x[r])))[:min(top, int((~np.isnan(x[r])).sum()))]
+            assert np.array_equal(got["ids"][r][:len(order)], order.astype(np.uint32))
+
+
 @pytest.mark.parametrize("n", [7, 5000, 70001])
 def test_rows_without_finite_answers(n):
     rng = np.random.default_rng(n)
