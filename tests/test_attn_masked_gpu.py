@@ -263,3 +263,45 @@ def test_other_stream_and_replayed_graph():
             g.replay()
             want, tol = c.exact()
             assert np.all(np.abs(c.result(b).astype(np.float64) - want) <= tol)
+
+
+@pytest.mark.parametrize("T,keys,qh,kvh,hd", [(400, 3000, 16, 2, 256), (40, 6000, 16, 2, 256), (25, 9000, 20, 4, 128), (300, 4000, 32, 8, 128)])
+@pytest.mark.parametrize("page,cap,slopes,by_row", [(0, 0.0, False, False), (64, 30.0, True, False), (24, 0.0, True, True)])
+def test_chunks_behind_a_long_text(T, keys, qh, kvh, hd, page, cap, slopes, by_row):
+    """chunks whose keys are split into few and into many parts, with either width of a work-group"""
+    before = keys - T
+    lo, hi = documents(T, before, [0, T // 3, T // 2], given=9, padded=2)
+    c = Case(T + keys, T, keys, qh, kvh, hd, cap=cap, slopes=slopes, page=page)
+    c.check(by_row=by_row)
+    c = Case(T + keys + 1, T, keys, qh, kvh, hd, cap=cap, slopes=slopes, page=page, lo=lo, hi=hi, prefix=before - 77)
+    got = c.check(by_row=by_row)
+    assert not got[T - 2:].any()
+
+
+class FarCase(Case):
+    """a cache whose last rows lie past 2^32 bytes, its first ones never written"""
+
+    def place(self, x, by_row):
+        T = torch()
+        if self.page:  # head-major pages
+            rows = self.n_pages * self.page
+            j = np.arange(self.keys)
+            at = self.order[j // self.page].astype(np.int64) * self.page + j % self.page
+            strides = (self.hd, rows * self.hd)
+        else:  # rows far apart
+            at, strides = np.arange(self.keys, dtype=np.int64), (1 << 23, self.hd)
+        c = T.empty(int(at.max() * strides[0] + (self.kvh - 1) * strides[1] + self.hd), dtype=T.int16, device="cuda")
+        view = c.as_strided((int(at.max()) + 1, self.kvh, self.hd), (strides[0], strides[1], 1))
+        view[T.from_numpy(at).cuda()] = T.from_numpy(np.ascontiguousarray(x.transpose(1, 0, 2)).view(np.int16)).cuda()
+        return c, strides
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("T", [1, 50])
+@pytest.mark.parametrize("page", [0, 64])
+def test_offsets_past_32_bits(T, hd, page):
+    c = FarCase(T + hd, T, 600, 8, 2, hd, page=page)
+    if page:
+        c.n_pages = 150000
+        c.order = (c.n_pages - 1 - 997 * np.arange(10)).astype(np.uint32)
+    c.check()
