@@ -92,7 +92,7 @@ def test_attention_refusals():
     for kw in ({"q": None}, {"k": None}, {"v": None}, {"out": None}, {"sh_ref": False}, {"mask_ref": False}, {"k": P + 8}, {"v": P + 2},
                {"q": P + 2}, {"out": P + 1}, {"rs": 132}, {"hs": (1 << 20) + 4}, {"pages": P, "page": 0, "n_pages": 5},
                {"pages": P, "page": 64, "n_pages": 0}, {"ws": None}, {"ws": P + 4}, {"nb": need - 1}, {"sh": shape(act=2)},
-               {"mask": mi.AttnMask(cap=-1.0)}, {"mask": mi.AttnMask(cap=float("nan"))}, {"mask": mi.AttnMask(cap=float("inf"))}):
+               {"mask": mi.AttnMask(cap=-1.0)}, {"mask": mi.AttnMask(cap=float("nan"))}, {"mask": mi.AttnMask(cap=float("inf"))}, {"mask": mi.AttnMask(cap=1e-30)}):
         assert attn(**kw) == ARG, kw
         assert b"attn_masked" in L.mi_last_error()
     for kw in ({"T": 0}, {"T": 65536}, {"kv_len": 0}, {"kv_len": (1 << 30) + 1}, {"sh": shape(hd=64)}, {"sh": shape(40, 7)}, {"sh": shape(40, 0)},
