@@ -267,22 +267,21 @@ __device__ __forceinline__ void load_fragment(uint32_t lds, const u4_t* from, ui
 // Many rows: WM x WN waves of 16 RM rows x 16 CN columns, KS times over the parts of k. Both operands go into LDS in
 // fragment order, by direct loads into a ring of NS chunks, and from there into registers a chunk ahead of the products.
 // A is the weights: a lane ends with four adjacent columns of a row.
-template <bool F32, uint32_t RM, uint32_t CN, uint32_t WM, uint32_t WN, uint32_t KS, uint32_t NS>
-__global__ __launch_bounds__(64 * WM * WN * KS, 2) void gemm_w8a8_kernel(GemmArgs a, uint32_t m_tiles) {
-  constexpr uint32_t TM = RM * WM, TN = CN * WN, TT = TM + TN;  // 16-row and 16-column tiles of the work-group
-  constexpr uint32_t PW = WM * WN;                              // waves of a part
-  constexpr uint32_t L = (TT + PW - 1) / PW;                    // fragments a wave loads per chunk
-  constexpr uint32_t kSums = KS > 1 ? (KS - 1) * RM * CN * PW * 64 : 1;  // 16-byte pieces of the other parts' sums
-  __shared__ __align__(16) union {
+template <uint32_t RM, uint32_t CN, uint32_t WM, uint32_t WN, uint32_t KS, uint32_t NS>
+struct Stage {
+  static constexpr uint32_t TM = RM * WM, TN = CN * WN, TT = TM + TN;  // 16-row and 16-column tiles of the work-group
+  union {
     u4_t stage[KS][NS][TT][64];
-    i4_t sums[kSums];
-  } sm;
-  // An XCD takes a run of column tiles with all their row tiles (the rows fastest): what it holds in its L2 at a time is
-  // shared by the work-groups it runs at a time.
-  const uint32_t per = gridDim.x / 8u, id = (blockIdx.x & 7u) * per + (blockIdx.x >> 3);
+    i4_t sums[KS > 1 ? (KS - 1) * RM * CN * WM * WN * 64 : 1];  // the other parts' sums
+  };
+};
+// the work-group's share from the 16-row tile m0 and the 16-column tile n0 on
+template <bool F32, uint32_t RM, uint32_t CN, uint32_t WM, uint32_t WN, uint32_t KS, uint32_t NS>
+__device__ __forceinline__ void multiply_tile(const GemmArgs& a, Stage<RM, CN, WM, WN, KS, NS>& sm, uint32_t m0, uint32_t n0) {
+  constexpr uint32_t TM = RM * WM, TN = CN * WN, TT = TM + TN;
+  constexpr uint32_t PW = WM * WN;            // waves of a part
+  constexpr uint32_t L = (TT + PW - 1) / PW;  // fragments a wave loads per chunk
   const uint32_t nt = a.N / 16u, mt = (a.M + 15u) / 16u, nc = a.K / 64u;
-  const uint32_t m0 = id % m_tiles * TM, n0 = id / m_tiles * TN;
-  if (n0 >= nt) return;
   const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const uint32_t ks = wave / PW, pw = wave % PW, wm = pw / WN, wn = pw % WN;
   // this wave's fragments of a chunk: tile ft of the rows, then the columns (a tile behind the matrix is its last one, and
@@ -385,10 +384,47 @@ __global__ __launch_bounds__(64 * WM * WN * KS, 2) void gemm_w8a8_kernel(GemmArg
   }
 }
 
+// An XCD takes a run of column tiles with all their row tiles (the rows fastest): what it holds in its L2 at a time is
+// shared by the work-groups it runs at a time. The id-th of `count` (a multiple of 8) work-groups' place in these runs:
+__device__ __forceinline__ uint32_t in_runs(uint32_t id, uint32_t count) { return (id & 7u) * (count / 8u) + (id >> 3); }
+template <bool F32, uint32_t RM, uint32_t CN, uint32_t WM, uint32_t WN, uint32_t KS, uint32_t NS>
+__global__ __launch_bounds__(64 * WM * WN * KS, 2) void gemm_w8a8_kernel(GemmArgs a, uint32_t m_tiles) {
+  __shared__ __align__(16) Stage<RM, CN, WM, WN, KS, NS> sm;
+  const uint32_t id = in_runs(blockIdx.x, gridDim.x), n0 = id / m_tiles * (CN * WN);
+  if (n0 < a.N / 16u) multiply_tile<F32, RM, CN, WM, WN, KS, NS>(a, sm, id % m_tiles * (RM * WM), n0);
+}
+// 256 x 256 where half a round of the CUs' tiles or less is left behind the whole rounds: those are cut into quarters of
+// 128 x 128, which take half a tile's time, all CUs at once. Measured (us; without): 1000 rows 5120 -> 34816, 544 tiles, 168
+// (194); 2048 rows 5120 -> 34816, 1088 tiles, 318 (344); 1000 rows 5120 -> 22528, 352 tiles, 123 (127); 500 rows
+// 5120 -> 151936, 1188 tiles with 164 behind the whole rounds, 390 (381).
+template <bool F32>
+__global__ __launch_bounds__(512, 2) void gemm_w8a8_quarters_kernel(GemmArgs a, uint32_t m_tiles, uint32_t whole) {
+  __shared__ __align__(16) union {
+    Stage<8, 4, 2, 4, 1, 4> whole;
+    Stage<4, 2, 2, 4, 1, 8> quarter;
+  } sm;
+  if (blockIdx.x < whole) {
+    const uint32_t id = in_runs(blockIdx.x, whole);
+    multiply_tile<F32, 8, 4, 2, 4, 1, 4>(a, sm.whole, id % m_tiles * 16u, id / m_tiles * 16u);
+  } else {
+    const uint32_t q = in_runs(blockIdx.x - whole, gridDim.x - whole), id = whole + q / 4u;
+    const uint32_t m0 = id % m_tiles * 16u + 8u * (q & 1u), n0 = id / m_tiles * 16u + 4u * (q & 2u);
+    if (n0 < a.N / 16u && 16u * m0 < a.M) multiply_tile<F32, 4, 2, 2, 4, 1, 8>(a, sm.quarter, m0, n0);
+  }
+}
+
 template <bool F32, uint32_t RM, uint32_t CN, uint32_t WM, uint32_t WN, uint32_t KS, uint32_t NS>
 void launch_tiles(const GemmArgs& a, hipStream_t st) {
   const uint32_t m_tiles = (a.M + 16u * RM * WM - 1u) / (16u * RM * WM), n_tiles = (a.N + 16u * CN * WN - 1u) / (16u * CN * WN);
   gemm_w8a8_kernel<F32, RM, CN, WM, WN, KS, NS><<<(m_tiles * n_tiles + 7u) / 8u * 8u, 64 * WM * WN * KS, 0, st>>>(a, m_tiles);
+}
+uint32_t tiles_256(uint32_t M, uint32_t N) { return (M + 255u) / 256u * ((N + 255u) / 256u); }
+bool in_quarters(uint32_t tiles) { return tiles >= 256u && tiles % 256u != 0 && tiles % 256u <= 128u; }
+template <bool F32>
+void launch_256(const GemmArgs& a, hipStream_t st) {
+  const uint32_t tiles = tiles_256(a.M, a.N), rest = tiles % 256u;
+  if (!in_quarters(tiles)) return launch_tiles<F32, 8, 4, 2, 4, 1, 4>(a, st);
+  gemm_w8a8_quarters_kernel<F32><<<tiles - rest + (4u * rest + 7u) / 8u * 8u, 512, 0, st>>>(a, (a.M + 255u) / 256u, tiles - rest);
 }
 template <bool F32, uint32_t MT, uint32_t NT, uint32_t W, uint32_t U>
 void launch_few(const GemmArgs& a, hipStream_t st) {
@@ -405,12 +441,13 @@ void launch_fused(const GemmArgs& a, uint32_t out_kind, const uint16_t* x, hipSt
 // The work-group's shape by the least modelled time in ns,
 //   launch + turn r + step s c + work w s / 256 + weights K N / 10^6 + out M N / 10^6
 // with w work-groups, s = K / (64 parts) steps of each, c = ceil(w / 256) work-groups a CU runs and r of them one after
-// another (`occ` fit a CU at once). The constants were fitted to every shape's times at 790 random sizes (1..2048 rows,
-// K 256..17408, N 256..151936; a fifth of them this library's layers): the choice is 2.8 % off the best shape on average.
+// another (`occ` fit a CU at once); a last round in quarters counts 0.52 in c for up to 64 tiles, 0.95 for up to 128. The
+// constants were fitted to every shape's times at 790 random sizes (1..2048 rows, K 256..17408, N 256..151936; a fifth of
+// them this library's layers): the choice is 2.8 % off the best shape on average.
 // Measured (us; the chosen shape, then others) at K -> N:
 //   5120 -> 7168:   1 row 7.4 (16 x 16, 16 parts), 16 x 32 8.3, 64 x 64 10.3; 128 rows 12.3 (64 x 64, 4 parts), 64 x 32 18.8, 128 x 128 21.6;
 //                   1000 rows 38.8 (128 x 256), 128 x 128 41.0, 256 x 256 55.6
-//   5120 -> 34816:  13 rows 30.4 (16 x 32), 16 x 16 32.7; 128 rows 54.3 (128 x 256), 64 x 128 69.5; 2048 rows 329 (256 x 256), 128 x 256 385
+//   5120 -> 34816:  13 rows 30.4 (16 x 32), 16 x 16 32.7; 128 rows 54.3 (128 x 256), 64 x 128 69.5; 2048 rows 318 (256 x 256), 128 x 256 381
 //   17408 -> 5120:  333 rows 53.8 (64 x 128), 64 x 64 67.0, 128 x 256 107; 1000 rows 106 (192 x 256), 128 x 256 111
 //   5120 -> 151936: 500 rows 374 (256 x 256), 128 x 256 453
 enum Shape { kFew16x16, kFew16x16w, kFew16x32, kFew32x32, kFew64x16, kTile64p4, kTile64, kTile64x128, kTile128, kTile128x256, kTile192x256, kTile256 };
@@ -437,7 +474,9 @@ Shape pick(uint32_t M, uint32_t K, uint32_t N) {
     if (M > s.most) continue;
     const uint64_t w = (uint64_t)((M + s.rows - 1u) / s.rows) * ((N + s.cols - 1u) / s.cols);
     const double steps = (K / 64u + s.parts - 1u) / s.parts;
-    const double t = s.launch + s.turn * (double)((w + 256u * s.occ - 1u) / (256u * s.occ)) + s.step * steps * (double)((w + 255u) / 256u) +
+    const double rounds = s.shape == kTile256 && in_quarters((uint32_t)w) ? (double)(w / 256u) + (w % 256u <= 64u ? 0.52 : 0.95)
+                                                                          : (double)((w + 255u) / 256u);
+    const double t = s.launch + s.turn * (double)((w + 256u * s.occ - 1u) / (256u * s.occ)) + s.step * steps * rounds +
                      s.work * steps * (double)w / 256.0 + s.weights * 1e-6 * K * N + s.out * 1e-6 * M * N;
     if (t < least) {
       least = t;
@@ -461,7 +500,7 @@ void launch_shape(Shape p, const GemmArgs& a, hipStream_t st) {
     case kTile128: return launch_tiles<F32, 4, 4, 2, 2, 1, 5>(a, st);
     case kTile128x256: return launch_tiles<F32, 4, 4, 2, 4, 1, 6>(a, st);
     case kTile192x256: return launch_tiles<F32, 6, 4, 2, 4, 1, 5>(a, st);
-    case kTile256: return launch_tiles<F32, 8, 4, 2, 4, 1, 4>(a, st);
+    case kTile256: return launch_256<F32>(a, st);
   }
 }
 int launch_gemm(const GemmArgs& a, uint32_t out_kind, hipStream_t st) {

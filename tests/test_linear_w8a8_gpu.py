@@ -198,7 +198,7 @@ def test_other_stream_and_replayed_graph():
 # inside one
 WIDE = [(9, 2112, 5136), (27, 1088, 6160), (33, 5184, 7184), (61, 1088, 10256), (515, 8256, 80), (250, 64, 4112), (131, 2112, 10256),
         (333, 5184, 5136), (390, 576, 7184), (131, 64, 20496), (515, 1088, 7184), (1021, 64, 10256), (131, 2112, 34832),
-        (1500, 192, 10256), (2045, 448, 7184)]
+        (1500, 192, 10256), (2045, 448, 7184), (500, 1088, 34848), (500, 1600, 45520)]
 
 
 @pytest.mark.parametrize("M,K,N", WIDE)
