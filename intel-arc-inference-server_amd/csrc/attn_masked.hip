@@ -16,8 +16,8 @@
 //
 // What bounds it (MI355X): one row the cache's bytes, 131072 keys of 8 heads of 128 104 us, 5.2 TB/s; a chunk the matrix
 // cores, whose products are 3 per score-and-value pair (q in two parts): 2048 rows causal over 2048, 40 / 8 heads of 128,
-// 86 us; where rows see little (7 documents in 2048 rows 39.6 us, 13 of it the products that they need) a work-group's chain of
-// loads before its first tile and the tiles' unseen parts.
+// 86 us; where rows see little (7 documents in 2048 rows 39.6 us, 14 of it the bytes of q and the outputs) a work-group's
+// chain of loads before its first tile, the tiles' unseen parts, and CUs that are done before the longest document's.
 //
 // A key that a row does not see has weight 0, but 0 times an infinity or a NaN of its V row is a NaN. A block whose
 // result is not finite is therefore formed again, key by key, over the keys that each row sees.
