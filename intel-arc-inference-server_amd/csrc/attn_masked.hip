@@ -262,9 +262,11 @@ __device__ __forceinline__ void load_q(const float* qp, h8_t (&qh)[KK], h8_t (&q
 }
 
 // One step of the softmax of a wave's CT column tiles. The references first: raised, with what was formed by them, where a
-// score passes one (each column by its own four lanes, whatever its neighbours need).
+// score passes one (each column by its own four lanes, whatever its neighbours need). NT 0: the accumulators are left to
+// the caller, with their factor.
 template <uint32_t CT, uint32_t NT>
-__device__ __forceinline__ void raise(const float (&w)[CT][8], uint32_t qi, float (&r)[CT], float (&l)[CT], f4_t (&acc)[CT][NT]) {
+__device__ __forceinline__ void raise(const float (&w)[CT][8], uint32_t qi, float (&r)[CT], float (&l)[CT], f4_t (*acc)[NT ? NT : 1],
+                                      float* factor) {
   float mx[CT];
   bool over = false;
 #pragma unroll
@@ -283,6 +285,7 @@ __device__ __forceinline__ void raise(const float (&w)[CT][8], uint32_t qi, floa
     l[ct] *= alpha;
 #pragma unroll
     for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] *= alpha;
+    if constexpr (NT == 0) *factor = alpha;
   }
 }
 // Then the weights, as the B operands of P V in f16 high and low parts; their sum goes to l.
@@ -412,7 +415,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) w[0][e] = d[e / 4][e % 4];
     scores(a, col, key + 4u * qq, b.masked(a, key), w[0]);
-    raise<1, NT>(w, qi, r, l, acc);
+    raise<1, NT>(w, qi, r, l, acc, nullptr);
     h8_t ph, pl;
     weights(w[0], r[0], l[0], ph, pl);
 #pragma unroll
@@ -475,14 +478,20 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
 //   the products of tile i + 1's scores, dealt out among the exponentials that make tile i's weights;
 //   P V of tile i, dealt out among the scaling (and the tanh) of tile i + 1's scores, whose maxima follow.
 // So the matrix core has products while the vector ALUs work in the same wave. The halves of the dims exchange their parts
-// of the scores through LDS across the barrier.
+// of the scores through LDS across the barrier. With two column tiles each of the two waves takes the softmax of one, its
+// tile 0 (the other wave's 1): the parts of the other's scores go over, and a step later the weights and the factor of a raised
+// reference come back.
 template <int HD, int CT, bool CAP, Order ORDER>
 __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   constexpr uint32_t DS = HD / 128, KK = 4, NT = 8, KROW = HD + 8, VROW = HD + 16, THREADS = 2 * HD;
   constexpr uint32_t PPR = HD / 8, RPP = THREADS / PPR, CH = kTile / RPP;  // 16-byte pieces per row, rows per pass, passes
+  constexpr bool OWN = DS == 2 && CT == 2;
+  constexpr uint32_t SC = OWN ? 1 : CT;  // column tiles whose softmax the wave takes
   __shared__ __align__(16) struct {
     uint16_t k[2][kTile * KROW], v[2][kTile * VROW];
-    f4_t s[DS > 1 ? 2 : 1][DS > 1 ? 4 * DS : 1][2 * CT][DS > 1 ? 64 : 1];
+    f4_t s[DS > 1 ? 2 : 1][DS > 1 ? 4 * DS : 1][2 * SC][DS > 1 ? 64 : 1];
+    h8_t p[OWN ? 2 : 1][OWN ? 8 : 1][OWN ? 64 : 1];
+    float f[OWN ? 2 : 1][OWN ? 8 : 1][OWN ? 64 : 1];  // the references' factors; the sums at the end
   } st;
   // the last row blocks of a causal chunk see the most keys: they are dispatched first
   const uint32_t j = blockIdx.x, t0 = (gridDim.y - 1u - blockIdx.y) * a.rows, split = blockIdx.z;
@@ -491,14 +500,17 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   const uint32_t rows_here = min(a.rows, a.T - t0);
   const Block b = block_of(a, t0, rows_here);
   uint32_t row[CT], g[CT];
-  Column col[CT];
+  Column col[SC];
+  bool live[CT];
   f4_t qraw[CT][2 * KK];  // (converted behind the first tiles' loads)
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
-    const uint32_t p = 16u * (CT * cw + ct) + qi;
+    const uint32_t p = 16u * (CT * cw + (OWN ? ct ^ ds : ct)) + qi;
     row[ct] = p / a.gqa;
     g[ct] = p % a.gqa;
-    col[ct] = column(a, j, t0, row[ct], g[ct], rows_here);
+    const Column c = column(a, j, t0, row[ct], g[ct], rows_here);
+    live[ct] = c.live;
+    if (ct < SC) col[ct] = c;
     const float* qp = a.q + ((size_t)(t0 + (row[ct] < rows_here ? row[ct] : 0u)) * a.q_heads + j * a.gqa + g[ct]) * HD + 128u * ds + 8u * qq;
 #pragma unroll
     for (uint32_t x = 0; x < 2 * KK; ++x) qraw[ct][x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2)));
@@ -551,14 +563,16 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
     load(a.v, 0, r0, vr);
     load(a.k, 1, r1, k1);
   }
-  float r[CT], l[CT];
+  float r[SC], l[SC], factor = 1.f;
   f4_t acc[CT][NT], d[CT][2];
   h8_t qh[CT][KK], ql[CT][KK];
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
     split_q<KK>(qraw[ct], qh[ct], ql[ct]);
-    r[ct] = kNoKey;
-    l[ct] = 0.f;
+    if (ct < SC) {
+      r[ct] = kNoKey;
+      l[ct] = 0.f;
+    }
 #pragma unroll
     for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
   }
@@ -578,27 +592,28 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   auto hand_over = [&](uint32_t buf) {
     if constexpr (DS > 1) {
 #pragma unroll
-      for (uint32_t ct = 0; ct < CT; ++ct)
+      for (uint32_t ct = 0; ct < SC; ++ct)
 #pragma unroll
-        for (uint32_t gg = 0; gg < 2; ++gg) st.s[buf][wave][2 * ct + gg][lane] = d[ct][gg];
+        for (uint32_t gg = 0; gg < 2; ++gg) st.s[buf][wave][2 * ct + gg][lane] = d[OWN ? 1 : ct][gg];
     }
   };
   auto take_over = [&](uint32_t buf) {
     if constexpr (DS > 1) {
 #pragma unroll
-      for (uint32_t ct = 0; ct < CT; ++ct)
+      for (uint32_t ct = 0; ct < SC; ++ct)
 #pragma unroll
         for (uint32_t gg = 0; gg < 2; ++gg) d[ct][gg] += st.s[buf][wave ^ 4u][2 * ct + gg][lane];
     }
   };
-  float w[CT][8];
+  float w[SC][8];
   // the scores w of tile i: bias, mask, and the columns' references
   auto settle = [&](uint32_t i) {
     const uint32_t key = b.key(from + i);
     const bool masked = b.masked(a, key);
 #pragma unroll
-    for (uint32_t ct = 0; ct < CT; ++ct) bias_and_mask(a, col[ct], key + 4u * qq, masked, w[ct]);
-    raise<CT, NT>(w, qi, r, l, acc);
+    for (uint32_t ct = 0; ct < SC; ++ct) bias_and_mask(a, col[ct], key + 4u * qq, masked, w[ct]);
+    if constexpr (OWN) raise<1, 0>(w, qi, r, l, nullptr, &factor);
+    else raise<CT, NT>(w, qi, r, l, acc, nullptr);
   };
   if (n) {
     store(st.k[0], KROW, kr);
@@ -616,7 +631,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
     lds_barrier();
     take_over(0);
 #pragma unroll
-    for (uint32_t ct = 0; ct < CT; ++ct)
+    for (uint32_t ct = 0; ct < SC; ++ct)
 #pragma unroll
       for (uint32_t e = 0; e < 8; ++e) w[ct][e] = score<CAP>(a, d[ct][e / 4][e % 4]);
     settle(0);
@@ -645,10 +660,11 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
       for (uint32_t s = 0; s < S; ++s) {
         if (s + AHEAD < S) kh[s + AHEAD] = k_operand(nxt, s + AHEAD);
 #pragma unroll
-        for (uint32_t h = 0; h < CT; ++h) {  // two products, one weight
+        for (uint32_t h = 0; h < CT; ++h) {  // two products, one weight (or a weight for every four)
           product(kh[s], s, 2 * h);
           product(kh[s], s, 2 * h + 1);
-          const uint32_t x = s * CT + h, ct = x / 8, e = x % 8;
+          if (h >= SC) continue;
+          const uint32_t x = s * SC + h, ct = x / 8, e = x % 8;
           w[ct][e] = __builtin_amdgcn_exp2f(w[ct][e] - r[ct]);
           l[ct] += w[ct][e];
           if (e % 2) {
@@ -660,6 +676,10 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
         }
       }
       hand_over(nxt);
+      if constexpr (OWN) {
+        st.p[cur][wave][lane] = p[0];
+        st.f[cur][wave][lane] = factor;
+      }
     }
     lds_barrier();
     {
@@ -668,6 +688,18 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
       h8_t av[NT];
 #pragma unroll
       for (uint32_t tt = 0; tt < AHEAD; ++tt) av[tt] = v_operand<VROW>(vb, tt);
+      if constexpr (OWN) {
+        p[1] = st.p[cur][wave ^ 4u][lane];
+        const float other = st.f[cur][wave ^ 4u][lane];
+        if (__ballot(factor != 1.f || other != 1.f)) {
+#pragma unroll
+          for (uint32_t tt = 0; tt < NT; ++tt) {
+            acc[0][tt] *= factor;
+            acc[1][tt] *= other;
+          }
+        }
+        factor = 1.f;
+      }
       take_over(nxt);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -676,7 +708,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
 #pragma unroll
         for (uint32_t ct = 0; ct < CT; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[tt], p[ct], acc[ct][tt], 0, 0, 0);
 #pragma unroll
-        for (uint32_t ct = 0; ct < CT; ++ct) w[ct][tt] = score<CAP>(a, d[ct][tt / 4][tt % 4]);
+        for (uint32_t ct = 0; ct < SC; ++ct) w[ct][tt] = score<CAP>(a, d[ct][tt / 4][tt % 4]);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (i + 1u < n) settle(i + 1u);
@@ -686,29 +718,34 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   bool bad = false;
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
-    sum[ct] = col_sum(l[ct]);
-    float z = sum[ct] - sum[ct];
+    float z = 0.f;
+    if (ct < SC) {
+      sum[ct] = col_sum(l[ct]);
+      z = sum[ct] - sum[ct];
+    }
 #pragma unroll
     for (uint32_t tt = 0; tt < NT; ++tt) z = not_finite(z, acc[ct][tt]);
-    bad |= col[ct].live && z != 0.f;
+    bad |= live[ct] && z != 0.f;
   }
+  if constexpr (OWN) st.f[n & 1u][wave][lane] = sum[0];  // (the last step's are in the other half)
   if (__syncthreads_or(bad)) {
     slow_block<HD>(a, b, j, t0, rows_here, from, from + n, split);
     return;
   }
+  if constexpr (OWN) sum[1] = st.f[n & 1u][wave ^ 4u][lane];
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
     if (row[ct] >= rows_here) continue;
     if (a.splits > 1) {
 #pragma unroll
       for (uint32_t tt = 0; tt < NT; ++tt) store_part<HD>(a, j, t0 + row[ct], g[ct], split, qq, 8u * ds + tt, acc[ct][tt]);
-      if (qq == 0 && ds == 0) {
+      if (qq == 0 && (OWN ? ct == 0 : ds == 0)) {
         float* o = part_at<HD>(a, j, t0 + row[ct], g[ct], split);
-        o[HD] = r[ct];
-        o[HD + 1] = col[ct].live ? sum[ct] : 0.f;
+        o[HD] = r[ct < SC ? ct : 0];
+        o[HD + 1] = live[ct] ? sum[ct] : 0.f;
       }
     } else {
-      const float inv = col[ct].live && sum[ct] != 0.f ? 1.0f / sum[ct] : 0.f;
+      const float inv = live[ct] && sum[ct] != 0.f ? 1.0f / sum[ct] : 0.f;
 #pragma unroll
       for (uint32_t tt = 0; tt < NT; ++tt)
         store_out<HD>(a, j, t0 + row[ct], g[ct], qq, 8u * ds + tt, inv == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : acc[ct][tt] * inv);
