@@ -19,7 +19,7 @@
 #include <cstdio>
 
 #include "mi_capi_internal.h"
-#include "mi_common.h"
+#include "mi_pieces.h"
 
 namespace mi {
 namespace {

@@ -22,7 +22,7 @@
 #include <type_traits>
 
 #include "mi_capi_internal.h"
-#include "mi_common.h"
+#include "mi_pieces.h"
 
 namespace mi {
 namespace {

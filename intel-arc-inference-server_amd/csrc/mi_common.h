@@ -22,11 +22,6 @@ typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef float f2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
-// outputs are stored in pieces of several elements at the elements' own alignment
-typedef f4_t f4_any __attribute__((aligned(4)));
-typedef uint32_t h2_any __attribute__((aligned(2)));
-typedef u2_t h4_any __attribute__((aligned(2)));
-typedef u4_t h8_any __attribute__((aligned(2)));
 
 // The control block (src/runtime/control.h:13-24): the only per-token state the host
 // and the captured step share, read by the kernels at execution time.
@@ -170,19 +165,6 @@ __device__ __forceinline__ void lane_swap32(float& a, float& b) {
 __device__ __forceinline__ void lane_swap16(float (&a)[4], float (&b)[4]) { MI_SWAP4("16"); }
 __device__ __forceinline__ void lane_swap32(float (&a)[4], float (&b)[4]) { MI_SWAP4("32"); }
 #undef MI_SWAP4
-
-// (v_maximum3_f32: fmaxf would quieten each operand first, an instruction per operand)
-__device__ __forceinline__ float max3(float x, float y, float z) {
-  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x, y), z);
-}
-// the max over the four lanes l % 16 + 16 k that hold one column's scores
-__device__ __forceinline__ float col_max(float x) {
-  float a0 = x, a1 = x;
-  lane_swap16(a0, a1);
-  float b0 = __builtin_elementwise_maximum(a0, a1), b1 = b0;
-  lane_swap32(b0, b1);
-  return __builtin_elementwise_maximum(b0, b1);
-}
 
 // The 64-lane pairwise tree v[i] += v[i + st], st = 32 .. 1, whose root lands in lane 0, on the vector
 // ALUs: st = 32 and 16 by lane swaps of v with itself (halves, then rows of 16), 8 .. 1 by DPP row

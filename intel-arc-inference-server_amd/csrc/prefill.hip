@@ -56,7 +56,7 @@
 #include <string>
 
 #include "mi_capi_internal.h"
-#include "mi_common.h"
+#include "mi_pieces.h"
 
 namespace mi {
 namespace {
