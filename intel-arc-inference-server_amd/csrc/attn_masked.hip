@@ -847,21 +847,27 @@ __global__ __launch_bounds__(256) void attn_masked_join_few_kernel(MaskedArgs a,
 //   few: as many parts as fill the CUs (two work-groups each at rows of 128, one at 256), of 128 keys at least. Measured
 //   (us): one row, 40 / 8 heads of 128, 4099 keys 17.6 / 12.9 / 11.3 / 10.0 / 11.2 in 4 / 8 / 16 / 32 / 64 parts; 131072 keys
 //   105 / 100 / 103 / 110 in 32 / 64 / 128 / 256; 16 / 2 heads of 256, 65536 keys 37.6 / 31.3 / 38.3 in 64 / 128 / 256.
-//   chunk: the least modelled time over both CT and the parts s, in us. What the rows see is the device's; the model takes
-//   them for the last T of the cache and causal, so that a work-group has between (keys - T) / 32 and keys / 32 tiles:
-//     the longest, 3 + most / s tau, or all of them over the CUs, rounds (3 + mean / s tau), and for s > 1
+//   chunk: the least modelled time over both CT and the parts s, in us. With `same` keys that all rows see and up to `own` keys
+//   more, a work-group has between same / 32 and (same + own) / 32 tiles:
+//     the longest, start + most / s tau, or all of them over the CUs, rounds (start + mean / s tau), and for s > 1
 //     join = 3 + T q_heads s (head_dim + 4) 8 bytes at 3.5 TB/s
 //   with cap the work-groups that a CU holds, tau a tile's time with that many on it, and rounds between w / (256 cap), where
-//   short work-groups fill up behind long ones, and the next whole number, where all are alike. Measured (us; CT 1 then 2, in
-//   1 / 2 / 3 / 4 parts): 500 rows over 4500 keys, 32 / 8 heads of 128: 108 / 88 / 79 / 82, 148 / 88 / 81 / 71; 777 over 3778,
-//   16 / 2 of 256: 124 / 127 / 132 / 138, 165 / 102 / 125 / 112 (102 in 5); 2048 over 2048, 40 / 8 of 128: 106 / 126, 86 / 112, 16 / 2 of 256:
-//   85 / 115, 98 / 92; 333 over 333, 40 / 8 of 128: 14 / 21 / 23, 20 / 24 / 26; 20 over 4020: 87 / 50 / 36 / 30 (16 parts 18), 129 / 71 / 51 / 42.
+//   short work-groups fill up behind long ones, and the next whole number, where all are alike. What the rows see is the
+//   device's. Without `lo` the model takes them for the last T of the cache and causal (own = T). With it (documents, a
+//   window) they see less, how much is not known: the least product of that time and the one at own = 512 behind the
+//   prefix, so that neither is far from its best; the parts stay within the first's, which the workspace is for. Measured
+//   (us; CT 1 then 2, in 1 / 2 / 3 / 4 parts): 500 rows over 4500 keys, 32 / 8 heads of 128: 108 / 88 / 79 / 82, 148 / 88 / 81 / 71;
+//   777 over 3778, 16 / 2 of 256: 124 / 127 / 132 / 138, 165 / 102 / 125 / 112 (102 in 5); 2048 over 2048, 40 / 8 of 128:
+//   106 / 126, 86 / 112, 16 / 2 of 256: 85 / 115, 98 / 92; 333 over 333, 40 / 8 of 128: 14 / 21 / 23, 20 / 24 / 26; 20 over 4020:
+//   87 / 50 / 36 / 30 (16 parts 18), 129 / 71 / 51 / 42. With `lo`, over 45 shapes (2 to 12 documents, windows of 256 and
+//   1024) 3 % off the best on average, 27 % by the causal time alone: 2048 rows, 12 documents, 16 / 16 heads of 128 20.2 us (43.8 in
+//   3 parts of CT 2), 1000 rows behind 4000, 3 documents, 40 / 8 23.5 (45.1).
 struct Pick {
   bool few;
   uint32_t ct, rows, splits;
 };
 constexpr uint32_t kCus = 256;
-Pick pick(uint32_t T, uint32_t keys, uint32_t kv_heads, uint32_t gqa, uint32_t hd) {
+Pick pick(uint32_t T, uint32_t keys, uint32_t kv_heads, uint32_t gqa, uint32_t hd, const mi_attn_mask* mask = nullptr) {
   Pick p{gqa <= 16 && (uint64_t)T * gqa <= 16, 1, 0, 1};
   if (p.few) {
     p.rows = 16u / gqa;
@@ -869,27 +875,32 @@ Pick pick(uint32_t T, uint32_t keys, uint32_t kv_heads, uint32_t gqa, uint32_t h
     p.splits = std::max(1u, std::min({slots / kv_heads, (keys + 127u) / 128u, kMaxSplits}));
     return p;
   }
-  static constexpr double kTau[2][2][3] = {{{0.73, 1.15, 1.53}, {1.05, 1.45, 1.45}}, {{1.2, 1.2, 1.2}, {1.85, 1.85, 1.85}}};
-  const double most = (keys + kTile - 1u) / kTile, mean = most - std::min(T, keys) / (2.0 * kTile);
-  const double alike = (double)(keys - std::min(T, keys)) / keys;
-  double least = 1e300;
-  for (uint32_t ct = 1; ct <= 2; ++ct) {
+  static constexpr double kTau[2][2][3] = {{{0.73, 1.15, 1.53}, {1.05, 1.45, 1.45}}, {{1.2, 1.2, 1.2}, {1.5, 1.5, 1.5}}};
+  static constexpr double kStart[2][2] = {{4.0, 8.0}, {6.0, 6.0}};
+  auto time = [&](uint32_t ct, uint32_t s, uint32_t same, uint32_t own) {
     const uint32_t rows = 64u * ct / gqa, cap = hd == 128 ? 4u - ct : 1u;
-    const double* tau = kTau[hd == 256][ct - 1];
-    const uint64_t blocks = (uint64_t)kv_heads * ((T + rows - 1u) / rows);
-    for (uint32_t s = 1; s <= 64u && (s == 1 || s * 4u <= most); ++s) {
-      const uint64_t w = blocks * s;
-      const double at = tau[std::min<uint64_t>((w + kCus - 1u) / kCus, cap) - 1u];
-      const double turns = (double)w / (kCus * cap), whole = (double)((w + kCus * cap - 1u) / (kCus * cap));
-      double us = std::max(3.0 + most / s * at, (turns + (whole - turns) * alike) * (3.0 + mean / s * at));
-      if (s > 1) us += 3.0 + (double)T * (kv_heads * gqa) * s * (hd + 4) * 8.0 / 3.5e6;
-      if (us < least) {
-        least = us;
-        p.ct = ct;
-        p.rows = rows;
-        p.splits = s;
+    const double most = (same + own + kTile - 1u) / kTile, mean = most - own / (2.0 * kTile), alike = (double)same / (same + own);
+    const uint64_t w = (uint64_t)kv_heads * ((T + rows - 1u) / rows) * s;
+    const double tau = kTau[hd == 256][ct - 1][std::min<uint64_t>((w + kCus - 1u) / kCus, cap) - 1u], start = kStart[hd == 256][ct - 1];
+    const double turns = (double)w / (kCus * cap), whole = (double)((w + kCus * cap - 1u) / (kCus * cap));
+    const double us = std::max(start + most / s * tau, (turns + (whole - turns) * alike) * (start + mean / s * tau));
+    return s == 1 ? us : us + 3.0 + (double)T * (kv_heads * gqa) * s * (hd + 4) * 8.0 / 3.5e6;
+  };
+  const uint32_t tiles = (keys + kTile - 1u) / kTile, own = std::min(T, keys);
+  auto choose = [&](uint32_t most_parts, auto cost) {
+    double least = 1e300;
+    for (uint32_t ct = 1; ct <= 2; ++ct)
+      for (uint32_t s = 1; s <= most_parts && (s == 1 || s * 4u <= tiles); ++s) {
+        const double c = cost(ct, s);
+        if (c >= least) continue;
+        least = c;
+        p = Pick{false, ct, 64u * ct / gqa, s};
       }
-    }
+  };
+  choose(64u, [&](uint32_t ct, uint32_t s) { return time(ct, s, keys - own, own); });
+  if (mask && mask->lo) {
+    const uint32_t same = std::min(mask->prefix, keys), near = std::min(keys - same, 512u);
+    choose(p.splits, [&](uint32_t ct, uint32_t s) { return time(ct, s, keys - own, own) * time(ct, s, same, near); });
   }
   return p;
 }
@@ -933,7 +944,7 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
   if (!(mask->cap == 0.f || (mask->cap >= 1e-20f && mask->cap <= 1e30f)))  // (2 c / cap stays finite)
     return mi_fail(MI_ERR_ARG, "attn_masked: cap is 0 (none) or between 1e-20 and 1e30");
   const uint32_t gqa = shape->q_heads / shape->kv_heads;
-  const Pick p = pick(T, kv_len, shape->kv_heads, gqa, shape->head_dim);
+  const Pick p = pick(T, kv_len, shape->kv_heads, gqa, shape->head_dim, mask);
   const size_t need = part_bytes(p, T, shape->q_heads, shape->head_dim);
   if (need && (!ws || off(ws, 16) || ws_bytes < need))
     return mi_fail(MI_ERR_ARG, "attn_masked: the workspace is null, misaligned (16 bytes) or below mi_attn_masked_ws");
