@@ -16,7 +16,7 @@
 //
 // What bounds it (MI355X): one row the cache's bytes, 131072 keys of 8 heads of 128 104 us, 5.2 TB/s; a chunk the matrix
 // cores, whose products are 3 per score-and-value pair (q in two parts): 2048 rows causal over 2048, 40 / 8 heads of 128,
-// 86 us; where rows see little (7 documents in 2048 rows 39.6 us, 14 of it the bytes of q and the outputs) a work-group's
+// 86 us; where rows see little (7 documents in 2048 rows 36.4 us, 14 of it the bytes of q and the outputs) a work-group's
 // chain of loads before its first tile, the tiles' unseen parts, and CUs that are done before the longest document's.
 //
 // A key that a row does not see has weight 0, but 0 times an infinity or a NaN of its V row is a NaN. A block whose
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
 // So the matrix core has products while the vector ALUs work in the same wave. The halves of the dims exchange their parts
 // of the scores through LDS across the barrier. With two column tiles each of the two waves takes the softmax of one, its
 // tile 0 (the other wave's 1): the parts of the other's scores go over, and a step later the weights and the factor of a raised
-// reference come back (777 rows over 3778 keys, 16 / 2 heads, with distances: 125 -> 110 us).
+// reference come back (777 rows over 3778 keys, 16 / 2 heads, with distances, in 5 parts: 125 -> 110 us).
 template <int HD, int CT, bool CAP, Order ORDER>
 __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   constexpr uint32_t DS = HD / 128, KK = 4, NT = 8, KROW = HD + 8, VROW = HD + 16, THREADS = 2 * HD;
