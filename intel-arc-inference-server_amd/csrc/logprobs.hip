@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
 // k = 20. The bound: of runs by their largest logit, equal ones by their place, the worst of the waves' ceil(k / W)-th best
 // (k runs have a token at least as good as any token of a run behind it). A token's place among the best is the number of
 // those read that are better. Where more tokens reach the bound than fit (equal logits, or fewer finite ones than k), the
-// waves keep lists. One row of 151936 with the 20 best takes 12.0 us, 16 rows 15.7, 333 with the 5 best 52.5 (lists from
+// waves keep lists. One row of 151936 with the 20 best takes 11.8 us, 16 rows 15.9, 333 with the 5 best 53 (lists from
 // every slice, as a row in one has them: 18.6, 23 and 54.2); one row of equal logits 21.4 (20.9).
 __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
   constexpr uint32_t W = 8, U = 4, B = 8, kFit = 1024;  // waves; a lane's runs looked at together; runs read together; tokens
@@ -391,34 +391,24 @@ __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
   uint32_t token;
   const float xt = token_logit(a, row, &token);
   if (threadIdx.x == 0) fits = 0;
-  if (a.top) {  // this wave's share of the bound, each lane with the best of its runs
-    float v = p[0], low = -INFINITY;
-    uint32_t run = W * lane + wave, worst = 0;
+  if (a.top) {  // this wave's share of the bound, from the best run of each lane
+    float v = p[0];
+    uint32_t run = W * lane + wave;
 #pragma unroll
     for (uint32_t u = 1; u < U; ++u)
       if (p[u] > v || v != v) {
         v = p[u];
         run = W * (64u * u + lane) + wave;
       }
-    uint64_t left = __ballot(run < runs);
-#pragma unroll 1
-    for (uint32_t i = 0; i < share; ++i) {
-      const float most = wave_max(v);
-      const uint64_t who = __ballot(v == most) & left;
-      if (!who) {  // (fewer runs than the share: every token reaches the bound)
-        low = -INFINITY;
-        worst = kNone;
-        break;
-      }
-      const uint32_t l = (uint32_t)__builtin_ctzll(who), r = (uint32_t)__builtin_amdgcn_readlane((int)run, (int)l);
-      worst = i && most == low ? max(worst, r) : r;
-      low = most;
-      left &= ~(1ull << l);
-      if (lane == l) v = -INFINITY;
-    }
+    // its value, and of the lanes that have just that one as many as the share takes, the lowest: the last of their runs
+    const float low = kth_largest(v, share, lane);
+    const uint64_t with = __ballot(run < runs && v == low), above = __ballot(run < runs && v > low);
+    const uint32_t need = share - min(share, (uint32_t)__popcll(above));
+    const bool mine = ((with >> lane) & 1u) && (uint32_t)__popcll(with & ((1ull << lane) - 1u)) < need;
+    const float last_of = wave_max(mine ? (float)run : 0.f);
     if (lane == 0) {
       least[wave] = low;
-      place[wave] = worst;
+      place[wave] = (uint32_t)__popcll(with) < need ? kNone : (uint32_t)last_of;  // (too few: every token reaches it)
     }
   }
   __syncthreads();
