@@ -131,7 +131,7 @@ struct Column {
 __device__ __forceinline__ Column column(const MaskedArgs& a, uint32_t j, uint32_t t0, uint32_t row, uint32_t g, uint32_t rows_here) {
   const Span s = row_span(a, t0 + min(row, rows_here - 1u));
   Column c{s.lo, s.hi, s.pos, 0.f, row < rows_here && s.hi != 0u};
-  if (!c.live) {  // (it sees every key and is not written)
+  if (!c.live) {  // (it sees every key, so no tile is masked for it; zeros are stored in place of what it sums)
     c.lo = 0u;
     c.hi = 0xFFFFFFFFu;
   }
@@ -461,6 +461,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
     for (uint32_t w = 0; w < 4; ++w)
 #pragma unroll
       for (uint32_t e = 0; e < 4; ++e) v[e] = __builtin_fmaf(slab[w].part.acc[4u * tt + e][lane], f[w], v[e]);
+    if (!col.live) v = f4_t{0.f, 0.f, 0.f, 0.f};  // (what it summed may be a NaN, which no factor makes a zero)
     if (a.splits > 1) store_part<HD>(a, j, t0 + row, g, split, qq, tt, v);
     else store_out<HD>(a, j, t0 + row, g, qq, tt, v * inv);
   }
@@ -738,7 +739,8 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
     if (row[ct] >= rows_here) continue;
     if (a.splits > 1) {
 #pragma unroll
-      for (uint32_t tt = 0; tt < NT; ++tt) store_part<HD>(a, j, t0 + row[ct], g[ct], split, qq, 8u * ds + tt, acc[ct][tt]);
+      for (uint32_t tt = 0; tt < NT; ++tt)
+        store_part<HD>(a, j, t0 + row[ct], g[ct], split, qq, 8u * ds + tt, live[ct] ? acc[ct][tt] : f4_t{0.f, 0.f, 0.f, 0.f});
       if (qq == 0 && (OWN ? ct == 0 : ds == 0)) {
         float* o = part_at<HD>(a, j, t0 + row[ct], g[ct], split);
         o[HD] = r[ct < SC ? ct : 0];
