@@ -545,8 +545,8 @@ int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, 
  *   packed documents   lo = the document's first position (with prefix: a prompt that all of them share)
  *   a prompt that sees itself whole   hi = max(pos + 1, the prompt's end)
  *   padding            hi = 0
- * cap > 0 (1e-20 to 1e30): scores become cap * tanh(score / cap). slopes: slopes[h] * |pos - j| is taken off a score of
- * head h (after the cap). */
+ * cap > 0 (1e-20 to 1e30): scores become cap * tanh(score / cap), off by 2^-21 of the cap for caps up to 256 and by 2^-20 of the
+ * score above. slopes: slopes[h] * |pos - j| is taken off a score of head h (after the cap). */
 typedef struct mi_attn_mask {
   const uint32_t* lo;
   const uint32_t* hi;

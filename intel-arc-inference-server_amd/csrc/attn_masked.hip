@@ -6,7 +6,8 @@
 //   s = scale q_t . k_j;  with a cap s = cap tanh(s / cap);  with slopes s -= slope_h |p_t - j|
 //   out_t = sum_j e^s v_j / sum_j e^s, zeros for a row that sees no key.
 // Scores are formed in base 2, y = s log2(e). cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1), which costs an
-// exponential, a reciprocal and two fused operations and is off by 2^-22 cap at most, where f16 weights are off by 2^-11.
+// exponential, a reciprocal and two fused operations and is off by 2^-21 cap at most; caps above 256, where that error would pass
+// the weights' rounding, take a form whose error is the score's own.
 // A column (a row and one of its q heads) keeps a reference r and forms its weights as 2^(y - r); r is raised, and the
 // accumulators rescaled, only when a score passes it by more than 15, and then to 7 below that score: the weights
 // are f16 numbers up to 2^15, and 2^-24 of the largest is still an f16 number to eight bits, so that the many small weights of
@@ -46,6 +47,7 @@ struct MaskedArgs {
   size_t row_stride, head_stride;
   uint32_t page, page_shift, n_pages, kv_len, T, pos0, prefix, q_heads, kv_heads, gqa, rows, splits, act;
   float c, c2, cap;      // y = c s, or cap - 2 cap / (2^(c2 s) + 1) (cap here in base 2)
+  uint32_t form;         // a Cap
 };
 
 // A row's span: lo <= hi <= kv_len; hi 0: it sees nothing.
@@ -141,11 +143,24 @@ __device__ __forceinline__ Column column(const MaskedArgs& a, uint32_t j, uint32
 __device__ __forceinline__ bool sees(const MaskedArgs& a, const Column& c, uint32_t key) {
   return key < c.hi && (key >= c.lo || key < a.prefix);
 }
+// The scores' cap: none; one up to kPlainCap, by its two exponentials' form; any, by a form that a cap far above the scores
+// leaves their bits.
+enum Cap { kNoCap, kPlain, kAnyCap };
+// The plain form's error is the cap's, 2^-21 of it: at 256 2^-13 of a weight, as much as the weights' rounding to f16.
+constexpr float kPlainCap = 256.f;
 // A score in base 2, the cap applied.
-template <bool CAP>
+template <Cap CAP>
 __device__ __forceinline__ float score(const MaskedArgs& a, float s) {
-  if constexpr (CAP) return __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.c2) + 1.f), a.cap);
-  return s * a.c;
+  if constexpr (CAP == kNoCap) return s * a.c;
+  if constexpr (CAP == kPlain)
+    return __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * a.c2) + 1.f), a.cap);
+  // With u = x / cap and t = 2 u log2(e): from |u| = 1/4 on the same form at |t|, with the sign of t, its error 2^-20 of the score;
+  // below, x (1 - u^2 / 3 + 2 u^4 / 15 - 17 u^6 / 315), off by 62 u^8 / 2835 < 2^-21 of it.
+  constexpr float kU2 = 0.25f * 0.4804530139182014f;  // u^2 = (ln 2 / 2)^2 t^2
+  const float t = s * a.c2, v = t * t;
+  const float far = __builtin_fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fabsf(t)) + 1.f), a.cap);
+  const float f = __builtin_fmaf(v, __builtin_fmaf(v, -17.f / 315.f * kU2 * kU2 * kU2, 2.f / 15.f * kU2 * kU2), -1.f / 3.f * kU2);
+  return v < 0.0625f / kU2 ? s * a.c * __builtin_fmaf(v, f, 1.f) : copysignf(far, t);
 }
 // The rest for the scores of keys key0 + 16 (e / 4) + e % 4 (e < 8): the bias, and -inf for a key that the column does not
 // see.
@@ -160,15 +175,18 @@ __device__ __forceinline__ void bias_and_mask(const MaskedArgs& a, const Column&
     for (uint32_t e = 0; e < 8; ++e) w[e] = sees(a, c, key0 + 16u * (e / 4) + e % 4) ? w[e] : -INFINITY;
   }
 }
-__device__ __forceinline__ void scores(const MaskedArgs& a, const Column& c, uint32_t key0, bool masked, float (&w)[8]) {
-  if (a.cap != 0.f) {
+// (where the cap's form is not the kernel's own)
+__device__ __forceinline__ void scores_by_form(const MaskedArgs& a, float (&w)[8]) {
+  if (a.form == kAnyCap) {
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) w[e] = score<true>(a, w[e]);
+    for (uint32_t e = 0; e < 8; ++e) w[e] = score<kAnyCap>(a, w[e]);
+  } else if (a.form == kPlain) {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) w[e] = score<kPlain>(a, w[e]);
   } else {
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) w[e] = score<false>(a, w[e]);
+    for (uint32_t e = 0; e < 8; ++e) w[e] = score<kNoCap>(a, w[e]);
   }
-  bias_and_mask(a, c, key0, masked, w);
 }
 // where a split leaves column `col` of its block: HD values (sums of weight times V), then r and the weights' sum
 template <int HD>
@@ -176,10 +194,11 @@ __device__ __forceinline__ float* part_at(const MaskedArgs& a, uint32_t j, uint3
   return a.part + ((size_t)(t * a.q_heads + j * a.gqa + g) * a.splits + split) * (HD + 4);
 }
 
-// The columns of a block one by one, over the keys that they see only: a lane holds dims lane + 64 i.
-template <int HD>
+// The columns of a block one by one, over the keys that they see only: a lane holds dims lane + 64 i. `capped` makes scores in
+// base 2 of products.
+template <int HD, typename F>
 __device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, uint32_t j, uint32_t t0,
-                                           uint32_t rows_here, uint32_t from, uint32_t to, uint32_t split) {
+                                           uint32_t rows_here, uint32_t from, uint32_t to, uint32_t split, F capped) {
   constexpr uint32_t D = HD / 64;
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
   const size_t hoff = (size_t)j * a.head_stride;
@@ -203,7 +222,8 @@ __device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, 
 #pragma unroll
           for (uint32_t d = 0; d < D; ++d) s = __builtin_fmaf(q[64u * d], h2f(a.k[at + 64u * d]), s);
           float w[8] = {wave_sum(s), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          scores(a, c, key, false, w);
+          capped(w);
+          bias_and_mask(a, c, key, false, w);
           if (w[0] > r + kRaise) {
             const float to_r = w[0] - kBelow, alpha = __builtin_amdgcn_exp2f(r - to_r);
             r = to_r;
@@ -414,7 +434,8 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
     float w[1][8];
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) w[0][e] = d[e / 4][e % 4];
-    scores(a, col, key + 4u * qq, b.masked(a, key), w[0]);
+    scores_by_form(a, w[0]);
+    bias_and_mask(a, col, key + 4u * qq, b.masked(a, key), w[0]);
     raise<1, NT>(w, qi, r, l, acc, nullptr);
     h8_t ph, pl;
     weights(w[0], r[0], l[0], ph, pl);
@@ -439,7 +460,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
   mine.r[lane] = r[0];
   mine.l[lane] = l[0];
   if (__syncthreads_or(col.live && bad != 0.f)) {
-    slow_block<HD>(a, b, j, t0, rows_here, from, to, split);
+    slow_block<HD>(a, b, j, t0, rows_here, from, to, split, [&](float(&w)[8]) { scores_by_form(a, w); });
     return;
   }
   // wave w joins the dims 16 tt + .. of its quarter of the tiles
@@ -482,7 +503,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
 // of the scores through LDS across the barrier. With two column tiles each of the two waves takes the softmax of one, its
 // tile 0 (the other wave's 1): the parts of the other's scores go over, and a step later the weights and the factor of a raised
 // reference come back (777 rows over 3778 keys, 16 / 2 heads, with distances, in 5 parts: 125 -> 110 us).
-template <int HD, int CT, bool CAP, Order ORDER>
+template <int HD, int CT, Cap CAP, Order ORDER>
 __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   constexpr uint32_t DS = HD / 128, KK = 4, NT = 8, KROW = HD + 8, VROW = HD + 16, THREADS = 2 * HD;
   constexpr uint32_t PPR = HD / 8, RPP = THREADS / PPR, CH = kTile / RPP;  // 16-byte pieces per row, rows per pass, passes
@@ -730,7 +751,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   }
   if constexpr (OWN) st.f[n & 1u][wave][lane] = sum[0];  // (the last step's are in the other half)
   if (__syncthreads_or(bad)) {
-    slow_block<HD>(a, b, j, t0, rows_here, from, from + n, split);
+    slow_block<HD>(a, b, j, t0, rows_here, from, from + n, split, [&](float(&w)[8]) { w[0] = score<CAP>(a, w[0]); });
     return;
   }
   if constexpr (OWN) sum[1] = st.f[n & 1u][wave ^ 4u][lane];
@@ -754,16 +775,21 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
     }
   }
 }
-template <int HD, int CT, bool CAP>
+template <int HD, int CT, Cap CAP>
 void launch_order(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
   if (!a.pages) attn_masked_kernel<HD, CT, CAP, kContiguous><<<grid, 2 * HD, 0, st>>>(a);
   else if (a.page % kTile == 0) attn_masked_kernel<HD, CT, CAP, kWholeTiles><<<grid, 2 * HD, 0, st>>>(a);
   else attn_masked_kernel<HD, CT, CAP, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
 }
+// Caps above kPlainCap take one column tile (two do not fit the registers), in one kernel for every order of the cache: they are
+// the rare ones. Measured (us; cap 257, then 30 or 256): 2048 rows causal, 40 / 8 heads of 128 113, 99; 7 documents in them 40.2, 36.2; 500
+// rows over 4500 keys, 32 / 8 134, 119; 777 over 3778, 16 / 2 of 256 206, 157. A single row over 131072 keys 101.5, 100.4.
 template <int HD, int CT>
 void launch_chunk(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
-  if (a.cap != 0.f) launch_order<HD, CT, true>(a, grid, st);
-  else launch_order<HD, CT, false>(a, grid, st);
+  if constexpr (CT == 1)
+    if (a.form == kAnyCap) return attn_masked_kernel<HD, 1, kAnyCap, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
+  if (a.form == kPlain) launch_order<HD, CT, kPlain>(a, grid, st);
+  else launch_order<HD, CT, kNoCap>(a, grid, st);
 }
 
 // grid (q_heads, T): one column's splits. Each split's factor first, a thread each; then HD / 4 threads side by side take
@@ -946,7 +972,9 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
   if (!(mask->cap == 0.f || (mask->cap >= 1e-20f && mask->cap <= 1e30f)))  // (2 c / cap stays finite)
     return mi_fail(MI_ERR_ARG, "attn_masked: cap is 0 (none) or between 1e-20 and 1e30");
   const uint32_t gqa = shape->q_heads / shape->kv_heads;
-  const Pick p = pick(T, kv_len, shape->kv_heads, gqa, shape->head_dim, mask);
+  Pick p = pick(T, kv_len, shape->kv_heads, gqa, shape->head_dim, mask);
+  const Cap form = mask->cap == 0.f ? kNoCap : mask->cap <= kPlainCap ? kPlain : kAnyCap;
+  if (form == kAnyCap && !p.few) p = Pick{false, 1, 64u / gqa, p.splits};
   const size_t need = part_bytes(p, T, shape->q_heads, shape->head_dim);
   if (need && (!ws || off(ws, 16) || ws_bytes < need))
     return mi_fail(MI_ERR_ARG, "attn_masked: the workspace is null, misaligned (16 bytes) or below mi_attn_masked_ws");
@@ -980,6 +1008,7 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
   a.c = shape->scale * kLog2e;
   a.cap = mask->cap * kLog2e;
   a.c2 = mask->cap != 0.f ? 2.f * a.c / mask->cap : 0.f;
+  a.form = form;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid(shape->kv_heads, (T + p.rows - 1u) / p.rows, p.splits);
   const bool narrow = shape->head_dim == 128;
