@@ -561,7 +561,8 @@ typedef struct mi_attn_mask {
  * kv_len are never read. attn_out [T][q_heads * head_dim] f16 (shape->act as mi_attn_reduce); a row that sees
  * no key gives zeros. What a row does not see has no part in it, infinities and NaN included. pages: cache row
  * of key j = pages[j / page] * page + j % page, n_pages the pages that the cache holds; an entry that is not
- * below n_pages sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL), the call's outputs are then not to be
+ * below n_pages sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL) if a row sees a key of that page (pages that no row
+ * sees, behind a window or not written yet, may be absent), the call's outputs are then not to be
  * used, and nothing outside the cache is read. head_dim 128 or 256, up to 64 q heads per kv head, not gated;
  * T up to 65535. ws: mi_attn_masked_ws(T, kv_len, shape) bytes of device scratch, 16-byte aligned (NULL
  * where that is 0). */

@@ -27,7 +27,9 @@ HIP_ONLY = ["--offload-arch=gfx950", "-Xclang", "-target-feature", "-Xclang", "-
 # fp32 accumulators by the vector ALUs at once, so it too is kept out of AGPRs (no copies out of
 # them: 27B step 4.23 -> 4.13 ms, verify steps at 2..8 rows 0.5-2 % faster).
 PER_FILE = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-            "attn_masked.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],  # as attn.hip
+            # as attn.hip; loops at 64 bytes: the same loop took 98 or 107 us (500 rows over 4500 keys, 32 / 8 heads of 128) by where
+            # the code before it happened to end
+            "attn_masked.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-falign-loops=64"],
             # as attn.hip (one work-group per CU leaves 512 registers, and the accumulators then go to AGPRs and
             # back: 128 x 5120 x 34816 in 128 x 128 tiles 72.5 us against 64.2)
             "gemm_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],

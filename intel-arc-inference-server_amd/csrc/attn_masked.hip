@@ -50,7 +50,7 @@ struct MaskedArgs {
   uint32_t form;         // a Cap
 };
 
-// A row's span: lo <= hi <= kv_len; hi 0: it sees nothing.
+// A row's span: lo <= hi <= kv_len; lo == hi: it sees the prefix alone, up to hi; hi 0: it sees nothing.
 struct Span {
   uint32_t lo, hi, pos;
 };
@@ -59,15 +59,22 @@ __device__ __forceinline__ Span row_span(const MaskedArgs& a, uint32_t t) {
   s.pos = a.pos ? a.pos[t] : a.pos0 + t;
   s.hi = min(a.hi ? a.hi[t] : s.pos + 1u, a.kv_len);
   s.lo = min(a.lo ? a.lo[t] : 0u, s.hi);
-  if (s.lo == s.hi && min(a.prefix, s.hi) == 0u) s.lo = s.hi = 0u;
+  if (s.lo == s.hi) s.lo = s.hi = min(a.prefix, s.hi);
   return s;
 }
 // What a block's rows see, and the 32-key tiles that hold it: tiles [0, n_a) of the prefix, then from b0 on. Every wave
 // forms it by itself from the rows' spans, a row (or two) per lane: no barrier stands before the first loads.
 struct Block {
   uint32_t min_hi, max_lo, last;  // the last key that a row sees
+  uint32_t prefix, gap;           // the prefix's end as far as a row sees it, and how many keys behind it no row sees
   uint32_t n_a, b0, n;
   __device__ __forceinline__ uint32_t key(uint32_t i) const { return kTile * (i < n_a ? i : b0 + (i - n_a)); }
+  // A key of tile i, or where it lies outside what the rows see one of that tile that does not: a page that holds such keys alone
+  // may not be there.
+  __device__ __forceinline__ uint32_t within(uint32_t i, uint32_t k) const {
+    k = min(k, last);
+    return k - prefix < gap ? (i < n_a ? prefix - 1u : prefix + gap) : k;
+  }
   // whether some column of the block does not see some key of the tile (uniform)
   __device__ __forceinline__ bool masked(const MaskedArgs& a, uint32_t key) const {
     return key + kTile > min_hi || (key < max_lo && key + kTile > a.prefix);
@@ -89,7 +96,7 @@ __device__ __forceinline__ Block block_of(const MaskedArgs& a, uint32_t t0, uint
   for (uint32_t r = lane; r < rows_here; r += 64u) {
     const Span s = row_span(a, t0 + r);
     if (s.hi) {
-      min_lo = min(min_lo, s.lo);
+      if (s.lo < s.hi) min_lo = min(min_lo, s.lo);
       max_lo = max(max_lo, s.lo);
       min_hi = min(min_hi, s.hi);
       max_hi = max(max_hi, s.hi);
@@ -99,9 +106,10 @@ __device__ __forceinline__ Block block_of(const MaskedArgs& a, uint32_t t0, uint
   auto greater = [](uint32_t x, uint32_t y) { return max(x, y); };
   min_lo = wave_fold(min_lo, lesser);
   max_hi = wave_fold(max_hi, greater);
-  Block b{wave_fold(min_hi, lesser), wave_fold(max_lo, greater), max_hi - 1u, 0u, 0u, 0u};
+  Block b{wave_fold(min_hi, lesser), wave_fold(max_lo, greater), max_hi - 1u, min(a.prefix, max_hi), 0u, 0u, 0u, 0u};
   if (max_hi) {
-    b.n_a = (min(a.prefix, max_hi) + kTile - 1u) / kTile;
+    b.gap = max(min_lo, b.prefix) - b.prefix;
+    b.n_a = (b.prefix + kTile - 1u) / kTile;
     b.b0 = max(min_lo / kTile, b.n_a);
     const uint32_t end = (max_hi + kTile - 1u) / kTile;
     b.n = b.n_a + (end > b.b0 ? end - b.b0 : 0u);
@@ -109,16 +117,35 @@ __device__ __forceinline__ Block block_of(const MaskedArgs& a, uint32_t t0, uint
   return b;
 }
 
-// the cache row of a key below kv_len
-__device__ __forceinline__ uint32_t cache_row(const MaskedArgs& a, uint32_t key) {
+__device__ __forceinline__ uint32_t page_of(const MaskedArgs& a, uint32_t key) {
+  return a.page_shift < 32u ? key >> a.page_shift : key / a.page;
+}
+// the cache row of a key below kv_len; `outside`: its page's entry is not the cache's, and the row is the first page's
+__device__ __forceinline__ uint32_t cache_row(const MaskedArgs& a, uint32_t key, bool& outside) {
   if (!a.pages) return key;
-  const uint32_t at = a.page_shift < 32u ? key >> a.page_shift : key / a.page;
+  const uint32_t at = page_of(a, key);
   uint32_t pg = a.pages[at];
   if (pg >= a.n_pages) {
-    if (a.flag) *a.flag = MI_STATUS_BAD_PAGE;
+    outside = true;
     pg = 0u;
   }
   return pg * a.page + (key - at * a.page);
+}
+// A wave that met such an entry among the tiles from, from + step .. of its block reports it if a row sees one of the keys: the
+// tiles between the rows' spans (far apart documents in one block) are walked too.
+__device__ __forceinline__ void report_pages(const MaskedArgs& a, const Block& b, uint32_t t0, uint32_t rows_here, uint32_t from,
+                                             uint32_t to, uint32_t step) {
+  if (!a.flag) return;
+#pragma unroll 1
+  for (uint32_t i = from; i < to; i += step) {
+    const uint32_t key = b.key(i) + (threadIdx.x & (kTile - 1u));
+    if (key > b.last || a.pages[page_of(a, key)] < a.n_pages) continue;
+#pragma unroll 1
+    for (uint32_t r = 0; r < rows_here; ++r) {
+      const Span s = row_span(a, t0 + r);
+      if (key < s.hi && (key >= s.lo || key < a.prefix)) *a.flag = MI_STATUS_BAD_PAGE;
+    }
+  }
 }
 
 // The cache's order: contiguous, pages that hold whole tiles (one table entry for a tile's 32 keys), any pages.
@@ -217,7 +244,8 @@ __device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, 
 #pragma unroll 1
         for (uint32_t key = k0; key < k0 + kTile; ++key) {
           if (!sees(a, c, key)) continue;
-          const size_t at = (size_t)cache_row(a, key) * a.row_stride + hoff + lane;
+          bool outside;  // (the block's walk has reported it)
+          const size_t at = (size_t)cache_row(a, key, outside) * a.row_stride + hoff + lane;
           float s = 0.f;
 #pragma unroll
           for (uint32_t d = 0; d < D; ++d) s = __builtin_fmaf(q[64u * d], h2f(a.k[at + 64u * d]), s);
@@ -389,8 +417,12 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
 
   const size_t hoff = (size_t)j * a.head_stride;
   u4_t kr[2][KK], vr[NV];
-  // a lane's cache row: of key 16 (lane / 16 % 2) + lane % 16 of the tile (keys behind the last one read it again)
-  auto rows_of = [&](uint32_t i) { return cache_row(a, min(b.key(i) + (lane & 31u), b.last)); };
+  // a lane's cache row: of key 16 (lane / 16 % 2) + lane % 16 of the tile
+  bool outside = false;
+  auto rows_of = [&](uint32_t i) {
+    const uint32_t key = b.key(i) + (lane & 31u);
+    return a.pages ? cache_row(a, b.within(i, key), outside) : min(key, b.last);
+  };
   auto load = [&](uint32_t crow) {
 #pragma unroll
     for (uint32_t gg = 0; gg < 2; ++gg) {
@@ -428,8 +460,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
     for (uint32_t n = 0; n < NV; ++n) *reinterpret_cast<u4_t*>(vs + (RPP * n + lane / PPR) * VROW + 8u * (lane % PPR)) = vr[n];
     wave_lds_sync();
     if (i + 4u < to) {
-      load(crow);
+      const uint32_t now = crow;  // (the next rows' page is asked for before these rows are)
       if (i + 8u < to) crow = rows_of(i + 8u);
+      load(now);
     }
     float w[1][8];
 #pragma unroll
@@ -446,6 +479,7 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel
       acc[0][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pl, acc[0][tt], 0, 0, 0);
     }
   }
+  if (__ballot(outside)) report_pages(a, b, t0, rows_here, from + wave, to, 4u);
   l[0] = col_sum(l[0]);
   float bad = 0.f;
 #pragma unroll
@@ -546,16 +580,17 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
   struct Rows {
     uint32_t r[CH];
   };
+  bool outside = false;
   auto rows_of = [&](uint32_t i) {
     Rows w;
-    const uint32_t key0 = b.key(from + min(i, n - 1u));
+    const uint32_t tile = from + min(i, n - 1u), key0 = b.key(tile);
     if constexpr (ORDER == kContiguous) {
       w.r[0] = key0;
     } else if constexpr (ORDER == kWholeTiles) {
-      w.r[0] = cache_row(a, key0);
+      w.r[0] = cache_row(a, key0, outside);
     } else {
 #pragma unroll
-      for (uint32_t c = 0; c < CH; ++c) w.r[c] = cache_row(a, min(key0 + RPP * c + srow, b.last));
+      for (uint32_t c = 0; c < CH; ++c) w.r[c] = cache_row(a, b.within(tile, key0 + RPP * c + srow), outside);
     }
     return w;
   };
@@ -736,6 +771,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
       if (i + 1u < n) settle(i + 1u);
     }
   }
+  if (ORDER != kContiguous && __ballot(outside)) report_pages(a, b, t0, rows_here, from, from + n, 1u);
   float sum[CT];
   bool bad = false;
 #pragma unroll
@@ -782,8 +818,8 @@ void launch_order(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
   else attn_masked_kernel<HD, CT, CAP, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
 }
 // Caps above kPlainCap take one column tile (two do not fit the registers), in one kernel for every order of the cache: they are
-// the rare ones. Measured (us; cap 257, then 30 or 256): 2048 rows causal, 40 / 8 heads of 128 113, 99; 7 documents in them 40.2, 36.2; 500
-// rows over 4500 keys, 32 / 8 134, 119; 777 over 3778, 16 / 2 of 256 206, 157. A single row over 131072 keys 101.5, 100.4.
+// the rare ones. Measured (us; cap 257, then 30 or 256): 2048 rows causal, 40 / 8 heads of 128 120, 104; 7 documents in them 41, 38; 500
+// rows over 4500 keys, 32 / 8 138, 115; 777 over 3778, 16 / 2 of 256 214, 158. A single row over 131072 keys 99.6, 99.5.
 template <int HD, int CT>
 void launch_chunk(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
   if constexpr (CT == 1)
