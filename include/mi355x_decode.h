@@ -533,7 +533,8 @@ int mi_linear_w8a8(const uint16_t* x, size_t x_stride, const int8_t* w_tiled, co
  * of -inf has probability 0 (and counts nothing in the entropy). A NaN, a +inf or nothing but -inf in a row makes its
  * probabilities and entropy NaN, as the formulas say; a NaN is behind every token, and has the rank
  * 0xFFFFFFFF. Places past vocab_used hold the id 0xFFFFFFFF and -inf. ws: mi_logprobs_ws bytes of device
- * scratch, 16-byte aligned (NULL where that is 0). M up to 65535, vocab_used up to 2^23. */
+ * scratch, 16-byte aligned (NULL where that is 0). M up to 65535, vocab_used up to 2^23; the size asked for others
+ * is 0. */
 size_t mi_logprobs_ws(uint32_t M, uint32_t vocab_used, uint32_t top);
 int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, uint32_t M,
                 uint32_t vocab_used, uint32_t top, float* logprob, uint32_t* rank, float* entropy,

@@ -34,6 +34,7 @@ namespace {
 constexpr float kNoKey = -1e30f, kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 15.f, kBelow = 7.f;
 constexpr uint32_t kTile = 32;      // keys per step of a wave
+constexpr uint32_t kMaxRows = 65535, kMaxKeys = 1u << 30;
 
 struct MaskedArgs {
   const float* q;        // [T][q_heads][HD]
@@ -984,7 +985,7 @@ using namespace mi;
 extern "C" {
 
 size_t mi_attn_masked_ws(uint32_t T, uint32_t kv_len, const mi_attn_shape* shape) {
-  if (T == 0 || kv_len == 0 || !shape_ok(shape)) return 0;
+  if (T == 0 || T > kMaxRows || kv_len == 0 || kv_len > kMaxKeys || !shape_ok(shape)) return 0;
   return part_bytes(pick(T, kv_len, shape->kv_heads, shape->q_heads / shape->kv_heads, shape->head_dim), T, shape->q_heads,
                     shape->head_dim);
 }
@@ -998,7 +999,7 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
     return mi_fail(MI_ERR_SHAPE, "attn_masked: head_dim 128 or 256, q_heads a multiple of kv_heads, up to 64 of them each");
   if (shape->gated) return mi_fail(MI_ERR_SHAPE, "attn_masked: gated shapes are not supported");
   if (shape->act > 1) return mi_fail(MI_ERR_ARG, "attn_masked: act is 0 or 1");
-  if (T == 0 || T > 65535 || kv_len == 0 || kv_len > 1u << 30) return mi_fail(MI_ERR_SHAPE, "attn_masked: T 1..65535, kv_len 1..2^30");
+  if (T == 0 || T > kMaxRows || kv_len == 0 || kv_len > kMaxKeys) return mi_fail(MI_ERR_SHAPE, "attn_masked: T 1..65535, kv_len 1..2^30");
   if (pages && (page == 0 || n_pages == 0)) return mi_fail(MI_ERR_ARG, "attn_masked: page size or page count 0");
   if (pages && (uint64_t)page * n_pages > 0xFFFFFFFFull) return mi_fail(MI_ERR_SHAPE, "attn_masked: above 2^32 cache rows");
   if (row_stride % 8 || head_stride % 8) return mi_fail(MI_ERR_ARG, "attn_masked: KV strides must keep 8-element alignment");

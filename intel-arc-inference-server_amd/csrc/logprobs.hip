@@ -27,7 +27,7 @@
 namespace mi {
 namespace {
 
-constexpr uint32_t kMaxTop = 64, kNone = 0xFFFFFFFFu;
+constexpr uint32_t kMaxRows = 65535, kMaxVocab = 1u << 23, kMaxTop = 64, kNone = 0xFFFFFFFFu;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogprobArgs {
@@ -556,7 +556,7 @@ using namespace mi;
 extern "C" {
 
 size_t mi_logprobs_ws(uint32_t M, uint32_t vocab_used, uint32_t top) {
-  if (M == 0 || vocab_used == 0) return 0;
+  if (M == 0 || M > kMaxRows || vocab_used == 0 || vocab_used > kMaxVocab) return 0;
   uint32_t slices, slice;
   pick_slices(M, vocab_used, &slices, &slice);
   return slices == 1 ? 0 : (size_t)M * (16u * (size_t)slices + (top ? (vocab_used + 255u) / 256u * 4u : 0u));
@@ -566,7 +566,7 @@ int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, 
                 uint32_t top, float* logprob, uint32_t* rank, float* entropy, uint32_t* top_ids, float* top_logprobs,
                 void* ws, size_t ws_bytes, void* stream) {
   if (!logits || (reinterpret_cast<uintptr_t>(logits) & 3u)) return mi_fail(MI_ERR_ARG, "logprobs: null or misaligned logits");
-  if (M == 0 || M > 65535 || vocab_used == 0 || vocab_used > 1u << 23)
+  if (M == 0 || M > kMaxRows || vocab_used == 0 || vocab_used > kMaxVocab)
     return mi_fail(MI_ERR_SHAPE, "logprobs: M 1..65535, vocab_used 1..2^23");
   if (row_stride < vocab_used) return mi_fail(MI_ERR_ARG, "logprobs: row_stride below vocab_used");
   if (top > kMaxTop) return mi_fail(MI_ERR_SHAPE, "logprobs: at most 64 top tokens");
