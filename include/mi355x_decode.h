@@ -533,8 +533,8 @@ int mi_linear_w8a8(const uint16_t* x, size_t x_stride, const int8_t* w_tiled, co
  * of -inf has probability 0 (and counts nothing in the entropy). A NaN, a +inf or nothing but -inf in a row makes its
  * probabilities and entropy NaN, as the formulas say; a NaN is behind every token, and has the rank
  * 0xFFFFFFFF. Places past vocab_used hold the id 0xFFFFFFFF and -inf. ws: mi_logprobs_ws bytes of device
- * scratch, 16-byte aligned (NULL where that is 0). M up to 65535, vocab_used up to 2^23; the size asked for others
- * is 0. */
+ * scratch, 16-byte aligned (NULL where that is 0), asked for each M: fewer rows are cut into more slices, 513 and more
+ * need none. M up to 65535, vocab_used up to 2^23; the size asked for others is 0. */
 size_t mi_logprobs_ws(uint32_t M, uint32_t vocab_used, uint32_t top);
 int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, uint32_t M,
                 uint32_t vocab_used, uint32_t top, float* logprob, uint32_t* rank, float* entropy,
@@ -565,8 +565,9 @@ typedef struct mi_attn_mask {
  * below n_pages sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL) if a row sees a key of that page (pages that no row
  * sees, behind a window or not written yet, may be absent), the call's outputs are then not to be
  * used, and nothing outside the cache is read. head_dim 128 or 256, up to 64 q heads per kv head, not gated;
- * T up to 65535. ws: mi_attn_masked_ws(T, kv_len, shape) bytes of device scratch, 16-byte aligned (NULL
- * where that is 0). */
+ * T up to 65535, kv_len up to 2^30. ws: mi_attn_masked_ws(T, kv_len, shape) bytes of device scratch, 16-byte
+ * aligned (NULL where that is 0). That size never falls as T or kv_len grows, so one that was asked for the largest of both
+ * serves every smaller call; 1032 bytes times 2^18 at most. */
 size_t mi_attn_masked_ws(uint32_t T, uint32_t kv_len, const mi_attn_shape* shape);
 int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v, size_t row_stride,
                    size_t head_stride, const uint32_t* pages, uint32_t page, uint32_t n_pages,

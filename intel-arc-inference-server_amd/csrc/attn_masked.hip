@@ -920,7 +920,7 @@ __global__ __launch_bounds__(256) void attn_masked_join_few_kernel(MaskedArgs a,
 //   short work-groups fill up behind long ones, and the next whole number, where all are alike. What the rows see is the
 //   device's. Without `lo` the model takes them for the last T of the cache and causal (own = T). With it (documents, a
 //   window) they see less, how much is not known: the least product of that time and the one at own = 512 behind the
-//   prefix, so that neither is far from its best; the parts stay within the first's, which the workspace is for. Measured
+//   prefix, so that neither is far from its best, with no more parts than the first's. Measured
 //   (us; CT 1 then 2, in 1 / 2 / 3 / 4 parts): 500 rows over 4500 keys, 32 / 8 heads of 128: 108 / 88 / 79 / 82, 148 / 88 / 81 / 71;
 //   777 over 3778, 16 / 2 of 256: 124 / 127 / 132 / 138, 165 / 102 / 125 / 112 (102 in 5); 2048 over 2048, 40 / 8 of 128:
 //   106 / 126, 86 / 112, 16 / 2 of 256: 85 / 115, 98 / 92; 333 over 333, 40 / 8 of 128: 14 / 21 / 23, 20 / 24 / 26; 20 over 4020:
@@ -932,6 +932,10 @@ struct Pick {
   uint32_t ct, rows, splits;
 };
 constexpr uint32_t kCus = 256;
+// A chunk's columns times its parts, each of at least four tiles: so many in a workspace at most (138 MB at rows of 128). Where more
+// would be chosen the work-groups fill the CUs many times over without them: up to 3000 rows over 16384 keys the limit is never met.
+constexpr uint32_t kMostColumns = 1u << 18;
+uint32_t most_parts(uint32_t keys) { return std::min(64u, std::max(1u, (keys + kTile - 1u) / kTile / 4u)); }
 Pick pick(uint32_t T, uint32_t keys, uint32_t kv_heads, uint32_t gqa, uint32_t hd, const mi_attn_mask* mask = nullptr) {
   Pick p{gqa <= 16 && (uint64_t)T * gqa <= 16, 1, 0, 1};
   if (p.few) {
@@ -951,27 +955,26 @@ Pick pick(uint32_t T, uint32_t keys, uint32_t kv_heads, uint32_t gqa, uint32_t h
     const double us = std::max(start + most / s * tau, (turns + (whole - turns) * alike) * (start + mean / s * tau));
     return s == 1 ? us : us + 3.0 + (double)T * (kv_heads * gqa) * s * (hd + 4) * 8.0 / 3.5e6;
   };
-  const uint32_t tiles = (keys + kTile - 1u) / kTile, own = std::min(T, keys);
-  auto choose = [&](uint32_t most_parts, auto cost) {
+  const uint32_t own = std::min(T, keys);
+  auto choose = [&](uint32_t most, auto cost) {
     double least = 1e300;
     for (uint32_t ct = 1; ct <= 2; ++ct)
-      for (uint32_t s = 1; s <= most_parts && (s == 1 || s * 4u <= tiles); ++s) {
+      for (uint32_t s = 1; s <= most; ++s) {
         const double c = cost(ct, s);
         if (c >= least) continue;
         least = c;
         p = Pick{false, ct, 64u * ct / gqa, s};
       }
   };
-  choose(64u, [&](uint32_t ct, uint32_t s) { return time(ct, s, keys - own, own); });
+  const uint32_t parts = std::min(most_parts(keys), std::max(1u, kMostColumns / (T * kv_heads * gqa)));
+  choose(parts, [&](uint32_t ct, uint32_t s) { return time(ct, s, keys - own, own); });
   if (mask && mask->lo) {
     const uint32_t same = std::min(mask->prefix, keys), near = std::min(keys - same, 512u);
     choose(p.splits, [&](uint32_t ct, uint32_t s) { return time(ct, s, keys - own, own) * time(ct, s, same, near); });
   }
   return p;
 }
-size_t part_bytes(const Pick& p, uint32_t T, uint32_t q_heads, uint32_t hd) {
-  return p.splits == 1 ? 0 : (size_t)T * q_heads * p.splits * (hd + 4) * 4;
-}
+size_t part_bytes(uint32_t columns, uint32_t hd) { return (size_t)columns * (hd + 4) * 4; }
 bool shape_ok(const mi_attn_shape* s) {
   return s && s->kv_heads && s->q_heads && s->q_heads % s->kv_heads == 0 && s->q_heads / s->kv_heads <= 64 &&
          s->q_heads <= 1024 && (s->head_dim == 128 || s->head_dim == 256);
@@ -984,10 +987,18 @@ using namespace mi;
 
 extern "C" {
 
+// What a call of up to T rows over up to kv_len keys takes at most: of as many rows as the few-rows kernel takes, or of a chunk.
 size_t mi_attn_masked_ws(uint32_t T, uint32_t kv_len, const mi_attn_shape* shape) {
   if (T == 0 || T > kMaxRows || kv_len == 0 || kv_len > kMaxKeys || !shape_ok(shape)) return 0;
-  return part_bytes(pick(T, kv_len, shape->kv_heads, shape->q_heads / shape->kv_heads, shape->head_dim), T, shape->q_heads,
-                    shape->head_dim);
+  const uint32_t gqa = shape->q_heads / shape->kv_heads, few = std::min(T, 16u / gqa), parts = most_parts(kv_len);
+  uint32_t columns = 0;
+  if (few) {
+    const Pick p = pick(few, kv_len, shape->kv_heads, gqa, shape->head_dim);
+    if (p.splits > 1) columns = few * shape->q_heads * p.splits;
+  }
+  if (T > few && parts > 1)
+    columns = std::max(columns, (uint32_t)std::min<uint64_t>((uint64_t)T * shape->q_heads * parts, kMostColumns));
+  return part_bytes(columns, shape->head_dim);
 }
 
 int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v, size_t row_stride, size_t head_stride,
@@ -1012,7 +1023,7 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
   Pick p = pick(T, kv_len, shape->kv_heads, gqa, shape->head_dim, mask);
   const Cap form = mask->cap == 0.f ? kNoCap : mask->cap <= kPlainCap ? kPlain : kAnyCap;
   if (form == kAnyCap && !p.few) p = Pick{false, 1, 64u / gqa, p.splits};
-  const size_t need = part_bytes(p, T, shape->q_heads, shape->head_dim);
+  const size_t need = p.splits == 1 ? 0 : part_bytes(T * shape->q_heads * p.splits, shape->head_dim);
   if (need && (!ws || off(ws, 16) || ws_bytes < need))
     return mi_fail(MI_ERR_ARG, "attn_masked: the workspace is null, misaligned (16 bytes) or below mi_attn_masked_ws");
   MaskedArgs a{};

@@ -21,3 +21,16 @@ def test_sizes_that_the_calls_refuse():
             for T in (1, 20, 2048):
                 assert L.mi_attn_masked_ws(T, n, shape(*heads)) == 0
     assert L.mi_attn_masked_ws(1, 1000, None) == 0
+
+
+def test_attention_workspace_never_falls():
+    """a workspace that was asked for the largest call serves the smaller ones"""
+    L = mi.lib()
+    rows = sorted(set(list(range(1, 80)) + [int(80 * 1.13 ** i) for i in range(55)] + [777, 1000, 2048, 65535]))
+    keys = sorted(set(list(range(1, 300, 7)) + [int(300 * 1.17 ** i) for i in range(97)] + [3406, 3503, 8000, 131072, 1 << 30]))
+    assert rows[-1] == 65535 and keys[-1] == 1 << 30
+    for heads in HEADS:
+        size = [[L.mi_attn_masked_ws(T, n, shape(*heads)) for n in keys] for T in rows]
+        assert all(r == sorted(r) for r in size), heads
+        assert all(list(c) == sorted(c) for c in zip(*size)), heads
+        assert size[-1][-1] <= (1 << 18) * (heads[2] + 4) * 4
