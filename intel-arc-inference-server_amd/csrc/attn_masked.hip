@@ -31,7 +31,8 @@
 namespace mi {
 namespace {
 
-constexpr float kNoKey = -1e30f, kLog2e = 1.4426950408889634f;
+constexpr float kNoKey = -0x1.fffffep127f;  // the reference before the first key: no finite score is below it
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRaise = 15.f, kBelow = 7.f;
 constexpr uint32_t kTile = 32;      // keys per step of a wave
 constexpr uint32_t kMaxRows = 65535, kMaxKeys = 1u << 30;

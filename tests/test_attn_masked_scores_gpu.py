@@ -1,6 +1,6 @@
-"""mi_attn_masked's scores over the range that it accepts: caps from small to far above the scores. The tolerances are
-test_attn_masked_gpu.py's, but for the cap's part, which does not grow with the cap: 2^-21 of one up to 256, of larger ones 2^-20
-of the score."""
+"""mi_attn_masked's scores over the range that it accepts: caps from small to far above the scores, and scores far below zero.
+The tolerances are test_attn_masked_gpu.py's, but for the cap's part, which does not grow with the cap: 2^-21 of one up to 256,
+of larger ones 2^-20 of the score."""
 import numpy as np
 import pytest
 
@@ -45,3 +45,14 @@ def test_caps(T, keys, qh, kvh, hd, page, cap):
 def test_caps_near_large_scores(T, keys, qh, kvh, hd, cap):
     """scores up to and past the cap, where the tanh bends and where it is 1"""
     Capped(T + keys, T, keys, qh, kvh, hd, cap=cap, q_std=cap / 2).check()
+
+
+@pytest.mark.parametrize("T,keys,qh,kvh,hd", [(1, 300, 10, 2, 128), (1, 5000, 10, 2, 128), (90, 400, 10, 2, 128), (50, 130, 16, 2, 256),
+                                              (20, 4020, 40, 8, 128)])
+def test_scores_far_below_zero(T, keys, qh, kvh, hd):
+    """a bias that takes every key that a row sees below -1e30: the nearest one has it all"""
+    hi = np.arange(T) + keys - T - 20
+    c = Case(T + keys, T, keys, qh, kvh, hd, hi=hi, pos=hi + 19, slopes=True)
+    c.slopes[:] = np.float32(1e30)
+    got = c.run().astype(np.float64)
+    assert np.array_equal(got, np.repeat(c.v[:, hi - 1].transpose(1, 0, 2), qh // kvh, axis=1).astype(np.float64))
