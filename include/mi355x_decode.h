@@ -503,7 +503,7 @@ int mi_moe_prefill(const uint32_t* route, const uint16_t* x, const uint32_t* gu_
  * with masks. No counterpart in the reference, which scores nothing; the conventions are those of the
  * entries above. Each may be captured into a hipGraph: sizes and pointers are the launch's, what the
  * device arrays hold (tokens, spans, positions, pages, activations) is read at every replay. Calls that
- * overlap need workspaces of their own. ---- */
+ * overlap need workspaces of their own. Arrays are aligned to their elements at least; one that is not is refused. ---- */
 enum { MI_OUT_F32 = 0, MI_OUT_F16 = 1 };
 /* Rows of activations to 8 bits: s[m] = max_k |x[m][k]| / 127 (fp32), q = rne(x / s), as
  * mi_lm_head_int8_quantise does to a head's rows; a zero row s = 0, q = 0; a row with a value that is not

@@ -1018,6 +1018,8 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
   auto off = [](const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1u)) != 0; };
   if (off(kv_k, 16) || off(kv_v, 16) || off(attn_q, 4) || off(attn_out, 2))
     return mi_fail(MI_ERR_ARG, "attn_masked: misaligned pointer (K and V 16 bytes)");
+  if (off(pages, 4) || off(mask->lo, 4) || off(mask->hi, 4) || off(mask->pos, 4) || off(mask->slopes, 4) || off(flag, 4))
+    return mi_fail(MI_ERR_ARG, "attn_masked: misaligned pages, spans, positions, slopes or flag (4 bytes)");
   if (!(mask->cap == 0.f || (mask->cap >= 1e-20f && mask->cap <= 1e30f)))  // (2 c / cap stays finite)
     return mi_fail(MI_ERR_ARG, "attn_masked: cap is 0 (none) or between 1e-20 and 1e30");
   const uint32_t gqa = shape->q_heads / shape->kv_heads;

@@ -573,6 +573,9 @@ int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, 
   if ((logprob || rank) && !tokens) return mi_fail(MI_ERR_ARG, "logprobs: logprob and rank need tokens");
   if (top ? !top_ids || !top_logprobs : top_ids || top_logprobs)
     return mi_fail(MI_ERR_ARG, "logprobs: top_ids and top_logprobs go with top > 0");
+  for (const void* p : {(const void*)tokens, (const void*)logprob, (const void*)rank, (const void*)entropy, (const void*)top_ids,
+                        (const void*)top_logprobs})
+    if (reinterpret_cast<uintptr_t>(p) & 3u) return mi_fail(MI_ERR_ARG, "logprobs: misaligned tokens or outputs (4 bytes)");
   if (!logprob && !rank && !entropy && !top) return mi_fail(MI_ERR_ARG, "logprobs: nothing is asked");
   const size_t need = mi_logprobs_ws(M, vocab_used, top);
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < need))
