@@ -540,7 +540,7 @@ int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, 
                 uint32_t vocab_used, uint32_t top, float* logprob, uint32_t* rank, float* entropy,
                 uint32_t* top_ids, float* top_logprobs, void* ws, size_t ws_bytes, void* stream);
 /* What the rows of mi_attn_masked see, device arrays of T (slopes: q_heads). Row t stands at cache position
- * pos[t] (NULL: pos0 + t) and sees the keys j < hi[t] (NULL: pos + 1, causal) that are at or behind lo[t]
+ * pos[t] (NULL: pos0 + t; below 2^31) and sees the keys j < hi[t] (NULL: pos + 1, causal) that are at or behind lo[t]
  * (NULL: 0) or before `prefix`:
  *   a sliding window   lo = pos + 1 - window
  *   packed documents   lo = the document's first position (with prefix: a prompt that all of them share)

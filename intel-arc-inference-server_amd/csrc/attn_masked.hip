@@ -1022,6 +1022,8 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
     return mi_fail(MI_ERR_ARG, "attn_masked: misaligned pages, spans, positions, slopes or flag (4 bytes)");
   if (!(mask->cap == 0.f || (mask->cap >= 1e-20f && mask->cap <= 1e30f)))  // (2 c / cap stays finite)
     return mi_fail(MI_ERR_ARG, "attn_masked: cap is 0 (none) or between 1e-20 and 1e30");
+  if (!mask->pos && (uint64_t)mask->pos0 + T > 1u << 31)  // (distances are int32)
+    return mi_fail(MI_ERR_SHAPE, "attn_masked: positions are below 2^31");
   const uint32_t gqa = shape->q_heads / shape->kv_heads;
   Pick p = pick(T, kv_len, shape->kv_heads, gqa, shape->head_dim, mask);
   const Cap form = mask->cap == 0.f ? kNoCap : mask->cap <= kPlainCap ? kPlain : kAnyCap;

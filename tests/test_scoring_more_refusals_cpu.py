@@ -2,7 +2,7 @@
 import pytest
 
 from mipkg import mi
-from test_scoring_cpu import ARG, P, shape
+from test_scoring_cpu import ARG, SHAPE, P, shape
 
 
 @pytest.mark.parametrize("name", ["tokens", "logprob", "rank", "entropy", "top_ids", "top_logprobs"])
@@ -26,3 +26,11 @@ def test_misaligned_arrays_of_attention(name):
         assert L.mi_attn_masked(P, P, P, 128, 1 << 20, pages, 64, 100, 1000, 1, mi.C.byref(sh), mi.C.byref(mask), P, 1 << 30, P, flag,
                                 None) == ARG
         assert b"misaligned" in L.mi_last_error()
+
+
+@pytest.mark.parametrize("T,pos0", [(1, 1 << 31), (2, (1 << 31) - 1), (65535, 0xFFFFFFFF), (1, 0xFFFFFFFF)])
+def test_positions_past_31_bits(T, pos0):
+    L = mi.lib()
+    sh, mask = shape(), mi.AttnMask(pos0=pos0)
+    assert L.mi_attn_masked(P, P, P, 128, 1 << 20, None, 0, 0, 1000, T, mi.C.byref(sh), mi.C.byref(mask), P, 1 << 30, P, None, None) == SHAPE
+    assert b"positions" in L.mi_last_error()
