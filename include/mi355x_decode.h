@@ -560,14 +560,16 @@ typedef struct mi_attn_mask {
 /* Attention of T rows, one or many (q fp32 [T][q_heads][head_dim] as mi_attn_prep and mi_attn_prep_rows
  * write it, magnitudes below 65504), over the f16 cache: row layout as mi_attn_prefill, keys at or behind
  * kv_len are never read. attn_out [T][q_heads * head_dim] f16 (shape->act as mi_attn_reduce); a row that sees
- * no key gives zeros. What a row does not see has no part in it, infinities and NaN included. pages: cache row
+ * no key gives zeros, whatever its q. Sums, softmax and probabilities are fp32; a call of more than 16 / (q heads per kv head)
+ * rows rounds each probability's numerator to f16 (2^-11 of it) before the product with V, fewer rows keep it in two f16
+ * halves, so a row's bits depend on T. What a row does not see has no part in it, infinities and NaN included. pages: cache row
  * of key j = pages[j / page] * page + j % page, n_pages the pages that the cache holds; an entry that is not
  * below n_pages sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL) if a row sees a key of that page (pages that no row
  * sees, behind a window or not written yet, may be absent), the call's outputs are then not to be
  * used, and nothing outside the cache is read. head_dim 128 or 256, up to 64 q heads per kv head, not gated;
  * T up to 65535, kv_len up to 2^30. ws: mi_attn_masked_ws(T, kv_len, shape) bytes of device scratch, 16-byte
  * aligned (NULL where that is 0). That size never falls as T or kv_len grows, so one that was asked for the largest of both
- * serves every smaller call; 1032 bytes times 2^18 at most. */
+ * serves every smaller call; 2^18 times 4 (head_dim + 4) bytes at most. */
 size_t mi_attn_masked_ws(uint32_t T, uint32_t kv_len, const mi_attn_shape* shape);
 int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v, size_t row_stride,
                    size_t head_stride, const uint32_t* pages, uint32_t page, uint32_t n_pages,

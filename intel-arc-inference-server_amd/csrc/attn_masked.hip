@@ -15,9 +15,9 @@
 // kernel takes the weights so too (it is bound by the cache's bytes, not by products); the chunk's rounds each to f16 once
 // (2^-11 of it, as much as the output's own rounding; the weights' sum is taken before).
 //
-// What bounds it (MI355X): one row the cache's bytes, 131072 keys of 8 heads of 128 104 us, 5.2 TB/s; a chunk the matrix
+// What bounds it (MI355X): one row the cache's bytes, 131072 keys of 8 heads of 128 99 us, 5.4 TB/s; a chunk the matrix
 // cores, whose products are 3 per score-and-value pair (q in two parts): 2048 rows causal over 2048, 40 / 8 heads of 128,
-// 86 us; where rows see little (7 documents in 2048 rows 36.4 us, 14 of it the bytes of q and the outputs) a work-group's
+// 83 us; where rows see little (7 documents in 2048 rows 35.4 us, 14 of it the bytes of q and the outputs) a work-group's
 // chain of loads before its first tile, the tiles' unseen parts, and CUs that are done before the longest document's.
 //
 // A key that a row does not see has weight 0, but 0 times an infinity or a NaN of its V row is a NaN. A block whose
@@ -820,8 +820,8 @@ void launch_order(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
   else attn_masked_kernel<HD, CT, CAP, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
 }
 // Caps above kPlainCap take one column tile (two do not fit the registers), in one kernel for every order of the cache: they are
-// the rare ones. Measured (us; cap 257, then 30 or 256): 2048 rows causal, 40 / 8 heads of 128 120, 104; 7 documents in them 41, 38; 500
-// rows over 4500 keys, 32 / 8 138, 115; 777 over 3778, 16 / 2 of 256 214, 158. A single row over 131072 keys 99.6, 99.5.
+// the rare ones. Measured (us; cap 257, then 30): 2048 rows causal, 40 / 8 heads of 128 117, 93; 7 documents in them 41, 38; 500
+// rows causal over 4500 keys, 32 / 8 101, 79; 777 over 3778, 16 / 2 of 256 159, 107. A single row over 131072 keys 99.6, 99.5.
 template <int HD, int CT>
 void launch_chunk(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
   if constexpr (CT == 1)
@@ -911,8 +911,8 @@ __global__ __launch_bounds__(256) void attn_masked_join_few_kernel(MaskedArgs a,
 // The launch: the few-rows kernel up to 16 columns, else the chunk's with CT column tiles, and the parts that the keys are
 // split in.
 //   few: as many parts as fill the CUs (two work-groups each at rows of 128, one at 256), of 128 keys at least. Measured
-//   (us): one row, 40 / 8 heads of 128, 4099 keys 17.6 / 12.9 / 11.3 / 10.0 / 11.2 in 4 / 8 / 16 / 32 / 64 parts; 131072 keys
-//   105 / 100 / 103 / 110 in 32 / 64 / 128 / 256; 16 / 2 heads of 256, 65536 keys 37.6 / 31.3 / 38.3 in 64 / 128 / 256.
+//   (us): one row, 40 / 8 heads of 128, 4099 keys 17.7 / 13.5 / 12.0 / 11.8 / 11.8 in 4 / 8 / 16 / 32 / 64 parts; 131072 keys
+//   97 / 99 / 102 / 106 in 32 / 64 / 128 / 256; 16 / 2 heads of 256, 65536 keys 40 / 34 / 42 in 64 / 128 / 256.
 //   chunk: the least modelled time over both CT and the parts s, in us. With `same` keys that all rows see and up to `own` keys
 //   more, a work-group has between same / 32 and (same + own) / 32 tiles:
 //     the longest, start + most / s tau, or all of them over the CUs, rounds (start + mean / s tau), and for s > 1
@@ -922,10 +922,10 @@ __global__ __launch_bounds__(256) void attn_masked_join_few_kernel(MaskedArgs a,
 //   device's. Without `lo` the model takes them for the last T of the cache and causal (own = T). With it (documents, a
 //   window) they see less, how much is not known: the least product of that time and the one at own = 512 behind the
 //   prefix, so that neither is far from its best, with no more parts than the first's. Measured
-//   (us; CT 1 then 2, in 1 / 2 / 3 / 4 parts): 500 rows over 4500 keys, 32 / 8 heads of 128: 108 / 88 / 79 / 82, 148 / 88 / 81 / 71;
-//   777 over 3778, 16 / 2 of 256: 124 / 127 / 132 / 138, 165 / 102 / 125 / 112 (102 in 5); 2048 over 2048, 40 / 8 of 128:
-//   106 / 126, 86 / 112, 16 / 2 of 256: 85 / 115, 98 / 92; 333 over 333, 40 / 8 of 128: 14 / 21 / 23, 20 / 24 / 26; 20 over 4020:
-//   87 / 50 / 36 / 30 (16 parts 18), 129 / 71 / 51 / 42. With `lo`, over 45 shapes (2 to 12 documents, windows of 256 and
+//   (us; CT 1 then 2, in 1 / 2 / 3 / 4 parts): 500 rows over 4500 keys, 32 / 8 heads of 128: 105 / 84 / 80 / 82, 140 / 84 / 79 / 71;
+//   777 over 3778, 16 / 2 of 256: 128 / 128 / 134 / 139, 172 / 104 / 125 / 112 (104 in 5); 2048 over 2048, 40 / 8 of 128:
+//   99 / 127, 81 / 112, 16 / 2 of 256: 85 / 115, 100 / 94; 333 over 333, 40 / 8 of 128: 14 / 19 / 20, 20 / 21 / 23; 20 over 4020:
+//   87 / 49 / 35 / 29 (16 parts 16), 126 / 69 / 49 / 40. With `lo`, over 45 shapes (2 to 12 documents, windows of 256 and
 //   1024) 3 % off the best on average, 27 % by the causal time alone: 2048 rows, 12 documents, 16 / 16 heads of 128 20.2 us (43.8 in
 //   3 parts of CT 2), 1000 rows behind 4000, 3 documents, 40 / 8 23.5 (45.1).
 struct Pick {

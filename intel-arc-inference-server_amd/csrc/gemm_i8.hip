@@ -15,7 +15,7 @@
 // columns also the row's own chain (maximum, quotients, then the products: 5120 -> 7168 9.4 us, 3.9 TB/s); many rows the
 // matrix cores with the reads of their operands from LDS close behind (2048 rows 5120 -> 34816: 318 us, 2.3 PTOP/s; the
 // largest library product on the card 2.06); some hundred rows the operands' way into LDS and out again, 192 rows and columns
-// for 64 x 128 products per k (333 rows 17408 -> 5120: 53.8 us).
+// for 64 x 128 products per k (333 rows 17408 -> 5120: 51 us, 60 with the quantiser).
 #include <cstdio>
 
 #include "mi_capi_internal.h"

@@ -15,9 +15,9 @@
 // launch joins them and reads again the few runs that can hold one of the k best.
 // What bounds it: the memory's stream, with the vector ALUs close behind (about ten instructions per logit); few rows are
 // bound by their two launches' chains of loads. Each wave's next 4 KiB are loaded ahead of the work on the present ones.
-// Measured (MI355X, vocabulary 151936): 2048 rows with the 20 best 323 -> 271 us by the bound (-30) and the loads ahead
-// (-22), 245 with the 5 best, 232 with none (5.4 TB/s; a plain read of those bytes 6.7); 333 rows with 5 66 -> 52.5; one
-// row with 20 33 -> 12.0 in 149 slices.
+// Measured (MI355X, vocabulary 151936): 2048 rows with the 20 best 257 us (323 without the bound, which takes 30 off, and the
+// loads ahead, 22), 244 with the 5 best, 232 with none (5.4 TB/s; a plain read of those bytes 6.7); 333 rows with 5 53 (66); one
+// row with 20 11.6 in 149 slices (33 in one).
 #include <algorithm>
 #include <type_traits>
 
@@ -357,8 +357,8 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
 // k = 20. The bound: of runs by their largest logit, equal ones by their place, the worst of the waves' ceil(k / W)-th best
 // (k runs have a token at least as good as any token of a run behind it). A token's place among the best is the number of
 // those read that are better. Where more tokens reach the bound than fit (equal logits, or fewer finite ones than k), the
-// waves keep lists. One row of 151936 with the 20 best takes 11.8 us, 16 rows 15.9, 333 with the 5 best 53 (lists from
-// every slice, as a row in one has them: 18.6, 23 and 54.2); one row of equal logits 21.4 (20.9).
+// waves keep lists. One row of 151936 with the 20 best takes 11.6 us, 16 rows 15.2, 333 with the 5 best 53 (lists from
+// every slice, as a row in one has them: 18.6, 23 and 54.2); one row of equal logits 21.6 (20.9).
 __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
   constexpr uint32_t W = 8, U = 4, B = 8, kFit = 1024;  // waves; a lane's runs looked at together; runs read together; tokens
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x, runs = (a.vocab + 255u) / 256u;
