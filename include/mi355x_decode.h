@@ -562,7 +562,8 @@ typedef struct mi_attn_mask {
  * kv_len are never read. attn_out [T][q_heads * head_dim] f16 (shape->act as mi_attn_reduce); a row that sees
  * no key gives zeros, whatever its q. Sums, softmax and probabilities are fp32; a call of more than 16 / (q heads per kv head)
  * rows rounds each probability's numerator to f16 (2^-11 of it) before the product with V, fewer rows keep it in two f16
- * halves, so a row's bits depend on T. What a row does not see has no part in it, infinities and NaN included. pages: cache row
+ * halves, so a row's bits depend on T. What a row does not see has no part in it, infinities and NaN included (in
+ * V rows within 32 keys of seen ones they cost time: such blocks are formed again key by key). pages: cache row
  * of key j = pages[j / page] * page + j % page, n_pages the pages that the cache holds; an entry that is not
  * below n_pages sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL) if a row sees a key of that page (pages that no row
  * sees, behind a window or not written yet, may be absent), the call's outputs are then not to be
