@@ -8,12 +8,7 @@
 // Scores are formed in base 2, y = s log2(e). cap tanh(x / cap) = cap - 2 cap / (e^(2 x / cap) + 1), which costs an
 // exponential, a reciprocal and two fused operations and is off by 2^-21 cap at most; caps above 256, where that error would come
 // near the weights' rounding, take a form whose error goes with the score.
-// A column (a row and one of its q heads) keeps a reference r and forms its weights as 2^(y - r); r is raised, and the
-// accumulators rescaled, only when a score passes it by more than 15, and then to 7 below that score: the weights
-// are f16 numbers up to 2^15, and 2^-24 of the largest is still an f16 number to eight bits, so that the many small weights of
-// a long cache are not lost. q is taken as f16 high and low parts, so scores carry fp32's error of the sum alone. The few-rows
-// kernel takes the weights so too (it is bound by the cache's bytes, not by products); the chunk's rounds each to f16 once
-// (2^-11 of it, as much as the output's own rounding; the weights' sum is taken before).
+// The kernels, and how their softmax and its roundings go, are attn_rows.h's.
 //
 // What bounds it (MI355X): one row the cache's bytes, 131072 keys of 8 heads of 128 99 us, 5.4 TB/s; a chunk the matrix
 // cores, whose products are 3 per score-and-value pair (q in two parts): 2048 rows causal over 2048, 40 / 8 heads of 128,
@@ -24,18 +19,13 @@
 // result is not finite is therefore formed again, key by key, over the keys that each row sees. That is slow: a NaN in an unseen V row
 // of one part in 64 takes one row over 131072 keys from 100 us to 2.5 ms, one between 7 documents 2048 rows from 38 to 1560.
 #include <algorithm>
-#include <type_traits>
 
+#include "attn_rows.h"
 #include "mi_capi_internal.h"
-#include "mi_pieces.h"
 
 namespace mi {
 namespace {
 
-constexpr float kNoKey = -0x1.fffffep127f;  // the reference before the first key: no finite score is below it
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRaise = 15.f, kBelow = 7.f;
-constexpr uint32_t kTile = 32;      // keys per step of a wave
 constexpr uint32_t kMaxRows = 65535, kMaxKeys = 1u << 30;
 
 struct MaskedArgs {
@@ -78,21 +68,7 @@ struct Block {
     k = min(k, last);
     return k - prefix < gap ? (i < n_a ? prefix - 1u : prefix + gap) : k;
   }
-  // whether some column of the block does not see some key of the tile (uniform)
-  __device__ __forceinline__ bool masked(const MaskedArgs& a, uint32_t key) const {
-    return key + kTile > min_hi || (key < max_lo && key + kTile > a.prefix);
-  }
 };
-template <typename F>
-__device__ __forceinline__ uint32_t wave_fold(uint32_t v, F f) {
-  auto swap = [](uint32_t x, auto c) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, decltype(c)::value, 0xF, 0xF, false); };
-  v = f(v, swap(v, std::integral_constant<int, 0xB1>{}));
-  v = f(v, swap(v, std::integral_constant<int, 0x4E>{}));
-  v = f(v, swap(v, std::integral_constant<int, 0x141>{}));
-  v = f(v, swap(v, std::integral_constant<int, 0x140>{}));
-  auto at = [&](int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); };
-  return f(f(at(0), at(16)), f(at(32), at(48)));
-}
 __device__ __forceinline__ Block block_of(const MaskedArgs& a, uint32_t t0, uint32_t rows_here) {
   const uint32_t lane = threadIdx.x & 63u;
   uint32_t min_lo = 0xFFFFFFFFu, min_hi = 0xFFFFFFFFu, max_lo = 0u, max_hi = 0u;
@@ -151,9 +127,6 @@ __device__ __forceinline__ void report_pages(const MaskedArgs& a, const Block& b
   }
 }
 
-// The cache's order: contiguous, pages that hold whole tiles (one table entry for a tile's 32 keys), any pages.
-enum Order { kContiguous, kWholeTiles, kAnyPages };
-
 // A column of a wave's 16 x CT: its span and what its scores take.
 struct Column {
   uint32_t lo, hi, pos;
@@ -173,9 +146,6 @@ __device__ __forceinline__ Column column(const MaskedArgs& a, uint32_t j, uint32
 __device__ __forceinline__ bool sees(const MaskedArgs& a, const Column& c, uint32_t key) {
   return key < c.hi && (key >= c.lo || key < a.prefix);
 }
-// The scores' cap: none; one up to kPlainCap, by one exponential; any, by a form that leaves the scores their bits where the cap is
-// far above them.
-enum Cap { kNoCap, kPlain, kAnyCap };
 // The plain form's error is the cap's, 2^-21 of it: at 256 2^-13 of a weight, below their own rounding to f16.
 constexpr float kPlainCap = 256.f;
 // A score in base 2, the cap applied.
@@ -218,615 +188,68 @@ __device__ __forceinline__ void scores_by_form(const MaskedArgs& a, float (&w)[8
     for (uint32_t e = 0; e < 8; ++e) w[e] = score<kNoCap>(a, w[e]);
   }
 }
-// where a split leaves column `col` of its block: HD values (sums of weight times V), then r and the weights' sum
-template <int HD>
-__device__ __forceinline__ float* part_at(const MaskedArgs& a, uint32_t j, uint32_t t, uint32_t g, uint32_t split) {
-  return a.part + ((size_t)(t * a.q_heads + j * a.gqa + g) * a.splits + split) * (HD + 4);
-}
+// The kernels' argument (attn_rows.h).
+struct Place {
+  uint32_t j, t0, rows, split, splits;
+};
+struct MaskedRows : MaskedArgs {
+  using Place = mi::Place;
+  using Block = mi::Block;
+  using Column = mi::Column;
+  static constexpr bool kMayIdle = false;
+  // grid (kv_heads, row blocks, splits); the last row blocks of a causal chunk see the most keys: they are dispatched first
+  __device__ __forceinline__ Place place(bool chunk) const {
+    const uint32_t t0 = (chunk ? gridDim.y - 1u - blockIdx.y : blockIdx.y) * rows;
+    return {blockIdx.x, t0, min(rows, T - t0), blockIdx.z, splits};
+  }
+  __device__ __forceinline__ Block block(const Place& p) const { return block_of(*this, p.t0, p.rows); }
+  __device__ __forceinline__ uint32_t part_begin(const Place& p, const Block& b, uint32_t split) const {
+    return (uint32_t)((uint64_t)b.n * split / p.splits);
+  }
+  __device__ __forceinline__ Column column(const Place& p, const Block&, uint32_t row, uint32_t g) const {
+    return mi::column(*this, p.j, p.t0, row, g, p.rows);
+  }
+  __device__ __forceinline__ bool masked(const Block& b, uint32_t key) const {
+    return key + kTile > b.min_hi || (key < b.max_lo && key + kTile > prefix);
+  }
+  __device__ __forceinline__ bool sees(const Column& c, uint32_t key) const { return mi::sees(*this, c, key); }
+  template <Cap CAP>
+  __device__ __forceinline__ float score(float s) const {
+    return mi::score<CAP>(*this, s);
+  }
+  __device__ __forceinline__ void scores_by_form(float (&w)[8]) const { mi::scores_by_form(*this, w); }
+  __device__ __forceinline__ void bias_and_mask(const Column& c, uint32_t key0, bool masked, float (&w)[8]) const {
+    mi::bias_and_mask(*this, c, key0, masked, w);
+  }
+  __device__ __forceinline__ uint32_t first_row(const Block&, uint32_t key) const { return key; }
+  __device__ __forceinline__ uint32_t cache_row(const Block&, uint32_t key, bool& outside) const {
+    return mi::cache_row(*this, key, outside);
+  }
+  __device__ __forceinline__ uint32_t row_of(const Block& b, uint32_t i, uint32_t key, bool& outside) const {
+    return pages ? mi::cache_row(*this, b.within(i, key), outside) : min(key, b.last);
+  }
+  __device__ __forceinline__ void report_pages(const Place& p, const Block& b, uint32_t from, uint32_t to, uint32_t step) const {
+    mi::report_pages(*this, b, p.t0, p.rows, from, to, step);
+  }
+  template <int HD>
+  __device__ __forceinline__ float* part_at(const Place& p, uint32_t row, uint32_t g) const {
+    return part + ((size_t)((p.t0 + row) * q_heads + p.j * gqa + g) * splits + p.split) * (HD + 4);
+  }
+};
 
-// The columns of a block one by one, over the keys that they see only: a lane holds dims lane + 64 i. `capped` makes scores in
-// base 2 of products.
-template <int HD, typename F>
-__device__ __forceinline__ void slow_block(const MaskedArgs& a, const Block& b, uint32_t j, uint32_t t0,
-                                           uint32_t rows_here, uint32_t from, uint32_t to, uint32_t split, F capped) {
-  constexpr uint32_t D = HD / 64;
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-  const size_t hoff = (size_t)j * a.head_stride;
-#pragma unroll 1
-  for (uint32_t p = wave; p < rows_here * a.gqa; p += blockDim.x / 64u) {
-    const uint32_t row = p / a.gqa, g = p % a.gqa;
-    const Column c = column(a, j, t0, row, g, rows_here);
-    const float* q = a.q + ((size_t)(t0 + row) * a.q_heads + j * a.gqa + g) * HD + lane;
-    float r = kNoKey, l = 0.f, acc[D];
-#pragma unroll
-    for (uint32_t i = 0; i < D; ++i) acc[i] = 0.f;
-    if (c.live) {
-#pragma unroll 1
-      for (uint32_t i = from; i < to; ++i) {
-        const uint32_t k0 = b.key(i);
-#pragma unroll 1
-        for (uint32_t key = k0; key < k0 + kTile; ++key) {
-          if (!sees(a, c, key)) continue;
-          bool outside;  // (the block's walk has reported it)
-          const size_t at = (size_t)cache_row(a, key, outside) * a.row_stride + hoff + lane;
-          float s = 0.f;
-#pragma unroll
-          for (uint32_t d = 0; d < D; ++d) s = __builtin_fmaf(q[64u * d], h2f(a.k[at + 64u * d]), s);
-          float w[8] = {wave_sum(s), 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-          capped(w);
-          bias_and_mask(a, c, key, false, w);
-          if (w[0] > r + kRaise) {
-            const float to_r = w[0] - kBelow, alpha = __builtin_amdgcn_exp2f(r - to_r);
-            r = to_r;
-            l *= alpha;
-#pragma unroll
-            for (uint32_t d = 0; d < D; ++d) acc[d] *= alpha;
-          }
-          const float pw = __builtin_amdgcn_exp2f(w[0] - r);
-          l += pw;
-#pragma unroll
-          for (uint32_t d = 0; d < D; ++d) acc[d] = __builtin_fmaf(pw, h2f(a.v[at + 64u * d]), acc[d]);
-        }
-      }
-    }
-    if (a.splits > 1) {
-      float* o = part_at<HD>(a, j, t0 + row, g, split);
-#pragma unroll
-      for (uint32_t d = 0; d < D; ++d) o[lane + 64u * d] = acc[d];
-      if (lane == 0) {
-        o[HD] = r;
-        o[HD + 1] = l;
-      }
-    } else {
-      uint16_t* o = a.out + ((size_t)(t0 + row) * a.q_heads + j * a.gqa + g) * HD + lane;
-#pragma unroll
-      for (uint32_t d = 0; d < D; ++d) o[64u * d] = act_enc(l == 0.f ? 0.f : acc[d] / l, a.act);
-    }
-  }
-}
-
-// KK x 32 dims of a column's q as the B operand, f16 high and low parts: k = 32 kk + 8 qq + e
-template <uint32_t KK>
-__device__ __forceinline__ void split_q(const f4_t (&q)[2 * KK], h8_t (&qh)[KK], h8_t (&ql)[KK]) {
-  float neg1 = -1.f;
-  asm("" : "+s"(neg1));
-#pragma unroll
-  for (uint32_t kk = 0; kk < KK; ++kk) {
-    u4_t h, l;
-#pragma unroll
-    for (uint32_t x = 0; x < 4; ++x) {
-      uint32_t hh, ll;
-      f16_parts(q[2 * kk + x / 2][2 * (x % 2)], q[2 * kk + x / 2][2 * (x % 2) + 1], neg1, hh, ll);
-      h[x] = hh;
-      l[x] = ll;
-    }
-    qh[kk] = __builtin_bit_cast(h8_t, h);
-    ql[kk] = __builtin_bit_cast(h8_t, l);
-  }
-}
-template <uint32_t KK>
-__device__ __forceinline__ void load_q(const float* qp, h8_t (&qh)[KK], h8_t (&ql)[KK]) {
-  f4_t q[2 * KK];
-#pragma unroll
-  for (uint32_t x = 0; x < 2 * KK; ++x) q[x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2)));
-  split_q<KK>(q, qh, ql);
-}
-
-// One step of the softmax of a wave's CT column tiles. The references first: raised, with what was formed by them, where a
-// score passes one (each column by its own four lanes, whatever its neighbours need). NT 0: the accumulators are left to
-// the caller, with their factor.
-template <uint32_t CT, uint32_t NT>
-__device__ __forceinline__ void raise(const float (&w)[CT][8], uint32_t qi, float (&r)[CT], float (&l)[CT], f4_t (*acc)[NT ? NT : 1],
-                                      float* factor) {
-  float mx[CT];
-  bool over = false;
-#pragma unroll
-  for (uint32_t ct = 0; ct < CT; ++ct) {
-    mx[ct] = max3(max3(w[ct][0], w[ct][1], w[ct][2]), max3(w[ct][3], w[ct][4], w[ct][5]), max3(w[ct][6], w[ct][7], w[ct][7]));
-    over |= mx[ct] > r[ct] + kRaise;
-  }
-  if (!__ballot(over)) return;
-#pragma unroll
-  for (uint32_t ct = 0; ct < CT; ++ct) {
-    const uint64_t lanes = __ballot(mx[ct] > r[ct] + kRaise);
-    const uint32_t o = (uint32_t)lanes | (uint32_t)(lanes >> 32);
-    const float cm = col_max(mx[ct]), to = ((o | o >> 16) >> qi) & 1u ? fmaxf(r[ct], cm - kBelow) : r[ct];
-    const float alpha = __builtin_amdgcn_exp2f(r[ct] - to);
-    r[ct] = to;
-    l[ct] *= alpha;
-#pragma unroll
-    for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] *= alpha;
-    if constexpr (NT == 0) *factor = alpha;
-  }
-}
-// Then the weights, as the B operands of P V in f16 high and low parts; their sum goes to l.
-__device__ __forceinline__ void weights(float (&w)[8], float r, float& l, h8_t& hi, h8_t& lo) {
-#pragma unroll
-  for (uint32_t e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_exp2f(w[e] - r);
-  l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-  float neg1 = -1.f;
-  asm("" : "+s"(neg1));
-  u4_t h, m;
-#pragma unroll
-  for (uint32_t e = 0; e < 4; ++e) {
-    uint32_t hh, mm;
-    f16_parts(w[2 * e], w[2 * e + 1], neg1, hh, mm);
-    h[e] = hh;
-    m[e] = mm;
-  }
-  hi = __builtin_bit_cast(h8_t, h);
-  lo = __builtin_bit_cast(h8_t, m);
-}
-typedef short v4s_t __attribute__((ext_vector_type(4)));
-typedef v4s_t __attribute__((address_space(3)))* v4s_lds;
-// V^T of a 32-key tile as the A operand: the k of the product are the keys 4 qq + e of the two 16-key groups, which is
-// how the lanes hold the weights; 4 keys' dims come from one transposing read
-template <uint32_t VROW>
-__device__ __forceinline__ h8_t v_operand(const uint16_t* vb, uint32_t tt) {
-  const v4s_t a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(vb + 16u * tt));
-  const v4s_t a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(vb + 16u * VROW + 16u * tt));
-  return __builtin_bit_cast(h8_t, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-// the sum over the four lanes of a column
-__device__ __forceinline__ float col_sum(float x) {
-  float a0 = x, a1 = x;
-  lane_swap16(a0, a1);
-  float b0 = a0 + a1, b1 = b0;
-  lane_swap32(b0, b1);
-  return b0 + b1;
-}
-template <int HD>
-__device__ __forceinline__ void store_part(const MaskedArgs& a, uint32_t j, uint32_t t, uint32_t g, uint32_t split, uint32_t qq,
-                                           uint32_t tt, f4_t v) {
-  *reinterpret_cast<f4_t*>(part_at<HD>(a, j, t, g, split) + 16u * tt + 4u * qq) = v;
-}
-template <int HD>
-__device__ __forceinline__ void store_out(const MaskedArgs& a, uint32_t j, uint32_t t, uint32_t g, uint32_t qq, uint32_t tt, f4_t v) {
-  const u2_t h = {(uint32_t)act_enc(v[0], a.act) | ((uint32_t)act_enc(v[1], a.act) << 16),
-                  (uint32_t)act_enc(v[2], a.act) | ((uint32_t)act_enc(v[3], a.act) << 16)};
-  *reinterpret_cast<h4_any*>(a.out + ((size_t)t * a.q_heads + j * a.gqa + g) * HD + 16u * tt + 4u * qq) = h;
-}
-__device__ __forceinline__ float not_finite(float z, f4_t v) {  // 0 (a zero z), or NaN
-#pragma unroll
-  for (uint32_t e = 0; e < 4; ++e) z = __builtin_fmaf(v[e], 0.f, z);
-  return z;
-}
-
-// Few rows (16 columns per block): grid (kv_heads, row blocks, splits), 4 waves. A wave walks its own 32-key tiles,
-// every fourth of the split's: K from memory as the A operand, V through its own part of LDS for the transposing
-// reads, the next tile's rows in registers meanwhile. The waves' sums join through LDS.
-template <int HD>
-__global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_masked_few_kernel(MaskedArgs a) {
-  constexpr uint32_t KK = HD / 32, NT = HD / 16, VROW = HD + 16;
-  constexpr uint32_t PPR = HD / 8, RPP = 64 / PPR, NV = kTile / RPP;  // 16-byte pieces per V row, rows per load, loads per tile
-  __shared__ __align__(16) union Slab {
-    uint16_t v[kTile * VROW];
-    struct {
-      float acc[NT * 4][64], r[64], l[64];
-    } part;
-  } slab[4];
-  const uint32_t j = blockIdx.x, t0 = blockIdx.y * a.rows, split = blockIdx.z;
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, qi = lane & 15u, qq = lane >> 4;
-  const uint32_t rows_here = min(a.rows, a.T - t0);
-  const uint32_t row = qi / a.gqa, g = qi % a.gqa;
-  const Block b = block_of(a, t0, rows_here);
-  const Column col = column(a, j, t0, row, g, rows_here);
-  const uint32_t from = (uint32_t)((uint64_t)b.n * split / a.splits), to = (uint32_t)((uint64_t)b.n * (split + 1u) / a.splits);
-  const float* qp = a.q + ((size_t)(t0 + (row < rows_here ? row : 0u)) * a.q_heads + j * a.gqa + g) * HD + 8u * qq;
-  float r[1] = {kNoKey}, l[1] = {0.f};
-  f4_t acc[1][NT];
-#pragma unroll
-  for (uint32_t tt = 0; tt < NT; ++tt) acc[0][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
-
-  const size_t hoff = (size_t)j * a.head_stride;
-  u4_t kr[2][KK], vr[NV];
-  // a lane's cache row: of key 16 (lane / 16 % 2) + lane % 16 of the tile
-  bool outside = false;
-  auto rows_of = [&](uint32_t i) {
-    const uint32_t key = b.key(i) + (lane & 31u);
-    return a.pages ? cache_row(a, b.within(i, key), outside) : min(key, b.last);
-  };
-  auto load = [&](uint32_t crow) {
-#pragma unroll
-    for (uint32_t gg = 0; gg < 2; ++gg) {
-      const uint16_t* p = a.k + (size_t)(uint32_t)__shfl((int)crow, (int)(16u * gg + qi), 64) * a.row_stride + hoff + 8u * qq;
-#pragma unroll
-      for (uint32_t kk = 0; kk < KK; ++kk) kr[gg][kk] = *reinterpret_cast<const u4_t*>(p + 32u * kk);
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < NV; ++i) {
-      const uint32_t cr = (uint32_t)__shfl((int)crow, (int)(RPP * i + lane / PPR), 64);
-      vr[i] = *reinterpret_cast<const u4_t*>(a.v + (size_t)cr * a.row_stride + hoff + 8u * (lane % PPR));
-    }
-  };
-  uint32_t i = from + wave, crow = 0;
-  if (i < to) {
-    load(rows_of(i));
-    if (i + 4u < to) crow = rows_of(i + 4u);
-  }
-  h8_t qh[KK], ql[KK];
-  load_q<KK>(qp, qh, ql);
-  uint16_t* vs = slab[wave].v;
-  const uint16_t* vb = vs + (4u * qq + (qi >> 2)) * VROW + 4u * (qi & 3u);
-  for (; i < to; i += 4u) {
-    const uint32_t key = b.key(i);
-    f4_t d[2] = {f4_t{0.f, 0.f, 0.f, 0.f}, f4_t{0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-    for (uint32_t kk = 0; kk < KK; ++kk)
-#pragma unroll
-      for (uint32_t gg = 0; gg < 2; ++gg) {
-        d[gg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[gg][kk]), qh[kk], d[gg], 0, 0, 0);
-        d[gg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, kr[gg][kk]), ql[kk], d[gg], 0, 0, 0);
-      }
-    wave_lds_sync();
-#pragma unroll
-    for (uint32_t n = 0; n < NV; ++n) *reinterpret_cast<u4_t*>(vs + (RPP * n + lane / PPR) * VROW + 8u * (lane % PPR)) = vr[n];
-    wave_lds_sync();
-    if (i + 4u < to) {
-      const uint32_t now = crow;  // (the next rows' page is asked for before these rows are)
-      if (i + 8u < to) crow = rows_of(i + 8u);
-      load(now);
-    }
-    float w[1][8];
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) w[0][e] = d[e / 4][e % 4];
-    scores_by_form(a, w[0]);
-    bias_and_mask(a, col, key + 4u * qq, b.masked(a, key), w[0]);
-    raise<1, NT>(w, qi, r, l, acc, nullptr);
-    h8_t ph, pl;
-    weights(w[0], r[0], l[0], ph, pl);
-#pragma unroll
-    for (uint32_t tt = 0; tt < NT; ++tt) {
-      const h8_t av = v_operand<VROW>(vb, tt);
-      acc[0][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ph, acc[0][tt], 0, 0, 0);
-      acc[0][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, pl, acc[0][tt], 0, 0, 0);
-    }
-  }
-  if (__ballot(outside)) report_pages(a, b, t0, rows_here, from + wave, to, 4u);
-  l[0] = col_sum(l[0]);
-  float bad = 0.f;
-#pragma unroll
-  for (uint32_t tt = 0; tt < NT; ++tt) bad = not_finite(bad, acc[0][tt]);
-  bad += l[0] - l[0];
-  wave_lds_sync();
-  auto& mine = slab[wave].part;
-#pragma unroll
-  for (uint32_t tt = 0; tt < NT; ++tt)
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) mine.acc[4u * tt + e][lane] = acc[0][tt][e];
-  mine.r[lane] = r[0];
-  mine.l[lane] = l[0];
-  if (__syncthreads_or(col.live && bad != 0.f)) {
-    slow_block<HD>(a, b, j, t0, rows_here, from, to, split, [&](float(&w)[8]) { scores_by_form(a, w); });
-    return;
-  }
-  // wave w joins the dims 16 tt + .. of its quarter of the tiles
-  float top = slab[0].part.r[lane], f[4], sum = 0.f;
-#pragma unroll
-  for (uint32_t w = 1; w < 4; ++w) top = fmaxf(top, slab[w].part.r[lane]);
-#pragma unroll
-  for (uint32_t w = 0; w < 4; ++w) {
-    f[w] = __builtin_amdgcn_exp2f(slab[w].part.r[lane] - top);
-    sum = __builtin_fmaf(slab[w].part.l[lane], f[w], sum);
-  }
-  if (row >= rows_here) return;
-  const float inv = col.live && sum != 0.f ? 1.0f / sum : 0.f;
-#pragma unroll
-  for (uint32_t n = 0; n < NT / 4; ++n) {
-    const uint32_t tt = wave * (NT / 4) + n;
-    f4_t v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (uint32_t w = 0; w < 4; ++w)
-#pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) v[e] = __builtin_fmaf(slab[w].part.acc[4u * tt + e][lane], f[w], v[e]);
-    if (!col.live) v = f4_t{0.f, 0.f, 0.f, 0.f};  // (what it summed may be a NaN, which no factor makes a zero)
-    if (a.splits > 1) store_part<HD>(a, j, t0 + row, g, split, qq, tt, v);
-    else store_out<HD>(a, j, t0 + row, g, qq, tt, v * inv);
-  }
-  if (a.splits > 1 && wave == 0 && qq == 0) {
-    float* o = part_at<HD>(a, j, t0 + row, g, split);
-    o[HD] = top;
-    o[HD + 1] = col.live ? sum : 0.f;
-  }
-}
-
-// A chunk: grid (kv_heads, row blocks, splits). Four waves side by side take CT column tiles each and 128 of the dims; at
-// rows of 256 four more take the other half (a wave's registers hold 32 columns of 128 dims with two waves per SIMD, and
-// every LDS read then serves 32 columns). All walk the same 32-key tiles, K and V staged in LDS for all of them, the rows
-// after them in registers meanwhile. A step i has two halves with a barrier between them:
-//   the products of tile i + 1's scores, dealt out among the exponentials that make tile i's weights;
-//   P V of tile i, dealt out among the scaling (and the tanh) of tile i + 1's scores, whose maxima follow.
-// So the matrix core has products while the vector ALUs work in the same wave. The halves of the dims exchange their parts
-// of the scores through LDS across the barrier. With two column tiles each of the two waves takes the softmax of one, its
-// tile 0 (the other wave's 1): the parts of the other's scores go over, and a step later the weights and the factor of a raised
-// reference come back (777 rows over 3778 keys, 16 / 2 heads, with distances, in 5 parts: 125 -> 110 us).
-template <int HD, int CT, Cap CAP, Order ORDER>
-__global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedArgs a) {
-  constexpr uint32_t DS = HD / 128, KK = 4, NT = 8, KROW = HD + 8, VROW = HD + 16, THREADS = 2 * HD;
-  constexpr uint32_t PPR = HD / 8, RPP = THREADS / PPR, CH = kTile / RPP;  // 16-byte pieces per row, rows per pass, passes
-  constexpr bool OWN = DS == 2 && CT == 2;
-  constexpr uint32_t SC = OWN ? 1 : CT;  // column tiles whose softmax the wave takes
-  __shared__ __align__(16) struct {
-    uint16_t k[2][kTile * KROW], v[2][kTile * VROW];
-    f4_t s[DS > 1 ? 2 : 1][DS > 1 ? 4 * DS : 1][2 * SC][DS > 1 ? 64 : 1];
-    h8_t p[OWN ? 2 : 1][OWN ? 8 : 1][OWN ? 64 : 1];
-    float f[OWN ? 2 : 1][OWN ? 8 : 1][OWN ? 64 : 1];  // the references' factors; the sums at the end
-  } st;
-  // the last row blocks of a causal chunk see the most keys: they are dispatched first
-  const uint32_t j = blockIdx.x, t0 = (gridDim.y - 1u - blockIdx.y) * a.rows, split = blockIdx.z;
-  const uint32_t t = threadIdx.x, lane = t & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 6)), qi = lane & 15u, qq = lane >> 4;
-  const uint32_t cw = wave % 4u, ds = wave / 4u;
-  const uint32_t rows_here = min(a.rows, a.T - t0);
-  const Block b = block_of(a, t0, rows_here);
-  uint32_t row[CT], g[CT];
-  Column col[SC];
-  bool live[CT];
-  f4_t qraw[CT][2 * KK];  // (converted behind the first tiles' loads)
-#pragma unroll
-  for (uint32_t ct = 0; ct < CT; ++ct) {
-    const uint32_t p = 16u * (CT * cw + (OWN ? ct ^ ds : ct)) + qi;
-    row[ct] = p / a.gqa;
-    g[ct] = p % a.gqa;
-    const Column c = column(a, j, t0, row[ct], g[ct], rows_here);
-    live[ct] = c.live;
-    if (ct < SC) col[ct] = c;
-    const float* qp = a.q + ((size_t)(t0 + (row[ct] < rows_here ? row[ct] : 0u)) * a.q_heads + j * a.gqa + g[ct]) * HD + 128u * ds + 8u * qq;
-#pragma unroll
-    for (uint32_t x = 0; x < 2 * KK; ++x) qraw[ct][x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2)));
-  }
-  const uint32_t from = (uint32_t)((uint64_t)b.n * split / a.splits), n = (uint32_t)((uint64_t)b.n * (split + 1u) / a.splits) - from;
-  auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
-  const size_t hoff = (size_t)j * a.head_stride;
-  const uint32_t srow = t / PPR, sp = 8u * (t % PPR);
-  u4_t kr[CH], vr[CH];
-  // the cache rows of tile i: its first (r[0]) where they follow one another, else those that the thread loads
-  struct Rows {
-    uint32_t r[CH];
-  };
-  bool outside = false;
-  auto rows_of = [&](uint32_t i) {
-    Rows w;
-    const uint32_t tile = from + min(i, n - 1u), key0 = b.key(tile);
-    if constexpr (ORDER == kContiguous) {
-      w.r[0] = key0;
-    } else if constexpr (ORDER == kWholeTiles) {
-      w.r[0] = cache_row(a, key0, outside);
-    } else {
-#pragma unroll
-      for (uint32_t c = 0; c < CH; ++c) w.r[c] = cache_row(a, b.within(tile, key0 + RPP * c + srow), outside);
-    }
-    return w;
-  };
-  // (a tile behind the last is that one again, and its loads are not used)
-  auto load = [&](const uint16_t* cache, uint32_t i, const Rows& w, u4_t (&to)[CH]) {
-    const uint32_t left = b.last - b.key(from + min(i, n - 1u));
-#pragma unroll
-    for (uint32_t c = 0; c < CH; ++c) {
-      const uint32_t r = ORDER == kAnyPages ? w.r[c] : uniform(w.r[0]) + min(RPP * c + srow, left);
-      to[c] = *as_global(reinterpret_cast<const u4_t*>(cache + (size_t)r * a.row_stride + hoff + sp));
-    }
-  };
-  auto store = [&](uint16_t* to, uint32_t pitch, const u4_t (&v)[CH]) {
-#pragma unroll
-    for (uint32_t c = 0; c < CH; ++c) *reinterpret_cast<u4_t*>(to + (RPP * c + srow) * pitch + sp) = v[c];
-  };
-  // the rows of the tiles i + 1 .. i + 3 of a step i: V of the first and K of the last are loaded in it (a page's entry is
-  // fetched a step before the loads that need it)
-  Rows r1, r2, r3;
-  u4_t k1[CH];
-  if (n) {
-    const Rows r0 = rows_of(0);
-    r1 = rows_of(1);
-    r2 = rows_of(2);
-    r3 = rows_of(3);
-    load(a.k, 0, r0, kr);
-    load(a.v, 0, r0, vr);
-    load(a.k, 1, r1, k1);
-  }
-  float r[SC], l[SC], factor = 1.f;
-  f4_t acc[CT][NT], d[CT][2];
-  h8_t qh[CT][KK], ql[CT][KK];
-#pragma unroll
-  for (uint32_t ct = 0; ct < CT; ++ct) {
-    split_q<KK>(qraw[ct], qh[ct], ql[ct]);
-    if (ct < SC) {
-      r[ct] = kNoKey;
-      l[ct] = 0.f;
-    }
-#pragma unroll
-    for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
-  }
-  // One K operand (16 keys x 32 dims, number s = 2 kk + gg) and its products: this wave's part of the scores
-  // S^T[key 16 gg + 4 qq + e][column qi].
-  auto k_operand = [&](uint32_t buf, uint32_t s) {
-    return *reinterpret_cast<const h8_t*>(st.k[buf] + (16u * (s % 2u) + qi) * KROW + 128u * ds + 8u * qq + 32u * (s / 2u));
-  };
-  auto product = [&](h8_t kh, uint32_t s, uint32_t part) {  // part < 2 CT: the columns' high parts, then the low ones
-    const uint32_t ct = part % CT;
-    d[ct][s % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, part < CT ? qh[ct][s / 2] : ql[ct][s / 2], d[ct][s % 2], 0, 0, 0);
-  };
-  auto clear = [&]() {
-#pragma unroll
-    for (uint32_t ct = 0; ct < CT; ++ct) d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
-  };
-  auto hand_over = [&](uint32_t buf) {
-    if constexpr (DS > 1) {
-#pragma unroll
-      for (uint32_t ct = 0; ct < SC; ++ct)
-#pragma unroll
-        for (uint32_t gg = 0; gg < 2; ++gg) st.s[buf][wave][2 * ct + gg][lane] = d[OWN ? 1 : ct][gg];
-    }
-  };
-  auto take_over = [&](uint32_t buf) {
-    if constexpr (DS > 1) {
-#pragma unroll
-      for (uint32_t ct = 0; ct < SC; ++ct)
-#pragma unroll
-        for (uint32_t gg = 0; gg < 2; ++gg) d[ct][gg] += st.s[buf][wave ^ 4u][2 * ct + gg][lane];
-    }
-  };
-  float w[SC][8];
-  // the scores w of tile i: bias, mask, and the columns' references
-  auto settle = [&](uint32_t i) {
-    const uint32_t key = b.key(from + i);
-    const bool masked = b.masked(a, key);
-#pragma unroll
-    for (uint32_t ct = 0; ct < SC; ++ct) bias_and_mask(a, col[ct], key + 4u * qq, masked, w[ct]);
-    if constexpr (OWN) raise<1, 0>(w, qi, r, l, nullptr, &factor);
-    else raise<CT, NT>(w, qi, r, l, acc, nullptr);
-  };
-  if (n) {
-    store(st.k[0], KROW, kr);
-    store(st.k[1], KROW, k1);
-    load(a.k, 2, r2, kr);
-    lds_barrier();
-    clear();
-#pragma unroll
-    for (uint32_t s = 0; s < 2 * KK; ++s) {
-      const h8_t kh = k_operand(0, s);
-#pragma unroll
-      for (uint32_t part = 0; part < 2 * CT; ++part) product(kh, s, part);
-    }
-    hand_over(0);
-    lds_barrier();
-    take_over(0);
-#pragma unroll
-    for (uint32_t ct = 0; ct < SC; ++ct)
-#pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) w[ct][e] = score<CAP>(a, d[ct][e / 4][e % 4]);
-    settle(0);
-  }
-  for (uint32_t i = 0; i < n; ++i) {
-    const uint32_t cur = i & 1u, nxt = cur ^ 1u;
-    // V of tile i and K of tile i + 2 into the buffers that were last read before the barrier behind us; then the loads of
-    // the next step's
-    store(st.v[cur], VROW, vr);
-    store(st.k[cur], KROW, kr);
-    const Rows r4 = rows_of(i + 4u);
-    load(a.v, i + 1u, r1, vr);
-    load(a.k, i + 3u, r3, kr);
-    r1 = r2;
-    r2 = r3;
-    r3 = r4;
-    h8_t p[CT];
-    {  // (behind the last tile the products are of a tile that is not used)
-      constexpr uint32_t S = 2 * KK, AHEAD = 3;
-      h8_t kh[S];
-      clear();
-#pragma unroll
-      for (uint32_t s = 0; s < AHEAD; ++s) kh[s] = k_operand(nxt, s);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (uint32_t s = 0; s < S; ++s) {
-        if (s + AHEAD < S) kh[s + AHEAD] = k_operand(nxt, s + AHEAD);
-#pragma unroll
-        for (uint32_t h = 0; h < CT; ++h) {  // two products, one weight (or a weight for every four)
-          product(kh[s], s, 2 * h);
-          product(kh[s], s, 2 * h + 1);
-          if (h >= SC) continue;
-          const uint32_t x = s * SC + h, ct = x / 8, e = x % 8;
-          w[ct][e] = __builtin_amdgcn_exp2f(w[ct][e] - r[ct]);
-          l[ct] += w[ct][e];
-          if (e % 2) {
-            u4_t pk = __builtin_bit_cast(u4_t, p[ct]);
-            pk[e / 2] = h2_bits(__builtin_convertvector((f2_t{w[ct][e - 1], w[ct][e]}), h2_t));
-            p[ct] = __builtin_bit_cast(h8_t, pk);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-      hand_over(nxt);
-      if constexpr (OWN) {
-        st.p[cur][wave][lane] = p[0];
-        st.f[cur][wave][lane] = factor;
-      }
-    }
-    lds_barrier();
-    {
-      const uint16_t* vb = st.v[cur] + (4u * qq + (qi >> 2)) * VROW + 128u * ds + 4u * (qi & 3u);
-      constexpr uint32_t AHEAD = 3;
-      h8_t av[NT];
-#pragma unroll
-      for (uint32_t tt = 0; tt < AHEAD; ++tt) av[tt] = v_operand<VROW>(vb, tt);
-      if constexpr (OWN) {
-        p[1] = st.p[cur][wave ^ 4u][lane];
-        const float other = st.f[cur][wave ^ 4u][lane];
-        if (__ballot(factor != 1.f || other != 1.f)) {
-#pragma unroll
-          for (uint32_t tt = 0; tt < NT; ++tt) {
-            acc[0][tt] *= factor;
-            acc[1][tt] *= other;
-          }
-        }
-        factor = 1.f;
-      }
-      take_over(nxt);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (uint32_t tt = 0; tt < NT; ++tt) {
-        if (tt + AHEAD < NT) av[tt + AHEAD] = v_operand<VROW>(vb, tt + AHEAD);
-#pragma unroll
-        for (uint32_t ct = 0; ct < CT; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[tt], p[ct], acc[ct][tt], 0, 0, 0);
-#pragma unroll
-        for (uint32_t ct = 0; ct < SC; ++ct) w[ct][tt] = score<CAP>(a, d[ct][tt / 4][tt % 4]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (i + 1u < n) settle(i + 1u);
-    }
-  }
-  if (ORDER != kContiguous && __ballot(outside)) report_pages(a, b, t0, rows_here, from, from + n, 1u);
-  float sum[CT];
-  bool bad = false;
-#pragma unroll
-  for (uint32_t ct = 0; ct < CT; ++ct) {
-    float z = 0.f;
-    if (ct < SC) {
-      sum[ct] = col_sum(l[ct]);
-      z = sum[ct] - sum[ct];
-    }
-#pragma unroll
-    for (uint32_t tt = 0; tt < NT; ++tt) z = not_finite(z, acc[ct][tt]);
-    bad |= live[ct] && z != 0.f;
-  }
-  if constexpr (OWN) st.f[n & 1u][wave][lane] = sum[0];  // (the last step's are in the other half)
-  if (__syncthreads_or(bad)) {
-    slow_block<HD>(a, b, j, t0, rows_here, from, from + n, split, [&](float(&w)[8]) { w[0] = score<CAP>(a, w[0]); });
-    return;
-  }
-  if constexpr (OWN) sum[1] = st.f[n & 1u][wave ^ 4u][lane];
-#pragma unroll
-  for (uint32_t ct = 0; ct < CT; ++ct) {
-    if (row[ct] >= rows_here) continue;
-    if (a.splits > 1) {
-#pragma unroll
-      for (uint32_t tt = 0; tt < NT; ++tt)
-        store_part<HD>(a, j, t0 + row[ct], g[ct], split, qq, 8u * ds + tt, live[ct] ? acc[ct][tt] : f4_t{0.f, 0.f, 0.f, 0.f});
-      if (qq == 0 && (OWN ? ct == 0 : ds == 0)) {
-        float* o = part_at<HD>(a, j, t0 + row[ct], g[ct], split);
-        o[HD] = r[ct < SC ? ct : 0];
-        o[HD + 1] = live[ct] ? sum[ct] : 0.f;
-      }
-    } else {
-      const float inv = live[ct] && sum[ct] != 0.f ? 1.0f / sum[ct] : 0.f;
-#pragma unroll
-      for (uint32_t tt = 0; tt < NT; ++tt)
-        store_out<HD>(a, j, t0 + row[ct], g[ct], qq, 8u * ds + tt, inv == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : acc[ct][tt] * inv);
-    }
-  }
-}
 template <int HD, int CT, Cap CAP>
-void launch_order(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
-  if (!a.pages) attn_masked_kernel<HD, CT, CAP, kContiguous><<<grid, 2 * HD, 0, st>>>(a);
-  else if (a.page % kTile == 0) attn_masked_kernel<HD, CT, CAP, kWholeTiles><<<grid, 2 * HD, 0, st>>>(a);
-  else attn_masked_kernel<HD, CT, CAP, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
+void launch_order(const MaskedRows& a, const dim3& grid, hipStream_t st) {
+  if (!a.pages) attn_rows_kernel<HD, CT, CAP, kContiguous><<<grid, 2 * HD, 0, st>>>(a);
+  else if (a.page % kTile == 0) attn_rows_kernel<HD, CT, CAP, kWholeTiles><<<grid, 2 * HD, 0, st>>>(a);
+  else attn_rows_kernel<HD, CT, CAP, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
 }
 // Caps above kPlainCap take one column tile (two do not fit the registers), in one kernel for every order of the cache: they are
 // the rare ones. Measured (us; cap 257, then 30): 2048 rows causal, 40 / 8 heads of 128 117, 93; 7 documents in them 41, 38; 500
 // rows causal over 4500 keys, 32 / 8 101, 79; 777 over 3778, 16 / 2 of 256 159, 107. A single row over 131072 keys 99.6, 99.5.
 template <int HD, int CT>
-void launch_chunk(const MaskedArgs& a, const dim3& grid, hipStream_t st) {
+void launch_chunk(const MaskedRows& a, const dim3& grid, hipStream_t st) {
   if constexpr (CT == 1)
-    if (a.form == kAnyCap) return attn_masked_kernel<HD, 1, kAnyCap, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
+    if (a.form == kAnyCap) return attn_rows_kernel<HD, 1, kAnyCap, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
   if (a.form == kPlain) launch_order<HD, CT, kPlain>(a, grid, st);
   else launch_order<HD, CT, kNoCap>(a, grid, st);
 }
@@ -1032,7 +455,7 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
   const size_t need = p.splits == 1 ? 0 : part_bytes(T * shape->q_heads * p.splits, shape->head_dim);
   if (need && (!ws || off(ws, 16) || ws_bytes < need))
     return mi_fail(MI_ERR_ARG, "attn_masked: the workspace is null, misaligned (16 bytes) or below mi_attn_masked_ws");
-  MaskedArgs a{};
+  MaskedRows a{};
   a.q = attn_q;
   a.k = kv_k;
   a.v = kv_v;
@@ -1067,8 +490,8 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
   const dim3 grid(shape->kv_heads, (T + p.rows - 1u) / p.rows, p.splits);
   const bool narrow = shape->head_dim == 128;
   if (p.few) {
-    if (narrow) attn_masked_few_kernel<128><<<grid, 256, 0, st>>>(a);
-    else attn_masked_few_kernel<256><<<grid, 256, 0, st>>>(a);
+    if (narrow) attn_rows_few_kernel<128><<<grid, 256, 0, st>>>(a);
+    else attn_rows_few_kernel<256><<<grid, 256, 0, st>>>(a);
   } else if (narrow) {
     if (p.ct == 2) launch_chunk<128, 2>(a, grid, st);
     else launch_chunk<128, 1>(a, grid, st);
