@@ -36,8 +36,13 @@ extern "C" {
  * activation left the fp16 range): the argmax kernels set it when the word was 0, and the
  * step's token is not to be used. */
 #define MI_STATUS_NONFINITE 0xDEAD0004u
-/* mi_attn_masked's flag word after a page table entry outside the cache. */
+/* mi_attn_masked's flag word after a page table entry outside the cache; also of the entries of a step of several
+ * sequences, where a cache row lies outside. */
 #define MI_STATUS_BAD_PAGE 0xDEAD0005u
+/* mi_block_tables' flag word where the ring has too few free pages, and where lengths, tables, ring or parents cannot be
+ * (mi_attn_tree's: where sequences overlap). */
+#define MI_STATUS_NO_PAGES 0xDEAD0006u
+#define MI_STATUS_BAD_ROWS 0xDEAD0007u
 
 enum {
   MI_OK = 0,
@@ -576,6 +581,137 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
                    size_t head_stride, const uint32_t* pages, uint32_t page, uint32_t n_pages,
                    uint32_t kv_len, uint32_t T, const mi_attn_shape* shape, const mi_attn_mask* mask,
                    void* ws, size_t ws_bytes, uint16_t* attn_out, uint32_t* flag, void* stream);
+
+/* ---- a step of several sequences over one paged cache, each with one row, a tree of drafted tokens, beams or a stretch of a
+ * prompt. No counterpart in the reference, whose lists and batched rows are chains; the conventions are those of the entries
+ * above, and of the scoring entries on capture, workspaces and alignment. Rows of all sequences lie one behind another: sequence b
+ * has the rows row_start[b] .. row_start[b + 1] - 1; arrays of ids hold 0xFFFFFFFF for none. A step is
+ *   mi_block_tables    pages, cache rows, positions and the trees' masks, once
+ *   mi_rope_rows, mi_attn_tree   in each layer, between the linears
+ *   mi_beam_select or the heads' argmax and mi_accept_tree, then mi_kv_move for the rows whose tokens stay ---- */
+/* The plan of a step from the requests' lengths. Request b has cached[b] keys in the pages that its table's first held[b] entries
+ * name, and adds added[b] rows (0 and 0: it is done). It takes pages from the ring where ceil((cached + added) / page) is more than
+ * held, request after request, and gives back those behind that number where it is less; the pages given back are free from
+ * the next call on. ring: ring_len page ids, ring_at {first free one's place, how many are free}; a ring as long as there are
+ * pages never overflows. held_out and ring_at_out may be held and ring_at themselves (a captured step then goes on from replay
+ * to replay); they, cached and added do not overlap otherwise.
+ *   row_start [requests + 1]; of row t = row_start[b] + i: seq[t] = b, slot[t] the cache row of key cached[b] + i, pos[t] that key
+ *   with parent [rows] (of each row the number of its parent among its sequence's rows, below its own, or none): mask [rows][words]
+ *   gets bit i and the bits of its ancestors, and pos[t] = cached[b] + how many ancestors it has. words >= added / 32.
+ * rows is the arrays' size: rows behind the last sequence's get seq and slot none, pos 0, an empty mask. Where a request does not
+ * fit (held < cached / page, more than table_stride pages or 32 words of nodes, more rows than `rows`) *flag = MI_STATUS_BAD_ROWS,
+ * where the ring has too few pages MI_STATUS_NO_PAGES: then row_start is all 0, no row has a slot, tables and ring are as they were
+ * and held_out and ring_at_out repeat held and ring_at. A parent that is not below its child counts as none (MI_STATUS_BAD_ROWS); a
+ * page id that is not below n_pages gives slot none (MI_STATUS_BAD_PAGE). flag may be NULL.
+ * 1..1024 requests, rows up to 65535, cached + added up to 2^30, words up to 64. ws: mi_block_tables_ws bytes, 4-byte aligned. */
+typedef struct mi_block_plan {
+  uint32_t requests, rows, page, n_pages, table_stride, ring_len, words;
+  const uint32_t* cached;
+  const uint32_t* added;
+  const uint32_t* held;
+  uint32_t* held_out;
+  uint32_t* tables; /* [requests][table_stride] */
+  uint32_t* ring;
+  const uint32_t* ring_at;
+  uint32_t* ring_at_out;
+  const uint32_t* parent; /* NULL: no trees, and no masks */
+  uint32_t* row_start;
+  uint32_t* seq;
+  uint32_t* slot;
+  uint32_t* pos;
+  uint32_t* mask;
+  uint32_t* flag;
+} mi_block_plan;
+size_t mi_block_tables_ws(uint32_t requests);
+int mi_block_tables(const mi_block_plan* plan, void* ws, size_t ws_bytes, void* stream);
+/* A rotation's frequencies: pair i of rot_dim / 2 has f_i = theta^(-2 i / rot_dim), divided by divisors[i] where those are
+ * given (host array), and then by `factor` as scaling says:
+ *   MI_ROPE_NONE        not (factor is not read)
+ *   MI_ROPE_LINEAR      every one
+ *   MI_ROPE_BASE        theta is multiplied by factor^(rot_dim / (rot_dim - 2)) instead
+ *   MI_ROPE_WAVELENGTH  pairs that turn `low` times or less within `original` positions whole, those of `high` turns or more not, and
+ *                       between them mixed linearly by their turns
+ *   MI_ROPE_YARN        the same two limits (usual: low 1, high 32), mixed linearly by the pair's number between the pairs that
+ *                       have them (rounded outwards)
+ * Cosines and sines are multiplied with `attention`; 0: its default, 0.1 ln(factor) + 1 for MI_ROPE_YARN with factors above 1, else 1. */
+enum { MI_ROPE_NONE = 0, MI_ROPE_LINEAR = 1, MI_ROPE_BASE = 2, MI_ROPE_WAVELENGTH = 3, MI_ROPE_YARN = 4 };
+typedef struct mi_rope {
+  uint32_t rot_dim;
+  float theta;
+  uint32_t scaling;
+  float factor;
+  uint32_t original;
+  float low, high;
+  float attention;
+  const float* divisors;
+} mi_rope;
+/* table [n][2][rot_dim / 2] fp32 = (cos, sin)(p f_i) of the positions pos0 .. pos0 + n - 1, formed in 64 bits and rounded once:
+ * what mi_attn_prep, mi_attn_prep_rows and mi_rope_rows read. rot_dim a multiple of 8 up to 256, positions below 2^31. */
+int mi_rope_table(const mi_rope* rope, uint32_t pos0, uint32_t n, float* table, void* stream);
+/* Rows of q||k||v (in_kind MI_OUT_F32 or MI_OUT_F16, rows in_stride elements apart): q and k are normed by head (RMSNorm with
+ * q_norm / k_norm fp32 [head_dim], NULL = none, shape->eps), their first rot_dim dims turned by the table's row of position pos[t]
+ * (NULL: pos0 + t), pairs (i, i + rot_dim / 2), or with paired = 1 the neighbours (2 i, 2 i + 1); q -> attn_q fp32
+ * [T][q_heads][head_dim], k and v as f16 (shape->act as mi_attn_prep) to cache row slots[t] (NULL: the position) at
+ * row * row_stride + head * head_stride. All of it in fp32, each k and v rounded once: mi_attn_prep_rows rounds to f16 before and
+ * behind the norm too. A slot of none: the row has no k and v to store. rows: the cache's; a slot that is not below it
+ * stores neither (MI_STATUS_BAD_PAGE); a position that is not below rope_len (the table's rows) stores nothing of its row
+ * (0xDEAD0002). flag may be NULL. Slots are distinct. head_dim 128 or 256, rot_dim a multiple of 8, T up to 65535, not gated. */
+int mi_rope_rows(const void* qkv, uint32_t in_kind, size_t in_stride, uint32_t T, const uint32_t* pos, uint32_t pos0,
+                 const uint32_t* slots, uint32_t rows, const mi_attn_shape* shape, uint32_t paired, const float* q_norm,
+                 const float* k_norm, const float* rope, uint32_t rope_len, float* attn_q, uint16_t* kv_k, uint16_t* kv_v,
+                 size_t row_stride, size_t head_stride, uint32_t* flag, void* stream);
+/* The sequences of mi_attn_tree, device arrays. Row i of sequence b sees the keys j < cached[b] and, of the step's own keys
+ * cached[b] + c (its rows' k and v are in the cache already), those whose bit c of mask [T][words] is set; without masks c <= i.
+ * Key j of sequence b lies in cache row tables[b][j / page] * page + j % page, or without tables in row b * table_stride + j. */
+typedef struct mi_attn_batch {
+  uint32_t sequences;
+  uint32_t kv_len; /* no sequence's keys at or behind it are read: tables hold that many */
+  const uint32_t* row_start;
+  const uint32_t* cached;
+  const uint32_t* tables;
+  uint32_t table_stride, page, n_pages;
+  const uint32_t* mask;
+  uint32_t words;
+} mi_attn_batch;
+/* Attention of T rows of several sequences (q fp32 [T][q_heads][head_dim], magnitudes below 65504) over the f16 cache; attn_out
+ * [T][q_heads * head_dim] f16 (shape->act as mi_attn_reduce). A row that sees nothing gives zeros; rows before row_start[0] and behind
+ * row_start[sequences] (T is the arrays' size) are left as they were, and a sequence may have no rows. Sums, softmax and
+ * probabilities are fp32; calls of more than 16 columns a sequence on average (T / sequences rows, rounded up, times q heads per kv
+ * head) round each probability's numerator to f16 before the product with V, the others keep it in two f16 halves. How the keys are cut into
+ * parts follows the lengths of all sequences, so a row's last bits depend on T and on the lengths beside it, never on the values.
+ * What a row does not see has no part in it, infinities and NaN included. A table entry that is not below n_pages, of a page that holds
+ * a key of a sequence with rows, sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL); nothing outside the cache is read. row_start
+ * does not fall; sequences that overlap so much that they are more than T rows are refused on the device (MI_STATUS_BAD_ROWS, no row
+ * is written). head_dim 128 or 256, up to 64 q heads per kv head, not gated; T up to 65535, 1..1024 sequences, kv_len up to 2^30,
+ * words 1..64 with masks, 0 without. ws: mi_attn_tree_ws bytes of device scratch, 16-byte aligned; its size never falls as T grows
+ * and is the same for any number of sequences. */
+size_t mi_attn_tree_ws(uint32_t T, uint32_t sequences, const mi_attn_shape* shape);
+int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v, size_t row_stride, size_t head_stride,
+                 uint32_t T, const mi_attn_shape* shape, const mi_attn_batch* batch, void* ws, size_t ws_bytes,
+                 uint16_t* attn_out, uint32_t* flag, void* stream);
+/* mi_accept_greedy for a tree, on the host: node 0 is the text's next token, tokens and parent those of the n nodes, argmax what the
+ * model says behind each. From node 0 on, the child whose token is its parent's argmax is accepted (the first of equal ones).
+ * Returns the number of accepted drafts, their nodes in path [n - 1]; *next = the argmax behind the last. */
+uint32_t mi_accept_tree(const uint32_t* argmax, const uint32_t* tokens, const uint32_t* parent, uint32_t n, uint32_t* path,
+                        uint32_t* next);
+/* The k best continuations of each of `batch` texts over its beams and the vocabulary: logits fp32 [batch * beams][vocab_used], rows
+ * row_stride apart; a candidate (beam w, token v) scores cum[w] + log softmax(logits of w)[v]; larger scores come first, equal ones
+ * by the lower beam, then the lower token (of one beam the order is the logits'). done [batch * beams] (NULL: none): a beam at its
+ * end has one candidate, the token eos with its own score. ids, from (the beam within its text), scores [batch][k]; where there are
+ * fewer candidates of a score above -inf: none, none, -inf (a NaN or a +inf among a beam's logits leaves it without
+ * candidates). 1..64 beams, batch * beams up to 65535, vocab_used up to 2^23, k 1..64. ws: mi_beam_select_ws bytes, 16-byte aligned. */
+size_t mi_beam_select_ws(uint32_t batch, uint32_t beams, uint32_t vocab_used, uint32_t k);
+int mi_beam_select(const float* logits, size_t row_stride, const float* cum, const uint32_t* done, uint32_t eos, uint32_t batch,
+                   uint32_t beams, uint32_t vocab_used, uint32_t k, uint32_t* ids, uint32_t* from, float* scores, void* ws,
+                   size_t ws_bytes, void* stream);
+/* Moves cache rows, in every layer (layer_stride elements apart) and kv head, K and V: row from[g][i] to row to[g][i], of `groups` lists
+ * of `per` (1..64). Within a list all rows are read before one is written: a tree's accepted rows closed up (list = sequence),
+ * beams that change places (list = the beams' rows of one position). No row is written by two entries, and none that another list
+ * writes is read or written. to = none: no move. A row that is not below `rows` (the cache's) is not moved (MI_STATUS_BAD_PAGE, flag may be
+ * NULL). head_dim 128 or 256. */
+int mi_kv_move(uint16_t* kv_k, uint16_t* kv_v, uint32_t layers, size_t layer_stride, size_t row_stride, size_t head_stride,
+               uint32_t kv_heads, uint32_t head_dim, uint32_t rows, const uint32_t* from, const uint32_t* to, uint32_t groups,
+               uint32_t per, uint32_t* flag, void* stream);
 
 /* ---- the decode loop (src/runtime/engine.h:52-331, capture.cc, control.h) ----
  * Model shape as data (model::ModelDesc, src/model/model_desc.h:67-229), restricted to the

@@ -117,6 +117,16 @@ SIGNATURES = {
     "mi_logprobs": (i32, [vp, sz, vp, u32, u32, u32, vp, vp, vp, vp, vp, vp, sz, vp]),
     "mi_attn_masked_ws": (sz, [u32, u32, vp]),
     "mi_attn_masked": (i32, [vp, vp, vp, sz, sz, vp, u32, u32, u32, u32, vp, vp, vp, sz, vp, vp, vp]),
+    "mi_block_tables_ws": (sz, [u32]),
+    "mi_block_tables": (i32, [vp, vp, sz, vp]),
+    "mi_rope_table": (i32, [vp, u32, u32, vp, vp]),
+    "mi_rope_rows": (i32, [vp, u32, sz, u32, vp, u32, vp, u32, vp, u32, vp, vp, vp, u32, vp, vp, vp, sz, sz, vp, vp]),
+    "mi_attn_tree_ws": (sz, [u32, u32, vp]),
+    "mi_attn_tree": (i32, [vp, vp, vp, sz, sz, u32, vp, vp, vp, sz, vp, vp, vp]),
+    "mi_accept_tree": (u32, [vp, vp, vp, u32, vp, vp]),
+    "mi_beam_select_ws": (sz, [u32, u32, u32, u32]),
+    "mi_beam_select": (i32, [vp, sz, vp, vp, u32, u32, u32, u32, u32, vp, vp, vp, vp, sz, vp]),
+    "mi_kv_move": (i32, [vp, vp, u32, sz, sz, sz, u32, u32, u32, vp, vp, u32, u32, vp, vp]),
 }
 
 
@@ -137,6 +147,10 @@ class GemvEpilogue(C.Structure):
 
 STATUS_HANDOFF_TIMEOUT = 0xDEAD0003
 STATUS_BAD_PAGE = 0xDEAD0005
+STATUS_NO_PAGES = 0xDEAD0006
+STATUS_BAD_ROWS = 0xDEAD0007
+NONE = 0xFFFFFFFF  # an array's id that is none (mi_block_tables, mi_beam_select, mi_kv_move)
+ROPE_NONE, ROPE_LINEAR, ROPE_BASE, ROPE_WAVELENGTH, ROPE_YARN = range(5)  # mi_rope.scaling
 OUT_F32, OUT_F16 = 0, 1  # mi_gemm_w8a8's and mi_linear_w8a8's out_kind
 
 
@@ -196,6 +210,25 @@ class AttnShape(C.Structure):
 class AttnMask(C.Structure):
     """mi_attn_mask: the rows' spans of keys, the cap of the scores and the bias by distance."""
     _fields_ = [("lo", vp), ("hi", vp), ("pos", vp), ("pos0", u32), ("prefix", u32), ("cap", f32), ("slopes", vp)]
+
+
+class BlockPlan(C.Structure):
+    """mi_block_plan: requests' lengths, tables and free pages, and what a step's plan writes."""
+    _fields_ = [(n, u32) for n in ("requests", "rows", "page", "n_pages", "table_stride", "ring_len", "words")] + \
+               [(n, vp) for n in ("cached", "added", "held", "held_out", "tables", "ring", "ring_at", "ring_at_out", "parent",
+                                  "row_start", "seq", "slot", "pos", "mask", "flag")]
+
+
+class Rope(C.Structure):
+    """mi_rope: a rotation's frequencies and how they are scaled."""
+    _fields_ = [("rot_dim", u32), ("theta", f32), ("scaling", u32), ("factor", f32), ("original", u32), ("low", f32),
+                ("high", f32), ("attention", f32), ("divisors", vp)]
+
+
+class AttnBatch(C.Structure):
+    """mi_attn_batch: the sequences of a call, where their keys are and what their rows see."""
+    _fields_ = [("sequences", u32), ("kv_len", u32), ("row_start", vp), ("cached", vp), ("tables", vp), ("table_stride", u32),
+                ("page", u32), ("n_pages", u32), ("mask", vp), ("words", u32)]
 
 
 def lib_shape(sh, act=0):
@@ -402,6 +435,15 @@ class Engine:
         import numpy as np
         lg = self.to_host(T_LOGITS, dtype=np.float32)
         return lg[:rows * self.desc.vocab].reshape(rows, self.desc.vocab)
+
+
+def accept_tree(argmax, tokens, parent):
+    """mi_accept_tree: (the accepted drafts' nodes, next token)."""
+    import numpy as np
+    a, t, p = (np.ascontiguousarray(x, np.uint32) for x in (argmax, tokens, parent))
+    path, nxt = np.zeros(a.size, np.uint32), u32()
+    j = lib().mi_accept_tree(a.ctypes.data, t.ctypes.data, p.ctypes.data, a.size, path.ctypes.data, C.byref(nxt))
+    return path[:j], int(nxt.value)
 
 
 def accept_greedy(verify_argmax, drafts):

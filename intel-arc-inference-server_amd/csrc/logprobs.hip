@@ -27,7 +27,7 @@
 namespace mi {
 namespace {
 
-constexpr uint32_t kMaxRows = 65535, kMaxVocab = 1u << 23, kMaxTop = 64, kNone = 0xFFFFFFFFu;
+constexpr uint32_t kMaxRows = 65535, kMaxVocab = 1u << 23, kMaxTop = 64, kMaxBeams = 64, kNone = 0xFFFFFFFFu;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogprobArgs {
@@ -40,6 +40,7 @@ struct LogprobArgs {
   // where a row has several slices: (m, Z, T, count) per (row, slice), the largest logit per (row, 256 tokens)
   f4_t* stats;
   float* peaks;
+  f2_t* sums;  // NULL, or the rows' (m, Z): top_logprobs are then the logits themselves
 };
 
 // ---- the statistics ----
@@ -215,10 +216,11 @@ __device__ __forceinline__ void answer(const LogprobArgs& a, uint32_t row, const
   if (a.entropy) a.entropy[row] = log_z - s.t / s.z * kLn2;
   if (a.logprob) a.logprob[row] = (xt - s.m) - log_z;
   if (a.rank) a.rank[row] = xt != xt ? kNone : count;
+  if (a.sums) a.sums[row] = f2_t{s.m, s.z};
 }
 __device__ __forceinline__ void answer_top(const LogprobArgs& a, uint32_t row, uint32_t place, Entry e, const Stats& s, float log_z) {
   a.top_ids[(size_t)row * a.top + place] = e.id;
-  a.top_logprobs[(size_t)row * a.top + place] = e.id == kNone ? -INFINITY : (e.v - s.m) - log_z;
+  a.top_logprobs[(size_t)row * a.top + place] = e.id == kNone ? -INFINITY : a.sums ? e.v : (e.v - s.m) - log_z;
 }
 
 // four values' maxima over the wave: lane 0 the first's, 32 the second's, 16 the third's, 48 the fourth's
@@ -540,12 +542,94 @@ __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
   if (lane < a.top) answer_top(a, row, lane, list, s, log_z);
 }
 
+// ---- the best continuations of beams ----
+// A candidate: a token of a beam with the score cum + (x - m) - log Z, in 64 bits, so that candidates of different beams are
+// told apart as far as Z (in 32 bits) tells them. A beam's candidates stand in the order of their logits; equal scores go to the
+// lower beam, then to the lower place.
+struct Candidate {
+  double score = -INFINITY;
+  uint32_t at = kNone;  // 64 beam + place; kNone: none
+};
+__device__ __forceinline__ bool better(const Candidate& a, const Candidate& b) {
+  return a.score > b.score || (a.score == b.score && a.at < b.at);
+}
+template <uint32_t X>
+__device__ __forceinline__ void half_clean(Candidate& e, uint32_t lane) {  // strides X .. 1, best first
+  const uint64_t s = __builtin_bit_cast(uint64_t, e.score);
+  const Candidate o = {__builtin_bit_cast(double, (uint64_t)xor_lane<X>((uint32_t)(s >> 32)) << 32 | xor_lane<X>((uint32_t)s)),
+                       xor_lane<X>(e.at)};
+  if (better(o, e) == ((lane & X) == 0)) e = o;
+  if constexpr (X > 1) half_clean<X / 2>(e, lane);
+}
+
+struct BeamArgs {
+  const float* cum;
+  const uint32_t* done;
+  const f2_t* sums;         // [rows]
+  const uint32_t* top_ids;  // [rows][k]
+  const float* top;         // [rows][k], logits
+  uint32_t eos, beams, k;
+  uint32_t *ids, *from;
+  float* scores;
+};
+// grid (batch), four waves: a wave merges every fourth beam's candidates, 64 at a time over its lanes, then the waves' join. Bound by
+// its chain: a few loads, six exchanges a beam.
+__global__ __launch_bounds__(256) void beam_select_kernel(BeamArgs a) {
+  __shared__ double score[4][64];
+  __shared__ uint32_t place[4][64];
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, batch = blockIdx.x;
+  Candidate list;
+  for (uint32_t w = wave; w < a.beams; w += 4u) {
+    const uint32_t row = batch * a.beams + w, n = 63u - lane;  // (best last)
+    Candidate c;
+    const double cum = (double)a.cum[row];
+    if (a.done && a.done[row]) {
+      if (n == 0u && cum > -INFINITY) c = Candidate{cum, 64u * w};
+    } else if (n < a.k && a.top_ids[(size_t)row * a.k + n] != kNone) {
+      const f2_t s = a.sums[row];
+      const double of = cum + ((double)a.top[(size_t)row * a.k + n] - (double)s.x) - log((double)s.y);
+      if (of > -INFINITY) c = Candidate{of, 64u * w + n};  // (nor a NaN)
+    }
+    if (better(c, list)) list = c;
+    half_clean<32>(list, lane);
+  }
+#pragma unroll 1
+  for (uint32_t step = 2; step; step /= 2) {
+    score[wave][lane] = list.score;
+    place[wave][lane] = list.at;
+    __syncthreads();
+    if (wave >= step) return;
+    const Candidate o = {score[wave + step][63u - lane], place[wave + step][63u - lane]};
+    if (better(o, list)) list = o;
+    half_clean<32>(list, lane);
+  }
+  if (lane >= a.k) return;
+  const size_t to = (size_t)batch * a.k + lane;
+  const uint32_t w = list.at / 64u, row = batch * a.beams + w;
+  const bool none = list.at == kNone;
+  a.ids[to] = none ? kNone : a.done && a.done[row] ? a.eos : a.top_ids[(size_t)row * a.k + list.at % 64u];
+  a.from[to] = none ? kNone : w;
+  a.scores[to] = (float)list.score;
+}
+
 // The slices of a row: one where the rows alone fill the chip.
 void pick_slices(uint32_t M, uint32_t vocab, uint32_t* slices, uint32_t* slice) {
   const uint32_t want = std::max(1u, 1024u / M), most = (vocab + 1023u) / 1024u;
   const uint32_t n = std::min(want, most);
   *slice = n == 1 ? vocab : ((vocab + n - 1u) / n + 1023u) / 1024u * 1024u;
   *slices = (vocab + *slice - 1u) / *slice;
+}
+
+void launch(LogprobArgs a, uint32_t M, void* ws, hipStream_t st) {
+  pick_slices(M, a.vocab, &a.slices, &a.slice);
+  if (a.slices == 1) {
+    logprobs_kernel<true><<<dim3(1, M), 256, 0, st>>>(a);
+  } else {
+    a.stats = static_cast<f4_t*>(ws);
+    a.peaks = reinterpret_cast<float*>(a.stats + (size_t)M * a.slices);
+    logprobs_kernel<false><<<dim3(a.slices, M), 256, 0, st>>>(a);
+    logprobs_join_kernel<<<M, 512, 0, st>>>(a);
+  }
 }
 
 }  // namespace
@@ -580,21 +664,44 @@ int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, 
   const size_t need = mi_logprobs_ws(M, vocab_used, top);
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < need))
     return mi_fail(MI_ERR_ARG, "logprobs: the workspace is null, misaligned (16 bytes) or below mi_logprobs_ws");
-  LogprobArgs a{logits, row_stride, tokens, vocab_used, top, 1, vocab_used, logprob, entropy, top_logprobs, rank, top_ids,
-                nullptr, nullptr};
-  pick_slices(M, vocab_used, &a.slices, &a.slice);
-  if (need) {
-    a.stats = static_cast<f4_t*>(ws);
-    a.peaks = reinterpret_cast<float*>(a.stats + (size_t)M * a.slices);
-  }
-  hipStream_t st = (hipStream_t)stream;
-  if (a.slices == 1) {
-    logprobs_kernel<true><<<dim3(1, M), 256, 0, st>>>(a);
-  } else {
-    logprobs_kernel<false><<<dim3(a.slices, M), 256, 0, st>>>(a);
-    logprobs_join_kernel<<<M, 512, 0, st>>>(a);
-  }
+  const LogprobArgs a{logits, row_stride, tokens, vocab_used, top, 1, vocab_used, logprob, entropy, top_logprobs, rank, top_ids,
+                      nullptr, nullptr, nullptr};
+  launch(a, M, ws, (hipStream_t)stream);
   return mi_hip((int)hipGetLastError(), "logprobs");
+}
+
+size_t mi_beam_select_ws(uint32_t batch, uint32_t beams, uint32_t vocab_used, uint32_t k) {
+  if (batch == 0 || beams == 0 || beams > kMaxBeams || (uint64_t)batch * beams > kMaxRows || vocab_used == 0 ||
+      vocab_used > kMaxVocab || k == 0 || k > kMaxTop)
+    return 0;
+  const uint32_t rows = batch * beams;
+  return (size_t)rows * (8u + 8u * k) + 16u + mi_logprobs_ws(rows, vocab_used, k);
+}
+
+int mi_beam_select(const float* logits, size_t row_stride, const float* cum, const uint32_t* done, uint32_t eos, uint32_t batch,
+                   uint32_t beams, uint32_t vocab_used, uint32_t k, uint32_t* ids, uint32_t* from, float* scores, void* ws,
+                   size_t ws_bytes, void* stream) {
+  for (const void* p : {(const void*)logits, (const void*)cum, (const void*)ids, (const void*)from, (const void*)scores})
+    if (!p || (reinterpret_cast<uintptr_t>(p) & 3u)) return mi_fail(MI_ERR_ARG, "beam_select: null or misaligned pointer (4 bytes)");
+  if (reinterpret_cast<uintptr_t>(done) & 3u) return mi_fail(MI_ERR_ARG, "beam_select: misaligned done (4 bytes)");
+  if (batch == 0 || beams == 0 || beams > kMaxBeams || (uint64_t)batch * beams > kMaxRows)
+    return mi_fail(MI_ERR_SHAPE, "beam_select: 1..64 beams, batch * beams 1..65535");
+  if (vocab_used == 0 || vocab_used > kMaxVocab || k == 0 || k > kMaxTop)
+    return mi_fail(MI_ERR_SHAPE, "beam_select: vocab_used 1..2^23, k 1..64");
+  if (row_stride < vocab_used) return mi_fail(MI_ERR_ARG, "beam_select: row_stride below vocab_used");
+  if (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < mi_beam_select_ws(batch, beams, vocab_used, k))
+    return mi_fail(MI_ERR_ARG, "beam_select: the workspace is null, misaligned (16 bytes) or below mi_beam_select_ws");
+  const uint32_t rows = batch * beams;
+  f2_t* sums = static_cast<f2_t*>(ws);
+  float* top = reinterpret_cast<float*>(sums + rows);
+  uint32_t* top_ids = reinterpret_cast<uint32_t*>(top + (size_t)rows * k);
+  const uintptr_t end = (reinterpret_cast<uintptr_t>(top_ids + (size_t)rows * k) + 15u) & ~(uintptr_t)15u;
+  const LogprobArgs a{logits, row_stride, nullptr, vocab_used, k, 1, vocab_used, nullptr, nullptr, top, nullptr, top_ids,
+                      nullptr, nullptr, sums};
+  hipStream_t st = (hipStream_t)stream;
+  launch(a, rows, reinterpret_cast<void*>(end), st);
+  beam_select_kernel<<<batch, 256, 0, st>>>(BeamArgs{cum, done, sums, top_ids, top, eos, beams, k, ids, from, scores});
+  return mi_hip((int)hipGetLastError(), "beam_select");
 }
 
 }  // extern "C"

@@ -1,0 +1,195 @@
+"""mi_beam_select and mi_kv_move.
+
+A score is cum + x - m - log Z. Z is a sum of positive terms in 32 bits: at most vocab / 256 + 30 of them one after another (2^-24 each),
+a term off by |x - m| 2^-22 of it (the exponent's two roundings) and an exponential's 2^-22. That holds for log Z, and the score rounds
+once more. Candidates whose exact scores are closer than that may change places."""
+import numpy as np
+import pytest
+
+from mipkg import dev, empty, host, mi, ptr, stream, sync, torch
+
+pytestmark = pytest.mark.gpu
+NONE, GUARD = mi.NONE, 16
+
+
+class Beams:
+    def __init__(self, seed, batch, beams, used, k, done=False, std=2.0, stride=0):
+        rng = np.random.default_rng(seed)
+        self.__dict__.update(batch=batch, beams=beams, used=used, k=k, stride=stride or used, eos=used // 2)
+        self.x = (rng.standard_normal((batch * beams, self.stride)) * std).astype(np.float32)
+        self.cum = rng.uniform(-9, -1, batch * beams).astype(np.float32)
+        self.done = (rng.random(batch * beams) < 0.4).astype(np.uint32) if done else None
+
+    def bind(self):
+        d = {n: dev(getattr(self, n)) for n in ("x", "cum", "done")}
+        for n, t in (("ids", np.uint32), ("from", np.uint32), ("scores", np.float32)):
+            d[n] = empty((self.batch * self.k + GUARD,), t)
+            d[n].fill_(99)
+        need = mi.lib().mi_beam_select_ws(self.batch, self.beams, self.used, self.k)
+        d["ws"], d["need"] = dev(np.full(need + GUARD, 77, np.uint8)), need
+        d["args"] = (ptr(d["x"]), self.stride, ptr(d["cum"]), ptr(d["done"]), self.eos, self.batch, self.beams, self.used, self.k, ptr(d["ids"]),
+                     ptr(d["from"]), ptr(d["scores"]), ptr(d["ws"]), need)
+        return d
+
+    def result(self, d):
+        sync()
+        assert (host(d["ws"], np.uint8)[d["need"]:] == 77).all()
+        out = []
+        for n, t in (("ids", np.uint32), ("from", np.uint32), ("scores", np.float32)):
+            a = host(d[n], t)
+            assert (a[-GUARD:] == 99).all()
+            out.append(a[:-GUARD].reshape(self.batch, self.k))
+        return out
+
+    def run(self, st=None):
+        d = self.bind()
+        mi.call("mi_beam_select", *d["args"], stream() if st is None else st)
+        return self.result(d)
+
+    def check(self, got=None):
+        ids, beams, scores = self.run() if got is None else got
+        for b in range(self.batch):
+            best, tol, lists = [], 0.0, {}
+            for w in range(self.beams):
+                r = b * self.beams + w
+                cum = np.float64(self.cum[r])
+                if self.done is not None and self.done[r]:
+                    lists[w] = {self.eos: cum} if cum > -np.inf else {}
+                    best += [(-cum, w, 0)] if cum > -np.inf else []
+                    continue
+                x = self.x[r, :self.used].astype(np.float64)
+                lists[w] = {}
+                if np.isnan(x).any() or (x == np.inf).any() or not (x > -np.inf).any() or not cum > -np.inf:
+                    continue
+                m = x.max()
+                e = np.exp(x - m)
+                s = cum + x - m - np.log(e.sum())
+                with np.errstate(invalid="ignore"):
+                    off = np.where(e > 0, e * np.abs(x - m), 0).sum() / e.sum()
+                tol = max(tol, (self.used / 256 + 30) * 2.0 ** -24 + 2.0 ** -22 * (1 + off))
+                order = np.lexsort((np.arange(self.used), -x))[:self.k]
+                order = order[s[order] > -np.inf]
+                lists[w] = {int(v): s[v] for v in order}
+                best += [(-s[v], w, n) for n, v in enumerate(order)]
+            best.sort()
+            n = min(len(best), self.k)
+            assert (ids[b, n:] == NONE).all() and (beams[b, n:] == NONE).all() and (scores[b, n:] == -np.inf).all()
+            taken = {w: 0 for w in lists}
+            for i in range(n):
+                w, v = int(beams[b, i]), int(ids[b, i])
+                assert list(lists[w])[taken[w]] == v  # a beam's own candidates in their order
+                taken[w] += 1
+                s = lists[w][v]
+                slack = tol + 2.0 ** -23 * abs(s)
+                assert abs(s + best[i][0]) <= 2 * slack and abs(scores[b, i] - s) <= slack
+            assert np.all(np.diff(scores[b, :n]) <= 0)
+        return ids, beams, scores
+
+
+@pytest.mark.parametrize("batch,beams,used,k", [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 7, 64), (1, 4, 151936, 8), (16, 8, 1000, 16), (3, 64, 500, 64),
+                                                (2, 5, 4099, 33), (129, 4, 2049, 5), (1, 1, 100000, 64), (40, 16, 300, 20)])
+@pytest.mark.parametrize("done", [False, True])
+def test_select(batch, beams, used, k, done):
+    Beams(used + k, batch, beams, used, k, done, stride=used + 3 if beams == 5 else 0).check()
+
+
+def test_equal_scores_go_to_the_lower_beam_then_the_lower_token():
+    c = Beams(1, 2, 4, 600, 40)
+    c.x[:] = np.round(c.x[0] * 2)  # equal rows, many equal logits
+    c.cum[:] = -3.0
+    ids, beams, _ = c.check()
+    x = c.x[0, :600]
+    want = sorted(((-x[v], w, v) for w in range(4) for v in range(600)))[:40]
+    for b in range(2):
+        assert [(int(w), int(v)) for w, v in zip(beams[b], ids[b])] == [(w, v) for _, w, v in want]
+
+
+def test_beams_without_candidates():
+    c = Beams(2, 3, 4, 900, 12)
+    c.cum[[1, 2, 3]] = -np.inf  # a text's first step: one beam lives
+    c.x[4, 7] = np.nan
+    c.x[5, 8] = np.inf
+    c.x[6] = -np.inf
+    c.x[7, 5:] = -np.inf  # a grammar that leaves five tokens
+    c.cum[8:] = -np.inf  # nothing lives
+    c.cum[9] = np.nan
+    ids, beams, scores = c.check()
+    assert (beams[0] == 0).all() and (beams[1, :5] == 3).all() and (ids[1, 5:] == NONE).all() and (ids[2] == NONE).all()
+    c = Beams(3, 1, 4, 900, 12)
+    c.done = np.array([1, 0, 1, 1], np.uint32)
+    c.cum = np.array([-1.0, -50.0, -np.inf, -2.0], np.float32)
+    ids, beams, scores = c.check()
+    assert list(beams[0, :2]) == [0, 3] and list(ids[0, :2]) == [c.eos] * 2 and (beams[0, 2:] == 1).all()
+
+
+def test_captured_select_and_other_stream():
+    T = torch()
+    c = Beams(4, 2, 8, 5000, 16, done=True)
+    d = c.bind()
+    g = T.cuda.CUDAGraph()
+    with T.cuda.graph(g):
+        mi.call("mi_beam_select", *d["args"], stream())
+    for seed in (5, 6, 7):
+        o = Beams(seed, 2, 8, 5000, 16, done=True)
+        for n in ("x", "cum", "done"):
+            d[n].copy_(dev(getattr(o, n)))
+        g.replay()
+        o.check(o.result(d))
+    side = T.cuda.Stream()
+    with T.cuda.stream(side):
+        c.check(c.run(side.cuda_stream))
+
+
+def move(k, v, rows, origin, to, by_row=False, flag=None, captured=False):
+    """k, v [layers][kv_heads][rows][hd] uint16; what mi_kv_move leaves of them"""
+    L, H, n, hd = k.shape
+    dk, dv = (dev(np.ascontiguousarray(x.transpose(0, 2, 1, 3)) if by_row else x) for x in (k, v))
+    strides = (H * hd, hd) if by_row else (hd, n * hd)
+    df, dt = dev(np.asarray(origin, np.uint32)), dev(np.asarray(to, np.uint32))
+    f = dev(np.zeros(1, np.uint32))
+    groups, per = np.shape(to)
+    mi.call("mi_kv_move", ptr(dk), ptr(dv), L, H * n * hd, *strides, H, hd, rows, ptr(df), ptr(dt), groups, per, ptr(f), stream())
+    sync()
+    assert int(host(f, np.uint32)[0]) == (flag or 0)
+    out = [host(x, np.uint16).reshape((L, n, H, hd) if by_row else (L, H, n, hd)) for x in (dk, dv)]
+    return [x.transpose(0, 2, 1, 3) if by_row else x for x in out]
+
+
+def moved(x, rows, origin, to):
+    y = x.copy()
+    for a, b in zip(np.ravel(origin), np.ravel(to)):
+        if b != NONE and a < rows and b < rows:
+            y[:, :, b] = x[:, :, a]
+    return y
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("groups,per", [(1, 1), (5, 3), (2, 16), (3, 17), (2, 33), (2, 64)])
+@pytest.mark.parametrize("by_row", [False, True])
+def test_moves_within_a_list_are_at_once(groups, per, hd, by_row):
+    """each list permutes, closes up or copies rows of its own stretch"""
+    rng = np.random.default_rng(groups * per + hd)
+    n = groups * 80 + 3
+    k, v = (rng.integers(0, 1 << 16, (3, 2, n, hd)).astype(np.uint16) for _ in range(2))
+    origin, to = [], []
+    for g in range(groups):
+        f, t = 80 * g + rng.integers(0, 80, per), 80 * g + rng.permutation(80)[:per]
+        if g % 3 == 1:
+            f = rng.permutation(t)
+        if g % 3 == 2:
+            f, t = 80 * g + np.sort(rng.permutation(80)[:per]), 80 * g + np.arange(per)
+        t = np.where(rng.random(per) < 0.2, NONE, t)
+        origin.append(f)
+        to.append(t)
+    got = move(k, v, n, origin, to, by_row)
+    for g, x in zip(got, (k, v)):
+        assert np.array_equal(g, moved(x, n, origin, to))
+
+
+def test_rows_outside_are_not_moved():
+    rng = np.random.default_rng(1)
+    k, v = (rng.integers(0, 1 << 16, (2, 3, 50, 128)).astype(np.uint16) for _ in range(2))
+    origin, to = [[1, 48, 3, NONE], [5, 6, 7, 8]], [[10, 11, 45, 12], [13, NONE, 44, 14]]
+    got = move(k, v, 45, origin, to, flag=mi.STATUS_BAD_PAGE)
+    for g, x in zip(got, (k, v)):
+        assert np.array_equal(g, moved(x, 45, origin, to))
