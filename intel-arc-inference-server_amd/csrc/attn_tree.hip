@@ -7,8 +7,8 @@
 // The kernels, and how their softmax and its roundings go, are attn_rows.h's.
 //
 // How the work is dealt out: a sequence's rows are cut into blocks of `rows`, its 32-key tiles into parts of `per` tiles, the same
-// for all sequences. A block, a part and a kv head are an item, and a work-group's. Lengths are the device's: every wave reads
-// them all, forms `per` and finds its item by itself. Items that read the same keys (a sequence's blocks) follow one another
+// for all sequences (a sequence's parts then as even as may be). A block, a part and a kv head are an item, and a work-group's.
+// Lengths are the device's: every wave reads them all, forms `per` and finds its item by itself. Items that read the same keys (a sequence's blocks) follow one another
 // and run on one XCD. Sequences of several parts leave sums, which a second launch joins.
 #include <algorithm>
 
@@ -18,7 +18,7 @@
 namespace mi {
 namespace {
 
-constexpr uint32_t kMaxRows = 65535, kMaxKeys = 1u << 30, kMaxSequences = 1024, kMaxWords = 64, kMaxSplits = 256, kXcds = 8;
+constexpr uint32_t kMaxRows = 65535, kMaxKeys = 1u << 30, kMaxSequences = 1024, kMaxWords = 64, kMaxSplits = 1024, kXcds = 8, kNone = 0xFFFFFFFFu;
 constexpr uint32_t kNoTree = 0x7FFFFFFFu;  // a column's `first` where it is none: every key lies before it
 
 struct TreeArgs {
@@ -30,8 +30,8 @@ struct TreeArgs {
   float* part;    // items of several parts: see part_at
   uint32_t* flag;
   size_t row_stride, head_stride;
-  uint32_t table_stride, page, page_shift, n_pages, kv_len, T, sequences, words, q_heads, kv_heads, gqa, rows, columns, share,
-      least, most_blocks, act;
+  uint32_t table_stride, page, page_shift, n_pages, kv_len, T, sequences, words, q_heads, kv_heads, gqa, rows, columns, slots,
+      share, least, most_blocks, act;
   float c;  // y = c q . k
 };
 
@@ -71,38 +71,77 @@ struct TreeRows : TreeArgs {
   };
   static constexpr bool kMayIdle = true;
 
+  static __device__ __forceinline__ uint32_t parts(const Sequence& s, uint32_t per) { return (s.tiles + per - 1u) / per; }
+  // Tiles of a part at most. With `even` tiles in each of the work-groups that run at once, and parts of `per` tiles that make `items`
+  // items, the call lasts per + 3 where all run at once, else even + per / 2 + 3 items / slots (in tiles; 3: an item's start).
+  // Few sequences of uneven lengths are near `even` in one round or none: of the candidates the least is taken. None is below
+  // total / share, so there are no more items than share and one for each block.
+  __device__ __forceinline__ uint32_t part_tiles(const Sequence& first, float total) const {
+    const uint32_t lane = threadIdx.x & 63u;
+    constexpr uint32_t N = 8;
+    constexpr float kOf[N] = {2.f, 1.5f, 1.25f, 1.125f, 1.f, 0.5f, 0.33f, 0.25f};
+    const float even = total * (float)kv_heads / (float)slots;
+    float items[N];
+    uint32_t per[N];
+#pragma unroll
+    for (uint32_t n = 0; n < N; ++n) {
+      per[n] = max(least, (uint32_t)fminf(fmaxf(even * kOf[n], total * 1.0001f / (float)share), (float)kMaxKeys) + 1u);
+      items[n] = 0.f;
+    }
+    for (uint32_t b = 0; b < sequences; b += 64u) {
+      const Sequence s = b ? sequence(*this, b + lane) : first;
+#pragma unroll
+      for (uint32_t n = 0; n < N; ++n)
+        items[n] += (float)s.blocks * ceilf((float)s.tiles * __builtin_amdgcn_rcpf((float)per[n]));
+    }
+    uint32_t best = 0;
+    float cost = INFINITY;
+#pragma unroll
+    for (uint32_t n = 0; n < N; ++n) {
+      const float turns = wave_sum(items[n]) * (float)kv_heads / (float)slots;
+      const float c = turns <= 1.f ? (float)per[n] + 3.f : even + 0.5f * (float)per[n] + 3.f * turns;
+      if (c < cost) {
+        cost = c;
+        best = per[n];
+      }
+    }
+    return best;
+  }
   __device__ __forceinline__ Place place(bool) const {
     const uint32_t lane = threadIdx.x & 63u;
     auto plus = [](uint32_t x, uint32_t y) { return x + y; };
-    // The parts: `share` of them, as the sum of all blocks' tiles has it (in fp32, a little too many rather than too few: so
-    // there are no more than share + the blocks' number). An item's number: the parts of the sequences before it.
+    Place p{};
+    if (sequences == 1u) {
+      const Sequence s = sequence(*this, 0u);
+      p.per = max(least, max(s.blocks, s.tiles) < 65536u ? (s.blocks * s.tiles + share - 1u) / share
+                                                         : (uint32_t)((float)s.blocks * (float)s.tiles * 1.0001f / (float)share) + 1u);
+      const uint32_t n = parts(s, p.per), item = item_of(s.blocks * n * kv_heads);
+      if (item == kNone) return p;
+      return inside(p, s, 0u, n, item, 0u);
+    }
     Sequence s = sequence(*this, lane);
     float total = (float)s.blocks * (float)s.tiles, blocks = (float)s.blocks;
-    for (uint32_t b = 64u + lane; b < sequences + lane; b += 64u) {
-      const Sequence o = sequence(*this, b);
+    for (uint32_t b = 64u; b < sequences; b += 64u) {
+      const Sequence o = sequence(*this, b + lane);
       total += (float)o.blocks * (float)o.tiles;
       blocks += (float)o.blocks;
     }
-    Place p{};
     if (wave_sum(blocks) > (float)most_blocks) {  // (sequences that overlap: their items would be more than are counted with)
       if (flag) *flag = MI_STATUS_BAD_ROWS;
       return p;
     }
-    const uint32_t per = max(least, (uint32_t)fminf(wave_sum(total) * 1.0001f / (float)share, (float)kMaxKeys) + 1u);
-    auto parts = [&](const Sequence& o) { return (o.tiles + per - 1u) / per; };
-    uint32_t items = s.blocks * parts(s);
-    for (uint32_t b = 64u + lane; b < sequences + lane; b += 64u) {
-      const Sequence o = sequence(*this, b);
-      items += o.blocks * parts(o);
+    p.per = part_tiles(s, wave_sum(total));
+    uint32_t items = s.blocks * parts(s, p.per);
+    for (uint32_t b = 64u; b < sequences; b += 64u) {
+      const Sequence o = sequence(*this, b + lane);
+      items += o.blocks * parts(o, p.per);
     }
-    items = wave_fold(items, plus) * kv_heads;
-    const uint32_t each = (items + kXcds - 1u) / kXcds, at = blockIdx.x / kXcds;
-    uint32_t item = (blockIdx.x % kXcds) * each + at;
-    if (at >= each || item >= items) return p;
+    uint32_t item = item_of(wave_fold(items, plus) * kv_heads);
+    if (item == kNone) return p;
     uint32_t part = 0;
     for (uint32_t b0 = 0; b0 < sequences; b0 += 64u) {
       if (b0) s = sequence(*this, b0 + lane);
-      const uint32_t n = parts(s), mine = s.blocks * n * kv_heads;
+      const uint32_t n = parts(s, p.per), mine = s.blocks * n * kv_heads;
       uint32_t sum = mine;  // of the lanes up to this one
 #pragma unroll
       for (uint32_t d = 1; d < 64u; d *= 2) {
@@ -117,23 +156,31 @@ struct TreeRows : TreeArgs {
         continue;
       }
       auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)found); };
-      item -= of(sum - mine);
-      const uint32_t n_blocks = of(s.blocks), split = item / (n_blocks * kv_heads), rest = item - split * n_blocks * kv_heads;
-      p.j = rest / n_blocks;
-      p.own = (rest - p.j * n_blocks) * this->rows;
-      p.rows = min(this->rows, of(s.rows) - p.own);
-      p.t0 = of(s.start) + p.own;
-      p.split = split;
-      p.splits = of(n);
-      p.b = b0 + found;
-      p.cached = of(s.cached);
-      p.keys = of(s.keys);
-      p.per = per;
-      p.part = part + item;
-      if (split == 0u && p.j == 0u && threadIdx.x < p.rows)
-        info[p.t0 + threadIdx.x] = u4_t{p.part, n_blocks, p.splits, threadIdx.x};
-      return p;
+      const Sequence f = {of(s.start), of(s.rows), of(s.cached), of(s.keys), of(s.blocks), of(s.tiles)};
+      return inside(p, f, b0 + found, of(n), item - of(sum - mine), part);
     }
+    return p;
+  }
+  // This work-group's of `items` items: XCD x (every eighth work-group is its) has those from x / 8 of them on.
+  __device__ __forceinline__ uint32_t item_of(uint32_t items) const {
+    const uint32_t each = (items + kXcds - 1u) / kXcds, at = blockIdx.x / kXcds, item = (blockIdx.x % kXcds) * each + at;
+    return at < each && item < items ? item : kNone;
+  }
+  // The place of item `item` of sequence b, of n parts, whose first item's sums are number `part`.
+  __device__ __forceinline__ Place inside(Place p, const Sequence& s, uint32_t b, uint32_t n, uint32_t item, uint32_t part) const {
+    const uint32_t each = s.blocks * kv_heads, split = item / each, rest = item - split * each;
+    p.j = rest / s.blocks;
+    p.own = (rest - p.j * s.blocks) * rows;
+    p.rows = min(rows, s.rows - p.own);
+    p.t0 = s.start + p.own;
+    p.split = split;
+    p.splits = n;
+    p.b = b;
+    p.cached = s.cached;
+    p.keys = s.keys;
+    p.part = part + item;
+    if (split == 0u && p.j == 0u && threadIdx.x < p.rows)
+      info[p.t0 + threadIdx.x] = u4_t{p.part, s.blocks, p.splits, threadIdx.x};
     return p;
   }
   __device__ __forceinline__ Block block(const Place& p) const {
@@ -148,7 +195,7 @@ struct TreeRows : TreeArgs {
     return b;
   }
   __device__ __forceinline__ uint32_t part_begin(const Place& p, const Block& b, uint32_t split) const {
-    return min(b.n, split * p.per);
+    return (uint32_t)((uint64_t)b.n * split / p.splits);
   }
   __device__ __forceinline__ Column column(const Place& p, const Block& b, uint32_t row, uint32_t) const {
     Column c{nullptr, p.own + row, p.cached, p.keys - p.cached, row < p.rows};
@@ -293,10 +340,14 @@ Pick pick(uint32_t T, uint32_t sequences, uint32_t gqa, uint32_t hd) {
   if (each <= 16u) return few_rows(gqa, hd);
   return chunk(each <= 64u ? 1u : 2u, gqa, hd);
 }
-uint32_t share_of(const Pick& p, uint32_t kv_heads) { return std::min(kMaxSplits - 1u, std::max(1u, p.slots / kv_heads)); }
+// The parts of all sequences at most, one for each block aside: as many as make every work-group that runs at once busy, where there
+// are several sequences some times as many.
+uint32_t share_of(const Pick& p, uint32_t kv_heads, uint32_t sequences) {
+  return std::min(kMaxSplits - 1u, std::max(1u, p.slots * (sequences == 1u ? 1u : p.few ? 4u : 2u) / kv_heads));
+}
 // The items of sequences of several parts: such a sequence has at most twice tiles / per parts.
-size_t part_floats(const Pick& p, uint32_t kv_heads, uint32_t hd) {
-  return (size_t)2u * share_of(p, kv_heads) * kv_heads * p.columns * (hd + 4u);
+size_t part_floats(const Pick& p, uint32_t kv_heads, uint32_t sequences, uint32_t hd) {
+  return (size_t)2u * share_of(p, kv_heads, sequences) * kv_heads * p.columns * (hd + 4u);
 }
 bool shape_ok(const mi_attn_shape* s) {
   return s && s->kv_heads && s->q_heads && s->q_heads % s->kv_heads == 0 && s->q_heads / s->kv_heads <= 64 &&
@@ -320,9 +371,9 @@ size_t mi_attn_tree_ws(uint32_t T, uint32_t sequences, const mi_attn_shape* shap
   if (T == 0 || T > kMaxRows || sequences == 0 || sequences > kMaxSequences || !shape_ok(shape)) return 0;
   const uint32_t gqa = shape->q_heads / shape->kv_heads, hd = shape->head_dim;
   // the most that any call of up to T rows takes
-  size_t floats = gqa <= 16u ? part_floats(few_rows(gqa, hd), shape->kv_heads, hd) : 0u;
+  size_t floats = gqa <= 16u ? part_floats(few_rows(gqa, hd), shape->kv_heads, 2u, hd) : 0u;
   for (uint32_t ct = 1; ct <= 2; ++ct)
-    if (T * gqa > (ct == 1u ? 16u : 64u)) floats = std::max(floats, part_floats(chunk(ct, gqa, hd), shape->kv_heads, hd));
+    if (T * gqa > (ct == 1u ? 16u : 64u)) floats = std::max(floats, part_floats(chunk(ct, gqa, hd), shape->kv_heads, 2u, hd));
   return (size_t)T * sizeof(u4_t) + floats * 4u;
 }
 
@@ -358,7 +409,7 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
     return mi_fail(MI_ERR_ARG, "attn_tree: misaligned row_start, cached, tables, mask or flag (4 bytes)");
   const uint32_t gqa = shape->q_heads / shape->kv_heads;
   const Pick p = pick(T, n, gqa, shape->head_dim);
-  const size_t floats = part_floats(p, shape->kv_heads, shape->head_dim);
+  const size_t floats = part_floats(p, shape->kv_heads, n, shape->head_dim);
   if (!ws || off(ws, 16) || ws_bytes < (size_t)T * sizeof(u4_t) + floats * 4u)
     return mi_fail(MI_ERR_ARG, "attn_tree: the workspace is null, misaligned (16 bytes) or below mi_attn_tree_ws");
   TreeRows a{};
@@ -388,14 +439,18 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
   a.gqa = gqa;
   a.rows = p.rows;
   a.columns = p.columns;
-  a.share = share_of(p, shape->kv_heads);
+  a.slots = p.slots;
+  a.share = share_of(p, shape->kv_heads, n);
   a.least = 4;
   a.act = shape->act;
   a.c = shape->scale * kLog2e;
   hipStream_t st = (hipStream_t)stream;
   a.most_blocks = T / p.rows + n;
-  // as many work-groups as there are items at most: share and one more for each block, of each kv head
-  const uint32_t items = shape->kv_heads * (a.share + a.most_blocks), grid = (items + kXcds - 1u) / kXcds * kXcds;
+  // as many work-groups as there are items at most: share and one more for each block, of each kv head, no more than the blocks have
+  // parts of the least size
+  const uint64_t least_parts = ((uint64_t)kv_len + a.least * kTile - 1u) / (a.least * kTile);
+  const uint32_t items = shape->kv_heads * (uint32_t)std::min<uint64_t>(a.share + a.most_blocks, a.most_blocks * least_parts);
+  const uint32_t grid = (items + kXcds - 1u) / kXcds * kXcds;
   const bool narrow = shape->head_dim == 128;
   if (p.few) {
     if (narrow) attn_rows_few_kernel<128><<<grid, 256, 0, st>>>(a);

@@ -206,23 +206,27 @@ __global__ __launch_bounds__(256) void kv_move_kernel(MoveArgs a) {
   const uint32_t* from = a.from + (size_t)blockIdx.x * a.per;
   const uint32_t* to = a.to + (size_t)blockIdx.x * a.per;
   u4_t k[U], v[U];
-  uint32_t at[U];
+  uint32_t whence[U], at[U];
+  // (all of the lists' entries first: loads come back in order, and an entry asked for behind rows would wait for them)
 #pragma unroll
   for (uint32_t u = 0; u < U; ++u) {
-    const uint32_t i = (256u * u + threadIdx.x) / PPR;
-    at[u] = kNone;
-    if (i < a.per) {
-      const uint32_t f = from[i], t = to[i];
-      if (f < a.rows && t < a.rows) {
-        at[u] = t;
-        const size_t o = base + (size_t)f * a.row_stride + 8u * (threadIdx.x % PPR);
-        k[u] = *as_global(reinterpret_cast<const u4_t*>(a.k + o));
-        v[u] = *as_global(reinterpret_cast<const u4_t*>(a.v + o));
-      } else if (t != kNone && a.flag) {
-        *a.flag = MI_STATUS_BAD_PAGE;
-      }
-    }
+    const uint32_t i = min((256u * u + threadIdx.x) / PPR, a.per - 1u);
+    whence[u] = from[i];
+    at[u] = to[i];
   }
+  bool outside = false;
+#pragma unroll
+  for (uint32_t u = 0; u < U; ++u) {
+    if ((256u * u + threadIdx.x) / PPR >= a.per) at[u] = kNone;
+    const bool moves = whence[u] < a.rows && at[u] < a.rows;
+    outside |= !moves && at[u] != kNone;
+    if (!moves) at[u] = kNone;
+    // (what does not move loads row 0: a branch would wait for what was loaded in it)
+    const size_t o = base + (size_t)(moves ? whence[u] : 0u) * a.row_stride + 8u * (threadIdx.x % PPR);
+    k[u] = *as_global(reinterpret_cast<const u4_t*>(a.k + o));
+    v[u] = *as_global(reinterpret_cast<const u4_t*>(a.v + o));
+  }
+  if (outside && a.flag) *a.flag = MI_STATUS_BAD_PAGE;
   wait_memory();
   __syncthreads();
 #pragma unroll
