@@ -41,6 +41,7 @@ struct LogprobArgs {
   f4_t* stats;
   float* peaks;
   f2_t* sums;  // NULL, or the rows' (m, Z): top_logprobs are then the logits themselves
+  const uint32_t* skip;  // NULL, or rows (not 0) of which nothing is asked
 };
 
 // ---- the statistics ----
@@ -243,6 +244,7 @@ __device__ __forceinline__ float wave_max4(float a, float b, float c, float d) {
 template <bool LISTS>
 __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.y;
+  if (a.skip && a.skip[row]) return;
   const float* x = a.logits + (size_t)row * a.row_stride;
   const uint32_t begin = blockIdx.x * a.slice, end = min(begin + a.slice, a.vocab);
   uint32_t token, ahead = 0;
@@ -364,6 +366,7 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
 __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
   constexpr uint32_t W = 8, U = 4, B = 8, kFit = 1024;  // waves; a lane's runs looked at together; runs read together; tokens
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x, runs = (a.vocab + 255u) / 256u;
+  if (a.skip && a.skip[row]) return;
   const float* x = a.logits + (size_t)row * a.row_stride;
   const f4_t* stats = a.stats + (size_t)row * a.slices;
   const float* peaks = a.peaks + (size_t)row * runs;
@@ -573,25 +576,45 @@ struct BeamArgs {
   float* scores;
 };
 // grid (batch), four waves: a wave merges every fourth beam's candidates, 64 at a time over its lanes, then the waves' join. Bound by
-// its chain: a few loads, six exchanges a beam.
+// its chain: two rounds of loads, a logarithm, six exchanges a beam.
 __global__ __launch_bounds__(256) void beam_select_kernel(BeamArgs a) {
   __shared__ double score[4][64];
   __shared__ uint32_t place[4][64];
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, batch = blockIdx.x;
-  Candidate list;
-  for (uint32_t w = wave; w < a.beams; w += 4u) {
-    const uint32_t row = batch * a.beams + w, n = 63u - lane;  // (best last)
-    Candidate c;
-    const double cum = (double)a.cum[row];
-    if (a.done && a.done[row]) {
-      if (n == 0u && cum > -INFINITY) c = Candidate{cum, 64u * w};
-    } else if (n < a.k && a.top_ids[(size_t)row * a.k + n] != kNone) {
-      const f2_t s = a.sums[row];
-      const double of = cum + ((double)a.top[(size_t)row * a.k + n] - (double)s.x) - log((double)s.y);
-      if (of > -INFINITY) c = Candidate{of, 64u * w + n};  // (nor a NaN)
+  constexpr uint32_t U = 4;  // beams whose candidates are loaded at once
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, batch = blockIdx.x, n = 63u - lane;  // (the best come last)
+  const uint32_t mine = batch * a.beams + min(lane, a.beams - 1u);
+  uint32_t id[U];
+  float top[U];
+  auto load = [&](uint32_t w0) {
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const size_t at = (size_t)(batch * a.beams + min(w0 + 4u * u, a.beams - 1u)) * a.k + min(n, a.k - 1u);
+      id[u] = *as_global(a.top_ids + at);
+      top[u] = *as_global(a.top + at);
     }
-    if (better(c, list)) list = c;
-    half_clean<32>(list, lane);
+  };
+  load(wave);
+  // a lane a beam: what its logits are added to
+  const float cum = *as_global(a.cum + mine);
+  const f2_t s = *as_global(a.sums + mine);
+  const uint64_t done = __ballot(a.done && a.done[mine]);
+  const uint64_t of = __builtin_bit_cast(uint64_t, (done >> lane) & 1u ? (double)cum : (double)cum - (double)s.x - log((double)s.y));
+  Candidate list;
+  for (uint32_t w0 = wave; w0 < a.beams; w0 += 4u * U) {
+    if (w0 != wave) load(w0);
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      const uint32_t w = w0 + 4u * u;
+      if (w >= a.beams) break;
+      const double base = __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(of >> 32), (int)w) << 32 |
+                                                         (uint32_t)__builtin_amdgcn_readlane((int)of, (int)w));
+      const bool ends = (done >> w) & 1u;
+      const double sum = ends ? base : base + (double)top[u];
+      Candidate c;
+      if ((ends ? n == 0u : n < a.k && id[u] != kNone) && sum > -INFINITY) c = Candidate{sum, 64u * w + n};  // (nor a NaN)
+      if (better(c, list)) list = c;
+      half_clean<32>(list, lane);
+    }
   }
 #pragma unroll 1
   for (uint32_t step = 2; step; step /= 2) {
@@ -665,7 +688,7 @@ int mi_logprobs(const float* logits, size_t row_stride, const uint32_t* tokens, 
   if (need && (!ws || (reinterpret_cast<uintptr_t>(ws) & 15u) || ws_bytes < need))
     return mi_fail(MI_ERR_ARG, "logprobs: the workspace is null, misaligned (16 bytes) or below mi_logprobs_ws");
   const LogprobArgs a{logits, row_stride, tokens, vocab_used, top, 1, vocab_used, logprob, entropy, top_logprobs, rank, top_ids,
-                      nullptr, nullptr, nullptr};
+                      nullptr, nullptr, nullptr, nullptr};
   launch(a, M, ws, (hipStream_t)stream);
   return mi_hip((int)hipGetLastError(), "logprobs");
 }
@@ -697,7 +720,7 @@ int mi_beam_select(const float* logits, size_t row_stride, const float* cum, con
   uint32_t* top_ids = reinterpret_cast<uint32_t*>(top + (size_t)rows * k);
   const uintptr_t end = (reinterpret_cast<uintptr_t>(top_ids + (size_t)rows * k) + 15u) & ~(uintptr_t)15u;
   const LogprobArgs a{logits, row_stride, nullptr, vocab_used, k, 1, vocab_used, nullptr, nullptr, top, nullptr, top_ids,
-                      nullptr, nullptr, sums};
+                      nullptr, nullptr, sums, done};
   hipStream_t st = (hipStream_t)stream;
   launch(a, rows, reinterpret_cast<void*>(end), st);
   beam_select_kernel<<<batch, 256, 0, st>>>(BeamArgs{cum, done, sums, top_ids, top, eos, beams, k, ids, from, scores});

@@ -15,7 +15,7 @@
 namespace mi {
 namespace {
 
-constexpr uint32_t kMaxRequests = 1024, kMaxRows = 65535, kMaxKeys = 1u << 30, kMaxWords = 64, kNone = 0xFFFFFFFFu;
+constexpr uint32_t kMaxRequests = 1024, kMaxRows = 65535, kMaxKeys = 1u << 30, kMaxWords = 64, kMaxTable = 1u << 21, kNone = 0xFFFFFFFFu;
 constexpr uint32_t kOneGroup = 4096;  // rows that the requests' work-group does itself
 
 struct PlanArgs {
@@ -48,15 +48,26 @@ __device__ __forceinline__ Three sums_before(Three v, Three& all) {
   return before;
 }
 
-// The rows `first` .. of a work-group: starts is row_start, in LDS.
-__device__ __forceinline__ void plan_rows(const PlanArgs& a, const uint32_t* starts, bool planned, uint32_t head, uint32_t begin,
-                                          uint32_t end, uint32_t* parents) {
-  const mi_block_plan& p = a.p;
-  const uint32_t total = planned ? starts[p.requests] : 0u;
-  if (p.parent && planned) {
-    for (uint32_t t = begin + threadIdx.x; t < min(end, total); t += blockDim.x) parents[t - begin] = p.parent[t];
-    __syncthreads();
+// What the rows of a work-group need of the requests, in LDS.
+struct Requests {
+  uint32_t start[kMaxRequests + 1];  // row_start
+  uint32_t cached[kMaxRequests], held[kMaxRequests], taken[kMaxRequests];
+};
+// the last of n + 1 ascending sums that is not above i, which is below the last one
+__device__ __forceinline__ uint32_t find(const uint32_t* sums, uint32_t n, uint32_t i) {
+  uint32_t lo = 0, hi = n;
+  while (hi - lo > 1u) {
+    const uint32_t mid = (lo + hi) / 2u;
+    if (sums[mid] <= i) lo = mid;
+    else hi = mid;
   }
+  return lo;
+}
+// The rows begin .. end - 1, and their parents in LDS.
+__device__ __forceinline__ void plan_rows(const PlanArgs& a, const Requests& r, bool planned, uint32_t head, uint32_t begin, uint32_t end,
+                                          const uint32_t* parents) {
+  const mi_block_plan& p = a.p;
+  const uint32_t total = planned ? r.start[p.requests] : 0u;
   for (uint32_t t = begin + threadIdx.x; t < end; t += blockDim.x) {
     if (t >= total) {
       p.seq[t] = p.slot[t] = kNone;
@@ -65,23 +76,12 @@ __device__ __forceinline__ void plan_rows(const PlanArgs& a, const uint32_t* sta
         for (uint32_t w = 0; w < p.words; ++w) p.mask[(size_t)t * p.words + w] = 0u;
       continue;
     }
-    uint32_t lo = 0, hi = p.requests;  // starts[lo] <= t < starts[hi]
-    while (hi - lo > 1u) {
-      const uint32_t mid = (lo + hi) / 2u;
-      if (starts[mid] <= t) lo = mid;
-      else hi = mid;
-    }
-    const uint32_t b = lo, start = starts[b], i = t - start, key = p.cached[b] + i;
-    const uint32_t held = a.ws[2u + 2u * b], taken = a.ws[3u + 2u * b];
-    const uint32_t at = key / p.page, in = key - at * p.page;
+    const uint32_t b = find(r.start, p.requests, t), start = r.start[b], i = t - start, key = r.cached[b] + i;
+    const uint32_t held = r.held[b], at = key / p.page, in = key - at * p.page;
     uint32_t* table = p.tables + (size_t)b * p.table_stride;
-    uint32_t page;
-    if (at < held) {
-      page = table[at];
-    } else {
-      page = p.ring[(uint32_t)(((uint64_t)head + taken + (at - held)) % p.ring_len)];
-      if (in == 0u) table[at] = page;  // (its first key is one of the step's: the cached ones have their pages)
-    }
+    const bool fresh = at >= held;
+    const uint32_t page = fresh ? p.ring[(uint32_t)(((uint64_t)head + r.taken[b] + (at - held)) % p.ring_len)] : table[at];
+    if (fresh && in == 0u) table[at] = page;  // (its first key is one of the step's: the cached ones have their pages)
     if (page >= p.n_pages && p.flag) *p.flag = MI_STATUS_BAD_PAGE;
     p.seq[t] = b;
     p.slot[t] = page < p.n_pages ? page * p.page + in : kNone;
@@ -108,86 +108,91 @@ __device__ __forceinline__ void plan_rows(const PlanArgs& a, const uint32_t* sta
       ++depth;
     }
     for (mask[w] = bits; w; --w) mask[w - 1u] = 0u;
-    p.pos[t] = p.cached[b] + depth;
+    p.pos[t] = r.cached[b] + depth;
   }
 }
 
-// One work-group of 1024: the requests; ROWS: then the rows too.
+// One work-group: the requests, a thread each; ROWS: then the rows too.
 template <bool ROWS>
 __global__ __launch_bounds__(kMaxRequests) void plan_kernel(PlanArgs a) {
   const mi_block_plan& p = a.p;
-  __shared__ uint32_t starts[kMaxRequests + 1], back_at[kMaxRequests], needs[kMaxRequests], helds[kMaxRequests], wrong;
-  __shared__ unsigned long long added_all, taken_all, back_all;
+  __shared__ Requests r;
+  __shared__ uint32_t back_at[kMaxRequests + 1], need_of[kMaxRequests], parents[ROWS ? kOneGroup : 1];
   const uint32_t b = threadIdx.x;
   const bool request = b < p.requests;
-  if (b == 0) {
-    wrong = 0u;
-    added_all = taken_all = back_all = 0ull;
-  }
   const uint32_t head = p.ring_at[0], count = p.ring_at[1];
-  uint32_t cached = 0, added = 0, held = 0, need = 0;
+  uint32_t cached = 0, added = 0, held = 0, need = 0, before_held = 0;
   bool ok = true;
   if (request) {
     cached = p.cached[b];
     added = p.added[b];
-    held = p.held[b];
+    before_held = held = p.held[b];
     const uint64_t keys = (uint64_t)cached + added;
     ok = keys <= kMaxKeys && held <= p.table_stride && (uint64_t)held * p.page >= cached && added <= p.rows &&
          (!p.parent || added <= 32u * p.words);
-    if (ok) {
-      need = (uint32_t)((keys + p.page - 1u) / p.page);
-      ok = need <= p.table_stride;
+    need = ok ? ((uint32_t)keys + p.page - 1u) / p.page : 0u;
+    ok = ok && need <= p.table_stride;
+  }
+  if constexpr (ROWS)
+    if (p.parent)
+      for (uint32_t t = b; t < p.rows; t += blockDim.x) parents[t] = p.parent[t];
+  if (!ok) {  // (one request that cannot be makes the sum of the rows too large)
+    added = kMaxRows + 1u;
+    need = held = 0u;
+  }
+  Three all;  // (1024 requests of 2^21 pages at most: none of the sums wraps)
+  const Three before = sums_before(Three{added, need > held ? need - held : 0u, held > need ? held - need : 0u}, all);
+  const bool sound = all.a <= p.rows && head < p.ring_len && count <= p.ring_len && (uint64_t)count + all.c <= p.ring_len;
+  const bool planned = sound && all.b <= count;
+  if (request) {
+    r.start[b] = p.row_start[b] = planned ? before.a : 0u;
+    r.cached[b] = cached;
+    r.held[b] = held;
+    r.taken[b] = before.b;
+    back_at[b] = before.c;
+    need_of[b] = need;
+    p.held_out[b] = planned ? need : before_held;
+    if constexpr (!ROWS) {
+      a.ws[2u + 2u * b] = held;
+      a.ws[3u + 2u * b] = before.b;
     }
   }
-  if (!ok) added = need = held = 0u;
-  const uint32_t taken = need > held ? need - held : 0u, back = held > need ? held - need : 0u;
-  __syncthreads();
-  if (!ok) wrong = 1u;
-  // (the sums in 64 bits: 32 would wrap where the lengths are wrong)
-  if (added) atomicAdd(&added_all, (unsigned long long)added);
-  if (taken) atomicAdd(&taken_all, (unsigned long long)taken);
-  if (back) atomicAdd(&back_all, (unsigned long long)back);
-  __syncthreads();
-  const bool sound = !wrong && added_all <= p.rows && head < p.ring_len && count <= p.ring_len && count + back_all <= p.ring_len;
-  const bool planned = sound && taken_all <= count;
-  Three all;
-  const Three before = sums_before(Three{added, taken, back}, all);
-  if (request) {
-    starts[b] = p.row_start[b] = planned ? before.a : 0u;
-    p.held_out[b] = planned ? need : p.held[b];
-    a.ws[2u + 2u * b] = held;
-    a.ws[3u + 2u * b] = before.b;
-    back_at[b] = before.c;
-    needs[b] = need;
-    helds[b] = held;
-  }
   if (b == 0) {
-    starts[p.requests] = p.row_start[p.requests] = planned ? all.a : 0u;
+    r.start[p.requests] = p.row_start[p.requests] = planned ? all.a : 0u;
+    back_at[p.requests] = all.c;
     p.ring_at_out[0] = planned ? (uint32_t)(((uint64_t)head + all.b) % p.ring_len) : head;
     p.ring_at_out[1] = planned ? count - all.b + all.c : count;
-    a.ws[0] = planned ? 1u : 0u;
-    a.ws[1] = head;
+    if constexpr (!ROWS) {
+      a.ws[0] = planned ? 1u : 0u;
+      a.ws[1] = head;
+    }
     if (!planned && p.flag) *p.flag = sound ? MI_STATUS_NO_PAGES : MI_STATUS_BAD_ROWS;
   }
   __syncthreads();
-  if (planned) {  // what goes back, a wave a request
-    const uint32_t lane = threadIdx.x & 63u, waves = blockDim.x / 64u;
-    for (uint32_t r = threadIdx.x >> 6; r < p.requests; r += waves)
-      for (uint32_t i = needs[r] + lane; i < helds[r]; i += 64u)
-        p.ring[(uint32_t)(((uint64_t)head + count + back_at[r] + (i - needs[r])) % p.ring_len)] = p.tables[(size_t)r * p.table_stride + i];
-  }
-  if constexpr (ROWS) {
-    __shared__ uint32_t parents[kOneGroup];
-    plan_rows(a, starts, planned, head, 0u, p.rows, parents);
-  }
+  if (planned)  // what goes back, a thread a page
+    for (uint32_t i = b; i < all.c; i += blockDim.x) {
+      const uint32_t of = find(back_at, p.requests, i), page = p.tables[(size_t)of * p.table_stride + need_of[of] + (i - back_at[of])];
+      p.ring[(uint32_t)(((uint64_t)head + count + i) % p.ring_len)] = page;
+    }
+  if constexpr (ROWS) plan_rows(a, r, planned, head, 0u, p.rows, parents);
 }
 __global__ __launch_bounds__(256) void plan_rows_kernel(PlanArgs a) {
-  __shared__ uint32_t starts[kMaxRequests + 1], parents[256];
-  for (uint32_t b = threadIdx.x; b <= a.p.requests; b += 256u) starts[b] = a.p.row_start[b];
+  const mi_block_plan& p = a.p;
+  __shared__ Requests r;
+  __shared__ uint32_t parents[256];
+  const uint32_t begin = blockIdx.x * 256u, end = min(begin + 256u, p.rows);
+  if (p.parent && begin + threadIdx.x < end) parents[threadIdx.x] = p.parent[begin + threadIdx.x];
+  for (uint32_t b = threadIdx.x; b < p.requests; b += 256u) {
+    r.start[b] = p.row_start[b];
+    r.cached[b] = p.cached[b];
+    r.held[b] = a.ws[2u + 2u * b];
+    r.taken[b] = a.ws[3u + 2u * b];
+  }
+  if (threadIdx.x == 0) r.start[p.requests] = p.row_start[p.requests];
   const bool planned = a.ws[0] != 0u;
-  const uint32_t head = a.ws[1], begin = blockIdx.x * 256u;
+  const uint32_t head = a.ws[1];
   __syncthreads();
-  plan_rows(a, starts, planned, head, begin, min(begin + 256u, a.p.rows), parents);
+  plan_rows(a, r, planned, head, begin, end, parents);
 }
 
 struct MoveArgs {
@@ -272,18 +277,20 @@ int mi_block_tables(const mi_block_plan* plan, void* ws, size_t ws_bytes, void* 
   if (p.page == 0 || p.n_pages == 0 || p.table_stride == 0 || p.ring_len == 0)
     return mi_fail(MI_ERR_ARG, "block_tables: page size, page count, table_stride or ring_len 0");
   if ((uint64_t)p.page * p.n_pages > 0xFFFFFFFFull) return mi_fail(MI_ERR_SHAPE, "block_tables: above 2^32 cache rows");
-  if ((uint64_t)p.table_stride * p.page > 0xFFFFFFFFull || p.ring_len > 1u << 31)
-    return mi_fail(MI_ERR_SHAPE, "block_tables: tables of 2^32 keys or a ring of 2^31 pages at most");
+  if (p.table_stride > kMaxTable || p.ring_len > 1u << 31)
+    return mi_fail(MI_ERR_SHAPE, "block_tables: tables of 2^21 pages and a ring of 2^31 pages at most");
   if (p.parent ? !p.mask || p.words == 0 || p.words > kMaxWords : p.mask || p.words)
     return mi_fail(MI_ERR_ARG, "block_tables: masks of 1..64 words go with parents");
   if (!ws || off(ws, 4) || ws_bytes < mi_block_tables_ws(p.requests))
     return mi_fail(MI_ERR_ARG, "block_tables: the workspace is null, misaligned (4 bytes) or below mi_block_tables_ws");
   const PlanArgs a{p, static_cast<uint32_t*>(ws)};
   hipStream_t st = (hipStream_t)stream;
+  // a thread a request, and some for the rows
+  const uint32_t threads = std::max((p.requests + 63u) / 64u * 64u, p.rows <= 256u ? 256u : 1024u);
   if (p.rows <= kOneGroup) {
-    plan_kernel<true><<<1, kMaxRequests, 0, st>>>(a);
+    plan_kernel<true><<<1, threads, 0, st>>>(a);
   } else {
-    plan_kernel<false><<<1, kMaxRequests, 0, st>>>(a);
+    plan_kernel<false><<<1, threads, 0, st>>>(a);
     plan_rows_kernel<<<(p.rows + 255u) / 256u, 256, 0, st>>>(a);
   }
   return mi_hip((int)hipGetLastError(), "block_tables");

@@ -27,7 +27,7 @@ def test_block_tables_refusals():
                {"nb": L.mi_block_tables_ws(4) - 1}):
         assert call(**kw) == ARG, kw
     for kw in ({"requests": 0}, {"requests": 1025}, {"rows": 0}, {"rows": 65536}, {"page": 1 << 31, "n_pages": 3}, {"ring_len": (1 << 31) + 1},
-               {"table_stride": 1 << 30, "page": 64}):
+               {"table_stride": (1 << 21) + 1}):
         assert call(**kw) == SHAPE, kw
     assert L.mi_block_tables(None, P, 1 << 20, None) == ARG
     assert L.mi_block_tables_ws(0) == L.mi_block_tables_ws(1025) == 0 < L.mi_block_tables_ws(1)
@@ -91,7 +91,8 @@ def test_attn_tree_refusals():
         assert b"attn_tree" in L.mi_last_error()
     for kw in ({"sh": shape(head_dim=64)}, {"sh": shape(q_heads=11)}, {"sh": shape(kv_heads=0)}, {"sh": shape(gated=1)}, {"T": 0}, {"T": 65536},
                {"kv_len": 0}, {"kv_len": (1 << 30) + 1, "table_stride": 1 << 28}, {"sequences": 0}, {"sequences": 1025},
-               {"page": 1 << 31, "n_pages": 3}, {"tables": None, "table_stride": 1 << 31}, {"sh": shape(q_heads=130)}):
+               {"page": 1 << 31, "n_pages": 3}, {"tables": None, "table_stride": 1 << 31}, {"sh": shape(q_heads=130)},
+               {"rs": (1 << 25) + 8}):
         assert call(**kw) == SHAPE, kw
 
 
