@@ -683,7 +683,7 @@ typedef struct mi_attn_batch {
  * a key of a sequence with rows, sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL); nothing outside the cache is read. row_start
  * does not fall; sequences that overlap so much that they are more than T rows are refused on the device (MI_STATUS_BAD_ROWS, no row
  * is written). head_dim 128 or 256, up to 64 q heads per kv head, not gated; T up to 65535, 1..1024 sequences, kv_len up to 2^30,
- * words 1..64 with masks, 0 without, row_stride up to 2^25. ws: mi_attn_tree_ws bytes of device scratch, 16-byte aligned; its size never falls as T grows
+ * words 1..64 with masks, 0 without. ws: mi_attn_tree_ws bytes of device scratch, 16-byte aligned; its size never falls as T grows
  * and is the same for any number of sequences. */
 size_t mi_attn_tree_ws(uint32_t T, uint32_t sequences, const mi_attn_shape* shape);
 int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v, size_t row_stride, size_t head_stride,

@@ -8,8 +8,6 @@
 //   Column column(...)           what a column sees; bool masked(Block, key): whether some column does not see some key of a tile
 //   bool sees(Column, key), bias_and_mask, score, scores_by_form: of products the scores in base 2
 //   row_of, first_row, cache_row the cache rows of keys, with whether a page's entry is outside the cache; report_pages
-//   kLean                        scores are products alone (no cap, no bias): the chunk kernel then takes c into q and the references into
-//                                the products' first summand, and steps through the cache by 32-bit offsets (row_stride below 2^25)
 //   part_at                      where a part's sums go: HD values (sums of weight times V), then the reference and the weights' sum
 //
 // For a column with scores y_j in base 2: out = sum_j 2^y_j v_j / sum_j 2^y_j.
@@ -163,36 +161,6 @@ __device__ __forceinline__ void raise(const float (&w)[CT][8], uint32_t qi, floa
     const float alpha = __builtin_amdgcn_exp2f(r[ct] - to);
     r[ct] = to;
     l[ct] *= alpha;
-#pragma unroll
-    for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] *= alpha;
-    if constexpr (NT == 0) *factor = alpha;
-  }
-}
-// The same where the scores come relative to their references (kLean): `limit` is the score that raises, kNoKey before the first key,
-// and `base` minus the reference (0 before the first key), the summand that the next products begin with.
-template <uint32_t CT, uint32_t NT>
-__device__ __forceinline__ void raise_by(float (&w)[CT][8], uint32_t qi, float (&limit)[CT], f4_t (&base)[CT], float (&l)[CT],
-                                         f4_t (*acc)[NT ? NT : 1], float* factor) {
-  float mx[CT];
-  bool over = false;
-#pragma unroll
-  for (uint32_t ct = 0; ct < CT; ++ct) {
-    mx[ct] = max3(max3(w[ct][0], w[ct][1], w[ct][2]), max3(w[ct][3], w[ct][4], w[ct][5]), max3(w[ct][6], w[ct][7], w[ct][7]));
-    over |= mx[ct] > limit[ct];
-  }
-  if (!__ballot(over)) return;
-#pragma unroll
-  for (uint32_t ct = 0; ct < CT; ++ct) {
-    const uint64_t lanes = __ballot(mx[ct] > limit[ct]);
-    const uint32_t o = (uint32_t)lanes | (uint32_t)(lanes >> 32);
-    const float by = col_max(mx[ct]) - kBelow;
-    const bool up = ((o | o >> 16) >> qi) & 1u;
-    const float alpha = up ? (limit[ct] == kNoKey ? 0.f : __builtin_amdgcn_exp2f(-by)) : 1.f, less = up ? by : 0.f;
-    if (up) limit[ct] = kRaise;
-    base[ct] -= less;
-    l[ct] *= alpha;
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) w[ct][e] -= less;
 #pragma unroll
     for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] *= alpha;
     if constexpr (NT == 0) *factor = alpha;
@@ -438,9 +406,6 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
   auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
   const size_t hoff = (size_t)j * a.head_stride;
   const uint32_t srow = t / PPR, sp = 8u * (t % PPR);
-  uint32_t step[CH];  // (kLean) this thread's elements behind a whole tile's first
-#pragma unroll
-  for (uint32_t c = 0; c < CH; ++c) step[c] = (RPP * c + srow) * (uint32_t)a.row_stride + sp;
   u4_t kr[CH], vr[CH];
   // the cache rows of tile i: its first (r[0]) where they follow one another, else those that the thread loads
   struct Rows {
@@ -463,15 +428,6 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
   // (a tile behind the last is that one again, and its loads are not used)
   auto load = [&](const uint16_t* cache, uint32_t i, const Rows& w, u4_t (&to)[CH]) {
     const uint32_t left = b.last - b.key(from + min(i, n - 1u));
-    if constexpr (A::kLean && ORDER != kAnyPages) {
-      const uint16_t* at = cache + (size_t)uniform(w.r[0]) * a.row_stride + hoff;
-#pragma unroll
-      for (uint32_t c = 0; c < CH; ++c) {
-        const uint32_t off = left >= kTile - 1u ? step[c] : min(RPP * c + srow, left) * (uint32_t)a.row_stride + sp;
-        to[c] = *as_global(reinterpret_cast<const u4_t*>(at + off));
-      }
-      return;
-    }
 #pragma unroll
     for (uint32_t c = 0; c < CH; ++c) {
       const uint32_t r = ORDER == kAnyPages ? w.r[c] : uniform(w.r[0]) + min(RPP * c + srow, left);
@@ -495,20 +451,15 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
     load(a.v, 0, r0, vr);
     load(a.k, 1, r1, k1);
   }
-  float r[SC], l[SC], factor = 1.f;  // (kLean: r the limits of raise_by)
-  f4_t acc[CT][NT], d[CT][2], base[SC];
+  float r[SC], l[SC], factor = 1.f;
+  f4_t acc[CT][NT], d[CT][2];
   h8_t qh[CT][KK], ql[CT][KK];
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
-    if constexpr (A::kLean) {
-#pragma unroll
-      for (uint32_t x = 0; x < 2 * KK; ++x) qraw[ct][x] *= a.c;
-    }
     split_q<KK>(qraw[ct], qh[ct], ql[ct]);
     if (ct < SC) {
       r[ct] = kNoKey;
       l[ct] = 0.f;
-      base[ct] = f4_t{0.f, 0.f, 0.f, 0.f};
     }
 #pragma unroll
     for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
@@ -524,16 +475,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
   };
   auto clear = [&]() {
 #pragma unroll
-    for (uint32_t ct = 0; ct < CT; ++ct) {
-      d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
-      // (of a column whose scores two waves share one begins with it)
-      if constexpr (A::kLean)
-        if (ct < SC && (DS == 1 || OWN || ds == 0u)) d[ct][0] = d[ct][1] = base[ct];
-    }
-  };
-  auto scored = [&](float s) {
-    if constexpr (A::kLean) return s;
-    else return a.template score<CAP>(s);
+    for (uint32_t ct = 0; ct < CT; ++ct) d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
   };
   auto hand_over = [&](uint32_t buf) {
     if constexpr (DS > 1) {
@@ -558,9 +500,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
     const bool masked = a.masked(b, key);
 #pragma unroll
     for (uint32_t ct = 0; ct < SC; ++ct) a.bias_and_mask(col[ct], key + 4u * qq, masked, w[ct]);
-    if constexpr (A::kLean && OWN) raise_by<1, 0>(w, qi, r, base, l, nullptr, &factor);
-    else if constexpr (A::kLean) raise_by<CT, NT>(w, qi, r, base, l, acc, nullptr);
-    else if constexpr (OWN) raise<1, 0>(w, qi, r, l, nullptr, &factor);
+    if constexpr (OWN) raise<1, 0>(w, qi, r, l, nullptr, &factor);
     else raise<CT, NT>(w, qi, r, l, acc, nullptr);
   };
   if (n) {
@@ -581,7 +521,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
 #pragma unroll
     for (uint32_t ct = 0; ct < SC; ++ct)
 #pragma unroll
-      for (uint32_t e = 0; e < 8; ++e) w[ct][e] = scored(d[ct][e / 4][e % 4]);
+      for (uint32_t e = 0; e < 8; ++e) w[ct][e] = a.template score<CAP>(d[ct][e / 4][e % 4]);
     settle(0);
   }
   for (uint32_t i = 0; i < n; ++i) {
@@ -613,7 +553,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
           product(kh[s], s, 2 * h + 1);
           if (h >= SC) continue;
           const uint32_t x = s * SC + h, ct = x / 8, e = x % 8;
-          w[ct][e] = __builtin_amdgcn_exp2f(A::kLean ? w[ct][e] : w[ct][e] - r[ct]);
+          w[ct][e] = __builtin_amdgcn_exp2f(w[ct][e] - r[ct]);
           l[ct] += w[ct][e];
           if (e % 2) {
             u4_t pk = __builtin_bit_cast(u4_t, p[ct]);
@@ -656,7 +596,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
 #pragma unroll
         for (uint32_t ct = 0; ct < CT; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[tt], p[ct], acc[ct][tt], 0, 0, 0);
 #pragma unroll
-        for (uint32_t ct = 0; ct < SC; ++ct) w[ct][tt] = scored(d[ct][tt / 4][tt % 4]);
+        for (uint32_t ct = 0; ct < SC; ++ct) w[ct][tt] = a.template score<CAP>(d[ct][tt / 4][tt % 4]);
         __builtin_amdgcn_sched_barrier(0);
       }
       if (i + 1u < n) settle(i + 1u);
@@ -691,7 +631,7 @@ __global__ __launch_bounds__(2 * HD, 2) void attn_rows_kernel(A a) {
         store_part<HD>(a, pl, row[ct], g[ct], qq, 8u * ds + tt, live[ct] ? acc[ct][tt] : f4_t{0.f, 0.f, 0.f, 0.f});
       if (qq == 0 && (OWN ? ct == 0 : ds == 0)) {
         float* o = a.template part_at<HD>(pl, row[ct], g[ct]);
-        o[HD] = A::kLean && r[ct < SC ? ct : 0] != kNoKey ? -base[ct < SC ? ct : 0][0] : r[ct < SC ? ct : 0];
+        o[HD] = r[ct < SC ? ct : 0];
         o[HD + 1] = live[ct] ? sum[ct] : 0.f;
       }
     } else {

@@ -69,7 +69,7 @@ struct TreeRows : TreeArgs {
     uint32_t own, first, count;  // its index, the first of the step's own keys and how many they are
     bool live;
   };
-  static constexpr bool kMayIdle = true, kLean = true;
+  static constexpr bool kMayIdle = true;
 
   static __device__ __forceinline__ uint32_t parts(const Sequence& s, uint32_t per) { return (s.tiles + per - 1u) / per; }
   // Tiles of a part at most. With `even` tiles in each of the work-groups that run at once, and parts of `per` tiles that make `items`
@@ -402,7 +402,6 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
   if (batch->mask ? batch->words == 0 || batch->words > kMaxWords : batch->words != 0)
     return mi_fail(MI_ERR_ARG, "attn_tree: 1..64 words go with masks, 0 with none");
   if (row_stride % 8 || head_stride % 8) return mi_fail(MI_ERR_ARG, "attn_tree: KV strides must keep 8-element alignment");
-  if (row_stride > 1u << 25) return mi_fail(MI_ERR_SHAPE, "attn_tree: row_stride up to 2^25");  // (32 rows by a 32-bit offset)
   auto off = [](const void* p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1u)) != 0; };
   if (off(kv_k, 16) || off(kv_v, 16) || off(attn_q, 4) || off(attn_out, 2))
     return mi_fail(MI_ERR_ARG, "attn_tree: misaligned pointer (K and V 16 bytes)");

@@ -91,8 +91,7 @@ def test_attn_tree_refusals():
         assert b"attn_tree" in L.mi_last_error()
     for kw in ({"sh": shape(head_dim=64)}, {"sh": shape(q_heads=11)}, {"sh": shape(kv_heads=0)}, {"sh": shape(gated=1)}, {"T": 0}, {"T": 65536},
                {"kv_len": 0}, {"kv_len": (1 << 30) + 1, "table_stride": 1 << 28}, {"sequences": 0}, {"sequences": 1025},
-               {"page": 1 << 31, "n_pages": 3}, {"tables": None, "table_stride": 1 << 31}, {"sh": shape(q_heads=130)},
-               {"rs": (1 << 25) + 8}):
+               {"page": 1 << 31, "n_pages": 3}, {"tables": None, "table_stride": 1 << 31}, {"sh": shape(q_heads=130)}):
         assert call(**kw) == SHAPE, kw
 
 
