@@ -1,7 +1,7 @@
 """mi_rope_table and mi_rope_rows against their definitions in more bits.
 
 Tolerances. Table: the angle p f is off by 4 roundings of 64 bits (f's power and its scaling, the product, its reduction), 2^-51 of it,
-and the value by that, the series (2^-46) and one rounding to 32 bits. Rows: the norm's factor is off by half of the sum's ten
+and the value by that, 2^-46 (the series, and up to seven turns of 64 bits) and one rounding to 32 bits. Rows: the norm's factor is off by half of the sum's ten
 roundings, a quotient, a root, a reciprocal and two products, ten of 2^-24; a turn adds two: 2^-20 (|x cos| + |y sin|) holds them, and k
 rounds to f16."""
 import numpy as np
