@@ -146,6 +146,9 @@ __device__ __forceinline__ Column column(const MaskedArgs& a, uint32_t j, uint32
 __device__ __forceinline__ bool sees(const MaskedArgs& a, const Column& c, uint32_t key) {
   return key < c.hi && (key >= c.lo || key < a.prefix);
 }
+// The scores' cap: none; one up to kPlainCap, by one exponential; any, by a form that leaves the scores their bits where the cap is
+// far above them.
+enum Cap { kNoCap, kPlain, kAnyCap };
 // The plain form's error is the cap's, 2^-21 of it: at 256 2^-13 of a weight, below their own rounding to f16.
 constexpr float kPlainCap = 256.f;
 // A score in base 2, the cap applied.
@@ -237,11 +240,294 @@ struct MaskedRows : MaskedArgs {
   }
 };
 
+// A chunk: grid (kv_heads, row blocks, splits). Four waves side by side take CT column tiles each and 128 of the dims; at
+// rows of 256 four more take the other half (a wave's registers hold 32 columns of 128 dims with two waves per SIMD, and
+// every LDS read then serves 32 columns). All walk the same 32-key tiles, K and V staged in LDS for all of them, the rows
+// after them in registers meanwhile. A step i has two halves with a barrier between them:
+//   the products of tile i + 1's scores, dealt out among the exponentials that make tile i's weights;
+//   P V of tile i, dealt out among the scaling (and the tanh) of tile i + 1's scores, whose maxima follow.
+// So the matrix core has products while the vector ALUs work in the same wave. The halves of the dims exchange their parts
+// of the scores through LDS across the barrier. With two column tiles each of the two waves takes the softmax of one, its
+// tile 0 (the other wave's 1): the parts of the other's scores go over, and a step later the weights and the factor of a raised
+// reference come back (777 rows over 3778 keys, 16 / 2 heads, with distances, in 5 parts: 125 -> 110 us).
+template <int HD, int CT, Cap CAP, Order ORDER>
+__global__ __launch_bounds__(2 * HD, 2) void attn_masked_kernel(MaskedRows a) {
+  constexpr uint32_t DS = HD / 128, KK = 4, NT = 8, KROW = HD + 8, VROW = HD + 16, THREADS = 2 * HD;
+  constexpr uint32_t PPR = HD / 8, RPP = THREADS / PPR, CH = kTile / RPP;  // 16-byte pieces per row, rows per pass, passes
+  constexpr bool OWN = DS == 2 && CT == 2;
+  constexpr uint32_t SC = OWN ? 1 : CT;  // column tiles whose softmax the wave takes
+  __shared__ __align__(16) struct {
+    uint16_t k[2][kTile * KROW], v[2][kTile * VROW];
+    f4_t s[DS > 1 ? 2 : 1][DS > 1 ? 4 * DS : 1][2 * SC][DS > 1 ? 64 : 1];
+    h8_t p[OWN ? 2 : 1][OWN ? 8 : 1][OWN ? 64 : 1];
+    float f[OWN ? 2 : 1][OWN ? 8 : 1][OWN ? 64 : 1];  // the references' factors; the sums at the end
+  } st;
+  const uint32_t t = threadIdx.x, lane = t & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(t >> 6)), qi = lane & 15u, qq = lane >> 4;
+  const uint32_t cw = wave % 4u, ds = wave / 4u;
+  const Place pl = a.place(true);
+  const uint32_t j = pl.j, t0 = pl.t0, rows_here = pl.rows;
+  const Block b = a.block(pl);
+  uint32_t row[CT], g[CT];
+  Column col[SC];
+  bool live[CT];
+  f4_t qraw[CT][2 * KK];  // (converted behind the first tiles' loads)
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    const uint32_t p = 16u * (CT * cw + (OWN ? ct ^ ds : ct)) + qi;
+    row[ct] = p / a.gqa;
+    g[ct] = p % a.gqa;
+    const auto c = a.column(pl, b, row[ct], g[ct]);
+    live[ct] = c.live;
+    if (ct < SC) col[ct] = c;
+    const float* qp = a.q + ((size_t)(t0 + (row[ct] < rows_here ? row[ct] : 0u)) * a.q_heads + j * a.gqa + g[ct]) * HD + 128u * ds + 8u * qq;
+#pragma unroll
+    for (uint32_t x = 0; x < 2 * KK; ++x) qraw[ct][x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2)));
+  }
+  const uint32_t from = a.part_begin(pl, b, pl.split), n = a.part_begin(pl, b, pl.split + 1u) - from;
+  auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+  const size_t hoff = (size_t)j * a.head_stride;
+  const uint32_t srow = t / PPR, sp = 8u * (t % PPR);
+  u4_t kr[CH], vr[CH];
+  // the cache rows of tile i: its first (r[0]) where they follow one another, else those that the thread loads
+  struct Rows {
+    uint32_t r[CH];
+  };
+  bool outside = false;
+  auto rows_of = [&](uint32_t i) {
+    Rows w;
+    const uint32_t tile = from + min(i, n - 1u), key0 = b.key(tile);
+    if constexpr (ORDER == kContiguous) {
+      w.r[0] = a.first_row(b, key0);
+    } else if constexpr (ORDER == kWholeTiles) {
+      w.r[0] = a.cache_row(b, key0, outside);
+    } else {
+#pragma unroll
+      for (uint32_t c = 0; c < CH; ++c) w.r[c] = a.cache_row(b, b.within(tile, key0 + RPP * c + srow), outside);
+    }
+    return w;
+  };
+  // (a tile behind the last is that one again, and its loads are not used)
+  auto load = [&](const uint16_t* cache, uint32_t i, const Rows& w, u4_t (&to)[CH]) {
+    const uint32_t left = b.last - b.key(from + min(i, n - 1u));
+#pragma unroll
+    for (uint32_t c = 0; c < CH; ++c) {
+      const uint32_t r = ORDER == kAnyPages ? w.r[c] : uniform(w.r[0]) + min(RPP * c + srow, left);
+      to[c] = *as_global(reinterpret_cast<const u4_t*>(cache + (size_t)r * a.row_stride + hoff + sp));
+    }
+  };
+  auto store = [&](uint16_t* to, uint32_t pitch, const u4_t (&v)[CH]) {
+#pragma unroll
+    for (uint32_t c = 0; c < CH; ++c) *reinterpret_cast<u4_t*>(to + (RPP * c + srow) * pitch + sp) = v[c];
+  };
+  // the rows of the tiles i + 1 .. i + 3 of a step i: V of the first and K of the last are loaded in it (a page's entry is
+  // fetched a step before the loads that need it)
+  Rows r1, r2, r3;
+  u4_t k1[CH];
+  if (n) {
+    const Rows r0 = rows_of(0);
+    r1 = rows_of(1);
+    r2 = rows_of(2);
+    r3 = rows_of(3);
+    load(a.k, 0, r0, kr);
+    load(a.v, 0, r0, vr);
+    load(a.k, 1, r1, k1);
+  }
+  float r[SC], l[SC], factor = 1.f;
+  f4_t acc[CT][NT], d[CT][2];
+  h8_t qh[CT][KK], ql[CT][KK];
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    split_q<KK>(qraw[ct], qh[ct], ql[ct]);
+    if (ct < SC) {
+      r[ct] = kNoKey;
+      l[ct] = 0.f;
+    }
+#pragma unroll
+    for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // One K operand (16 keys x 32 dims, number s = 2 kk + gg) and its products: this wave's part of the scores
+  // S^T[key 16 gg + 4 qq + e][column qi].
+  auto k_operand = [&](uint32_t buf, uint32_t s) {
+    return *reinterpret_cast<const h8_t*>(st.k[buf] + (16u * (s % 2u) + qi) * KROW + 128u * ds + 8u * qq + 32u * (s / 2u));
+  };
+  auto product = [&](h8_t kh, uint32_t s, uint32_t part) {  // part < 2 CT: the columns' high parts, then the low ones
+    const uint32_t ct = part % CT;
+    d[ct][s % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, part < CT ? qh[ct][s / 2] : ql[ct][s / 2], d[ct][s % 2], 0, 0, 0);
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (uint32_t ct = 0; ct < CT; ++ct) d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+  };
+  auto hand_over = [&](uint32_t buf) {
+    if constexpr (DS > 1) {
+#pragma unroll
+      for (uint32_t ct = 0; ct < SC; ++ct)
+#pragma unroll
+        for (uint32_t gg = 0; gg < 2; ++gg) st.s[buf][wave][2 * ct + gg][lane] = d[OWN ? 1 : ct][gg];
+    }
+  };
+  auto take_over = [&](uint32_t buf) {
+    if constexpr (DS > 1) {
+#pragma unroll
+      for (uint32_t ct = 0; ct < SC; ++ct)
+#pragma unroll
+        for (uint32_t gg = 0; gg < 2; ++gg) d[ct][gg] += st.s[buf][wave ^ 4u][2 * ct + gg][lane];
+    }
+  };
+  float w[SC][8];
+  // the scores w of tile i: bias, mask, and the columns' references
+  auto settle = [&](uint32_t i) {
+    const uint32_t key = b.key(from + i);
+    const bool masked = a.masked(b, key);
+#pragma unroll
+    for (uint32_t ct = 0; ct < SC; ++ct) a.bias_and_mask(col[ct], key + 4u * qq, masked, w[ct]);
+    if constexpr (OWN) raise<1, 0>(w, qi, r, l, nullptr, &factor);
+    else raise<CT, NT>(w, qi, r, l, acc, nullptr);
+  };
+  if (n) {
+    store(st.k[0], KROW, kr);
+    store(st.k[1], KROW, k1);
+    load(a.k, 2, r2, kr);
+    lds_barrier();
+    clear();
+#pragma unroll
+    for (uint32_t s = 0; s < 2 * KK; ++s) {
+      const h8_t kh = k_operand(0, s);
+#pragma unroll
+      for (uint32_t part = 0; part < 2 * CT; ++part) product(kh, s, part);
+    }
+    hand_over(0);
+    lds_barrier();
+    take_over(0);
+#pragma unroll
+    for (uint32_t ct = 0; ct < SC; ++ct)
+#pragma unroll
+      for (uint32_t e = 0; e < 8; ++e) w[ct][e] = a.score<CAP>(d[ct][e / 4][e % 4]);
+    settle(0);
+  }
+  for (uint32_t i = 0; i < n; ++i) {
+    const uint32_t cur = i & 1u, nxt = cur ^ 1u;
+    // V of tile i and K of tile i + 2 into the buffers that were last read before the barrier behind us; then the loads of
+    // the next step's
+    store(st.v[cur], VROW, vr);
+    store(st.k[cur], KROW, kr);
+    const Rows r4 = rows_of(i + 4u);
+    load(a.v, i + 1u, r1, vr);
+    load(a.k, i + 3u, r3, kr);
+    r1 = r2;
+    r2 = r3;
+    r3 = r4;
+    h8_t p[CT];
+    {  // (behind the last tile the products are of a tile that is not used)
+      constexpr uint32_t S = 2 * KK, AHEAD = 3;
+      h8_t kh[S];
+      clear();
+#pragma unroll
+      for (uint32_t s = 0; s < AHEAD; ++s) kh[s] = k_operand(nxt, s);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (uint32_t s = 0; s < S; ++s) {
+        if (s + AHEAD < S) kh[s + AHEAD] = k_operand(nxt, s + AHEAD);
+#pragma unroll
+        for (uint32_t h = 0; h < CT; ++h) {  // two products, one weight (or a weight for every four)
+          product(kh[s], s, 2 * h);
+          product(kh[s], s, 2 * h + 1);
+          if (h >= SC) continue;
+          const uint32_t x = s * SC + h, ct = x / 8, e = x % 8;
+          w[ct][e] = __builtin_amdgcn_exp2f(w[ct][e] - r[ct]);
+          l[ct] += w[ct][e];
+          if (e % 2) {
+            u4_t pk = __builtin_bit_cast(u4_t, p[ct]);
+            pk[e / 2] = h2_bits(__builtin_convertvector((f2_t{w[ct][e - 1], w[ct][e]}), h2_t));
+            p[ct] = __builtin_bit_cast(h8_t, pk);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      hand_over(nxt);
+      if constexpr (OWN) {
+        st.p[cur][wave][lane] = p[0];
+        st.f[cur][wave][lane] = factor;
+      }
+    }
+    lds_barrier();
+    {
+      const uint16_t* vb = st.v[cur] + (4u * qq + (qi >> 2)) * VROW + 128u * ds + 4u * (qi & 3u);
+      constexpr uint32_t AHEAD = 3;
+      h8_t av[NT];
+#pragma unroll
+      for (uint32_t tt = 0; tt < AHEAD; ++tt) av[tt] = v_operand<VROW>(vb, tt);
+      if constexpr (OWN) {
+        p[1] = st.p[cur][wave ^ 4u][lane];
+        const float other = st.f[cur][wave ^ 4u][lane];
+        if (__ballot(factor != 1.f || other != 1.f)) {
+#pragma unroll
+          for (uint32_t tt = 0; tt < NT; ++tt) {
+            acc[0][tt] *= factor;
+            acc[1][tt] *= other;
+          }
+        }
+        factor = 1.f;
+      }
+      take_over(nxt);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (uint32_t tt = 0; tt < NT; ++tt) {
+        if (tt + AHEAD < NT) av[tt + AHEAD] = v_operand<VROW>(vb, tt + AHEAD);
+#pragma unroll
+        for (uint32_t ct = 0; ct < CT; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[tt], p[ct], acc[ct][tt], 0, 0, 0);
+#pragma unroll
+        for (uint32_t ct = 0; ct < SC; ++ct) w[ct][tt] = a.score<CAP>(d[ct][tt / 4][tt % 4]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (i + 1u < n) settle(i + 1u);
+    }
+  }
+  if (ORDER != kContiguous && __ballot(outside)) a.report_pages(pl, b, from, from + n, 1u);
+  float sum[CT];
+  bool bad = false;
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    float z = 0.f;
+    if (ct < SC) {
+      sum[ct] = col_sum(l[ct]);
+      z = sum[ct] - sum[ct];
+    }
+#pragma unroll
+    for (uint32_t tt = 0; tt < NT; ++tt) z = not_finite(z, acc[ct][tt]);
+    bad |= live[ct] && z != 0.f;
+  }
+  if constexpr (OWN) st.f[n & 1u][wave][lane] = sum[0];  // (the last step's are in the other half)
+  if (__syncthreads_or(bad)) {
+    slow_block<HD>(a, pl, b, from, from + n, [&](float(&w)[8]) { w[0] = a.score<CAP>(w[0]); });
+    return;
+  }
+  if constexpr (OWN) sum[1] = st.f[n & 1u][wave ^ 4u][lane];
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    if (row[ct] >= rows_here) continue;
+    if (pl.splits > 1) {
+#pragma unroll
+      for (uint32_t tt = 0; tt < NT; ++tt)
+        store_part<HD>(a, pl, row[ct], g[ct], qq, 8u * ds + tt, live[ct] ? acc[ct][tt] : f4_t{0.f, 0.f, 0.f, 0.f});
+      if (qq == 0 && (OWN ? ct == 0 : ds == 0)) {
+        float* o = a.part_at<HD>(pl, row[ct], g[ct]);
+        o[HD] = r[ct < SC ? ct : 0];
+        o[HD + 1] = live[ct] ? sum[ct] : 0.f;
+      }
+    } else {
+      const float inv = live[ct] && sum[ct] != 0.f ? 1.0f / sum[ct] : 0.f;
+#pragma unroll
+      for (uint32_t tt = 0; tt < NT; ++tt)
+        store_out<HD>(a, j, t0 + row[ct], g[ct], qq, 8u * ds + tt, inv == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : acc[ct][tt] * inv);
+    }
+  }
+}
 template <int HD, int CT, Cap CAP>
 void launch_order(const MaskedRows& a, const dim3& grid, hipStream_t st) {
-  if (!a.pages) attn_rows_kernel<HD, CT, CAP, kContiguous><<<grid, 2 * HD, 0, st>>>(a);
-  else if (a.page % kTile == 0) attn_rows_kernel<HD, CT, CAP, kWholeTiles><<<grid, 2 * HD, 0, st>>>(a);
-  else attn_rows_kernel<HD, CT, CAP, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
+  if (!a.pages) attn_masked_kernel<HD, CT, CAP, kContiguous><<<grid, 2 * HD, 0, st>>>(a);
+  else if (a.page % kTile == 0) attn_masked_kernel<HD, CT, CAP, kWholeTiles><<<grid, 2 * HD, 0, st>>>(a);
+  else attn_masked_kernel<HD, CT, CAP, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
 }
 // Caps above kPlainCap take one column tile (two do not fit the registers), in one kernel for every order of the cache: they are
 // the rare ones. Measured (us; cap 257, then 30): 2048 rows causal, 40 / 8 heads of 128 117, 93; 7 documents in them 41, 38; 500
@@ -249,7 +535,7 @@ void launch_order(const MaskedRows& a, const dim3& grid, hipStream_t st) {
 template <int HD, int CT>
 void launch_chunk(const MaskedRows& a, const dim3& grid, hipStream_t st) {
   if constexpr (CT == 1)
-    if (a.form == kAnyCap) return attn_rows_kernel<HD, 1, kAnyCap, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
+    if (a.form == kAnyCap) return attn_masked_kernel<HD, 1, kAnyCap, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
   if (a.form == kPlain) launch_order<HD, CT, kPlain>(a, grid, st);
   else launch_order<HD, CT, kNoCap>(a, grid, st);
 }

@@ -62,7 +62,6 @@ struct TreeRows : TreeArgs {
     uint32_t last, n, free, base;  // free: so many keys every row of the block sees
     const uint32_t* pages;
     __device__ __forceinline__ uint32_t key(uint32_t i) const { return kTile * i; }
-    __device__ __forceinline__ uint32_t within(uint32_t, uint32_t k) const { return min(k, last); }
   };
   struct Column {
     const uint32_t* bits;
@@ -215,10 +214,6 @@ struct TreeRows : TreeArgs {
     const int32_t n = (int32_t)(key - c.first);
     return (word(c, n >> 5) >> (n & 31)) & 1u;
   }
-  template <Cap>
-  __device__ __forceinline__ float score(float s) const {
-    return s * c;
-  }
   __device__ __forceinline__ void scores_by_form(float (&w)[8]) const {
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) w[e] *= c;
@@ -231,7 +226,6 @@ struct TreeRows : TreeArgs {
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) w[e] = (bits >> (16u * (e / 4) + e % 4)) & 1u ? w[e] : -INFINITY;
   }
-  __device__ __forceinline__ uint32_t first_row(const Block& b, uint32_t key) const { return b.base + key; }
   // the cache row of a key of the sequence; `outside`: its page's entry is not the cache's, and the row is the first page's
   __device__ __forceinline__ uint32_t cache_row(const Block& b, uint32_t key, bool& outside) const {
     if (!b.pages) return b.base + key;
@@ -255,17 +249,300 @@ struct TreeRows : TreeArgs {
   }
 };
 
-// Joins the parts of columns: HD / 4 threads side by side take a column, each four dims of all its parts, eight parts at a time; a
+// 16 bytes per lane from base + off straight into LDS [lds, lds + 1024), lane L at lds + 16 L. The compiler neither sees what this
+// writes nor counts the load: the kernel waits by vmcnt itself (the compiler's own loads only make such a wait stricter).
+__device__ __forceinline__ void load_lds(uint32_t lds, const uint16_t* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds(uint32_t lds, const uint16_t* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(from) : "memory");
+}
+template <uint32_t N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+// Blocks of more than 16 columns: four waves side by side, CT column tiles and all dims each, all walking the same 32-key tiles. K and V
+// go straight into LDS, into rings of three and four tiles: a tile's loads have two steps. A step i:
+//   the products of tile i + 1's scores, dealt out among the exponentials that make tile i's weights;
+//   the barrier: behind it every wave has read K of tile i + 1 and V of tile i - 1, whose places take K of tile i + 4 and V of
+//   tile i + 3, and the loads of two steps ago (K of i + 2, V of i + 1) are there;
+//   P V of tile i, dealt out among tile i + 1's masks and maxima.
+// The first operands of each half are read in the one before. Rows of a tile lie 2 HD bytes apart in LDS, the 16-byte pieces of row r
+// in the order p ^ (r % 16): the 16 rows of a read fall on distinct banks.
+template <int HD, int CT, Order ORDER>
+__global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void attn_tree_kernel(TreeRows a) {
+  constexpr uint32_t KK = HD / 32, NT = HD / 16, S = 2 * KK, ROW = 2 * HD, TILE = kTile * ROW;
+  constexpr uint32_t NI = TILE / 4096, RPI = 1024 / ROW, PPR = ROW / 16;  // a wave's loads of a tile, rows of each, pieces of a row
+  constexpr uint32_t AK = 3, AV = 3, PER = KK / 2;  // operands read ahead; products for each weight
+  __shared__ __align__(1024) uint8_t ring[7 * TILE];
+  const typename TreeRows::Place p = a.place(true);
+  if (p.rows == 0u) return;
+  const TreeRows::Block b = a.block(p);
+  const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), qi = lane & 15u,
+                 qq = lane >> 4;
+  auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
+  const uint32_t from = uniform(a.part_begin(p, b, p.split)), n = uniform(a.part_begin(p, b, p.split + 1u)) - from;
+  const uint32_t last = uniform(b.last);
+  uint32_t row[CT], g[CT];
+  h8_t qh[CT][KK], ql[CT][KK];
+  // ---- the loads ----
+  const uint32_t lds = (uint32_t)(uintptr_t)ring;
+  const size_t hoff = (size_t)uniform(p.j) * a.head_stride;
+  // a load's row of the tile, its piece's elements, and its bytes behind the tile's first row, in the last tile too
+  uint32_t place[NI], piece[NI], off[NI], off_last[NI];
+#pragma unroll
+  for (uint32_t c = 0; c < NI; ++c) {
+    place[c] = (4u * c + wave) * RPI + lane / PPR;
+    piece[c] = 8u * ((lane % PPR) ^ (place[c] & 15u));
+    off[c] = 2u * (place[c] * (uint32_t)a.row_stride + piece[c]);
+    off_last[c] = 2u * (min(place[c], (last - b.key(from + n - 1u))) * (uint32_t)a.row_stride + piece[c]);
+  }
+  bool outside = false;
+  struct Rows {
+    uint32_t r[ORDER == kAnyPages ? NI : 1];  // the cache rows of a tile: its first, or each load's
+  };
+  // (whole tiles) 64 entries of the page table from that of tile i on, a lane each, and the first's number
+  uint32_t entries = 0, entries_at = 0;
+  auto fetch = [&](uint32_t i) {
+    entries_at = b.key(from + min(i, n - 1u)) >> a.page_shift;
+    entries = b.pages[min(entries_at + lane, last >> a.page_shift)];
+    asm volatile("" ::"v"(entries));  // (waited for here, not in the loop)
+  };
+  auto rows_of = [&](uint32_t i) {
+    const uint32_t key = b.key(from + min(i, n - 1u));
+    Rows w;
+    if constexpr (ORDER == kContiguous) {
+      w.r[0] = b.base + key;
+    } else if constexpr (ORDER == kWholeTiles) {
+      const uint32_t at = key >> a.page_shift, pg = (uint32_t)__builtin_amdgcn_readlane((int)entries, (int)(at - entries_at));
+      outside |= pg >= a.n_pages;
+      w.r[0] = (pg < a.n_pages ? pg << a.page_shift : 0u) + (key - (at << a.page_shift));
+    } else {
+#pragma unroll
+      for (uint32_t c = 0; c < NI; ++c) w.r[c] = a.cache_row(b, min(key + place[c], b.last), outside);
+    }
+    return w;
+  };
+  auto load = [&](const uint16_t* cache, uint32_t to, uint32_t i, const Rows& w) {
+    if constexpr (ORDER == kAnyPages) {
+#pragma unroll
+      for (uint32_t c = 0; c < NI; ++c)
+        load_lds(lds + to + (4u * c + wave) * 1024u, cache + ((size_t)w.r[c] * a.row_stride + hoff + piece[c]));
+    } else {
+      const uint16_t* base = cache + ((size_t)uniform(w.r[0]) * a.row_stride + hoff);
+#pragma unroll
+      for (uint32_t c = 0; c < NI; ++c)
+        load_lds(lds + to + (4u * c + wave) * 1024u, base, i + 1u < n ? off[c] : off_last[c]);
+    }
+  };
+  auto k_at = [](uint32_t i) { return i % 3u * TILE; };
+  auto v_at = [](uint32_t i) { return (3u + i % 4u) * TILE; };
+  // the columns' queries, scaled, as the B operand in f16 high and low parts: k = 32 kk + 8 qq + e
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    const uint32_t col = 16u * (CT * wave + ct) + qi;
+    row[ct] = col / a.gqa;
+    g[ct] = col % a.gqa;
+    const float* qp = a.q + ((size_t)(p.t0 + (row[ct] < p.rows ? row[ct] : 0u)) * a.q_heads + p.j * a.gqa + g[ct]) * HD + 8u * qq;
+    f4_t q[2 * KK];
+#pragma unroll
+    for (uint32_t x = 0; x < 2 * KK; ++x) q[x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2))) * a.c;
+    split_q<KK>(q, qh[ct], ql[ct]);
+    if constexpr (HD * CT > 256) {  // (in accumulation registers, which the products read too: the others are the vector ALUs')
+#pragma unroll
+      for (uint32_t kk = 0; kk < KK; ++kk) asm volatile("" : "+a"(qh[ct][kk]), "+a"(ql[ct][kk]));
+    }
+  }
+  Rows r2{}, r3{};
+  if (n) {
+    if constexpr (ORDER == kWholeTiles) fetch(0);
+    const Rows r0 = rows_of(0), r1 = rows_of(1);
+    r2 = rows_of(2);
+    r3 = rows_of(3);
+    load(a.k, k_at(0), 0, r0);
+    load(a.k, k_at(1), 1, r1);
+    load(a.v, v_at(0), 0, r0);
+    load(a.k, k_at(2), 2, r2);
+    load(a.v, v_at(1), 1, r1);
+    wait_loads<2 * NI>();
+    lds_barrier();
+    // V of tile 2 and K of tile 3 follow behind the first scores
+  }
+  float r[CT], l[CT], w[CT][8];
+  f4_t acc[CT][NT], d[CT][2];
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    r[ct] = kNoKey;
+    l[ct] = 0.f;
+#pragma unroll
+    for (uint32_t tt = 0; tt < NT; ++tt) acc[ct][tt] = f4_t{0.f, 0.f, 0.f, 0.f};
+  }
+  // K operand s = 2 kk + gg: 16 keys x 32 dims
+  auto k_operand = [&](uint32_t to, uint32_t s) {
+    const uint32_t at = qi * ROW + 16u * ((4u * (s / 2u) + qq) ^ qi);
+    return *reinterpret_cast<const h8_t*>(ring + to + at + (s % 2u) * 16u * ROW);
+  };
+  // V^T of 32 keys x 16 dims: the k of the product are the keys 4 qq + e of the two 16-key groups, which is how the lanes hold the
+  // weights
+  auto v_operand_at = [&](uint32_t to, uint32_t tt) {
+    const uint32_t vrow = 4u * qq + (qi >> 2), at = vrow * ROW + 16u * ((2u * tt + ((qi >> 1) & 1u)) ^ vrow) + 8u * (qi & 1u);
+    const v4s_t a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(reinterpret_cast<const uint16_t*>(ring + to + at)));
+    const v4s_t a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(reinterpret_cast<const uint16_t*>(ring + to + at + 16u * ROW)));
+    return __builtin_bit_cast(h8_t, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  auto product = [&](h8_t kh, uint32_t s, uint32_t part) {  // part < 2 CT: the columns' high parts, then the low ones
+    const uint32_t ct = part % CT;
+    d[ct][s % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, part < CT ? qh[ct][s / 2] : ql[ct][s / 2], d[ct][s % 2], 0, 0, 0);
+  };
+  auto clear = [&]() {
+#pragma unroll
+    for (uint32_t ct = 0; ct < CT; ++ct) d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+  };
+  // a tile's scores of column tile ct and the largest of them; behind that tile i's masks and the references
+  float mx[CT];
+  auto scores = [&](uint32_t ct) {
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) w[ct][e] = d[ct][e / 4][e % 4];
+    mx[ct] = most_of(w[ct]);
+    asm volatile("" : "+v"(mx[ct]));  // (formed here, between the products, not where it is used)
+  };
+  auto settle = [&](uint32_t i) {
+    const uint32_t key = b.key(from + i);
+    if (a.masked(b, key)) {
+#pragma unroll
+      for (uint32_t ct = 0; ct < CT; ++ct) {
+        a.bias_and_mask(a.column(p, b, row[ct], g[ct]), key + 4u * qq, true, w[ct]);
+        mx[ct] = most_of(w[ct]);
+      }
+    }
+    raise_to<CT, NT>(mx, qi, r, l, acc, nullptr);
+  };
+  h8_t kh[S], av[NT];
+  if (n) {
+    clear();
+#pragma unroll
+    for (uint32_t s = 0; s < S; ++s) {
+      const h8_t k0 = k_operand(k_at(0), s);
+#pragma unroll
+      for (uint32_t part = 0; part < 2 * CT; ++part) product(k0, s, part);
+    }
+#pragma unroll
+    for (uint32_t ct = 0; ct < CT; ++ct) scores(ct);
+    settle(0);
+    lds_barrier();
+    load(a.k, k_at(3), 3, r3);
+    load(a.v, v_at(2), 2, r2);
+#pragma unroll
+    for (uint32_t s = 0; s < AK; ++s) kh[s] = k_operand(k_at(1), s);
+  }
+  uint32_t k1 = TILE, k2 = 2u * TILE, k3 = 0u, v0 = 3u * TILE, v1 = 4u * TILE, v2 = 5u * TILE, v3 = 6u * TILE;  // of tiles i + ..
+#pragma unroll 1
+  for (uint32_t i = 0; i < n; ++i) {
+    if constexpr (ORDER == kWholeTiles)
+      if (i % 32u == 0u) fetch(i + 4u);  // (pages hold a tile at least: 64 entries serve 64 steps)
+    h8_t pw[CT];
+    {  // (behind the last tile the products are of a tile that is not used)
+      clear();
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (uint32_t s = 0; s < S; ++s) {
+        if (s + AK < S) kh[s + AK] = k_operand(k1, s + AK);
+        if (s + AV >= S) av[s + AV - S] = v_operand_at(v0, s + AV - S);
+#pragma unroll
+        for (uint32_t part = 0; part < 2 * CT; ++part) {
+          product(kh[s], s, part);
+          const uint32_t done = s * 2 * CT + part + 1u;
+          if (done % PER) continue;
+          const uint32_t x = done / PER - 1u, ct = x / 8, e = x % 8;
+          w[ct][e] = __builtin_amdgcn_exp2f(w[ct][e] - r[ct]);
+          l[ct] += w[ct][e];
+          asm volatile("" : "+v"(l[ct]));
+          if (e % 2) {
+            u4_t pk = __builtin_bit_cast(u4_t, pw[ct]);
+            pk[e / 2] = h2_bits(__builtin_convertvector((f2_t{w[ct][e - 1], w[ct][e]}), h2_t));
+            pw[ct] = __builtin_bit_cast(h8_t, pk);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    wait_loads<2 * NI>();
+    lds_barrier();
+    {
+      const Rows r4 = rows_of(i + 4u);
+      load(a.k, k1, i + 4u, r4);
+      load(a.v, v3, i + 3u, r3);
+      r3 = r4;
+    }
+    {
+#pragma unroll
+      for (uint32_t tt = 0; tt < NT; ++tt) {
+        if (tt + AV < NT) av[tt + AV] = v_operand_at(v0, tt + AV);
+        if (tt + AK >= NT) kh[tt + AK - NT] = k_operand(k2, tt + AK - NT);
+#pragma unroll
+        for (uint32_t ct = 0; ct < CT; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[tt], pw[ct], acc[ct][tt], 0, 0, 0);
+        if (tt >= 1 && tt <= CT) scores(tt - 1);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    if (i + 1u < n) settle(i + 1u);
+    const uint32_t k = k1, v = v0;
+    k1 = k2;
+    k2 = k3;
+    k3 = k;
+    v0 = v1;
+    v1 = v2;
+    v2 = v3;
+    v3 = v;
+  }
+  wait_loads<0>();
+  if (ORDER != kContiguous && __ballot(outside)) a.report_pages(p, b, from, from + n, 1u);
+  float sum[CT];
+  bool bad = false;
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    sum[ct] = col_sum(l[ct]);
+    float z = sum[ct] - sum[ct];
+#pragma unroll
+    for (uint32_t tt = 0; tt < NT; ++tt) z = not_finite(z, acc[ct][tt]);
+    bad |= row[ct] < p.rows && z != 0.f;
+  }
+  if (__syncthreads_or(bad)) {
+    slow_block<HD>(a, p, b, from, from + n, [&](float(&w)[8]) { a.scores_by_form(w); });
+    return;
+  }
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+    if (row[ct] >= p.rows) continue;
+    if (p.splits > 1) {
+#pragma unroll
+      for (uint32_t tt = 0; tt < NT; ++tt) store_part<HD>(a, p, row[ct], g[ct], qq, tt, acc[ct][tt]);
+      if (qq == 0) {
+        float* o = a.template part_at<HD>(p, row[ct], g[ct]);
+        o[HD] = r[ct];
+        o[HD + 1] = sum[ct];
+      }
+    } else {
+      const float inv = sum[ct] != 0.f ? 1.0f / sum[ct] : 0.f;
+#pragma unroll
+      for (uint32_t tt = 0; tt < NT; ++tt)
+        store_out<HD>(a, p.j, p.t0 + row[ct], g[ct], qq, tt, inv == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : acc[ct][tt] * inv);
+    }
+  }
+}
+
+// Joins the parts of columns: HD / 4 threads side by side take a column, each four dims of all its parts, U parts at a time; a
 // work-group `C` columns of one row (C 1: all its threads one column's, which then share the parts out).
 template <int HD, bool MANY>
 __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a, uint32_t most) {
-  constexpr uint32_t L = HD / 4, G = 256 / L, U = 8;
+  constexpr uint32_t L = HD / 4, G = 256 / L, U = MANY ? 8 : 4;
   const uint32_t t = blockIdx.y, g = threadIdx.x / L, d = threadIdx.x % L;
   const uint32_t h = MANY ? blockIdx.x : blockIdx.x * G + g;
-  if (t < a.row_start[0] || t >= min(a.row_start[a.sequences], a.T)) return;  // (uniform: no sequence's row)
-  const u4_t info = a.info[t];
-  const uint32_t splits = min(info[2], kMaxSplits);
-  if (splits < 2u) return;  // (uniform: its work-group stored it)
+  const u4_t info = *as_global(a.info + t);
+  const uint32_t first = a.row_start[0], end = min(a.row_start[a.sequences], a.T), splits = min(info[2], kMaxSplits);
+  asm volatile("" ::"v"(info), "s"(first), "s"(end));  // (one round trip for all three)
+  if (t < first || t >= end || splits < 2u) return;  // (uniform: no sequence's row, or its work-group stored it)
   if (!MANY && h >= a.q_heads) return;
   const uint32_t j = h / a.gqa, col = info[3] * a.gqa + h % a.gqa;
   auto part = [&](uint32_t s) {  // (within the workspace whatever row_start held)
@@ -333,12 +610,12 @@ struct Pick {
 constexpr uint32_t kCus = 256;
 Pick few_rows(uint32_t gqa, uint32_t hd) { return Pick{true, 1, 16u / gqa, 16, (hd == 128 ? 2u : 1u) * kCus}; }
 Pick chunk(uint32_t ct, uint32_t gqa, uint32_t hd) {
-  return Pick{false, ct, 64u * ct / gqa, 64u * ct, hd == 128 ? (4u - ct) * kCus : kCus};
+  return Pick{false, ct, 64u * ct / gqa, 64u * ct, hd == 128 ? 2u * kCus : kCus};
 }
 Pick pick(uint32_t T, uint32_t sequences, uint32_t gqa, uint32_t hd) {
   const uint32_t each = (T + sequences - 1u) / sequences * gqa;  // columns
   if (each <= 16u) return few_rows(gqa, hd);
-  return chunk(each <= 64u ? 1u : 2u, gqa, hd);
+  return chunk(hd == 256 && each <= 64u ? 1u : 2u, gqa, hd);
 }
 // The parts of all sequences at most, one for each block aside: as many as make every work-group that runs at once busy, where there
 // are several sequences some times as many.
@@ -355,9 +632,10 @@ bool shape_ok(const mi_attn_shape* s) {
 }
 template <int HD, int CT>
 void launch_chunk(const TreeRows& a, uint32_t grid, hipStream_t st) {
-  if (!a.tables) attn_rows_kernel<HD, CT, kNoCap, kContiguous><<<grid, 2 * HD, 0, st>>>(a);
-  else if (a.page % kTile == 0) attn_rows_kernel<HD, CT, kNoCap, kWholeTiles><<<grid, 2 * HD, 0, st>>>(a);
-  else attn_rows_kernel<HD, CT, kNoCap, kAnyPages><<<grid, 2 * HD, 0, st>>>(a);
+  const bool near = a.row_stride <= 1u << 25;  // (a tile's rows by a 32-bit offset)
+  if (!a.tables && near) attn_tree_kernel<HD, CT, kContiguous><<<grid, 256, 0, st>>>(a);
+  else if (a.tables && a.page >= kTile && a.page_shift < 32u && near) attn_tree_kernel<HD, CT, kWholeTiles><<<grid, 256, 0, st>>>(a);
+  else attn_tree_kernel<HD, CT, kAnyPages><<<grid, 256, 0, st>>>(a);
 }
 
 }  // namespace
@@ -373,7 +651,7 @@ size_t mi_attn_tree_ws(uint32_t T, uint32_t sequences, const mi_attn_shape* shap
   // the most that any call of up to T rows takes
   size_t floats = gqa <= 16u ? part_floats(few_rows(gqa, hd), shape->kv_heads, 2u, hd) : 0u;
   for (uint32_t ct = 1; ct <= 2; ++ct)
-    if (T * gqa > (ct == 1u ? 16u : 64u)) floats = std::max(floats, part_floats(chunk(ct, gqa, hd), shape->kv_heads, 2u, hd));
+    if (hd == 256 ? T * gqa > (ct == 1u ? 16u : 64u) : ct == 2u && T * gqa > 16u) floats = std::max(floats, part_floats(chunk(ct, gqa, hd), shape->kv_heads, 2u, hd));
   return (size_t)T * sizeof(u4_t) + floats * 4u;
 }
 
@@ -456,8 +734,7 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
     if (narrow) attn_rows_few_kernel<128><<<grid, 256, 0, st>>>(a);
     else attn_rows_few_kernel<256><<<grid, 256, 0, st>>>(a);
   } else if (narrow) {
-    if (p.ct == 2) launch_chunk<128, 2>(a, grid, st);
-    else launch_chunk<128, 1>(a, grid, st);
+    launch_chunk<128, 2>(a, grid, st);
   } else {
     if (p.ct == 2) launch_chunk<256, 2>(a, grid, st);
     else launch_chunk<256, 1>(a, grid, st);
