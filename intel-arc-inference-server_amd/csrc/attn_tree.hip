@@ -603,6 +603,15 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a, uint32_
   store_out<HD>(a, j, t, h % a.gqa, d % 4u, d / 4u, o * inv);
 }
 
+// The launch: the few-rows kernel up to 16 columns a sequence, else the other with CT column tiles a wave (64 CT columns a
+// work-group; two work-groups a CU of rows of 128 with CT 2).
+//   rows of 256: CT 1 up to 64 columns, else 2. Measured (us): 6 ragged sequences up to 8200 keys, 16 / 2 heads, 8 rows 28.5
+//   against 32.7; 8 sequences, 30 rows 57.4 against 55.8; one of 131072, 60 rows 254 against 204.
+//   rows of 128: one sequence's rows make blocks / CT work-groups of a known number: the least modelled time of 2, 3 and 4, a
+//   block's tile 1.1, 1.375 and 1.7 us of a CU. Measured (us; CT 2, 3, 4): over 65536 keys, 40 / 8 heads, 25 rows 81 / 101 / 127, 38
+//   rows 117 / 100 / 121, 51 rows 211 / 167 / 121, 64 rows 209 / 168 / 200; over 8192 keys 27 / 27 / 31, 32 / 30 / 33, 37 / 37 / 36,
+//   38 / 38 / 44. Of several sequences only the mean is known: CT 2, which loses least where they are ragged (8 trees of 30 to 61
+//   rows 118 / 144 / 170; of 51 each, 4000 keys, 77 / 84 / 70).
 struct Pick {
   bool few;
   uint32_t ct, rows, columns, slots;
@@ -610,12 +619,24 @@ struct Pick {
 constexpr uint32_t kCus = 256;
 Pick few_rows(uint32_t gqa, uint32_t hd) { return Pick{true, 1, 16u / gqa, 16, (hd == 128 ? 2u : 1u) * kCus}; }
 Pick chunk(uint32_t ct, uint32_t gqa, uint32_t hd) {
-  return Pick{false, ct, 64u * ct / gqa, 64u * ct, hd == 128 ? 2u * kCus : kCus};
+  return Pick{false, ct, 64u * ct / gqa, 64u * ct, hd == 128 && ct == 2u ? 2u * kCus : kCus};
 }
 Pick pick(uint32_t T, uint32_t sequences, uint32_t gqa, uint32_t hd) {
   const uint32_t each = (T + sequences - 1u) / sequences * gqa;  // columns
   if (each <= 16u) return few_rows(gqa, hd);
-  return chunk(hd == 256 && each <= 64u ? 1u : 2u, gqa, hd);
+  if (hd == 256) return chunk(each <= 64u ? 1u : 2u, gqa, hd);
+  Pick best = chunk(2u, gqa, hd);
+  if (sequences > 1u) return best;
+  static constexpr double kTau[5] = {0.0, 0.0, 1.1, 1.375, 1.7};
+  double least = 1e300;
+  for (uint32_t ct = 2; ct <= 4; ++ct) {
+    const Pick p = chunk(ct, gqa, hd);
+    const double c = ((T + p.rows - 1u) / p.rows) * kTau[ct];
+    if (c >= least) continue;
+    least = c;
+    best = p;
+  }
+  return best;
 }
 // The parts of all sequences at most, one for each block aside: as many as make every work-group that runs at once busy, where there
 // are several sequences some times as many.
@@ -650,8 +671,9 @@ size_t mi_attn_tree_ws(uint32_t T, uint32_t sequences, const mi_attn_shape* shap
   const uint32_t gqa = shape->q_heads / shape->kv_heads, hd = shape->head_dim;
   // the most that any call of up to T rows takes
   size_t floats = gqa <= 16u ? part_floats(few_rows(gqa, hd), shape->kv_heads, 2u, hd) : 0u;
-  for (uint32_t ct = 1; ct <= 2; ++ct)
-    if (hd == 256 ? T * gqa > (ct == 1u ? 16u : 64u) : ct == 2u && T * gqa > 16u) floats = std::max(floats, part_floats(chunk(ct, gqa, hd), shape->kv_heads, 2u, hd));
+  if (T * gqa > 16u)
+    for (uint32_t ct = 1; ct <= 4; ++ct)
+      floats = std::max(floats, part_floats(chunk(ct, gqa, hd), shape->kv_heads, ct <= 2u ? 2u : 1u, hd));
   return (size_t)T * sizeof(u4_t) + floats * 4u;
 }
 
@@ -734,7 +756,9 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
     if (narrow) attn_rows_few_kernel<128><<<grid, 256, 0, st>>>(a);
     else attn_rows_few_kernel<256><<<grid, 256, 0, st>>>(a);
   } else if (narrow) {
-    launch_chunk<128, 2>(a, grid, st);
+    if (p.ct == 2) launch_chunk<128, 2>(a, grid, st);
+    else if (p.ct == 3) launch_chunk<128, 3>(a, grid, st);
+    else launch_chunk<128, 4>(a, grid, st);
   } else {
     if (p.ct == 2) launch_chunk<256, 2>(a, grid, st);
     else launch_chunk<256, 1>(a, grid, st);

@@ -171,7 +171,8 @@ def test_small(lengths, qh, kvh, hd, trees):
 @pytest.mark.parametrize("lengths,qh,kvh,hd", [
     ([(20000, 1)], 10, 2, 128), ([(9000, 2)], 16, 2, 256), ([(5000, 61)], 40, 8, 128), ([(6000, 60)], 16, 2, 256), ([(1500, 130)], 16, 2, 256),
     ([(700, 700)], 40, 8, 128), ([(3000, 12), (10, 12), (900, 12)], 10, 2, 128), ([(100 * i, 1) for i in range(30)], 10, 2, 128),
-    ([(4000, 40), (100, 64), (2000, 7)], 32, 8, 128)])
+    ([(4000, 40), (100, 64), (2000, 7)], 32, 8, 128), ([(3000, 38)], 10, 2, 128), ([(2500, 51)], 40, 8, 128), ([(100, 51)], 10, 2, 128),
+    ([(1000, 256)], 3, 3, 128), ([(600, 24)], 16, 2, 128), ([(50, 5)], 64, 1, 128)])
 @pytest.mark.parametrize("page", [0, 16, 24, 64])
 def test_long(lengths, qh, kvh, hd, page):
     Case(len(lengths) + page, lengths, qh, kvh, hd, page=page, trees="causal" if lengths[0][1] > 200 else "tree").check()
