@@ -27,7 +27,7 @@
 namespace mi {
 namespace {
 
-constexpr uint32_t kMaxRows = 65535, kMaxVocab = 1u << 23, kMaxTop = 64, kMaxBeams = 64, kNone = 0xFFFFFFFFu;
+constexpr uint32_t kMaxRows = 65535, kMaxVocab = 1u << 23, kMaxTop = 64, kNone = 0xFFFFFFFFu;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogprobArgs {
@@ -575,11 +575,41 @@ struct BeamArgs {
   uint32_t *ids, *from;
   float* scores;
 };
-// grid (batch), four waves: a wave merges every fourth beam's candidates, 64 at a time over its lanes, then the waves' join. Bound by
-// its chain: two rounds of loads, a logarithm, six exchanges a beam.
+// what a beam's logits are added to, of its maximum and sum
+__device__ __forceinline__ double beam_base(float cum, float m, float z) { return (double)cum - (double)m - log((double)z); }
+__device__ __forceinline__ void take_best(Candidate& list, const Candidate& c, uint32_t lane) {  // (c: the best last)
+  if (better(c, list)) list = c;
+  half_clean<32>(list, lane);
+}
+// W waves' lists into the first's: whether this wave holds the joint one
+template <uint32_t W>
+struct JointCandidates {
+  double score[W][64];
+  uint32_t at[W][64];
+};
+template <uint32_t W>
+__device__ __forceinline__ bool join_candidates(JointCandidates<W>& j, Candidate& list, uint32_t wave, uint32_t lane) {
+#pragma unroll 1
+  for (uint32_t step = W / 2; step; step /= 2) {
+    j.score[wave][lane] = list.score;
+    j.at[wave][lane] = list.at;
+    __syncthreads();
+    if (wave >= step) return false;
+    take_best(list, Candidate{j.score[wave + step][63u - lane], j.at[wave + step][63u - lane]}, lane);
+  }
+  return true;
+}
+__device__ __forceinline__ void answer_beam(const BeamArgs& a, uint32_t batch, uint32_t place, bool none, uint32_t id, uint32_t w,
+                                            double score) {
+  const size_t to = (size_t)batch * a.k + place;
+  a.ids[to] = none ? kNone : id;
+  a.from[to] = none ? kNone : w;
+  a.scores[to] = none ? -INFINITY : (float)score;
+}
+// Behind lists of every row's best. grid (batch), four waves: a wave merges every fourth beam's candidates, 64 at a time over its
+// lanes, then the waves' join. Bound by its chain: two rounds of loads, a logarithm, six exchanges a beam.
 __global__ __launch_bounds__(256) void beam_select_kernel(BeamArgs a) {
-  __shared__ double score[4][64];
-  __shared__ uint32_t place[4][64];
+  __shared__ JointCandidates<4> joint;
   constexpr uint32_t U = 4;  // beams whose candidates are loaded at once
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, batch = blockIdx.x, n = 63u - lane;  // (the best come last)
   const uint32_t mine = batch * a.beams + min(lane, a.beams - 1u);
@@ -594,11 +624,11 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamArgs a) {
     }
   };
   load(wave);
-  // a lane a beam: what its logits are added to
+  // a lane a beam
   const float cum = *as_global(a.cum + mine);
   const f2_t s = *as_global(a.sums + mine);
   const uint64_t done = __ballot(a.done && a.done[mine]);
-  const uint64_t of = __builtin_bit_cast(uint64_t, (done >> lane) & 1u ? (double)cum : (double)cum - (double)s.x - log((double)s.y));
+  const uint64_t of = __builtin_bit_cast(uint64_t, (done >> lane) & 1u ? (double)cum : beam_base(cum, s.x, s.y));
   Candidate list;
   for (uint32_t w0 = wave; w0 < a.beams; w0 += 4u * U) {
     if (w0 != wave) load(w0);
@@ -612,27 +642,205 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamArgs a) {
       const double sum = ends ? base : base + (double)top[u];
       Candidate c;
       if ((ends ? n == 0u : n < a.k && id[u] != kNone) && sum > -INFINITY) c = Candidate{sum, 64u * w + n};  // (nor a NaN)
-      if (better(c, list)) list = c;
-      half_clean<32>(list, lane);
+      take_best(list, c, lane);
     }
   }
-#pragma unroll 1
-  for (uint32_t step = 2; step; step /= 2) {
-    score[wave][lane] = list.score;
-    place[wave][lane] = list.at;
-    __syncthreads();
-    if (wave >= step) return;
-    const Candidate o = {score[wave + step][63u - lane], place[wave + step][63u - lane]};
-    if (better(o, list)) list = o;
-    half_clean<32>(list, lane);
-  }
-  if (lane >= a.k) return;
-  const size_t to = (size_t)batch * a.k + lane;
+  if (!join_candidates<4>(joint, list, wave, lane) || lane >= a.k) return;
   const uint32_t w = list.at / 64u, row = batch * a.beams + w;
   const bool none = list.at == kNone;
-  a.ids[to] = none ? kNone : a.done && a.done[row] ? a.eos : a.top_ids[(size_t)row * a.k + list.at % 64u];
-  a.from[to] = none ? kNone : w;
-  a.scores[to] = (float)list.score;
+  answer_beam(a, batch, lane, none, none ? kNone : a.done && a.done[row] ? a.eos : a.top_ids[(size_t)row * a.k + list.at % 64u], w,
+              list.score);
+}
+
+// Behind slices, in place of logprobs_join_kernel and beam_select_kernel: grid (batch), eight waves. They join each beam's
+// statistics; form a bound that k runs of 256 tokens reach by the score of their largest logit (as logprobs_join_kernel's); read again
+// the runs that reach it, of all beams about k; and a token's place is the number of those read that are better. Where more tokens reach
+// the bound than fit, the waves keep a list of every beam. One text of 4 beams with k = 8 takes 14.1 us in all, 16 of 8 with k = 16
+// 29.4 (16.0 and 32 with the rows' lists first); equal logits 45, rising ones 104. Bound by its chain of loads.
+constexpr uint32_t kFit = 1024, kMaxBeams = 64;
+constexpr uint32_t kJoinWaves = 16, kJoinRuns = 8;  // a lane's runs
+uint32_t runs_of_wave(uint32_t vocab) { return ((vocab + 255u) / 256u + kJoinWaves - 1u) / kJoinWaves; }
+__global__ __launch_bounds__(64 * kJoinWaves) void beam_join_kernel(LogprobArgs a, BeamArgs o) {
+  constexpr uint32_t W = kJoinWaves, U = kJoinRuns, B = 4;  // B: runs read together
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, batch = blockIdx.x, runs = (a.vocab + 255u) / 256u;
+  const uint32_t row0 = batch * o.beams;
+  __shared__ double base[kMaxBeams];  // what a beam's logits are added to; NaN: it has no candidates among them
+  __shared__ float m[kMaxBeams], z[kMaxBeams], least[W];
+  __shared__ uint32_t fits, hit_runs[W][64 * U];  // beam, run (below 2^15)
+  __shared__ union {
+    struct {
+      double score[kFit];
+      float v[kFit];
+      uint32_t id[kFit], w[kFit];
+    } fit;
+    struct {
+      JointCandidates<W> joint;
+      uint32_t id[kMaxBeams][64];
+    } lists;
+  } sm;
+  // (every load that the bound waits for goes out at once; a wave has every W-th run of every beam)
+  float p[U];
+  uint32_t run[U], beam_of[U];
+  const uint32_t each = (runs + W - 1u) / W;
+#pragma unroll
+  for (uint32_t u = 0; u < U; ++u) {
+    const uint32_t i = lane + 64u * u;
+    beam_of[u] = i / each;
+    run[u] = (i - beam_of[u] * each) * W + wave;
+    p[u] = beam_of[u] < o.beams && run[u] < runs ? a.peaks[(size_t)(row0 + beam_of[u]) * runs + run[u]] : -INFINITY;
+  }
+  const uint32_t mine = min(lane, o.beams - 1u);
+  const float cum = *as_global(o.cum + row0 + mine);
+  const bool ends = o.done && o.done[row0 + mine];
+  if (threadIdx.x == 0) fits = 0;
+  for (uint32_t w = wave; w < o.beams; w += W) {
+    const f4_t* stats = a.stats + (size_t)(row0 + w) * a.slices;
+    Stats s;
+    for (uint32_t i0 = 0; i0 < a.slices; i0 += 256u) {
+      f4_t r[4];
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t i = i0 + 64u * j + lane;
+        r[j] = i < a.slices ? stats[i] : f4_t{-INFINITY, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 4; ++j) {
+        Stats of;
+        of.m = r[j][0];
+        of.z = r[j][1];
+        s.merge(of);
+      }
+    }
+    merge_lanes(s);
+    if (lane == 0) {
+      m[w] = s.m;
+      z[w] = s.z;
+    }
+  }
+  __syncthreads();
+  if (wave == 0 && lane < o.beams) base[lane] = ends ? __builtin_bit_cast(double, 0x7FF8000000000000ull) : beam_base(cum, m[lane], z[lane]);
+  __syncthreads();
+  // `see` gets the score of each run's largest logit, -inf where there is none
+  auto walk = [&](auto see) {
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u) {
+      if (64u * u >= o.beams * each) break;
+      const double of = beam_of[u] < o.beams ? base[beam_of[u]] + (double)p[u] : -INFINITY;
+      see(of > -INFINITY ? of : -INFINITY, beam_of[u], run[u]);  // (nor a NaN)
+    }
+  };
+  float top = -INFINITY;
+  walk([&](double of, uint32_t, uint32_t) { top = fmaxf(top, __double2float_rd(of)); });
+  const uint32_t share = (o.k + W - 1u) / W;
+  const float low = kth_largest(top, share, lane);
+  if (lane == 0) least[wave] = low;
+  __syncthreads();
+  float cut = INFINITY;
+#pragma unroll
+  for (uint32_t w = 0; w < W; ++w) cut = fminf(cut, least[w]);
+  auto put_in = [&](double score, float v, uint32_t id, uint32_t w) {
+    const uint32_t to = atomicAdd(&fits, 1u);
+    if (to < kFit) {
+      sm.fit.score[to] = score;
+      sm.fit.v[to] = v;
+      sm.fit.id[to] = id;
+      sm.fit.w[to] = w;
+    }
+  };
+  // the wave's runs that reach it, then their tokens
+  uint32_t hits = 0;
+  walk([&](double of, uint32_t w, uint32_t r) {
+    const bool hit = of > -INFINITY && of >= (double)cut;
+    const uint64_t who = __ballot(hit);
+    if (hit) hit_runs[wave][hits + (uint32_t)__popcll(who & ((1ull << lane) - 1u))] = w << 16 | r;
+    hits += (uint32_t)__popcll(who);
+  });
+  wave_lds_sync();
+#pragma unroll 1
+  for (uint32_t h = 0; h < hits; h += B) {
+    f4_t v[B];
+    uint32_t at[B], beam[B];
+    const uint32_t n = min(B, hits - h);
+#pragma unroll
+    for (uint32_t b = 0; b < B; ++b) {
+      const uint32_t r = hit_runs[wave][min(h + b, hits - 1u)];
+      beam[b] = r >> 16;
+      at[b] = 256u * (r & 0xFFFFu) + 4u * lane;
+      const float* x = a.logits + (size_t)(row0 + beam[b]) * a.row_stride;
+      v[b] = f4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      if (at[b] + 4u <= a.vocab) v[b] = *as_global(reinterpret_cast<const f4_any*>(x + at[b]));
+      else
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+          if (at[b] + i < a.vocab) v[b][i] = *as_global(x + at[b] + i);
+    }
+#pragma unroll
+    for (uint32_t b = 0; b < B; ++b) {
+      if (b >= n) break;
+      const double of_beam = base[beam[b]];
+#pragma unroll
+      for (uint32_t i = 0; i < 4; ++i) {
+        const double s = of_beam + (double)v[b][i];
+        if (s > -INFINITY && s >= (double)cut) put_in(s, v[b][i], at[b] + i, beam[b]);
+      }
+    }
+  }
+  if (wave == 0 && lane < o.beams && ends && cum > -INFINITY) put_in((double)cum, 0.f, o.eos, lane);
+  __syncthreads();
+  const uint32_t n = fits;
+  if (n <= kFit) {
+    for (uint32_t i0 = 0; i0 < n; i0 += 8u * W) {  // 8 lanes for each
+      const uint32_t i = i0 + threadIdx.x / 8u, at = min(i, n - 1u);
+      const double score = sm.fit.score[at];
+      const Entry e = {sm.fit.v[at], sm.fit.id[at]};
+      const uint32_t w = sm.fit.w[at];
+      uint32_t place = 0;
+#pragma unroll 2
+      for (uint32_t j = lane & 7u; j < n; j += 8u) {
+        const double other = sm.fit.score[j];
+        const uint32_t ow = sm.fit.w[j];
+        place += other > score || (other == score && (ow < w || (ow == w && better(Entry{sm.fit.v[j], sm.fit.id[j]}, e)))) ? 1u : 0u;
+      }
+      place += xor_lane<1>(place);
+      place += xor_lane<2>(place);
+      place += xor_lane<4>(place);
+      if (i < n && place < o.k && (lane & 7u) == 0) answer_beam(o, batch, place, false, e.id, w, score);
+    }
+    for (uint32_t i = n + threadIdx.x; i < o.k; i += 64u * W) answer_beam(o, batch, i, true, 0u, 0u, 0.0);
+    return;
+  }
+  __syncthreads();  // (the waves have read `fits`; what it counted is written over)
+  Candidate list;
+  for (uint32_t w = wave; w < o.beams; w += W) {
+    const double of = base[w];
+    Entry best, last;
+    const float* x = a.logits + (size_t)(row0 + w) * a.row_stride;
+    const float* peaks = a.peaks + (size_t)(row0 + w) * runs;
+    const bool over = o.done && o.done[row0 + w];
+    for (uint32_t r0 = 0; !over && of == of && r0 < runs; r0 += 64u) {
+      const float peak = r0 + lane < runs ? peaks[r0 + lane] : -INFINITY;
+      // (in the runs' order: an equal logit behind a full list's last is not better)
+      for (uint64_t who = __ballot(peak > last.v && of + (double)peak >= (double)cut); who; who &= who - 1u) {
+        const int r = __builtin_ctzll(who);
+        if (!(lane_f(peak, r) > last.v)) continue;
+        const uint32_t i = 256u * (r0 + (uint32_t)r) + lane;
+#pragma unroll
+        for (uint32_t q = 0; q < 4; ++q)  // (64 ids at a time, ascending)
+          put(best, last, i + 64u * q < a.vocab ? Entry{x[i + 64u * q], i + 64u * q} : Entry{}, -INFINITY, o.k, lane);
+      }
+    }
+    sm.lists.id[w][lane] = best.id;
+    const float v = __shfl(best.v, (int)(63u - lane), 64);
+    const uint32_t id = (uint32_t)__shfl((int)best.id, (int)(63u - lane), 64), place = 63u - lane;
+    const double score = over ? (double)o.cum[row0 + w] : of + (double)v;
+    Candidate c;
+    if ((over ? place == 0u : place < o.k && id != kNone) && score > -INFINITY) c = Candidate{score, 64u * w + place};
+    take_best(list, c, lane);
+  }
+  if (!join_candidates<W>(sm.lists.joint, list, wave, lane) || lane >= o.k) return;
+  const uint32_t w = list.at / 64u;
+  const bool none = list.at == kNone;
+  answer_beam(o, batch, lane, none, none ? kNone : o.done && o.done[row0 + w] ? o.eos : sm.lists.id[w][list.at % 64u], w, list.score);
 }
 
 // The slices of a row: one where the rows alone fill the chip.
@@ -643,16 +851,20 @@ void pick_slices(uint32_t M, uint32_t vocab, uint32_t* slices, uint32_t* slice) 
   *slices = (vocab + *slice - 1u) / *slice;
 }
 
-void launch(LogprobArgs a, uint32_t M, void* ws, hipStream_t st) {
+// (beams: the rows' slices are joined by texts, and nothing is left to do)
+bool launch(LogprobArgs a, uint32_t M, void* ws, hipStream_t st, const BeamArgs* beams = nullptr) {
   pick_slices(M, a.vocab, &a.slices, &a.slice);
   if (a.slices == 1) {
     logprobs_kernel<true><<<dim3(1, M), 256, 0, st>>>(a);
-  } else {
-    a.stats = static_cast<f4_t*>(ws);
-    a.peaks = reinterpret_cast<float*>(a.stats + (size_t)M * a.slices);
-    logprobs_kernel<false><<<dim3(a.slices, M), 256, 0, st>>>(a);
-    logprobs_join_kernel<<<M, 512, 0, st>>>(a);
+    return false;
   }
+  a.stats = static_cast<f4_t*>(ws);
+  a.peaks = reinterpret_cast<float*>(a.stats + (size_t)M * a.slices);
+  logprobs_kernel<false><<<dim3(a.slices, M), 256, 0, st>>>(a);
+  const bool whole = beams && beams->beams * runs_of_wave(a.vocab) <= 64u * kJoinRuns;
+  if (whole) beam_join_kernel<<<M / beams->beams, 64 * kJoinWaves, 0, st>>>(a, *beams);
+  else logprobs_join_kernel<<<M, 512, 0, st>>>(a);
+  return whole;
 }
 
 }  // namespace
@@ -722,8 +934,8 @@ int mi_beam_select(const float* logits, size_t row_stride, const float* cum, con
   const LogprobArgs a{logits, row_stride, nullptr, vocab_used, k, 1, vocab_used, nullptr, nullptr, top, nullptr, top_ids,
                       nullptr, nullptr, sums, done};
   hipStream_t st = (hipStream_t)stream;
-  launch(a, rows, reinterpret_cast<void*>(end), st);
-  beam_select_kernel<<<batch, 256, 0, st>>>(BeamArgs{cum, done, sums, top_ids, top, eos, beams, k, ids, from, scores});
+  const BeamArgs o{cum, done, sums, top_ids, top, eos, beams, k, ids, from, scores};
+  if (!launch(a, rows, reinterpret_cast<void*>(end), st, &o)) beam_select_kernel<<<batch, 256, 0, st>>>(o);
   return mi_hip((int)hipGetLastError(), "beam_select");
 }
 

@@ -87,25 +87,39 @@ class Beams:
 
 
 @pytest.mark.parametrize("batch,beams,used,k", [(1, 1, 1, 1), (1, 1, 5, 8), (2, 3, 7, 64), (1, 4, 151936, 8), (16, 8, 1000, 16), (3, 64, 500, 64),
-                                                (2, 5, 4099, 33), (129, 4, 2049, 5), (1, 1, 100000, 64), (40, 16, 300, 20)])
+                                                (2, 5, 4099, 33), (129, 4, 2049, 5), (1, 1, 100000, 64), (40, 16, 300, 20), (3, 5, 20001, 64),
+                                                (1, 64, 66001, 64), (128, 4, 1025, 9), (513, 1, 1500, 7)])
 @pytest.mark.parametrize("done", [False, True])
 def test_select(batch, beams, used, k, done):
     Beams(used + k, batch, beams, used, k, done, stride=used + 3 if beams == 5 else 0).check()
 
 
-def test_equal_scores_go_to_the_lower_beam_then_the_lower_token():
-    c = Beams(1, 2, 4, 600, 40)
+@pytest.mark.parametrize("used", [600, 5000])
+def test_equal_scores_go_to_the_lower_beam_then_the_lower_token(used):
+    c = Beams(1, 2, 4, used, 40)
     c.x[:] = np.round(c.x[0] * 2)  # equal rows, many equal logits
     c.cum[:] = -3.0
     ids, beams, _ = c.check()
-    x = c.x[0, :600]
-    want = sorted(((-x[v], w, v) for w in range(4) for v in range(600)))[:40]
+    x = c.x[0, :used]
+    want = sorted(((-x[v], w, v) for w in range(4) for v in range(used)))[:40]
     for b in range(2):
         assert [(int(w), int(v)) for w, v in zip(beams[b], ids[b])] == [(w, v) for _, w, v in want]
 
 
-def test_beams_without_candidates():
-    c = Beams(2, 3, 4, 900, 12)
+@pytest.mark.parametrize("used,k", [(2000, 64), (30000, 20), (30000, 1)])
+@pytest.mark.parametrize("levels", [1, 2, 40])
+def test_rows_of_few_different_logits(used, k, levels):
+    """many tokens as good as the k-th best: of the lowest beams and tokens, whatever reads them"""
+    c = Beams(used + levels, 2, 3, used, k, done=levels == 2)
+    c.x[:] = np.random.default_rng(levels).integers(0, levels, c.x.shape) * np.float32(0.5)
+    c.x[3] = c.x[4]
+    c.cum[[3, 4]] = -2.0
+    c.check()
+
+
+@pytest.mark.parametrize("used", [900, 20000])
+def test_beams_without_candidates(used):
+    c = Beams(2, 3, 4, used, 12)
     c.cum[[1, 2, 3]] = -np.inf  # a text's first step: one beam lives
     c.x[4, 7] = np.nan
     c.x[5, 8] = np.inf
@@ -115,7 +129,7 @@ def test_beams_without_candidates():
     c.cum[9] = np.nan
     ids, beams, scores = c.check()
     assert (beams[0] == 0).all() and (beams[1, :5] == 3).all() and (ids[1, 5:] == NONE).all() and (ids[2] == NONE).all()
-    c = Beams(3, 1, 4, 900, 12)
+    c = Beams(3, 1, 4, used, 12)
     c.done = np.array([1, 0, 1, 1], np.uint32)
     c.cum = np.array([-1.0, -50.0, -np.inf, -2.0], np.float32)
     ids, beams, scores = c.check()
