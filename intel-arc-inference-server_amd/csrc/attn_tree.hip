@@ -127,6 +127,8 @@ struct TreeRows : TreeArgs {
     }
     if (wave_sum(blocks) > (float)most_blocks) {  // (sequences that overlap: their items would be more than are counted with)
       if (flag) *flag = MI_STATUS_BAD_ROWS;
+      if (blockIdx.x == 0u)
+        for (uint32_t t = threadIdx.x; t < T; t += blockDim.x) info[t] = u4_t{0u, 0u, 0u, 0u};  // (nothing to join)
       return p;
     }
     p.per = part_tiles(s, wave_sum(total));
@@ -532,30 +534,32 @@ __global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void attn_tree_kernel(
   }
 }
 
-// Joins the parts of columns: HD / 4 threads side by side take a column, each four dims of all its parts, U parts at a time; a
-// work-group `C` columns of one row (C 1: all its threads one column's, which then share the parts out).
-template <int HD, bool MANY>
-__global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a, uint32_t most) {
-  constexpr uint32_t L = HD / 4, G = 256 / L, U = MANY ? 8 : 4;
-  const uint32_t t = blockIdx.y, g = threadIdx.x / L, d = threadIdx.x % L;
-  const uint32_t h = MANY ? blockIdx.x : blockIdx.x * G + g;
-  const u4_t info = *as_global(a.info + t);
-  const uint32_t first = a.row_start[0], end = min(a.row_start[a.sequences], a.T), splits = min(info[2], kMaxSplits);
-  asm volatile("" ::"v"(info), "s"(first), "s"(end));  // (one round trip for all three)
-  if (t < first || t >= end || splits < 2u) return;  // (uniform: no sequence's row, or its work-group stored it)
-  if (!MANY && h >= a.q_heads) return;
-  const uint32_t j = h / a.gqa, col = info[3] * a.gqa + h % a.gqa;
-  auto part = [&](uint32_t s) {  // (within the workspace whatever row_start held)
-    return a.part + ((size_t)min(info[0] + (s * a.kv_heads + j) * info[1], most) * a.columns + min(col, a.columns - 1u)) * (HD + 4);
-  };
+// The sums of a column's parts s0, s0 + step .., four dims of them, U parts at a time.
+struct Sums {
   f4_t o = {0.f, 0.f, 0.f, 0.f};
   float top = kNoKey, sum = 0.f;
-  for (uint32_t s0 = MANY ? g : 0u; s0 < splits; s0 += U * (MANY ? G : 1u)) {
+  __device__ __forceinline__ void turn(float to) {
+    const float f = __builtin_amdgcn_exp2f(top - to);
+    sum *= f;
+    o *= f;
+    top = to;
+  }
+  __device__ __forceinline__ void add(f4_t v, float r, float l) {  // (r up to top)
+    const float w = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(r - top);  // (0: no key of the row in that part)
+    sum = __builtin_fmaf(l, w, sum);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[e], w, o[e]);
+  }
+};
+template <int HD, uint32_t U, typename F>
+__device__ __forceinline__ Sums join_parts(uint32_t s0, uint32_t step, uint32_t splits, uint32_t d, F part) {
+  Sums a;
+  for (; s0 < splits; s0 += U * step) {
     f4_t v[U];
-    float r[U], l[U], now = top;
+    float r[U], l[U], now = a.top;
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
-      const uint32_t s = s0 + u * (MANY ? G : 1u);
+      const uint32_t s = s0 + u * step;
       const float* p = part(s < splits ? s : s0);
       v[u] = *as_global(reinterpret_cast<const f4_t*>(p + 4u * d));
       r[u] = *as_global(p + HD);
@@ -563,44 +567,53 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a, uint32_
     }
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) now = l[u] == 0.f ? now : fmaxf(now, r[u]);
-    const float f = __builtin_amdgcn_exp2f(top - now);
-    sum *= f;
-    o *= f;
-    top = now;
+    a.turn(now);
 #pragma unroll
-    for (uint32_t u = 0; u < U; ++u) {
-      const float w = l[u] == 0.f ? 0.f : __builtin_amdgcn_exp2f(r[u] - top);  // (no key of the row in that part)
-      sum = __builtin_fmaf(l[u], w, sum);
-#pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) o[e] = __builtin_fmaf(v[u][e], w, o[e]);
-    }
+    for (uint32_t u = 0; u < U; ++u) a.add(v[u], r[u], l[u]);
   }
+  return a;
+}
+// Joins the parts of row blockIdx.y: HD / 4 threads side by side take a column, four dims each. MANY: all threads of a work-group are
+// one column's and share its parts out; else each HD / 4 take columns in turn.
+template <int HD, bool MANY>
+__global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a, uint32_t most) {
+  constexpr uint32_t L = HD / 4, G = 256 / L;
+  const uint32_t t = blockIdx.y, g = threadIdx.x / L, d = threadIdx.x % L;
+  const u4_t info = *as_global(a.info + t);
+  const uint32_t first = a.row_start[0], end = min(a.row_start[a.sequences], a.T), splits = min(info[2], kMaxSplits);
+  asm volatile("" ::"v"(info), "s"(first), "s"(end));  // (one round trip for all three)
+  if (t < first || t >= end || splits < 2u) return;  // (uniform: no sequence's row, or its work-group stored it)
+  auto part_of = [&](uint32_t h) {
+    const uint32_t j = h / a.gqa, col = info[3] * a.gqa + h % a.gqa;
+    return [&a, info, j, col, most](uint32_t s) {  // (within the workspace whatever row_start held)
+      return a.part + ((size_t)min(info[0] + (s * a.kv_heads + j) * info[1], most) * a.columns + min(col, a.columns - 1u)) * (HD + 4);
+    };
+  };
+  auto store = [&](uint32_t h, const Sums& s) {
+    const float inv = s.sum == 0.f ? 0.f : 1.0f / s.sum;
+    store_out<HD>(a, h / a.gqa, t, h % a.gqa, d % 4u, d / 4u, s.o * inv);
+  };
   if constexpr (MANY) {
     __shared__ __align__(16) f4_t sums[G][L];
     __shared__ float tops[G], totals[G];
-    sums[g][d] = o;
+    Sums s = join_parts<HD, 8>(g, G, splits, d, part_of(blockIdx.x));
+    sums[g][d] = s.o;
     if (d == 0) {
-      tops[g] = top;
-      totals[g] = sum;
+      tops[g] = s.top;
+      totals[g] = s.sum;
     }
     __syncthreads();
     if (g) return;
+    float top = s.top;
 #pragma unroll
     for (uint32_t n = 1; n < G; ++n) top = fmaxf(top, tops[n]);
-    const float f = __builtin_amdgcn_exp2f(tops[0] - top);
-    sum *= f;
-    o *= f;
+    s.turn(top);
 #pragma unroll
-    for (uint32_t n = 1; n < G; ++n) {
-      const float w = __builtin_amdgcn_exp2f(tops[n] - top);
-      const f4_t x = sums[n][d];
-      sum = __builtin_fmaf(totals[n], w, sum);
-#pragma unroll
-      for (uint32_t e = 0; e < 4; ++e) o[e] = __builtin_fmaf(x[e], w, o[e]);
-    }
+    for (uint32_t n = 1; n < G; ++n) s.add(sums[n][d], tops[n], totals[n]);
+    store(blockIdx.x, s);
+  } else {
+    for (uint32_t h = blockIdx.x * G + g; h < a.q_heads; h += gridDim.x * G) store(h, join_parts<HD, 4>(0u, 1u, splits, d, part_of(h)));
   }
-  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  store_out<HD>(a, j, t, h % a.gqa, d % 4u, d / 4u, o * inv);
 }
 
 // The launch: the few-rows kernel up to 16 columns a sequence, else the other with CT column tiles a wave (64 CT columns a
@@ -768,9 +781,10 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
     if (a.most_blocks * 8u <= a.share) {
       if (narrow) attn_tree_join_kernel<128, true><<<dim3(shape->q_heads, T), 256, 0, st>>>(a, most);
       else attn_tree_join_kernel<256, true><<<dim3(shape->q_heads, T), 256, 0, st>>>(a, most);
-    } else {
-      if (narrow) attn_tree_join_kernel<128, false><<<dim3((shape->q_heads + 7u) / 8u, T), 256, 0, st>>>(a, most);
-      else attn_tree_join_kernel<256, false><<<dim3((shape->q_heads + 3u) / 4u, T), 256, 0, st>>>(a, most);
+    } else {  // (of many rows most have one part: few work-groups a row)
+      const uint32_t heads = narrow ? 8u : 4u, x = std::min((shape->q_heads + heads - 1u) / heads, std::max(1u, 4096u / T));
+      if (narrow) attn_tree_join_kernel<128, false><<<dim3(x, T), 256, 0, st>>>(a, most);
+      else attn_tree_join_kernel<256, false><<<dim3(x, T), 256, 0, st>>>(a, most);
     }
   }
   return mi_hip((int)hipGetLastError(), "attn_tree");

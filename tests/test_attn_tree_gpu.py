@@ -295,8 +295,9 @@ def test_a_page_outside_the_cache_is_reported(rows, page):
     sync()
 
 
-def test_sequences_that_overlap_are_refused():
-    c = Case(9, [(100, 3)] * 20)
+@pytest.mark.parametrize("rows,cached,page", [(3, 100, 16), (3, 900, 64), (40, 900, 64)])
+def test_sequences_that_overlap_are_refused(rows, cached, page):
+    c = Case(9, [(cached, rows)] * 20, page=page)
     b = c.bind()
     b["row_start"].copy_(dev(np.where(np.arange(21) % 2, c.T, 0).astype(np.uint32)))
     mi.call("mi_attn_tree", *b["args"], stream())
