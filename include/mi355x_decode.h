@@ -603,7 +603,7 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
  * where the ring has too few pages MI_STATUS_NO_PAGES: then row_start is all 0, no row has a slot, tables and ring are as they were
  * and held_out and ring_at_out repeat held and ring_at. A parent that is not below its child counts as none (MI_STATUS_BAD_ROWS); a
  * page id that is not below n_pages gives slot none (MI_STATUS_BAD_PAGE). flag may be NULL.
- * 1..1024 requests, rows up to 65535, cached + added up to 2^30, table_stride up to 2^21, words up to 64. ws: mi_block_tables_ws bytes, 4-byte aligned. */
+ * 1..1024 requests, rows up to 65535, cached + added up to 2^30, table_stride up to 2^21, page up to 2^20, words up to 64. ws: mi_block_tables_ws bytes, 4-byte aligned. */
 typedef struct mi_block_plan {
   uint32_t requests, rows, page, n_pages, table_stride, ring_len, words;
   const uint32_t* cached;

@@ -15,7 +15,7 @@
 namespace mi {
 namespace {
 
-constexpr uint32_t kMaxRequests = 1024, kMaxRows = 65535, kMaxKeys = 1u << 30, kMaxWords = 64, kMaxTable = 1u << 21, kNone = 0xFFFFFFFFu;
+constexpr uint32_t kMaxRequests = 1024, kMaxRows = 65535, kMaxKeys = 1u << 30, kMaxWords = 64, kMaxTable = 1u << 21, kMaxPage = 1u << 20, kNone = 0xFFFFFFFFu;
 constexpr uint32_t kOneGroup = 4096;  // rows that the requests' work-group does itself
 
 struct PlanArgs {
@@ -277,8 +277,8 @@ int mi_block_tables(const mi_block_plan* plan, void* ws, size_t ws_bytes, void* 
   if (p.page == 0 || p.n_pages == 0 || p.table_stride == 0 || p.ring_len == 0)
     return mi_fail(MI_ERR_ARG, "block_tables: page size, page count, table_stride or ring_len 0");
   if ((uint64_t)p.page * p.n_pages > 0xFFFFFFFFull) return mi_fail(MI_ERR_SHAPE, "block_tables: above 2^32 cache rows");
-  if (p.table_stride > kMaxTable || p.ring_len > 1u << 31)
-    return mi_fail(MI_ERR_SHAPE, "block_tables: tables of 2^21 pages and a ring of 2^31 pages at most");
+  if (p.table_stride > kMaxTable || p.ring_len > 1u << 31 || p.page > kMaxPage)
+    return mi_fail(MI_ERR_SHAPE, "block_tables: pages of 2^20 positions, tables of 2^21 pages, a ring of 2^31 at most");
   if (p.parent ? !p.mask || p.words == 0 || p.words > kMaxWords : p.mask || p.words)
     return mi_fail(MI_ERR_ARG, "block_tables: masks of 1..64 words go with parents");
   if (!ws || off(ws, 4) || ws_bytes < mi_block_tables_ws(p.requests))

@@ -27,7 +27,7 @@ def test_block_tables_refusals():
                {"nb": L.mi_block_tables_ws(4) - 1}):
         assert call(**kw) == ARG, kw
     for kw in ({"requests": 0}, {"requests": 1025}, {"rows": 0}, {"rows": 65536}, {"page": 1 << 31, "n_pages": 3}, {"ring_len": (1 << 31) + 1},
-               {"table_stride": (1 << 21) + 1}):
+               {"table_stride": (1 << 21) + 1}, {"page": (1 << 20) + 1, "n_pages": 9}):
         assert call(**kw) == SHAPE, kw
     assert L.mi_block_tables(None, P, 1 << 20, None) == ARG
     assert L.mi_block_tables_ws(0) == L.mi_block_tables_ws(1025) == 0 < L.mi_block_tables_ws(1)
