@@ -603,7 +603,8 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
  * where the ring has too few pages MI_STATUS_NO_PAGES: then row_start is all 0, no row has a slot, tables and ring are as they were
  * and held_out and ring_at_out repeat held and ring_at. A parent that is not below its child counts as none (MI_STATUS_BAD_ROWS); a
  * page id that is not below n_pages gives slot none (MI_STATUS_BAD_PAGE). flag may be NULL.
- * 1..1024 requests, rows up to 65535, cached + added up to 2^30, table_stride up to 2^21, page up to 2^20, words up to 64. ws: mi_block_tables_ws bytes, 4-byte aligned. */
+ * 1..1024 requests, rows up to 65535, cached + added up to 2^30, table_stride up to 2^21, page up to 2^20, words up to
+ * 64. ws: mi_block_tables_ws bytes, 4-byte aligned. */
 typedef struct mi_block_plan {
   uint32_t requests, rows, page, n_pages, table_stride, ring_len, words;
   const uint32_t* cached;
@@ -646,7 +647,8 @@ typedef struct mi_rope {
   const float* divisors;
 } mi_rope;
 /* table [n][2][rot_dim / 2] fp32 = (cos, sin)(p f_i) of the positions pos0 .. pos0 + n - 1, formed in 64 bits and rounded once:
- * what mi_attn_prep, mi_attn_prep_rows and mi_rope_rows read. rot_dim a multiple of 8 up to 256, positions below 2^31. */
+ * what mi_attn_prep, mi_attn_prep_rows and mi_rope_rows read. rot_dim a multiple of 8 up to 256, positions below 2^31, theta above 1,
+ * f_i up to 2^20 (an angle is off by 2^-53 of itself: below 2^-24 up to angles of 2^29). */
 int mi_rope_table(const mi_rope* rope, uint32_t pos0, uint32_t n, float* table, void* stream);
 /* Rows of q||k||v (in_kind MI_OUT_F32 or MI_OUT_F16, rows in_stride elements apart): q and k are normed by head (RMSNorm with
  * q_norm / k_norm fp32 [head_dim], NULL = none, shape->eps), their first rot_dim dims turned by the table's row of position pos[t]

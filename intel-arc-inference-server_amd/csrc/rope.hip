@@ -223,6 +223,8 @@ int mi_rope_table(const mi_rope* rope, uint32_t pos0, uint32_t n, float* table, 
     if (rope->scaling == MI_ROPE_YARN) part = 1.0 - (i - lo) / std::max(hi - lo, 0.001);
     part = std::min(std::max(part, 0.0), 1.0);
     a.f[i] = part == 1.0 ? f : part * f + (1.0 - part) * f / by;
+    // (so that a position's angle stays below 2^51, where its number of quarter turns is a whole number of 64 bits)
+    if (!(a.f[i] <= 1048576.0)) return mi_fail(MI_ERR_ARG, "rope_table: a frequency above 2^20");
     a.cos_f[i] = std::cos(a.f[i]);
     a.sin_f[i] = std::sin(a.f[i]);
   }

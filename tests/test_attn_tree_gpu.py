@@ -188,6 +188,9 @@ def test_many_sequences(n):
 def test_one_long_sequence_among_many_short_ones():
     Case(1, [(30000, 1) if b == 77 else (b, 1) for b in range(300)], qh=8, kvh=8, page=64).check()
     Case(2, [(9000, 30) if b == 5 else (3 * b, 20) for b in range(40)], qh=8, kvh=4, page=64).check()
+    # (so many rows that a work-group of the join takes several heads)
+    Case(3, [(20000, 1) if b == 5 else (b, 50) for b in range(41)], qh=60, kvh=12, page=64).check()
+    Case(4, [(9000, 2) if b == 7 else (0, 300) for b in range(11)], qh=12, kvh=2, hd=256, page=64).check()
 
 
 @pytest.mark.parametrize("qh,kvh,hd", [(10, 2, 128), (16, 2, 256), (20, 1, 128)])

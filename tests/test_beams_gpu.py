@@ -207,3 +207,58 @@ def test_rows_outside_are_not_moved():
     got = move(k, v, 45, origin, to, flag=mi.STATUS_BAD_PAGE)
     for g, x in zip(got, (k, v)):
         assert np.array_equal(g, moved(x, 45, origin, to))
+
+
+def test_captured_moves_and_other_stream():
+    """a captured move reads its lists anew, and the rows as the replay before left them"""
+    T = torch()
+    rng = np.random.default_rng(5)
+    n, groups, per = 90, 3, 7
+    k, v = (rng.integers(0, 1 << 16, (2, 3, n, 128)).astype(np.uint16) for _ in range(2))
+    dk, dv = dev(k), dev(v)
+    df, dt = (dev(np.zeros((groups, per), np.uint32)) for _ in range(2))
+
+    def call(st):
+        mi.call("mi_kv_move", ptr(dk), ptr(dv), 2, 3 * n * 128, 128, n * 128, 3, 128, n, ptr(df), ptr(dt), groups, per, None, st)
+
+    def lists():
+        f, t = ([30 * g + rng.permutation(30)[:per] for g in range(groups)] for _ in range(2))
+        df.copy_(dev(np.array(f, np.uint32)))
+        dt.copy_(dev(np.array(t, np.uint32)))
+        return f, t
+
+    g = T.cuda.CUDAGraph()
+    with T.cuda.graph(g):
+        call(stream())
+    side = T.cuda.Stream()
+    for i in range(5):
+        f, t = lists()
+        sync()
+        if i < 3:
+            g.replay()
+        else:
+            call(side.cuda_stream)
+        sync()
+        k, v = moved(k, n, f, t), moved(v, n, f, t)
+        assert np.array_equal(host(dk, np.uint16).reshape(k.shape), k) and np.array_equal(host(dv, np.uint16).reshape(v.shape), v)
+
+
+@pytest.mark.parametrize("strides", [((1 << 32) + 8, 128, 128 * 40), (128 * 80, 128, (1 << 32) + 8), (128, 1 << 27, 0)])
+def test_moves_past_32_bits(strides):
+    """rows whose offsets pass 2^32 elements, by layers, by heads and by rows, the elements between them never written"""
+    T = torch()
+    L, H, n = (1 if strides[1] > 128 else 2), (1 if strides[1] > 128 else 2), 40
+    rng = np.random.default_rng(6)
+    k, v = (rng.integers(0, 1 << 16, (L, H, n, 128)).astype(np.uint16) for _ in range(2))
+    f, t = [np.r_[39, 1, 38]], [np.r_[37, 39, 2]]
+    views = []
+    size = (L - 1) * strides[0] + (H - 1) * strides[2] + (n - 1) * strides[1] + 128
+    for x in (k, v):
+        d = T.empty(size, dtype=T.int16, device="cuda").as_strided((L, H, n, 128), (strides[0], strides[2], strides[1], 1))
+        d.copy_(dev(x).reshape(x.shape))
+        views.append(d)
+    df, dt = dev(np.array(f, np.uint32)), dev(np.array(t, np.uint32))
+    mi.call("mi_kv_move", ptr(views[0]), ptr(views[1]), L, strides[0], strides[1], strides[2], H, 128, n, ptr(df), ptr(dt), 1, 3, None, stream())
+    sync()
+    for d, x in zip(views, (k, v)):
+        assert np.array_equal(host(d.contiguous(), np.uint16).reshape(x.shape), moved(x, n, f, t))

@@ -259,3 +259,42 @@ def test_captured_and_other_stream():
     side = T.cuda.Stream()
     with T.cuda.stream(side):
         c.check(c.run(side.cuda_stream))
+
+
+def test_tables_captured_and_on_another_stream():
+    """the frequencies are read when the call is made"""
+    T = torch()
+    d = np.linspace(1.0, 9.0, 32).astype(np.float32)
+    rope = mi.Rope(rot_dim=64, theta=10000.0, divisors=d.ctypes.data)
+    outs = [T.zeros(100 * 64, dtype=T.float32, device="cuda") for _ in range(3)]
+    mi.call("mi_rope_table", mi.C.byref(rope), 70, 100, ptr(outs[0]), stream())
+    g = T.cuda.CUDAGraph()
+    with T.cuda.graph(g):
+        mi.call("mi_rope_table", mi.C.byref(rope), 70, 100, ptr(outs[1]), stream())
+    side = T.cuda.Stream()
+    mi.call("mi_rope_table", mi.C.byref(rope), 70, 100, ptr(outs[2]), side.cuda_stream)
+    d[:] = 3.0
+    rope.theta = 5.0
+    for _ in range(3):
+        outs[1].zero_()
+        g.replay()
+        sync()
+        assert T.equal(outs[0], outs[1]) and T.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("by_row", [False, True])
+def test_rows_past_32_bits(by_row):
+    """cache rows whose offsets pass 2^32 elements, by heads or by rows"""
+    T = torch()
+    c = Rows(13, 3, kvh=2, cache=41)
+    b = c.bind()
+    rs, hs = (1 << 27, 128) if by_row else (128, (1 << 32) + 8)
+    caches = [T.empty(40 * rs + hs + 128, dtype=T.int16, device="cuda").as_strided((2, 41, 128), (hs, rs, 1)) for _ in range(2)]
+    for x in caches:
+        x.fill_(77)
+    c.slot = np.array([40, 3, 39], np.uint32)
+    b["slot"].copy_(dev(c.slot))
+    mi.call("mi_rope_rows", *b["args"][:15], ptr(caches[0]), ptr(caches[1]), rs, hs, ptr(b["flag"]), stream())
+    for n, x in zip("kv", caches):
+        b[n][:-GUARD] = x.reshape(-1)
+    c.check(c.result(b))

@@ -42,8 +42,10 @@ def test_rope_table_refusals():
 
     nan = float("nan")
     bad = np.array([1.0] * 31 + [0.0], np.float32)
+    half = np.full(32, 0.5, np.float32)  # with a factor of 1e-6: a frequency of 2e6, above 2^20
     for kw in ({"table": None}, {"table": P + 2}, {"theta": 1.0}, {"theta": nan}, {"scaling": 5}, {"factor": 0.0}, {"factor": nan}, {"original": 0},
-               {"low": 0.0}, {"high": 1.0}, {"high": nan}, {"attention": -1.0}, {"attention": nan}, {"divisors": bad.ctypes.data}):
+               {"low": 0.0}, {"high": 1.0}, {"high": nan}, {"attention": -1.0}, {"attention": nan}, {"divisors": bad.ctypes.data},
+               {"factor": 1e-6, "scaling": mi.ROPE_LINEAR, "theta": 1.5, "divisors": half.ctypes.data}):
         assert call(**kw) == ARG, kw
         assert b"rope_table" in L.mi_last_error()
     for kw in ({"rot_dim": 0}, {"rot_dim": 12}, {"rot_dim": 264}, {"n": 0}, {"n": (1 << 24) + 1}, {"pos0": (1 << 31) - 9}):
