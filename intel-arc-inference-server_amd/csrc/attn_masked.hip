@@ -199,7 +199,7 @@ struct MaskedRows : MaskedArgs {
   using Place = mi::Place;
   using Block = mi::Block;
   using Column = mi::Column;
-  static constexpr bool kMayIdle = false;
+  static constexpr bool kItems = false;
   // grid (kv_heads, row blocks, splits); the last row blocks of a causal chunk see the most keys: they are dispatched first
   __device__ __forceinline__ Place place(bool chunk) const {
     const uint32_t t0 = (chunk ? gridDim.y - 1u - blockIdx.y : blockIdx.y) * rows;

@@ -3,7 +3,7 @@
 // row sees, where a work-group's rows and keys are and where a key lies in the cache is the caller's type A (MaskedRows in
 // attn_masked.hip, TreeRows in attn_tree.hip), the kernels' argument:
 //   Place place(bool chunk)      kv head j, the rows t0 .. t0 + rows - 1, and which of `splits` parts of their keys it takes
-//                                (kMayIdle: rows may be 0, and the work-group has nothing to do)
+//                                (kItems: each_item instead, for the places of a work-group one behind another)
 //   Block block(Place)           the 32-key tiles that the rows see: n of them, the first key of each, the last key that a row sees
 //   uint32_t part_begin(...)     the first tile of a part
 //   Column column(...)           what a column sees; bool masked(Block, key): whether some column does not see some key of a tile
@@ -142,8 +142,8 @@ __device__ __forceinline__ float most_of(const float (&w)[8]) {
 // One step of the softmax of a wave's CT column tiles, whose lanes' largest scores are mx. The references first: raised, with what
 // was formed by them, where a score passes one (each column by its own four lanes, whatever its neighbours need). NT 0: the
 // accumulators are left to the caller, with their factor.
-template <uint32_t CT, uint32_t NT>
-__device__ __forceinline__ void raise_to(const float (&mx)[CT], uint32_t qi, float (&r)[CT], float (&l)[CT], f4_t (*acc)[NT ? NT : 1],
+template <uint32_t CT, uint32_t NT, uint32_t N, uint32_t M>
+__device__ __forceinline__ void raise_to(const float (&mx)[N], uint32_t qi, float (&r)[M], float (&l)[M], f4_t (*acc)[NT ? NT : 1],
                                          float* factor) {
   bool over = false;
 #pragma unroll
@@ -227,7 +227,7 @@ __device__ __forceinline__ float not_finite(float z, f4_t v) {  // 0 (a zero z),
 // every fourth of the split's: K from memory as the A operand, V through its own part of LDS for the transposing
 // reads, the next tile's rows in registers meanwhile. The waves' sums join through LDS.
 template <int HD, typename A>
-__global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_rows_few_kernel(A a) {
+__device__ __forceinline__ void few_rows_of(const A& a, const typename A::Place& p) {
   constexpr uint32_t KK = HD / 32, NT = HD / 16, VROW = HD + 16;
   constexpr uint32_t PPR = HD / 8, RPP = 64 / PPR, NV = kTile / RPP;  // 16-byte pieces per V row, rows per load, loads per tile
   __shared__ __align__(16) union Slab {
@@ -236,9 +236,9 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_rows_few_kernel(A
       float acc[NT * 4][64], r[64], l[64];
     } part;
   } slab[4];
-  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, qi = lane & 15u, qq = lane >> 4;
-  const typename A::Place p = a.place(false);
-  if (A::kMayIdle && p.rows == 0u) return;
+  uint32_t thread = threadIdx.x;
+  if constexpr (A::kItems) asm volatile("" : "+v"(thread));  // (what follows from it is formed anew in each item, not kept)
+  const uint32_t lane = thread & 63u, wave = thread >> 6, qi = lane & 15u, qq = lane >> 4;
   const uint32_t j = p.j, t0 = p.t0, rows_here = p.rows;
   const uint32_t row = qi / a.gqa, g = qi % a.gqa;
   const typename A::Block b = a.block(p);
@@ -359,6 +359,14 @@ __global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_rows_few_kernel(A
     float* o = a.template part_at<HD>(p, row, g);
     o[HD] = top;
     o[HD + 1] = col.live ? sum : 0.f;
+  }
+}
+template <int HD, typename A>
+__global__ __launch_bounds__(256, HD == 128 ? 2 : 1) void attn_rows_few_kernel(A a) {
+  if constexpr (A::kItems) {
+    a.each_item([&](const typename A::Place& p) { few_rows_of<HD>(a, p); });
+  } else {
+    few_rows_of<HD>(a, a.place(false));
   }
 }
 

@@ -7,9 +7,12 @@
 // The kernels, and how their softmax and its roundings go, are attn_rows.h's.
 //
 // How the work is dealt out: a sequence's rows are cut into blocks of `rows`, its 32-key tiles into parts of `per` tiles, the same
-// for all sequences (a sequence's parts then as even as may be). A block, a part and a kv head are an item, and a work-group's.
-// Lengths are the device's: every wave reads them all, forms `per` and finds its item by itself. Items that read the same keys (a sequence's blocks) follow one another
-// and run on one XCD. Sequences of several parts leave sums, which a second launch joins.
+// for all sequences (a sequence's parts then as even as may be). A block, a part and a kv head are an item; as many work-groups as run
+// at once take them. Lengths are the device's: every wave reads them all, forms `per` and finds its items by itself. The items
+// of a kv head follow one another, those that read the same keys (a sequence's blocks) side by side, and an XCD takes an even stretch
+// of all: with 8 kv heads one head, so that the XCDs' loads are alike whatever the lengths are. Sequences of several parts leave
+// sums, which a second launch joins. Code is short here and its loops are not unrolled: every work-group fetches it anew (sixteen
+// candidates of `per` one behind another took 5 us more than eight of them).
 #include <algorithm>
 
 #include "attn_rows.h"
@@ -56,7 +59,7 @@ __device__ __forceinline__ Sequence sequence(const TreeArgs& a, uint32_t b) {
 struct TreeRows : TreeArgs {
   struct Place {
     uint32_t j, t0, rows, split, splits;
-    uint32_t b, own, cached, keys, per, part;  // the sequence, its index of the first row, where the part's sums go
+    uint32_t b, own, cached, keys, part;  // the sequence, its index of the first row, where the part's sums go
   };
   struct Block {
     uint32_t last, n, free, base;  // free: so many keys every row of the block sees
@@ -68,110 +71,116 @@ struct TreeRows : TreeArgs {
     uint32_t own, first, count;  // its index, the first of the step's own keys and how many they are
     bool live;
   };
-  static constexpr bool kMayIdle = true;
+  static constexpr bool kItems = true;
 
   static __device__ __forceinline__ uint32_t parts(const Sequence& s, uint32_t per) { return (s.tiles + per - 1u) / per; }
-  // Tiles of a part at most. With `even` tiles in each of the work-groups that run at once, and parts of `per` tiles that make `items`
-  // items, the call lasts per + 3 where all run at once, else even + per / 2 + 3 items / slots (in tiles; 3: an item's start).
-  // Few sequences of uneven lengths are near `even` in one round or none: of the candidates the least is taken. None is below
-  // total / share, so there are no more items than share and one for each block.
+  // Tiles of a part at most, for several sequences of `total` tiles in all blocks. With `even` tiles in each of the work-groups that
+  // run at once, and parts of `per` tiles that make `items` items, the call lasts per + 3 where all run at once, else
+  // even + per / 2 + 3 items / slots (in tiles; 3: an item's start). Few sequences of uneven lengths are near `even` in one round or
+  // none: of 64 candidates, a lane each, the least is taken. With many sequences items / slots is near even / per, and the second form least
+  // at per = sqrt(6 even). None is below total / share, so there are no more items than share and one for each block.
   __device__ __forceinline__ uint32_t part_tiles(const Sequence& first, float total) const {
     const uint32_t lane = threadIdx.x & 63u;
-    constexpr uint32_t N = 8;
-    constexpr float kOf[N] = {2.f, 1.5f, 1.25f, 1.125f, 1.f, 0.5f, 0.33f, 0.25f};
-    const float even = total * (float)kv_heads / (float)slots;
-    float items[N];
-    uint32_t per[N];
-#pragma unroll
-    for (uint32_t n = 0; n < N; ++n) {
-      per[n] = max(least, (uint32_t)fminf(fmaxf(even * kOf[n], total * 1.0001f / (float)share), (float)kMaxKeys) + 1u);
-      items[n] = 0.f;
+    const float even = total * (float)kv_heads / (float)slots, floor = total * 1.0001f / (float)share;
+    auto from = [&](float tiles) { return max(least, (uint32_t)fminf(fmaxf(tiles, floor), (float)kMaxKeys) + 1u); };
+    if (sequences > 64u) return from(sqrtf(6.f * even));
+    const uint32_t per = from(even * (lane < 48u ? 1.f + (float)lane * (1.f / 48.f) : (float)(lane - 46u) * (1.f / 18.f)));
+    const float one = __builtin_amdgcn_rcpf((float)per);
+    float items = 0.f;
+#pragma unroll 1
+    for (uint32_t b = 0; b < sequences; ++b) {
+      const float tiles = (float)__builtin_amdgcn_readlane((int)first.tiles, (int)b);
+      items += (float)__builtin_amdgcn_readlane((int)first.blocks, (int)b) * ceilf(tiles * one);
     }
-    for (uint32_t b = 0; b < sequences; b += 64u) {
-      const Sequence s = b ? sequence(*this, b + lane) : first;
-#pragma unroll
-      for (uint32_t n = 0; n < N; ++n)
-        items[n] += (float)s.blocks * ceilf((float)s.tiles * __builtin_amdgcn_rcpf((float)per[n]));
-    }
-    uint32_t best = 0;
-    float cost = INFINITY;
-#pragma unroll
-    for (uint32_t n = 0; n < N; ++n) {
-      const float turns = wave_sum(items[n]) * (float)kv_heads / (float)slots;
-      const float c = turns <= 1.f ? (float)per[n] + 3.f : even + 0.5f * (float)per[n] + 3.f * turns;
-      if (c < cost) {
-        cost = c;
-        best = per[n];
-      }
-    }
-    return best;
+    const float turns = items * (float)kv_heads / (float)slots;
+    const float c = turns <= 1.f ? (float)per + 3.f : even + 0.5f * (float)per + 3.f * turns;
+    const uint32_t cost = __builtin_bit_cast(uint32_t, c);  // (above 0: the bits are in the numbers' order)
+    const uint64_t least_cost = __ballot(cost == wave_fold(cost, [](uint32_t x, uint32_t y) { return min(x, y); }));
+    return (uint32_t)__builtin_amdgcn_readlane((int)per, (int)__builtin_ctzll(least_cost));
   }
-  __device__ __forceinline__ Place place(bool) const {
+  // All items of a work-group, blockIdx.x and every gridDim.x-th behind it: of(place).
+  template <typename F>
+  __device__ __forceinline__ void each_item(F of) const {
     const uint32_t lane = threadIdx.x & 63u;
+    const bool one = sequences == 1u;
     auto plus = [](uint32_t x, uint32_t y) { return x + y; };
-    Place p{};
-    if (sequences == 1u) {
-      const Sequence s = sequence(*this, 0u);
-      p.per = max(least, max(s.blocks, s.tiles) < 65536u ? (s.blocks * s.tiles + share - 1u) / share
-                                                         : (uint32_t)((float)s.blocks * (float)s.tiles * 1.0001f / (float)share) + 1u);
-      const uint32_t n = parts(s, p.per), item = item_of(s.blocks * n * kv_heads);
-      if (item == kNone) return p;
-      return inside(p, s, 0u, n, item, 0u);
+    Sequence s = sequence(*this, one ? 0u : lane);
+    uint32_t per, items;  // (items of a kv head)
+    if (one) {
+      per = max(least, max(s.blocks, s.tiles) < 65536u ? (s.blocks * s.tiles + share - 1u) / share
+                                                       : (uint32_t)((float)s.blocks * (float)s.tiles * 1.0001f / (float)share) + 1u);
+      items = s.blocks * parts(s, per);
+    } else {
+      float total = (float)s.blocks * (float)s.tiles, blocks = (float)s.blocks;
+      for (uint32_t b = 64u; b < sequences; b += 64u) {
+        const Sequence o = sequence(*this, b + lane);
+        total += (float)o.blocks * (float)o.tiles;
+        blocks += (float)o.blocks;
+      }
+      if (wave_sum(blocks) > (float)most_blocks) {  // (sequences that overlap: their items would be more than are counted with)
+        if (flag) *flag = MI_STATUS_BAD_ROWS;
+        if (blockIdx.x == 0u)
+          for (uint32_t t = threadIdx.x; t < T; t += blockDim.x) info[t] = u4_t{0u, 0u, 0u, 0u};  // (nothing to join)
+        return;
+      }
+      per = part_tiles(s, wave_sum(total));
+      items = s.blocks * parts(s, per);
+      for (uint32_t b = 64u; b < sequences; b += 64u) {
+        const Sequence o = sequence(*this, b + lane);
+        items += o.blocks * parts(o, per);
+      }
+      items = wave_fold(items, plus);
     }
-    Sequence s = sequence(*this, lane);
-    float total = (float)s.blocks * (float)s.tiles, blocks = (float)s.blocks;
-    for (uint32_t b = 64u; b < sequences; b += 64u) {
-      const Sequence o = sequence(*this, b + lane);
-      total += (float)o.blocks * (float)o.tiles;
-      blocks += (float)o.blocks;
-    }
-    if (wave_sum(blocks) > (float)most_blocks) {  // (sequences that overlap: their items would be more than are counted with)
-      if (flag) *flag = MI_STATUS_BAD_ROWS;
-      if (blockIdx.x == 0u)
-        for (uint32_t t = threadIdx.x; t < T; t += blockDim.x) info[t] = u4_t{0u, 0u, 0u, 0u};  // (nothing to join)
-      return p;
-    }
-    p.per = part_tiles(s, wave_sum(total));
-    uint32_t items = s.blocks * parts(s, p.per);
-    for (uint32_t b = 64u; b < sequences; b += 64u) {
-      const Sequence o = sequence(*this, b + lane);
-      items += o.blocks * parts(o, p.per);
-    }
-    uint32_t item = item_of(wave_fold(items, plus) * kv_heads);
-    if (item == kNone) return p;
-    uint32_t part = 0;
-    for (uint32_t b0 = 0; b0 < sequences; b0 += 64u) {
-      if (b0) s = sequence(*this, b0 + lane);
-      const uint32_t n = parts(s, p.per), mine = s.blocks * n * kv_heads;
-      uint32_t sum = mine;  // of the lanes up to this one
+#pragma unroll 1
+    for (uint32_t at = blockIdx.x;; at += gridDim.x) {
+      uint32_t item = item_of(items * kv_heads, at), part = 0, b = 0;
+      if (item == kNone) return;
+      const uint32_t j = item / items;
+      item -= j * items;
+      uint32_t found = 0;
+      if (one) {
+        if (at != blockIdx.x) s = sequence(*this, 0u);
+      } else {
+#pragma unroll 1
+        for (;; b += 64u) {
+          if (at != blockIdx.x || b) s = sequence(*this, b + lane);
+          const uint32_t n = parts(s, per), mine = s.blocks * n;
+          uint32_t sum = mine;  // of the lanes up to this one
 #pragma unroll
-      for (uint32_t d = 1; d < 64u; d *= 2) {
-        const uint32_t o = (uint32_t)__shfl_up((int)sum, d, 64);
-        sum += lane >= d ? o : 0u;
+          for (uint32_t d = 1; d < 64u; d *= 2) {
+            const uint32_t o = (uint32_t)__shfl_up((int)sum, d, 64);
+            sum += lane >= d ? o : 0u;
+          }
+          const uint64_t behind = __ballot(sum > item);
+          found = behind ? (uint32_t)__builtin_ctzll(behind) : 64u;
+          part += wave_fold(lane < found && n > 1u ? mine : 0u, plus);
+          if (found < 64u) {
+            item -= (uint32_t)__builtin_amdgcn_readlane((int)(sum - mine), (int)found);
+            break;
+          }
+          if (b + 64u >= sequences) return;  // (not reached: item is below the sum of all)
+          item -= (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        }
       }
-      const uint64_t behind = __ballot(sum > item);
-      const uint32_t found = behind ? (uint32_t)__builtin_ctzll(behind) : 64u;
-      part += wave_fold(lane < found && n > 1u ? mine : 0u, plus);
-      if (found == 64u) {
-        item -= (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
-        continue;
-      }
-      auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)found); };
-      const Sequence f = {of(s.start), of(s.rows), of(s.cached), of(s.keys), of(s.blocks), of(s.tiles)};
-      return inside(p, f, b0 + found, of(n), item - of(sum - mine), part);
+      auto of_found = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)found); };
+      const Sequence f = {of_found(s.start), of_found(s.rows), of_found(s.cached), of_found(s.keys), of_found(s.blocks), of_found(s.tiles)};
+      b += found;
+      s = Sequence{};  // (not kept in registers meanwhile)
+      of(inside(f, b, parts(f, per), j, item, part));
+      __syncthreads();
     }
-    return p;
   }
-  // This work-group's of `items` items: XCD x (every eighth work-group is its) has those from x / 8 of them on.
-  __device__ __forceinline__ uint32_t item_of(uint32_t items) const {
-    const uint32_t each = (items + kXcds - 1u) / kXcds, at = blockIdx.x / kXcds, item = (blockIdx.x % kXcds) * each + at;
+  // Work-group `group`'s of `items` items: XCD x (every eighth work-group is its) has those from x / 8 of them on.
+  __device__ __forceinline__ uint32_t item_of(uint32_t items, uint32_t group) const {
+    const uint32_t each = (items + kXcds - 1u) / kXcds, at = group / kXcds, item = (group % kXcds) * each + at;
     return at < each && item < items ? item : kNone;
   }
-  // The place of item `item` of sequence b, of n parts, whose first item's sums are number `part`.
-  __device__ __forceinline__ Place inside(Place p, const Sequence& s, uint32_t b, uint32_t n, uint32_t item, uint32_t part) const {
-    const uint32_t each = s.blocks * kv_heads, split = item / each, rest = item - split * each;
-    p.j = rest / s.blocks;
-    p.own = (rest - p.j * s.blocks) * rows;
+  // The place of kv head j's item `item` of sequence b, of n parts; behind `part` items of a head that leave sums.
+  __device__ __forceinline__ Place inside(const Sequence& s, uint32_t b, uint32_t n, uint32_t j, uint32_t item, uint32_t part) const {
+    Place p{};
+    const uint32_t split = item / s.blocks, block = item - split * s.blocks;
+    p.j = j;
+    p.own = block * rows;
     p.rows = min(rows, s.rows - p.own);
     p.t0 = s.start + p.own;
     p.split = split;
@@ -179,8 +188,8 @@ struct TreeRows : TreeArgs {
     p.b = b;
     p.cached = s.cached;
     p.keys = s.keys;
-    p.part = part + item;
-    if (split == 0u && p.j == 0u && threadIdx.x < p.rows)
+    p.part = part * kv_heads + (split * kv_heads + j) * s.blocks + block;
+    if (split == 0u && j == 0u && threadIdx.x < p.rows)
       info[p.t0 + threadIdx.x] = u4_t{p.part, s.blocks, p.splits, threadIdx.x};
     return p;
   }
@@ -270,18 +279,19 @@ __device__ __forceinline__ void wait_loads() {
 //   the barrier: behind it every wave has read K of tile i + 1 and V of tile i - 1, whose places take K of tile i + 4 and V of
 //   tile i + 3, and the loads of two steps ago (K of i + 2, V of i + 1) are there;
 //   P V of tile i, dealt out among tile i + 1's masks and maxima.
-// The first operands of each half are read in the one before. Rows of a tile lie 2 HD bytes apart in LDS, the 16-byte pieces of row r
+// A wave's column tiles are every fourth, and those behind the block's columns are left out: each wave walks with as many as it
+// has. The first operands of each half are read in the one before. Rows of a tile lie 2 HD bytes apart in LDS, the 16-byte pieces of row r
 // in the order p ^ (r % 16): the 16 rows of a read fall on distinct banks.
 template <int HD, int CT, Order ORDER>
-__global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void attn_tree_kernel(TreeRows a) {
+__device__ __forceinline__ void rows_of_block(const TreeRows& a, const TreeRows::Place& p) {
   constexpr uint32_t KK = HD / 32, NT = HD / 16, S = 2 * KK, ROW = 2 * HD, TILE = kTile * ROW;
   constexpr uint32_t NI = TILE / 4096, RPI = 1024 / ROW, PPR = ROW / 16;  // a wave's loads of a tile, rows of each, pieces of a row
   constexpr uint32_t AK = 3, AV = 3, PER = KK / 2;  // operands read ahead; products for each weight
   __shared__ __align__(1024) uint8_t ring[7 * TILE];
-  const typename TreeRows::Place p = a.place(true);
-  if (p.rows == 0u) return;
+  uint32_t thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));  // (what follows from it is formed anew in each item, not kept)
   const TreeRows::Block b = a.block(p);
-  const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), qi = lane & 15u,
+  const uint32_t lane = thread & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(thread >> 6)), qi = lane & 15u,
                  qq = lane >> 4;
   auto uniform = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); };
   const uint32_t from = uniform(a.part_begin(p, b, p.split)), n = uniform(a.part_begin(p, b, p.split + 1u)) - from;
@@ -309,7 +319,6 @@ __global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void attn_tree_kernel(
   auto fetch = [&](uint32_t i) {
     entries_at = b.key(from + min(i, n - 1u)) >> a.page_shift;
     entries = b.pages[min(entries_at + lane, last >> a.page_shift)];
-    asm volatile("" ::"v"(entries));  // (waited for here, not in the loop)
   };
   auto rows_of = [&](uint32_t i) {
     const uint32_t key = b.key(from + min(i, n - 1u));
@@ -340,33 +349,46 @@ __global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void attn_tree_kernel(
   };
   auto k_at = [](uint32_t i) { return i % 3u * TILE; };
   auto v_at = [](uint32_t i) { return (3u + i % 4u) * TILE; };
-  // the columns' queries, scaled, as the B operand in f16 high and low parts: k = 32 kk + 8 qq + e
+  // the page table's entries and the columns' queries, asked for together; then the first tiles; then, meanwhile, the queries as the B
+  // operand, scaled, in f16 high and low parts: k = 32 kk + 8 qq + e
+  if constexpr (ORDER == kWholeTiles) fetch(0);
+  f4_t q[CT][2 * KK];
 #pragma unroll
   for (uint32_t ct = 0; ct < CT; ++ct) {
-    const uint32_t col = 16u * (CT * wave + ct) + qi;
+    const uint32_t col = 16u * (4u * ct + wave) + qi;
     row[ct] = col / a.gqa;
     g[ct] = col % a.gqa;
     const float* qp = a.q + ((size_t)(p.t0 + (row[ct] < p.rows ? row[ct] : 0u)) * a.q_heads + p.j * a.gqa + g[ct]) * HD + 8u * qq;
-    f4_t q[2 * KK];
 #pragma unroll
-    for (uint32_t x = 0; x < 2 * KK; ++x) q[x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2))) * a.c;
-    split_q<KK>(q, qh[ct], ql[ct]);
-    if constexpr (HD * CT > 256) {  // (in accumulation registers, which the products read too: the others are the vector ALUs')
-#pragma unroll
-      for (uint32_t kk = 0; kk < KK; ++kk) asm volatile("" : "+a"(qh[ct][kk]), "+a"(ql[ct][kk]));
-    }
+    for (uint32_t x = 0; x < 2 * KK; ++x) q[ct][x] = *as_global(reinterpret_cast<const f4_any*>(qp + 32u * (x / 2) + 4u * (x % 2)));
   }
   Rows r2{}, r3{};
   if (n) {
-    if constexpr (ORDER == kWholeTiles) fetch(0);
+    asm volatile("" ::"v"(entries));
     const Rows r0 = rows_of(0), r1 = rows_of(1);
     r2 = rows_of(2);
     r3 = rows_of(3);
+#pragma unroll
+    for (uint32_t ct = 0; ct < CT; ++ct)
+#pragma unroll
+      for (uint32_t x = 0; x < 2 * KK; ++x) asm volatile("" : "+v"(q[ct][x]));  // (waited for here: behind the tiles' loads it would be for them too)
     load(a.k, k_at(0), 0, r0);
     load(a.k, k_at(1), 1, r1);
     load(a.v, v_at(0), 0, r0);
     load(a.k, k_at(2), 2, r2);
     load(a.v, v_at(1), 1, r1);
+  }
+#pragma unroll
+  for (uint32_t ct = 0; ct < CT; ++ct) {
+#pragma unroll
+    for (uint32_t x = 0; x < 2 * KK; ++x) q[ct][x] *= a.c;
+    split_q<KK>(q[ct], qh[ct], ql[ct]);
+    if constexpr (HD * CT > 256) {  // (in accumulation registers, which the products read too: the others are the vector ALUs')
+#pragma unroll
+      for (uint32_t kk = 0; kk < KK; ++kk) asm volatile("" : "+a"(qh[ct][kk]), "+a"(ql[ct][kk]));
+    }
+  }
+  if (n) {
     wait_loads<2 * NI>();
     lds_barrier();
     // V of tile 2 and K of tile 3 follow behind the first scores
@@ -393,111 +415,128 @@ __global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void attn_tree_kernel(
     const v4s_t a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s_lds)(reinterpret_cast<const uint16_t*>(ring + to + at + 16u * ROW)));
     return __builtin_bit_cast(h8_t, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  auto product = [&](h8_t kh, uint32_t s, uint32_t part) {  // part < 2 CT: the columns' high parts, then the low ones
-    const uint32_t ct = part % CT;
-    d[ct][s % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, part < CT ? qh[ct][s / 2] : ql[ct][s / 2], d[ct][s % 2], 0, 0, 0);
-  };
-  auto clear = [&]() {
+  // the walk of a wave with NC column tiles that hold columns
+  auto walk = [&](auto tiles) {
+    constexpr uint32_t NC = decltype(tiles)::value;
+    auto product = [&](h8_t kh, uint32_t s, uint32_t part) {  // part < 2 NC: the columns' high parts, then the low ones
+      const uint32_t ct = part % NC;
+      d[ct][s % 2] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, part < NC ? qh[ct][s / 2] : ql[ct][s / 2], d[ct][s % 2], 0, 0, 0);
+    };
+    auto clear = [&]() {
 #pragma unroll
-    for (uint32_t ct = 0; ct < CT; ++ct) d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
-  };
-  // a tile's scores of column tile ct and the largest of them; behind that tile i's masks and the references
-  float mx[CT];
-  auto scores = [&](uint32_t ct) {
+      for (uint32_t ct = 0; ct < NC; ++ct) d[ct][0] = d[ct][1] = f4_t{0.f, 0.f, 0.f, 0.f};
+    };
+    // a tile's scores of column tile ct and the largest of them; behind that tile i's masks and the references
+    float mx[NC ? NC : 1];
+    auto scores = [&](uint32_t ct) {
 #pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) w[ct][e] = d[ct][e / 4][e % 4];
-    mx[ct] = most_of(w[ct]);
-    asm volatile("" : "+v"(mx[ct]));  // (formed here, between the products, not where it is used)
-  };
-  auto settle = [&](uint32_t i) {
-    const uint32_t key = b.key(from + i);
-    if (a.masked(b, key)) {
+      for (uint32_t e = 0; e < 8; ++e) w[ct][e] = d[ct][e / 4][e % 4];
+      mx[ct] = most_of(w[ct]);
+      asm volatile("" : "+v"(mx[ct]));  // (formed here, between the products, not where it is used)
+    };
+    auto settle = [&](uint32_t i) {
+      const uint32_t key = b.key(from + i);
+      if (a.masked(b, key)) {
 #pragma unroll
-      for (uint32_t ct = 0; ct < CT; ++ct) {
-        a.bias_and_mask(a.column(p, b, row[ct], g[ct]), key + 4u * qq, true, w[ct]);
-        mx[ct] = most_of(w[ct]);
+        for (uint32_t ct = 0; ct < NC; ++ct) {
+          a.bias_and_mask(a.column(p, b, row[ct], g[ct]), key + 4u * qq, true, w[ct]);
+          mx[ct] = most_of(w[ct]);
+        }
       }
-    }
-    raise_to<CT, NT>(mx, qi, r, l, acc, nullptr);
-  };
-  h8_t kh[S], av[NT];
-  if (n) {
-    clear();
-#pragma unroll
-    for (uint32_t s = 0; s < S; ++s) {
-      const h8_t k0 = k_operand(k_at(0), s);
-#pragma unroll
-      for (uint32_t part = 0; part < 2 * CT; ++part) product(k0, s, part);
-    }
-#pragma unroll
-    for (uint32_t ct = 0; ct < CT; ++ct) scores(ct);
-    settle(0);
-    lds_barrier();
-    load(a.k, k_at(3), 3, r3);
-    load(a.v, v_at(2), 2, r2);
-#pragma unroll
-    for (uint32_t s = 0; s < AK; ++s) kh[s] = k_operand(k_at(1), s);
-  }
-  uint32_t k1 = TILE, k2 = 2u * TILE, k3 = 0u, v0 = 3u * TILE, v1 = 4u * TILE, v2 = 5u * TILE, v3 = 6u * TILE;  // of tiles i + ..
-#pragma unroll 1
-  for (uint32_t i = 0; i < n; ++i) {
-    if constexpr (ORDER == kWholeTiles)
-      if (i % 32u == 0u) fetch(i + 4u);  // (pages hold a tile at least: 64 entries serve 64 steps)
-    h8_t pw[CT];
-    {  // (behind the last tile the products are of a tile that is not used)
+      if constexpr (NC != 0) raise_to<NC, NT>(mx, qi, r, l, acc, nullptr);
+    };
+    h8_t kh[S], av[NT];
+    if (n) {
       clear();
-      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (uint32_t s = 0; s < S; ++s) {
-        if (s + AK < S) kh[s + AK] = k_operand(k1, s + AK);
-        if (s + AV >= S) av[s + AV - S] = v_operand_at(v0, s + AV - S);
+        const h8_t k0 = k_operand(k_at(0), s);
 #pragma unroll
-        for (uint32_t part = 0; part < 2 * CT; ++part) {
-          product(kh[s], s, part);
-          const uint32_t done = s * 2 * CT + part + 1u;
-          if (done % PER) continue;
-          const uint32_t x = done / PER - 1u, ct = x / 8, e = x % 8;
-          w[ct][e] = __builtin_amdgcn_exp2f(w[ct][e] - r[ct]);
-          l[ct] += w[ct][e];
-          asm volatile("" : "+v"(l[ct]));
-          if (e % 2) {
-            u4_t pk = __builtin_bit_cast(u4_t, pw[ct]);
-            pk[e / 2] = h2_bits(__builtin_convertvector((f2_t{w[ct][e - 1], w[ct][e]}), h2_t));
-            pw[ct] = __builtin_bit_cast(h8_t, pk);
+        for (uint32_t part = 0; part < 2 * NC; ++part) product(k0, s, part);
+      }
+#pragma unroll
+      for (uint32_t ct = 0; ct < NC; ++ct) scores(ct);
+      settle(0);
+      lds_barrier();
+      load(a.k, k_at(3), 3, r3);
+      load(a.v, v_at(2), 2, r2);
+#pragma unroll
+      for (uint32_t s = 0; s < AK; ++s) kh[s] = k_operand(k_at(1), s);
+    }
+    uint32_t k1 = TILE, k2 = 2u * TILE, k3 = 0u, v0 = 3u * TILE, v1 = 4u * TILE, v2 = 5u * TILE, v3 = 6u * TILE;  // of tiles i + ..
+#pragma unroll 1
+    for (uint32_t i = 0; i < n; ++i) {
+      if constexpr (ORDER == kWholeTiles)
+        if (i % 32u == 0u) {  // (pages hold a tile at least: 64 entries serve 64 steps)
+          fetch(i + 4u);
+          asm volatile("" ::"v"(entries));  // (waited for here, not in the loop)
+        }
+      h8_t pw[NC ? NC : 1];
+      {  // (behind the last tile the products are of a tile that is not used)
+        clear();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (uint32_t s = 0; s < S; ++s) {
+          if (s + AK < S) kh[s + AK] = k_operand(k1, s + AK);
+          if (s + AV >= S) av[s + AV - S] = v_operand_at(v0, s + AV - S);
+#pragma unroll
+          for (uint32_t part = 0; part < 2 * NC; ++part) {
+            product(kh[s], s, part);
+            const uint32_t done = s * 2 * NC + part + 1u;
+            if (done % PER) continue;
+            const uint32_t x = done / PER - 1u, ct = x / 8, e = x % 8;
+            w[ct][e] = __builtin_amdgcn_exp2f(w[ct][e] - r[ct]);
+            l[ct] += w[ct][e];
+            asm volatile("" : "+v"(l[ct]));
+            if (e % 2) {
+              u4_t pk = __builtin_bit_cast(u4_t, pw[ct]);
+              pk[e / 2] = h2_bits(__builtin_convertvector((f2_t{w[ct][e - 1], w[ct][e]}), h2_t));
+              pw[ct] = __builtin_bit_cast(h8_t, pk);
+            }
+            __builtin_amdgcn_sched_barrier(0);
           }
+        }
+      }
+      wait_loads<2 * NI>();
+      lds_barrier();
+      {
+        const Rows r4 = rows_of(i + 4u);
+        load(a.k, k1, i + 4u, r4);
+        load(a.v, v3, i + 3u, r3);
+        r3 = r4;
+      }
+      {
+#pragma unroll
+        for (uint32_t tt = 0; tt < NT; ++tt) {
+          if (tt + AV < NT) av[tt + AV] = v_operand_at(v0, tt + AV);
+          if (tt + AK >= NT) kh[tt + AK - NT] = k_operand(k2, tt + AK - NT);
+#pragma unroll
+          for (uint32_t ct = 0; ct < NC; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[tt], pw[ct], acc[ct][tt], 0, 0, 0);
+          if (tt >= 1 && tt <= NC) scores(tt - 1);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
+      if (NC != 0 && i + 1u < n) settle(i + 1u);
+      const uint32_t k = k1, v = v0;
+      k1 = k2;
+      k2 = k3;
+      k3 = k;
+      v0 = v1;
+      v1 = v2;
+      v2 = v3;
+      v3 = v;
     }
-    wait_loads<2 * NI>();
-    lds_barrier();
-    {
-      const Rows r4 = rows_of(i + 4u);
-      load(a.k, k1, i + 4u, r4);
-      load(a.v, v3, i + 3u, r3);
-      r3 = r4;
-    }
-    {
-#pragma unroll
-      for (uint32_t tt = 0; tt < NT; ++tt) {
-        if (tt + AV < NT) av[tt + AV] = v_operand_at(v0, tt + AV);
-        if (tt + AK >= NT) kh[tt + AK - NT] = k_operand(k2, tt + AK - NT);
-#pragma unroll
-        for (uint32_t ct = 0; ct < CT; ++ct) acc[ct][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av[tt], pw[ct], acc[ct][tt], 0, 0, 0);
-        if (tt >= 1 && tt <= CT) scores(tt - 1);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    if (i + 1u < n) settle(i + 1u);
-    const uint32_t k = k1, v = v0;
-    k1 = k2;
-    k2 = k3;
-    k3 = k;
-    v0 = v1;
-    v1 = v2;
-    v2 = v3;
-    v3 = v;
-  }
+  };
+  const uint32_t used = (p.rows * a.gqa + 15u) / 16u, live = uniform(used > wave ? (used - wave + 3u) / 4u : 0u);
+  auto walk_if = [&](auto tiles) {
+    if constexpr (decltype(tiles)::value <= CT)
+      if (live == tiles) walk(tiles);
+  };
+  walk_if(std::integral_constant<uint32_t, 0>{});
+  walk_if(std::integral_constant<uint32_t, 1>{});
+  walk_if(std::integral_constant<uint32_t, 2>{});
+  walk_if(std::integral_constant<uint32_t, 3>{});
+  walk_if(std::integral_constant<uint32_t, 4>{});
   wait_loads<0>();
   if (ORDER != kContiguous && __ballot(outside)) a.report_pages(p, b, from, from + n, 1u);
   float sum[CT];
@@ -532,6 +571,11 @@ __global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void attn_tree_kernel(
         store_out<HD>(a, p.j, p.t0 + row[ct], g[ct], qq, tt, inv == 0.f ? f4_t{0.f, 0.f, 0.f, 0.f} : acc[ct][tt] * inv);
     }
   }
+}
+
+template <int HD, int CT, Order ORDER>
+__global__ __launch_bounds__(256, HD * CT <= 256 ? 2 : 1) void attn_tree_kernel(TreeRows a) {
+  a.each_item([&](const TreeRows::Place& p) { rows_of_block<HD, CT, ORDER>(a, p); });
 }
 
 // The sums of a column's parts s0, s0 + step .., four dims of them, U parts at a time.
@@ -623,8 +667,8 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a, uint32_
 //   rows of 128: one sequence's rows make blocks / CT work-groups of a known number: the least modelled time of 2, 3 and 4, a
 //   block's tile 1.1, 1.375 and 1.7 us of a CU. Measured (us; CT 2, 3, 4): over 65536 keys, 40 / 8 heads, 25 rows 81 / 101 / 127, 38
 //   rows 117 / 100 / 121, 51 rows 211 / 167 / 121, 64 rows 209 / 168 / 200; over 8192 keys 27 / 27 / 31, 32 / 30 / 33, 37 / 37 / 36,
-//   38 / 38 / 44. Of several sequences only the mean is known: CT 2, which loses least where they are ragged (8 trees of 30 to 61
-//   rows 118 / 144 / 170; of 51 each, 4000 keys, 77 / 84 / 70).
+//   38 / 38 / 44. Of several sequences only the mean is known: CT 2, which loses least where they are ragged (8 trees of 38 to 61
+//   rows 107 / 141 / 162; of 51 each, 4000 keys, 77 / 84 / 70).
 struct Pick {
   bool few;
   uint32_t ct, rows, columns, slots;
@@ -652,7 +696,7 @@ Pick pick(uint32_t T, uint32_t sequences, uint32_t gqa, uint32_t hd) {
   return best;
 }
 // The parts of all sequences at most, one for each block aside: as many as make every work-group that runs at once busy, where there
-// are several sequences some times as many.
+// are several sequences some times as many, which its work-groups take one behind another.
 uint32_t share_of(const Pick& p, uint32_t kv_heads, uint32_t sequences) {
   return std::min(kMaxSplits - 1u, std::max(1u, p.slots * (sequences == 1u ? 1u : p.few ? 4u : 2u) / kv_heads));
 }
@@ -759,11 +803,11 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
   a.c = shape->scale * kLog2e;
   hipStream_t st = (hipStream_t)stream;
   a.most_blocks = T / p.rows + n;
-  // as many work-groups as there are items at most: share and one more for each block, of each kv head, no more than the blocks have
-  // parts of the least size
+  // as many work-groups as run at once, and as there are items at most: share and one more for each block, of each kv head, no more
+  // than the blocks have parts of the least size
   const uint64_t least_parts = ((uint64_t)kv_len + a.least * kTile - 1u) / (a.least * kTile);
   const uint32_t items = shape->kv_heads * (uint32_t)std::min<uint64_t>(a.share + a.most_blocks, a.most_blocks * least_parts);
-  const uint32_t grid = (items + kXcds - 1u) / kXcds * kXcds;
+  const uint32_t grid = std::min((items + kXcds - 1u) / kXcds * kXcds, p.slots);
   const bool narrow = shape->head_dim == 128;
   if (p.few) {
     if (narrow) attn_rows_few_kernel<128><<<grid, 256, 0, st>>>(a);
