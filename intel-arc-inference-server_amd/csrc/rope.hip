@@ -91,17 +91,16 @@ struct RowsArgs {
 template <bool F16>
 __device__ __forceinline__ f4_t load4(const void* base, size_t at) {
   if constexpr (F16) {
-    const u2_t h = *as_global(reinterpret_cast<const h4_any*>(static_cast<const uint16_t*>(base) + at));
+    const u2_t h = __builtin_nontemporal_load(as_global(reinterpret_cast<const h4_any*>(static_cast<const uint16_t*>(base) + at)));
     return f4_t{h2f((uint16_t)h[0]), h2f((uint16_t)(h[0] >> 16)), h2f((uint16_t)h[1]), h2f((uint16_t)(h[1] >> 16))};
   } else {
-    return *as_global(reinterpret_cast<const f4_any*>(static_cast<const float*>(base) + at));
+    return __builtin_nontemporal_load(as_global(reinterpret_cast<const f4_any*>(static_cast<const float*>(base) + at)));
   }
 }
 // HD / 8 threads take a head of a row, two pieces of four elements each: with pairs of halves the two pieces that turn together (and
 // two of those behind the rotated part that do not turn), with pairs of neighbours any two. The norm's sum goes over these threads.
-// Nothing is rounded before the stores. Bound by the bytes: 2048 rows of 40 / 8 heads of 128 (110 MB) 19.2 us where they are in the
-// last cache, 24 where they are not (a copy 7.2 and 4.9 TB/s). Four heads a thread took 18.7, but 6.6 in place of 4.2 at 256
-// rows and 8.8 in place of 6.9 at 512.
+// Nothing is rounded before the stores. Bound by the bytes: 2048 rows of 40 / 8 heads of 128 (110 MB) 23.3 us, 4.7 TB/s (a copy
+// 4.9; with loads that the caches keep 24.3). Four heads a thread took 2 us more at 256 and 512 rows and little less at 2048.
 template <int HD, bool F16, bool PAIRED>
 __global__ __launch_bounds__(256) void rope_rows_kernel(RowsArgs a) {
   constexpr uint32_t L = HD / 8;
