@@ -6,7 +6,9 @@
 //   first, and gives back max(held_b - need_b, 0) behind the ring's last
 //   row t = row_start_b + i (row_start: the sums of added): key cached_b + i, cache row table_b[key / page] page + key % page
 //   a tree's node i: mask_t the bits of i and its ancestors, position cached_b + their number; else position = key
-// One work-group does the requests, a thread each; a thread does a row. Bound by chains of loads: 8 trees of 61 nodes are 10 KB.
+// One work-group does the requests, a thread each; a thread does a row. Bound by chains of loads, not by bytes: 8 trees of 61 nodes
+// (10 KB) 5.6 us, a launch that does nothing 3.5; 509 requests with 10000 rows 8.3 in two launches. More rows than kOneGroup are
+// more than one work-group's loads hide.
 #include <algorithm>
 
 #include "mi_capi_internal.h"
