@@ -77,8 +77,8 @@ struct TreeRows : TreeArgs {
   // Tiles of a part at most, for several sequences of `total` tiles in all blocks. With `even` tiles in each of the work-groups that
   // run at once, and parts of `per` tiles that make `items` items, the call lasts per + 3 where all run at once, else
   // even + per / 2 + 3 items / slots (in tiles; 3: an item's start). Few sequences of uneven lengths are near `even` in one round or
-  // none: of 64 candidates, a lane each, the least is taken. With many sequences items / slots is near even / per, and the second form least
-  // at per = sqrt(6 even). None is below total / share, so there are no more items than share and one for each block.
+  // none: of 64 candidates, a lane each, the least is taken. Of many sequences items / slots is near even / per, and the second
+  // form is least at per = sqrt(6 even). None is below total / share, so there are no more items than share and one for each block.
   __device__ __forceinline__ uint32_t part_tiles(const Sequence& first, float total) const {
     const uint32_t lane = threadIdx.x & 63u;
     const float even = total * (float)kv_heads / (float)slots, floor = total * 1.0001f / (float)share;
