@@ -693,7 +693,7 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
                  uint16_t* attn_out, uint32_t* flag, void* stream);
 /* mi_accept_greedy for a tree, on the host: node 0 is the text's next token, tokens and parent those of the n nodes, argmax what the
  * model says behind each. From node 0 on, the child whose token is its parent's argmax is accepted (the first of equal ones).
- * Returns the number of accepted drafts, their nodes in path [n - 1]; *next = the argmax behind the last. */
+ * Returns the number of accepted drafts, their nodes in path [n - 1]; *next = the argmax behind the last. n 0: 0, *next as it was. */
 uint32_t mi_accept_tree(const uint32_t* argmax, const uint32_t* tokens, const uint32_t* parent, uint32_t n, uint32_t* path,
                         uint32_t* next);
 /* The k best continuations of each of `batch` texts over its beams and the vocabulary: logits fp32 [batch * beams][vocab_used], rows

@@ -91,6 +91,7 @@ extern "C" uint32_t mi_accept_greedy(const uint32_t* verify_argmax, const uint32
 extern "C" uint32_t mi_accept_tree(const uint32_t* argmax, const uint32_t* tokens, const uint32_t* parent, uint32_t n,
                                    uint32_t* path, uint32_t* next) {
   uint32_t at = 0, j = 0;
+  if (n == 0) return 0;  // (no node, no next token)
   for (uint32_t i = 1; i < n; ++i)  // (a child's number is above its parent's)
     if (parent[i] == at && tokens[i] == argmax[at]) path[j++] = at = i;
   if (next) *next = argmax[at];

@@ -150,6 +150,8 @@ def test_accept_tree():
     # equal drafts of one parent: the first
     got, n = mi.accept_tree([5, 1, 2, 3], [0, 5, 5, 1], [none, 0, 0, 1])
     assert list(got) == [1, 3] and n == 3
+    nxt = mi.u32(77)  # (no node: nothing is read)
+    assert mi.lib().mi_accept_tree(None, None, None, 0, None, mi.C.byref(nxt)) == 0 and nxt.value == 77
     got, n = mi.accept_tree([7], [0], [none])
     assert list(got) == [] and n == 7
     # a chain is accepted as mi_accept_greedy has it
