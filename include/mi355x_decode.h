@@ -657,7 +657,8 @@ int mi_rope_table(const mi_rope* rope, uint32_t pos0, uint32_t n, float* table, 
  * row * row_stride + head * head_stride. All of it in fp32, each k and v rounded once: mi_attn_prep_rows rounds to f16 before and
  * behind the norm too. A slot of none: the row has no k and v to store. rows: the cache's; a slot that is not below it
  * stores neither (MI_STATUS_BAD_PAGE); a position that is not below rope_len (the table's rows) stores nothing of its row
- * (0xDEAD0002). flag may be NULL. Slots are distinct. head_dim 128 or 256, rot_dim a multiple of 8, T up to 65535, not gated. */
+ * (0xDEAD0002). flag may be NULL. Slots are distinct. head_dim 128 or 256, rot_dim a multiple of 8, T up to 65535 and
+ * T (q_heads + 2 kv_heads) up to 2^26, not gated. */
 int mi_rope_rows(const void* qkv, uint32_t in_kind, size_t in_stride, uint32_t T, const uint32_t* pos, uint32_t pos0,
                  const uint32_t* slots, uint32_t rows, const mi_attn_shape* shape, uint32_t paired, const float* q_norm,
                  const float* k_norm, const float* rope, uint32_t rope_len, float* attn_q, uint16_t* kv_k, uint16_t* kv_v,

@@ -652,11 +652,11 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamArgs a) {
               list.score);
 }
 
-// Behind slices, in place of logprobs_join_kernel and beam_select_kernel: grid (batch), eight waves. They join each beam's
+// Behind slices, in place of logprobs_join_kernel and beam_select_kernel: grid (batch), sixteen waves. They join each beam's
 // statistics; form a bound that k runs of 256 tokens reach by the score of their largest logit (as logprobs_join_kernel's); read again
 // the runs that reach it, of all beams about k; and a token's place is the number of those read that are better. Where more tokens reach
-// the bound than fit, the waves keep a list of every beam. One text of 4 beams with k = 8 takes 14.1 us in all, 16 of 8 with k = 16
-// 29.4 (16.0 and 32 with the rows' lists first); equal logits 45, rising ones 104. Bound by its chain of loads.
+// the bound than fit, the waves keep a list of every beam. One text of 4 beams with k = 8 takes 13.4 us in all, 16 of 8 with k = 16
+// 28.7 (16.0 and 32 with the rows' lists first); equal logits 45, rising ones 104. Bound by its chain of loads.
 constexpr uint32_t kFit = 1024, kMaxBeams = 64;
 constexpr uint32_t kJoinWaves = 16, kJoinRuns = 8;  // a lane's runs
 uint32_t runs_of_wave(uint32_t vocab) { return ((vocab + 255u) / 256u + kJoinWaves - 1u) / kJoinWaves; }

@@ -247,6 +247,7 @@ int mi_rope_rows(const void* qkv, uint32_t in_kind, size_t in_stride, uint32_t T
     return mi_fail(MI_ERR_SHAPE, "rope_rows: rot_dim a multiple of 8 up to head_dim");
   if (T == 0 || T > kMaxRows || rows == 0 || rope_len == 0)
     return mi_fail(MI_ERR_SHAPE, "rope_rows: T 1..65535, rows and rope_len from 1");
+  if ((uint64_t)T * (qh + 2u * kvh) > 1u << 26) return mi_fail(MI_ERR_SHAPE, "rope_rows: 2^26 heads of rows at most");
   if (!pos && (uint64_t)pos0 + T > 0xFFFFFFFFull) return mi_fail(MI_ERR_SHAPE, "rope_rows: positions are below 2^32");
   if (in_stride < shape->qkv_n) return mi_fail(MI_ERR_ARG, "rope_rows: in_stride below qkv_n");
   if (off(qkv, in_kind == MI_OUT_F16 ? 2 : 4) || off(attn_q, 4) || off(kv_k, 2) || off(kv_v, 2) || off(rope, 4) || off(q_norm, 4) ||

@@ -74,6 +74,8 @@ def test_rope_rows_refusals():
                {"sh": shape(rot_dim=136)}, {"sh": shape(rot_dim=0)}, {"sh": shape(rot_dim=12)}, {"sh": shape(kv_heads=0)},
                {"pos": None, "pos0": 0xFFFFFFFE}):
         assert call(**kw) == SHAPE, kw
+    wide = mi.AttnShape(1024, 512, 128, 128, 0, 2048 * 128, 1024 * 128, 1536 * 128, 0.1, 1e-6, 0)  # (a launch of more than 2^32 threads)
+    assert call(sh=wide, T=65535, stride=2048 * 128) == SHAPE
     assert L.mi_rope_rows(P, 0, 1792, 4, P, 0, P, 100, None, 0, P, P, P, 50, P, P, P, 128, 12800, None, None) == ARG
 
 
