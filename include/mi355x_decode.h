@@ -40,7 +40,7 @@ extern "C" {
  * sequences, where a cache row lies outside. */
 #define MI_STATUS_BAD_PAGE 0xDEAD0005u
 /* mi_block_tables' flag word where the ring has too few free pages, and where lengths, tables, ring or parents cannot be
- * (mi_attn_tree's: where sequences overlap). */
+ * (mi_attn_tree's: where row_start falls). */
 #define MI_STATUS_NO_PAGES 0xDEAD0006u
 #define MI_STATUS_BAD_ROWS 0xDEAD0007u
 
@@ -684,8 +684,8 @@ typedef struct mi_attn_batch {
  * parts follows the lengths of all sequences, so a row's last bits depend on T and on the lengths beside it, never on the values.
  * What a row does not see has no part in it, infinities and NaN included. A table entry that is not below n_pages, of a page that holds
  * a key of a sequence with rows, sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL); nothing outside the cache is read. row_start
- * does not fall; sequences that overlap so much that they are more than T rows are refused on the device (MI_STATUS_BAD_ROWS, no row
- * is written). head_dim 128 or 256, up to 64 q heads per kv head, not gated; T up to 65535, 1..1024 sequences, kv_len up to 2^30,
+ * does not fall, so that no two sequences share a row: where an entry is below the one before it the call is refused on the device
+ * (MI_STATUS_BAD_ROWS, no row is written). head_dim 128 or 256, up to 64 q heads per kv head, not gated; T up to 65535, 1..1024 sequences, kv_len up to 2^30,
  * words 1..64 with masks, 0 without. ws: mi_attn_tree_ws bytes of device scratch, 16-byte aligned; its size never falls as T grows
  * and is the same for any number of sequences. */
 size_t mi_attn_tree_ws(uint32_t T, uint32_t sequences, const mi_attn_shape* shape);

@@ -34,19 +34,21 @@ struct TreeArgs {
   uint32_t* flag;
   size_t row_stride, head_stride;
   uint32_t table_stride, page, page_shift, n_pages, kv_len, T, sequences, words, q_heads, kv_heads, gqa, rows, columns, slots,
-      share, least, most_blocks, act;
+      share, least, act;
   float c;  // y = c q . k
 };
 
 // A sequence's rows, keys and tiles, whatever the arrays hold.
 struct Sequence {
   uint32_t start, rows, cached, keys, blocks, tiles;
+  bool falls;  // it ends before it starts: where none does, no two share a row
 };
 __device__ __forceinline__ Sequence sequence(const TreeArgs& a, uint32_t b) {
-  Sequence s{0u, 0u, 0u, 0u, 0u, 0u};
+  Sequence s{0u, 0u, 0u, 0u, 0u, 0u, false};
   if (b < a.sequences) {
     s.start = a.row_start[b];
-    const uint32_t end = min(a.row_start[b + 1u], a.T);
+    const uint32_t next = a.row_start[b + 1u], end = min(next, a.T);
+    s.falls = next < s.start;
     s.cached = min(a.cached[b], a.kv_len);
     s.rows = end > s.start ? end - s.start : 0u;
     s.keys = s.cached + min(s.rows, a.kv_len - s.cached);
@@ -106,22 +108,23 @@ struct TreeRows : TreeArgs {
     auto plus = [](uint32_t x, uint32_t y) { return x + y; };
     Sequence s = sequence(*this, one ? 0u : lane);
     uint32_t per, items;  // (items of a kv head)
+    bool falls = s.falls;
+    for (uint32_t b = 64u; b < sequences; b += 64u) falls |= sequence(*this, b + lane).falls;
+    if (__ballot(falls)) {  // (sequences may share rows: two work-groups would store one)
+      if (flag) *flag = MI_STATUS_BAD_ROWS;
+      if (blockIdx.x == 0u)
+        for (uint32_t t = threadIdx.x; t < T; t += blockDim.x) info[t] = u4_t{0u, 0u, 0u, 0u};  // (nothing to join)
+      return;
+    }
     if (one) {
       per = max(least, max(s.blocks, s.tiles) < 65536u ? (s.blocks * s.tiles + share - 1u) / share
                                                        : (uint32_t)((float)s.blocks * (float)s.tiles * 1.0001f / (float)share) + 1u);
       items = s.blocks * parts(s, per);
     } else {
-      float total = (float)s.blocks * (float)s.tiles, blocks = (float)s.blocks;
+      float total = (float)s.blocks * (float)s.tiles;
       for (uint32_t b = 64u; b < sequences; b += 64u) {
         const Sequence o = sequence(*this, b + lane);
         total += (float)o.blocks * (float)o.tiles;
-        blocks += (float)o.blocks;
-      }
-      if (wave_sum(blocks) > (float)most_blocks) {  // (sequences that overlap: their items would be more than are counted with)
-        if (flag) *flag = MI_STATUS_BAD_ROWS;
-        if (blockIdx.x == 0u)
-          for (uint32_t t = threadIdx.x; t < T; t += blockDim.x) info[t] = u4_t{0u, 0u, 0u, 0u};  // (nothing to join)
-        return;
       }
       per = part_tiles(s, wave_sum(total));
       items = s.blocks * parts(s, per);
@@ -163,7 +166,8 @@ struct TreeRows : TreeArgs {
         }
       }
       auto of_found = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)found); };
-      const Sequence f = {of_found(s.start), of_found(s.rows), of_found(s.cached), of_found(s.keys), of_found(s.blocks), of_found(s.tiles)};
+      const Sequence f = {of_found(s.start),  of_found(s.rows),  of_found(s.cached), of_found(s.keys),
+                          of_found(s.blocks), of_found(s.tiles), false};
       b += found;
       s = Sequence{};  // (not kept in registers meanwhile)
       of(inside(f, b, parts(f, per), j, item, part));
@@ -802,11 +806,11 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
   a.act = shape->act;
   a.c = shape->scale * kLog2e;
   hipStream_t st = (hipStream_t)stream;
-  a.most_blocks = T / p.rows + n;
+  const uint32_t most_blocks = T / p.rows + n;  // (no two sequences share a row)
   // as many work-groups as run at once, and as there are items at most: share and one more for each block, of each kv head, no more
   // than the blocks have parts of the least size
   const uint64_t least_parts = ((uint64_t)kv_len + a.least * kTile - 1u) / (a.least * kTile);
-  const uint32_t items = shape->kv_heads * (uint32_t)std::min<uint64_t>(a.share + a.most_blocks, a.most_blocks * least_parts);
+  const uint32_t items = shape->kv_heads * (uint32_t)std::min<uint64_t>(a.share + most_blocks, most_blocks * least_parts);
   const uint32_t grid = std::min((items + kXcds - 1u) / kXcds * kXcds, p.slots);
   const bool narrow = shape->head_dim == 128;
   if (p.few) {
@@ -822,7 +826,7 @@ int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v
   }
   if (kv_len > a.least * kTile) {  // (there may be several parts)
     const uint32_t most = 2u * a.share * shape->kv_heads - 1u;
-    if (a.most_blocks * 8u <= a.share) {
+    if (most_blocks * 8u <= a.share) {
       if (narrow) attn_tree_join_kernel<128, true><<<dim3(shape->q_heads, T), 256, 0, st>>>(a, most);
       else attn_tree_join_kernel<256, true><<<dim3(shape->q_heads, T), 256, 0, st>>>(a, most);
     } else {  // (of many rows most have one part: few work-groups a row)

@@ -390,3 +390,29 @@ def test_offsets_past_32_bits(rows, hd, page):
 
     c.place = place
     c.check()
+
+
+@pytest.mark.parametrize("rows,cached,hd", [(3, 100, 128), (20, 50, 128), (20, 900, 256)])
+@pytest.mark.parametrize("starts", [(0, 1, 0, 1), (0, 1, 1, 0), (1, 0, 0, 1), (1, 0)])
+def test_a_row_start_that_falls_is_refused(starts, rows, cached, hd):
+    """few enough rows for the arrays, but two sequences of the same ones: no row is written"""
+    c = Case(9, [(cached, rows)] + [(cached, 0)] * (len(starts) - 2), hd=hd)
+    b = c.bind()
+    b["row_start"].copy_(dev((np.array(starts) * rows).astype(np.uint32)))
+    mi.call("mi_attn_tree", *b["args"], stream())
+    sync()
+    assert int(host(b["flag"], np.uint32)[0]) == mi.STATUS_BAD_ROWS
+    assert (host(b["out"], np.uint16) == 1234).all()
+
+
+@pytest.mark.parametrize("n,at", [(64, 64), (65, 64), (130, 70), (1024, 1023)])
+def test_a_row_start_that_falls_far_behind_is_refused(n, at):
+    c = Case(9, [(40, 1)] * n)
+    b = c.bind()
+    starts = c.start.astype(np.uint32)
+    starts[at] = starts[at - 1] - 1
+    b["row_start"].copy_(dev(starts))
+    mi.call("mi_attn_tree", *b["args"], stream())
+    sync()
+    assert int(host(b["flag"], np.uint32)[0]) == mi.STATUS_BAD_ROWS
+    assert (host(b["out"], np.uint16) == 1234).all()
