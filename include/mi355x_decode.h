@@ -648,7 +648,7 @@ typedef struct mi_rope {
 } mi_rope;
 /* table [n][2][rot_dim / 2] fp32 = (cos, sin)(p f_i) of the positions pos0 .. pos0 + n - 1, formed in 64 bits and rounded once:
  * what mi_attn_prep, mi_attn_prep_rows and mi_rope_rows read. rot_dim a multiple of 8 up to 256, positions below 2^31, theta above 1,
- * f_i up to 2^20 (an angle is off by 2^-53 of itself: below 2^-24 up to angles of 2^29). */
+ * f_i up to 2^20 (an angle is off by 2^-52 of itself: below 2^-24 up to angles of 2^28). */
 int mi_rope_table(const mi_rope* rope, uint32_t pos0, uint32_t n, float* table, void* stream);
 /* Rows of q||k||v (in_kind MI_OUT_F32 or MI_OUT_F16, rows in_stride elements apart): q and k are normed by head (RMSNorm with
  * q_norm / k_norm fp32 [head_dim], NULL = none, shape->eps), their first rot_dim dims turned by the table's row of position pos[t]

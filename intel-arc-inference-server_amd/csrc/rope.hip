@@ -20,11 +20,12 @@ struct TableArgs {
   double much;
   double f[kMaxRot / 2], cos_f[kMaxRot / 2], sin_f[kMaxRot / 2];  // a pair's angle from a position to the next
 };
-// A thread takes four pairs of kStep positions. The first position's angle is formed in 64 bits and brought to |r| <= pi / 4 by
-// pi / 2 in two parts (off by 2^-53 of the angle, as the product p f_i is); the series of sine and cosine there go to r^15 and r^14
-// (off by 2^-49). Every position behind it turns by f_i, four products of 64 bits in place of some thirty operations, off by 2^-52
-// more each. Bound by the stores: 131072 positions of 64 pairs (67 MB) 12.3 us (16.0 with each angle's own series, bound by
-// the 64-bit operations; steps of 2 / 4 / 8 positions 12.6 / 12.3 / 14.2; a plain fill 11.2).
+// A thread takes four pairs of kStep positions. The first position's angle is formed in 64 bits, off by 2^-52 of itself (f_i, which
+// the host forms in more bits, and the product p f_i are rounded once each), and brought to |r| <= pi / 4 by pi / 2 in two parts, off
+// by 2^-53 of r; the series of sine and cosine there go to r^15 and r^14 (off by 2^-49). Every position behind it turns by f_i, four
+// products of 64 bits in place of some thirty operations, off by 2^-52 more each. Bound by the stores: 131072 positions of 64 pairs
+// (67 MB) 12.3 us (16.0 with each angle's own series, bound by the 64-bit operations; steps of 2 / 4 / 8 positions 12.6 / 12.3 / 14.2;
+// a plain fill 11.2).
 constexpr uint32_t kStep = 4;
 __global__ __launch_bounds__(256) void rope_table_kernel(TableArgs a) {
   const uint32_t per = a.half / 4u, i = blockIdx.x * 256u + threadIdx.x;
@@ -200,28 +201,36 @@ int mi_rope_table(const mi_rope* rope, uint32_t pos0, uint32_t n, float* table, 
   if (ranged && !(rope->original && rope->low > 0.0f && rope->high > rope->low && rope->high <= 1e9f))
     return mi_fail(MI_ERR_ARG, "rope_table: original from 1, 0 < low < high turns");
   TableArgs a{table, pos0, n, r / 2u, 1.0, {}, {}, {}};
-  const double by = rope->factor, pi = 3.141592653589793;
-  double theta = rope->theta, lo = 0.0, hi = 0.0;
-  if (rope->scaling == MI_ROPE_BASE) theta *= std::pow(by, (double)r / (double)(r - 2u));
+  // (in 64 bits the exponent's rounding alone would take a frequency ln(theta) 2^-53 of itself off)
+  using wide = long double;
+  const wide by = rope->factor, pi = 3.14159265358979323846L;
+  wide theta = rope->theta, lo = 0, hi = 0;
+  if (rope->scaling == MI_ROPE_BASE) theta *= std::pow(by, (wide)r / (wide)(r - 2u));
   if (rope->scaling == MI_ROPE_YARN) {
-    auto pair = [&](double turns) { return r * std::log(rope->original / (turns * 2.0 * pi)) / (2.0 * std::log(theta)); };
-    lo = std::max(std::floor(pair(rope->high)), 0.0);
-    hi = std::min(std::ceil(pair(rope->low)), (double)(r - 1u));
-    a.much = by > 1.0 ? 0.1 * std::log(by) + 1.0 : 1.0;
+    auto pair = [&](wide turns) { return r * std::log(rope->original / (turns * 2 * pi)) / (2 * std::log(theta)); };
+    lo = std::max(std::floor(pair(rope->high)), (wide)0);
+    hi = std::min(std::ceil(pair(rope->low)), (wide)(r - 1u));
+    a.much = by > 1 ? (double)(0.1L * std::log(by) + 1) : 1.0;
   }
   if (rope->attention != 0.0f) a.much = rope->attention;
+  // theta^(-2 i / r), from those whose i is a power of two (a power of each took the host 31 us a call, these 7, of 64 bits 6)
+  wide plain[kMaxRot / 2] = {1};
+  for (uint32_t i = 1; i < a.half; ++i) {
+    const uint32_t low = i & (0u - i);
+    plain[i] = i == low ? std::pow(theta, (wide)-2 * i / r) : plain[i - low] * plain[low];
+  }
   for (uint32_t i = 0; i < a.half; ++i) {
-    double f = std::pow(theta, -2.0 * i / r);
+    wide f = plain[i];
     if (rope->divisors) {
       if (!(rope->divisors[i] > 0.0f)) return mi_fail(MI_ERR_ARG, "rope_table: divisors above 0");
       f /= rope->divisors[i];
     }
-    double part = 1.0;  // of the frequency as it is; the rest of it divided by the factor
-    if (rope->scaling == MI_ROPE_LINEAR) part = 0.0;
-    if (rope->scaling == MI_ROPE_WAVELENGTH) part = (rope->original * f / (2.0 * pi) - rope->low) / ((double)rope->high - rope->low);
-    if (rope->scaling == MI_ROPE_YARN) part = 1.0 - (i - lo) / std::max(hi - lo, 0.001);
-    part = std::min(std::max(part, 0.0), 1.0);
-    a.f[i] = part == 1.0 ? f : part * f + (1.0 - part) * f / by;
+    wide part = 1;  // of the frequency as it is; the rest of it divided by the factor
+    if (rope->scaling == MI_ROPE_LINEAR) part = 0;
+    if (rope->scaling == MI_ROPE_WAVELENGTH) part = (rope->original * f / (2 * pi) - rope->low) / ((wide)rope->high - rope->low);
+    if (rope->scaling == MI_ROPE_YARN) part = 1 - (i - lo) / std::max(hi - lo, (wide)0.001);
+    part = std::min(std::max(part, (wide)0), (wide)1);
+    a.f[i] = (double)(part == 1 ? f : part * f + (1 - part) * f / by);
     // (so that a position's angle stays below 2^51, where its number of quarter turns is a whole number of 64 bits)
     if (!(a.f[i] <= 1048576.0)) return mi_fail(MI_ERR_ARG, "rope_table: a frequency above 2^20");
     a.cos_f[i] = std::cos(a.f[i]);

@@ -298,3 +298,37 @@ def test_rows_past_32_bits(by_row):
     for n, x in zip("kv", caches):
         b[n][:-GUARD] = x.reshape(-1)
     c.check(c.result(b))
+
+
+def check_far_table(rope, pos0, n, **kw):
+    """as check_table, with what two roundings of 64 bits leave of the angle (the frequency's and the product's): 2^-52 of it"""
+    got = table(rope, pos0, n)
+    angle = (pos0 + np.arange(n)).astype(LD)[:, None] * frequencies(rope.rot_dim, rope.theta, rope.scaling, **kw)
+    for k, fn in enumerate((np.cos, np.sin)):
+        want = fn(angle)
+        tol = 2.0 ** -24 * np.abs(want) + 1.01 * (2.0 ** -52 * angle + 2.0 ** -46)
+        assert np.all(np.abs(got[:, k] - want) <= tol), np.max(np.abs(got[:, k] - want) / tol)
+
+
+@pytest.mark.parametrize("r", [24, 96, 128, 248, 256])
+@pytest.mark.parametrize("theta", [1.5, 10000.0, 1e6, 1e30])
+@pytest.mark.parametrize("pos0", [0, 1 << 24, 1 << 28, (1 << 31) - 999])
+def test_table_of_far_positions(r, theta, pos0):
+    check_far_table(mi.Rope(rot_dim=r, theta=theta), pos0, 999)
+
+
+@pytest.mark.parametrize("r", [24, 64, 248])
+@pytest.mark.parametrize("scaling,factor,low,high", [
+    (mi.ROPE_LINEAR, 40.0, 0, 0), (mi.ROPE_LINEAR, 0.3, 0, 0), (mi.ROPE_BASE, 8.0, 0, 0), (mi.ROPE_WAVELENGTH, 32.0, 1.0, 4.0),
+    (mi.ROPE_YARN, 40.0, 1.0, 32.0)])
+@pytest.mark.parametrize("pos0", [1 << 20, (1 << 31) - 300])
+def test_scaled_table_of_far_positions(r, scaling, factor, low, high, pos0):
+    rope = mi.Rope(rot_dim=r, theta=1e6, scaling=scaling, factor=factor, original=4096, low=low, high=high, attention=1.0)
+    check_far_table(rope, pos0, 300, factor=factor, original=4096, low=low, high=high)
+
+
+def test_table_of_frequencies_above_one():
+    """up to the most that is allowed, 2^20 a position"""
+    d = np.geomspace(2.0 ** -20, 3.0, 120).astype(np.float32)
+    for pos0 in (0, 100000, 1 << 24):
+        check_far_table(mi.Rope(rot_dim=240, theta=1e6, divisors=d.ctypes.data), pos0, 200, divisors=d)
