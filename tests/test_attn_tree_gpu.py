@@ -416,3 +416,74 @@ def test_a_row_start_that_falls_far_behind_is_refused(n, at):
     sync()
     assert int(host(b["flag"], np.uint32)[0]) == mi.STATUS_BAD_ROWS
     assert (host(b["out"], np.uint16) == 1234).all()
+
+
+def in_few_rows(c):
+    """of a case whose sequences have at most 16 columns: the exact outputs, what the kernel that keeps its weights in two f16 halves may be
+    off, and the outputs with each weight rounded to f16 once. A half is off by at most 2^-10 of what it holds, two halves by 2^-20; the
+    difference that the exponential takes (up to 8) by 2^-22 and the exponential by 2^-23 of it, 2^-21 with the weights' sum's; the sums
+    and the waves' join by 2^-19 of their terms. The other terms as above."""
+    want, tol, once = c.exact()[0], np.zeros((c.T, c.qh, c.hd)), np.zeros((c.T, c.qh, c.hd))
+    g = c.qh // c.kvh
+    for b, n in enumerate(c.rows):
+        rows, seen = slice(c.start[b], c.start[b] + n), c.seen(b)
+        for h in range(c.qh):
+            kd, vd, qd = c.k[b][h // g].astype(np.float64), c.v[b][h // g].astype(np.float64), c.q[rows, h].astype(np.float64)
+            s = np.where(seen, qd @ kd.T * c.scale, -np.inf)
+            ds = abs(c.scale) * (2.0 ** -21 + c.hd * 2.0 ** -23) * (np.abs(qd) @ np.abs(kd).T).max()
+            e = np.exp(s - s.max(1, keepdims=True)) * 128  # (the reference is 2^7 below the largest score)
+            z = e.sum(1, keepdims=True)
+            tol[rows, h] = (2.0 ** -20 + 2.0 ** -21 + 2.1 * ds + 2.0 ** -19) * (e / z @ np.abs(vd)) + kd.shape[0] * 2.0 ** -32 * np.abs(vd).max()
+            once[rows, h] = e.astype(np.float16).astype(np.float64) @ vd / z
+    return want, tol + 2.0 ** -11 * np.abs(want) + 2.0 ** -25, once
+
+
+@pytest.mark.parametrize("qh,kvh,hd", [(10, 2, 128), (16, 2, 256), (7, 1, 128), (8, 8, 256)])
+@pytest.mark.parametrize("lengths", [[(1, 1)], [(5, 1), (29, 1), (0, 2)], [(199, 1), (77, 1)]])
+@pytest.mark.parametrize("page", [0, 16, 64])
+def test_few_rows_keep_their_weights_in_two_halves(lengths, page, qh, kvh, hd):
+    """values that cancel, near scores: the outputs are small beside sum p|v|, and their own rounding hides nothing of the weights'"""
+    c = Case(page + hd, lengths, qh, kvh, hd, page=page, trees="causal", q_std=0.02)
+    for v in c.v:
+        n = v.shape[1] // 2
+        v[:, n:2 * n] = -v[:, :n]
+    want, tol, once = in_few_rows(c)
+    assert np.any(np.abs(once - want) > 2 * tol)  # (one half would be seen)
+    got = c.run().astype(np.float64)
+    assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+@pytest.mark.parametrize("rows", [1, 30])
+@pytest.mark.parametrize("page", [0, 64])
+def test_rows_so_far_apart_that_a_tile_passes_32_bits(rows, hd, page):
+    """above 2^25 elements a row, where the many columns' tiles are not addressed from their first rows"""
+    T = torch()
+    c = Case(rows + hd, [(70, rows), (9, rows)], 8, 2, hd, page=page)
+    strides = ((1 << 25) + 8, hd)
+
+    def place(x, by_row):
+        top = max(int(c.at(b).max()) for b in range(2))
+        t = T.empty(top * strides[0] + (c.kvh - 1) * strides[1] + hd, dtype=T.int16, device="cuda")
+        view = t.as_strided((top + 1, c.kvh, hd), (strides[0], strides[1], 1))
+        for b in range(2):
+            view[T.from_numpy(c.at(b)).cuda()] = T.from_numpy(np.ascontiguousarray(x[b].transpose(1, 0, 2)).view(np.int16)).cuda()
+        return t, strides
+
+    c.place = place
+    c.check()
+
+
+@pytest.mark.parametrize("lengths,qh,kvh,hd", [([(900, 61), (300, 40), (2000, 55)], 40, 8, 128), ([(5000, 60)], 16, 2, 256), ([(4000, 64)], 40, 8, 128),
+                                               ([(3000, 1), (70, 1), (800, 1)], 16, 2, 256)])
+def test_a_call_gives_the_same_bits_again(lengths, qh, kvh, hd):
+    """whatever the workspace held before"""
+    c = Case(7, lengths, qh, kvh, hd, page=64)
+    b = c.bind()
+    outs = []
+    for fill in (0, 77, 255):
+        b["ws"][:b["need"]] = fill
+        b["out"].fill_(1234)
+        mi.call("mi_attn_tree", *b["args"], stream())
+        outs.append(c.result(b).view(np.uint16))
+    assert np.array_equal(outs[0], outs[1]) and np.array_equal(outs[0], outs[2])
