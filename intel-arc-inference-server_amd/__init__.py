@@ -441,6 +441,8 @@ def accept_tree(argmax, tokens, parent):
     """mi_accept_tree: (the accepted drafts' nodes, next token)."""
     import numpy as np
     a, t, p = (np.ascontiguousarray(x, np.uint32) for x in (argmax, tokens, parent))
+    if not a.size == t.size == p.size:  # (tokens and parent have the text's next token too: node 0)
+        raise ValueError(f"accept_tree: {a.size} argmaxes, {t.size} tokens and {p.size} parents of as many nodes")
     path, nxt = np.zeros(a.size, np.uint32), u32()
     j = lib().mi_accept_tree(a.ctypes.data, t.ctypes.data, p.ctypes.data, a.size, path.ctypes.data, C.byref(nxt))
     return path[:j], int(nxt.value)

@@ -163,3 +163,12 @@ def test_accept_tree():
         argmax, drafts = rng.integers(0, 2, k + 1), rng.integers(0, 2, k)
         got, n = mi.accept_tree(argmax, [0, *drafts], [none, *range(k)])
         assert (len(got), n) == mi.accept_greedy(argmax, drafts) and list(got) == list(range(1, len(got) + 1))
+
+
+def test_accept_tree_takes_arrays_of_one_size():
+    none = mi.NONE
+    for argmax, tokens, parent in (([1, 2, 3], [5, 6], [none, 0, 1]), ([1, 2, 3], [5, 6, 7], [none, 0]), ([1], [], [none]), ([], [1], [none])):
+        with pytest.raises(ValueError, match="accept_tree"):
+            mi.accept_tree(argmax, tokens, parent)
+    path, _ = mi.accept_tree([], [], [])
+    assert path.size == 0
