@@ -40,8 +40,9 @@ struct LogprobArgs {
   // where a row has several slices: (m, Z, T, count) per (row, slice), the largest logit per (row, 256 tokens)
   f4_t* stats;
   float* peaks;
-  f2_t* sums;  // NULL, or the rows' (m, Z): top_logprobs are then the logits themselves
-  const uint32_t* skip;  // NULL, or rows (not 0) of which nothing is asked
+  // of beams: the rows' (m, Z) (top_logprobs are then the logits themselves); NULL, or rows (not 0) of which nothing is asked
+  f2_t* sums;
+  const uint32_t* skip;
 };
 
 // ---- the statistics ----
@@ -211,17 +212,19 @@ __device__ __forceinline__ float token_logit(const LogprobArgs& a, uint32_t row,
   return t < a.vocab ? a.logits[(size_t)row * a.row_stride + t] : __builtin_bit_cast(float, kNanBits);
 }
 // the row's answers, from its whole statistics (log_z = logf(s.z)) and its token's logit
+template <bool BEAMS>
 __device__ __forceinline__ void answer(const LogprobArgs& a, uint32_t row, const Stats& s, uint32_t count, float log_z, float xt,
                                        uint32_t lane) {
   if (lane != 0) return;
   if (a.entropy) a.entropy[row] = log_z - s.t / s.z * kLn2;
   if (a.logprob) a.logprob[row] = (xt - s.m) - log_z;
   if (a.rank) a.rank[row] = xt != xt ? kNone : count;
-  if (a.sums) a.sums[row] = f2_t{s.m, s.z};
+  if constexpr (BEAMS) a.sums[row] = f2_t{s.m, s.z};
 }
+template <bool BEAMS>
 __device__ __forceinline__ void answer_top(const LogprobArgs& a, uint32_t row, uint32_t place, Entry e, const Stats& s, float log_z) {
   a.top_ids[(size_t)row * a.top + place] = e.id;
-  a.top_logprobs[(size_t)row * a.top + place] = e.id == kNone ? -INFINITY : a.sums ? e.v : (e.v - s.m) - log_z;
+  a.top_logprobs[(size_t)row * a.top + place] = e.id == kNone ? -INFINITY : BEAMS ? e.v : (e.v - s.m) - log_z;
 }
 
 // four values' maxima over the wave: lane 0 the first's, 32 the second's, 16 the third's, 48 the fourth's
@@ -240,12 +243,14 @@ __device__ __forceinline__ float wave_max4(float a, float b, float c, float d) {
 }
 
 // grid (slices, rows): 4 waves walk a slice of the row's tokens, each 256 at a time. LISTS: the slice is the whole row, and
-// the waves keep its best tokens; otherwise they leave the largest logit of each 256. ONCE: by loads that the caches need not keep
-// (beams: 128 texts of 4 67.5 us in all, 77.5 with the others).
-template <bool LISTS, bool ONCE>
+// the waves keep its best tokens; otherwise they leave the largest logit of each 256. BEAMS: by loads that the caches need not keep
+// (128 texts of 4 67.5 us in all, 77.5 with the others), and with `sums` and `skip` (asked for when the kernel runs they took one row of
+// 151936 tokens of mi_logprobs from 11.6 to 11.9 us, 333 rows from 53.8 to 54.6).
+template <bool LISTS, bool BEAMS>
 __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.y;
-  if (a.skip && a.skip[row]) return;
+  if constexpr (BEAMS)
+    if (a.skip && a.skip[row]) return;
   const float* x = a.logits + (size_t)row * a.row_stride;
   const uint32_t begin = blockIdx.x * a.slice, end = min(begin + a.slice, a.vocab);
   uint32_t token, ahead = 0;
@@ -263,7 +268,7 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
       to[u] = f4_t{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (i + 4u <= end) {
         const auto* from = as_global(reinterpret_cast<const f4_any*>(x + i));
-        if constexpr (ONCE) to[u] = __builtin_nontemporal_load(from);
+        if constexpr (BEAMS) to[u] = __builtin_nontemporal_load(from);
         else to[u] = *from;
       } else if (i < end)
 #pragma unroll
@@ -355,8 +360,8 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
   if (!join_waves<4>(joint, s, count, list, LISTS ? a.top : 0u, wave, lane)) return;
   if constexpr (LISTS) {
     const float log_z = logf(s.z);
-    answer(a, row, s, count, log_z, xt, lane);
-    if (lane < a.top) answer_top(a, row, lane, list, s, log_z);
+    answer<BEAMS>(a, row, s, count, log_z, xt, lane);
+    if (lane < a.top) answer_top<BEAMS>(a, row, lane, list, s, log_z);
   } else if (lane == 0) a.stats[(size_t)row * a.slices + blockIdx.x] = f4_t{s.m, s.z, s.t, (float)count};
 }
 
@@ -367,10 +372,12 @@ __global__ __launch_bounds__(256, 5) void logprobs_kernel(LogprobArgs a) {
 // those read that are better. Where more tokens reach the bound than fit (equal logits, or fewer finite ones than k), the
 // waves keep lists. One row of 151936 with the 20 best takes 11.6 us, 16 rows 15.2, 333 with the 5 best 53 (lists from
 // every slice, as a row in one has them: 18.6, 23 and 54.2); one row of equal logits 21.6 (20.9).
+template <bool BEAMS>
 __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
   constexpr uint32_t W = 8, U = 4, B = 8, kFit = 1024;  // waves; a lane's runs looked at together; runs read together; tokens
   const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, row = blockIdx.x, runs = (a.vocab + 255u) / 256u;
-  if (a.skip && a.skip[row]) return;
+  if constexpr (BEAMS)
+    if (a.skip && a.skip[row]) return;
   const float* x = a.logits + (size_t)row * a.row_stride;
   const f4_t* stats = a.stats + (size_t)row * a.slices;
   const float* peaks = a.peaks + (size_t)row * runs;
@@ -508,7 +515,7 @@ __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
   merge_lanes(s);
   count = (uint32_t)wave_sum(lane < W ? (float)counts[lane] : 0.f);
   const float log_z = logf(s.z);
-  if (wave == 0) answer(a, row, s, count, log_z, xt, lane);
+  if (wave == 0) answer<BEAMS>(a, row, s, count, log_z, xt, lane);
   const uint32_t n = fits;
   if (n <= kFit) {
     for (uint32_t i0 = 0; i0 < n; i0 += 8u * W) {  // 8 lanes for each
@@ -520,9 +527,9 @@ __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
       place += xor_lane<1>(place);
       place += xor_lane<2>(place);
       place += xor_lane<4>(place);
-      if (i < n && place < a.top && (lane & 7u) == 0) answer_top(a, row, place, e, s, log_z);
+      if (i < n && place < a.top && (lane & 7u) == 0) answer_top<BEAMS>(a, row, place, e, s, log_z);
     }
-    for (uint32_t i = n + threadIdx.x; i < a.top; i += 64u * W) answer_top(a, row, i, Entry{}, s, log_z);  // (no such token)
+    for (uint32_t i = n + threadIdx.x; i < a.top; i += 64u * W) answer_top<BEAMS>(a, row, i, Entry{}, s, log_z);  // (no such token)
     return;
   }
   Entry list, last;
@@ -546,7 +553,7 @@ __global__ __launch_bounds__(512) void logprobs_join_kernel(LogprobArgs a) {
   __syncthreads();  // (the waves have read `fits`; what it counted is written over)
   Stats none;
   if (!join_waves<W>(sm.joint, none, count, list, a.top, wave, lane)) return;
-  if (lane < a.top) answer_top(a, row, lane, list, s, log_z);
+  if (lane < a.top) answer_top<BEAMS>(a, row, lane, list, s, log_z);
 }
 
 // ---- the best continuations of beams ----
@@ -869,7 +876,8 @@ bool launch(LogprobArgs a, uint32_t M, void* ws, hipStream_t st, const BeamArgs*
   else logprobs_kernel<false, false><<<dim3(a.slices, M), 256, 0, st>>>(a);
   const bool whole = beams && beams->beams * runs_of_wave(a.vocab) <= 64u * kJoinRuns;
   if (whole) beam_join_kernel<<<M / beams->beams, 64 * kJoinWaves, 0, st>>>(a, *beams);
-  else logprobs_join_kernel<<<M, 512, 0, st>>>(a);
+  else if (beams) logprobs_join_kernel<true><<<M, 512, 0, st>>>(a);
+  else logprobs_join_kernel<false><<<M, 512, 0, st>>>(a);
   return whole;
 }
 
