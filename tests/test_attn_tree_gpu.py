@@ -487,3 +487,23 @@ def test_a_call_gives_the_same_bits_again(lengths, qh, kvh, hd):
         mi.call("mi_attn_tree", *b["args"], stream())
         outs.append(c.result(b).view(np.uint16))
     assert np.array_equal(outs[0], outs[1]) and np.array_equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("page", [0, 64])
+def test_tokens_and_a_stretch_of_a_prompt_in_one_call_and_in_two(page):
+    lengths = [(100 * i, 1) for i in range(9)] + [(300, 90), (0, 40)]
+    c = Case(11, lengths, 10, 2, 128, page=page, trees="causal")
+    want, tol = c.check(), c.exact()[1]
+    b = c.bind()
+    L, n, T = mi.lib(), 9, c.T
+    for first, count, rows in ((0, n, n), (n, 2, T)):
+        off = 0 if page else first * c.stride * c.hd * 2
+        batch = mi.AttnBatch(sequences=count, kv_len=c.kv_len, table_stride=c.stride, page=c.page, n_pages=c.n_pages, words=0, mask=None,
+                             row_start=ptr(b["row_start"]) + 4 * first, cached=ptr(b["cached"]) + 4 * first,
+                             tables=ptr(b["tables"]) + 4 * first * c.stride if page else None)
+        assert L.mi_attn_tree_ws(rows, count, mi.C.byref(b["sh"])) <= b["need"]
+        mi.call("mi_attn_tree", ptr(b["q"]), ptr(b["k"]) + off, ptr(b["v"]) + off, *b["args"][3:5], rows, mi.C.byref(b["sh"]),
+                mi.C.byref(batch), *b["args"][8:], stream())
+    got = c.result(b).astype(np.float64)
+    assert np.all(np.abs(got - want) <= 2 * tol)
+    assert int(host(b["flag"], np.uint32)[0]) == 0
