@@ -592,9 +592,10 @@ int mi_attn_masked(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv
 /* The plan of a step from the requests' lengths. Request b has cached[b] keys in the pages that its table's first held[b] entries
  * name, and adds added[b] rows (0 and 0: it is done). It takes pages from the ring where ceil((cached + added) / page) is more than
  * held, request after request, and gives back those behind that number where it is less; the pages given back are free from
- * the next call on. ring: ring_len page ids, ring_at {first free one's place, how many are free}; a ring as long as there are
- * pages never overflows. held_out and ring_at_out may be held and ring_at themselves (a captured step then goes on from replay
- * to replay); they, cached and added do not overlap otherwise.
+ * the next call on. A page belongs to one request: of pages that several share no count is kept, and each would give them back.
+ * ring: ring_len page ids, ring_at {first free one's place, how many are free}; a ring as long as there are pages never overflows.
+ * held_out and ring_at_out may be held and ring_at themselves (a captured step then goes on from replay to replay); they, cached and
+ * added do not overlap otherwise.
  *   row_start [requests + 1]; of row t = row_start[b] + i: seq[t] = b, slot[t] the cache row of key cached[b] + i, pos[t] that key
  *   with parent [rows] (of each row the number of its parent among its sequence's rows, below its own, or none): mask [rows][words]
  *   gets bit i and the bits of its ancestors, and pos[t] = cached[b] + how many ancestors it has. words >= added / 32.
@@ -647,7 +648,8 @@ typedef struct mi_rope {
   const float* divisors;
 } mi_rope;
 /* table [n][2][rot_dim / 2] fp32 = (cos, sin)(p f_i) of the positions pos0 .. pos0 + n - 1, formed in 64 bits and rounded once:
- * what mi_attn_prep, mi_attn_prep_rows and mi_rope_rows read. rot_dim a multiple of 8 up to 256, positions below 2^31, theta above 1,
+ * what mi_attn_prep, mi_attn_prep_rows and mi_rope_rows read. rot_dim a multiple of 8 up to 256, n up to 2^24, positions below 2^31,
+ * theta above 1 up to 1e30, factor and attention up to 1e6, 0 < low < high up to 1e9, original from 1, divisors above 0,
  * f_i up to 2^20 (an angle is off by 2^-52 of itself: below 2^-24 up to angles of 2^28). */
 int mi_rope_table(const mi_rope* rope, uint32_t pos0, uint32_t n, float* table, void* stream);
 /* Rows of q||k||v (in_kind MI_OUT_F32 or MI_OUT_F16, rows in_stride elements apart): q and k are normed by head (RMSNorm with
@@ -657,8 +659,8 @@ int mi_rope_table(const mi_rope* rope, uint32_t pos0, uint32_t n, float* table, 
  * row * row_stride + head * head_stride. All of it in fp32, each k and v rounded once: mi_attn_prep_rows rounds to f16 before and
  * behind the norm too. A slot of none: the row has no k and v to store. rows: the cache's; a slot that is not below it
  * stores neither (MI_STATUS_BAD_PAGE); a position that is not below rope_len (the table's rows) stores nothing of its row
- * (0xDEAD0002). flag may be NULL. Slots are distinct. head_dim 128 or 256, rot_dim a multiple of 8, T up to 65535 and
- * T (q_heads + 2 kv_heads) up to 2^26, not gated. */
+ * (0xDEAD0002). flag may be NULL. Slots are distinct. head_dim 128 or 256, rot_dim a multiple of 8, up to 1024 q and 1024 kv heads,
+ * T up to 65535 and T (q_heads + 2 kv_heads) up to 2^26, not gated. */
 int mi_rope_rows(const void* qkv, uint32_t in_kind, size_t in_stride, uint32_t T, const uint32_t* pos, uint32_t pos0,
                  const uint32_t* slots, uint32_t rows, const mi_attn_shape* shape, uint32_t paired, const float* q_norm,
                  const float* k_norm, const float* rope, uint32_t rope_len, float* attn_q, uint16_t* kv_k, uint16_t* kv_v,
@@ -682,12 +684,15 @@ typedef struct mi_attn_batch {
  * probabilities are fp32; calls of more than 16 columns a sequence on average (T / sequences rows, rounded up, times q heads per kv
  * head) round each probability's numerator to f16 before the product with V, the others keep it in two f16 halves. How the keys are cut into
  * parts follows the lengths of all sequences, so a row's last bits depend on T and on the lengths beside it, never on the values.
+ * The average chooses the kernel: single tokens beside a stretch of a prompt may be faster as two calls (by up to a fifth), the
+ * tokens' sequences first with T their rows, then the others with row_start, cached and tables (without tables kv_k and kv_v) from
+ * theirs on and T all rows.
  * What a row does not see has no part in it, infinities and NaN included. A table entry that is not below n_pages, of a page that holds
  * a key of a sequence with rows, sets *flag = MI_STATUS_BAD_PAGE (flag may be NULL); nothing outside the cache is read. row_start
  * does not fall, so that no two sequences share a row: where an entry is below the one before it the call is refused on the device
- * (MI_STATUS_BAD_ROWS, no row is written). head_dim 128 or 256, up to 64 q heads per kv head, not gated; T up to 65535, 1..1024 sequences, kv_len up to 2^30,
- * words 1..64 with masks, 0 without. ws: mi_attn_tree_ws bytes of device scratch, 16-byte aligned; its size never falls as T grows
- * and is the same for any number of sequences. */
+ * (MI_STATUS_BAD_ROWS, no row is written). head_dim 128 or 256, up to 64 q heads per kv head and 1024 in all, not gated; T up to
+ * 65535, 1..1024 sequences, kv_len up to 2^30, words 1..64 with masks, 0 without. ws: mi_attn_tree_ws bytes of device scratch,
+ * 16-byte aligned; its size never falls as T grows and is the same for any number of sequences. */
 size_t mi_attn_tree_ws(uint32_t T, uint32_t sequences, const mi_attn_shape* shape);
 int mi_attn_tree(const float* attn_q, const uint16_t* kv_k, const uint16_t* kv_v, size_t row_stride, size_t head_stride,
                  uint32_t T, const mi_attn_shape* shape, const mi_attn_batch* batch, void* ws, size_t ws_bytes,
@@ -711,7 +716,7 @@ int mi_beam_select(const float* logits, size_t row_stride, const float* cum, con
  * of `per` (1..64). Within a list all rows are read before one is written: a tree's accepted rows closed up (list = sequence),
  * beams that change places (list = the beams' rows of one position). No row is written by two entries, and none that another list
  * writes is read or written. to = none: no move. A row that is not below `rows` (the cache's) is not moved (MI_STATUS_BAD_PAGE, flag may be
- * NULL). head_dim 128 or 256. */
+ * NULL). head_dim 128 or 256, up to 65535 layers and kv heads, up to 2^20 lists. */
 int mi_kv_move(uint16_t* kv_k, uint16_t* kv_v, uint32_t layers, size_t layer_stride, size_t row_stride, size_t head_stride,
                uint32_t kv_heads, uint32_t head_dim, uint32_t rows, const uint32_t* from, const uint32_t* to, uint32_t groups,
                uint32_t per, uint32_t* flag, void* stream);

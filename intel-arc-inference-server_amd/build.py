@@ -30,7 +30,7 @@ PER_FILE = {"attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
             # as attn.hip; loops at 64 bytes: the same loop took 98 or 107 us (500 rows over 4500 keys, 32 / 8 heads of 128) by where
             # the code before it happened to end
             "attn_masked.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-falign-loops=64"],
-            "attn_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-falign-loops=64"],  # attn_masked.hip's kernels
+            "attn_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-falign-loops=64"],  # (the few rows' kernel is the same, the other alike)
             # as attn.hip (one work-group per CU leaves 512 registers, and the accumulators then go to AGPRs and
             # back: 128 x 5120 x 34816 in 128 x 128 tiles 72.5 us against 64.2)
             "gemm_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],

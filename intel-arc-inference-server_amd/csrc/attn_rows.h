@@ -20,7 +20,9 @@
 // own rounding; the weights' sum is taken before).
 //
 // A key that a row does not see has weight 0, but 0 times an infinity or a NaN of its V row is a NaN. A block whose
-// result is not finite is therefore formed again, key by key, over the keys that each row sees.
+// result is not finite is therefore formed again, key by key, over the keys that each row sees. That is slow, and a call lasts as long
+// as its slowest block: with one NaN among the keys that one of 48 texts' next tokens sees they take 2.3 ms (0.27), 8 trees of up to 61
+// rows 36 ms (0.09).
 #pragma once
 #include <type_traits>
 
@@ -230,9 +232,9 @@ __device__ __forceinline__ u4_t load_row(const uint16_t* p) {
   if constexpr (ONCE) return __builtin_nontemporal_load(as_global(reinterpret_cast<const u4_t*>(p)));
   else return *reinterpret_cast<const u4_t*>(p);
 }
-// Few rows (16 columns per block): grid (kv_heads, row blocks, splits), 4 waves. A wave walks its own 32-key tiles,
-// every fourth of the split's: K from memory as the A operand, V through its own part of LDS for the transposing
-// reads, the next tile's rows in registers meanwhile. The waves' sums join through LDS.
+// Few rows (16 columns per block): grid (kv_heads, row blocks, splits), or with kItems work-groups that take such places one behind
+// another; 4 waves. A wave walks its own 32-key tiles, every fourth of the split's: K from memory as the A operand, V through its own
+// part of LDS for the transposing reads, the next tile's rows in registers meanwhile. The waves' sums join through LDS.
 template <int HD, typename A>
 __device__ __forceinline__ void few_rows_of(const A& a, const typename A::Place& p) {
   constexpr uint32_t KK = HD / 32, NT = HD / 16, VROW = HD + 16;

@@ -12,7 +12,7 @@
 // of a kv head follow one another, those that read the same keys (a sequence's blocks) side by side, and an XCD takes an even stretch
 // of all: with 8 kv heads one head, so that the XCDs' loads are alike whatever the lengths are. Sequences of several parts leave
 // sums, which a second launch joins. Code is short here and its loops are not unrolled: every work-group fetches it anew (sixteen
-// candidates of `per` one behind another took 5 us more than eight of them).
+// candidates of `per` in unrolled code took 5 us more than eight; the 64 of part_tiles are a lane each).
 #include <algorithm>
 
 #include "attn_rows.h"
@@ -669,10 +669,13 @@ __global__ __launch_bounds__(256) void attn_tree_join_kernel(TreeArgs a, uint32_
 //   rows of 256: CT 1 up to 64 columns, else 2. Measured (us): 6 ragged sequences up to 8200 keys, 16 / 2 heads, 8 rows 28.5
 //   against 32.7; 8 sequences, 30 rows 57.4 against 55.8; one of 131072, 60 rows 254 against 204.
 //   rows of 128: one sequence's rows make blocks / CT work-groups of a known number: the least modelled time of 2, 3 and 4, a
-//   block's tile 1.1, 1.375 and 1.7 us of a CU. Measured (us; CT 2, 3, 4): over 65536 keys, 40 / 8 heads, 25 rows 81 / 101 / 127, 38
-//   rows 117 / 100 / 121, 51 rows 211 / 167 / 121, 64 rows 209 / 168 / 200; over 8192 keys 27 / 27 / 31, 32 / 30 / 33, 37 / 37 / 36,
-//   38 / 38 / 44. Of several sequences only the mean is known: CT 2, which loses least where they are ragged (8 trees of 38 to 61
-//   rows 107 / 141 / 162; of 51 each, 4000 keys, 77 / 84 / 70).
+//   block's tile 1.1, 1.375 and 1.7 us of a CU. Measured (us; CT 2, 3, 4; 40 / 8 heads; 25, 38, 51 and 64 rows): over 65536 keys
+//   83 / 82 / 82, 111 / 97 / 97, 184 / 151 / 117, 193 / 155 / 185; over 8192 29 / 27 / 27, 33 / 32 / 32, 37 / 38 / 38, 39 / 40 / 46;
+//   over 4096 27 / 23 / 23, 28 / 27 / 28, 31 / 30 / 32, 32 / 31 / 36. Of several sequences only the mean is known: CT 2, which
+//   loses least where they are ragged (8 trees of 38 to 61 rows 93 / 105 / 125; of 51 each, 4000 keys, 93 / 85 / 72).
+// The mean says little of single tokens beside a stretch of a prompt, 40 / 8 heads, taken as one call / as two (us): 48 tokens up to 16000
+// keys and 100 rows behind 2000 329 / 301, and 512 rows 351 / 337; 63 tokens up to 4000 and 128 rows behind 4000 187 / 155; 300 and
+// 300 rows 665 / 560; 31 and 512 rows behind none 88 / 91.
 struct Pick {
   bool few;
   uint32_t ct, rows, columns, slots;

@@ -667,7 +667,9 @@ __global__ __launch_bounds__(256) void beam_select_kernel(BeamArgs a) {
 // statistics; form a bound that k runs of 256 tokens reach by the score of their largest logit (as logprobs_join_kernel's); read again
 // the runs that reach it, of all beams about k; and a token's place is the number of those read that are better. Where more tokens reach
 // the bound than fit, the waves keep a list of every beam. One text of 4 beams with k = 8 takes 13.4 us in all, 16 of 8 with k = 16
-// 28.7 (16.0 and 32 with the rows' lists first); equal logits 45, rising ones 104. Bound by its chain of loads.
+// 28.7 (16.0 and 32 with the rows' lists first); equal logits 45, rising ones 104. Bound by its chain of loads. A wave with fewer runs
+// than its share of k leaves no bound (all vocabularies of 1025 to 3840 tokens; one beam of 8000 with k = 64): the lists then do it all
+// again, one text of 16 beams of 3800 tokens 59 us with k = 20 and 84 with 64, where 8000 tokens take 13 and 22.
 constexpr uint32_t kFit = 1024, kMaxBeams = 64;
 constexpr uint32_t kJoinWaves = 16, kJoinRuns = 8;  // a lane's runs
 uint32_t runs_of_wave(uint32_t vocab) { return ((vocab + 255u) / 256u + kJoinWaves - 1u) / kJoinWaves; }
